@@ -310,6 +310,70 @@ int k8v4_prefill_uses_tiles(int64_t seq_len, int64_t q_len, int hkv, int head_di
 int64_t k8v4_attn_workspace_bytes(int64_t batch, int64_t table_width, int pages_per_block,
                                   int q_len, int hkv, int head_dim, int num_splits);
 
+/*
+ * Reading the cache back: K and V rows of a ragged batch of token ranges,
+ * dequantized (the inverse of k8v4_kv_store_paged; the gather and
+ * dequantization of k8v4_v030/dequant.py:96-106 as an entry of its own).
+ *
+ * Row r of k_out / v_out ([rows][hkv][head_dim] of out_dtype, token strides
+ * k_out_stride / v_out_stride elements; either may be NULL) belongs to the
+ * sequence b with row_starts[b] <= r < row_starts[b + 1] and receives its
+ * token seq_starts[b] + r - row_starts[b]: K = code * k_scale, V = (nibble -
+ * v_zero) * v_scale in fp32, rounded once more to a 16-bit out_dtype (a value
+ * beyond fp16's range becomes an infinity, as a conversion makes it).
+ * row_starts: int32 [batch + 1] (device), not decreasing; seq_starts: int32
+ * [batch] (device) or NULL for 0.  block_table as in k8v4_attn_batch.  A token
+ * outside its table row or on a page outside the cache gives zeros; rows of
+ * no sequence (before row_starts[0], from row_starts[batch] on) are left as
+ * they were, and no row from `rows` on is written whatever row_starts holds.
+ */
+int k8v4_kv_load_paged(const int8_t *k_cache, const float *k_scale, const uint8_t *v_cache, const float *v_scale,
+                       const float *v_zero, int64_t num_pages, int64_t k_page_stride, int64_t ks_page_stride,
+                       int64_t v_page_stride, int64_t vs_page_stride, int64_t vz_page_stride,
+                       const int32_t *block_table, int64_t bt_stride, int64_t table_width, int pages_per_block,
+                       const int32_t *seq_starts, const int32_t *row_starts, int64_t batch, int hkv, int head_dim,
+                       void *k_out, void *v_out, int out_dtype, int64_t k_out_stride, int64_t v_out_stride,
+                       int64_t rows, void *stream);
+
+/*
+ * Verification of drafted tokens (no counterpart in the reference, whose
+ * engine samples): accepts a prefix of each sequence's drafts and draws the
+ * token behind it, so that the tokens are distributed as the target's own.
+ *
+ * target_probs: [batch][max_drafts + 1][vocab] of `dtype`, strides in
+ * elements, unit stride over the vocabulary; position i is the target's
+ * distribution after i drafts.  draft_probs: [batch][max_drafts][vocab] of the
+ * same dtype, or NULL for drafts chosen outright (probability 1 each).
+ * draft_tokens: int32, or int64 where tokens_are_int64, [batch][max_drafts].
+ * num_drafts: int32 [batch] (clamped to 0 .. max_drafts) or NULL for
+ * max_drafts.  accept_uniform: fp32 [batch][max_drafts], sample_uniform: fp32
+ * [batch], both in [0, 1).
+ * Draft i is accepted iff accept_uniform[i] * q_i(x_i) < p_i(x_i); a draft
+ * outside the vocabulary is refused.  With a drafts accepted before the first
+ * refusal, weights w = max(p_a - q_a, 0) (p_a without x_a for drafts chosen
+ * outright) where draft a was refused, p_a where none was or where those leave
+ * no weight; the drawn token is the lowest v with w_0 + .. + w_v >
+ * sample_uniform * sum(w).  Weights need not add up to 1; a negative or NaN
+ * one counts as none; a row without any draws -1.  Products, weights and sums
+ * are formed in float64, in a fixed order.
+ * out_tokens: int64 [batch][max_drafts + 1], the a accepted drafts, the drawn
+ * token, then -1.  accepted: int32 [batch], a.  next_lens (NULL: not wanted;
+ * may be seq_lens): int32 [batch], seq_lens + a + 1: where seq_lens counts a
+ * step's query tokens, what the next step of as many query tokens takes.
+ * workspace: >= k8v4_verify_drafts_workspace_bytes(batch, vocab) bytes, 16-byte
+ * aligned.  max_drafts <= 63, vocab <= 2^24, batch <= 65535.
+ */
+int k8v4_verify_drafts(const void *target_probs, int dtype, int64_t target_seq_stride, int64_t target_row_stride,
+                       const void *draft_probs, int64_t draft_seq_stride, int64_t draft_row_stride,
+                       const void *draft_tokens, int tokens_are_int64, int64_t token_stride,
+                       const int32_t *num_drafts, const float *accept_uniform, int64_t uniform_stride,
+                       const float *sample_uniform, const int32_t *seq_lens, int64_t batch, int max_drafts,
+                       int64_t vocab, int64_t *out_tokens, int64_t out_stride, int32_t *accepted,
+                       int32_t *next_lens, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Workspace bytes k8v4_verify_drafts needs (-1 on bad arguments). */
+int64_t k8v4_verify_drafts_workspace_bytes(int64_t batch, int64_t vocab);
+
 #ifdef __cplusplus
 }
 #endif

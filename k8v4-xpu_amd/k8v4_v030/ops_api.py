@@ -97,6 +97,19 @@ _EXTRA_SYMBOLS.append((
 _EXTRA_SYMBOLS.append(("k8v4_attn_batch_noalloc", _EXTRA_SYMBOLS[0][1][:28] + [_i32, _vp], _i32))
 _EXTRA_SYMBOLS.append(("k8v4_attn_noalloc_max_bytes", [], _i64))
 _EXTRA_SYMBOLS.append(("k8v4_decode_fault_count", [], _i64))
+_EXTRA_SYMBOLS.append((
+    "k8v4_kv_load_paged",
+    [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64,
+     _vp, _i64, _i64, _i32, _vp, _vp, _i64, _i32, _i32, _vp, _vp, _i32, _i64, _i64, _i64, _vp],
+    _i32,
+))
+_EXTRA_SYMBOLS.append((
+    "k8v4_verify_drafts",
+    [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _i64, _vp, _vp, _i64, _vp, _vp,
+     _i64, _i32, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp],
+    _i32,
+))
+_EXTRA_SYMBOLS.append(("k8v4_verify_drafts_workspace_bytes", [_i64, _i64], _i64))
 Q_TOKENS, Q_PADDED = 0, 1
 
 
@@ -268,6 +281,19 @@ class BoundCall:
             _require(self._profiled is not None, "this op has no staged variant")
             rc = self._profiled(*self._args, stream, int(split_done_event or 0), int(stages))
         _check(rc, self._lib)
+
+
+class DeviceCall(BoundCall):
+    """A :class:`BoundCall` that launches on its tensors' device, whichever is current."""
+
+    __slots__ = ()
+
+    def __call__(self) -> None:
+        if torch.cuda.current_device() == self._dev.index:
+            _check(self._fn(*self._args, _stream(self._dev)), self._lib)
+            return
+        with torch.cuda.device(self._dev):
+            _check(self._fn(*self._args, _stream(self._dev)), self._lib)
 
 
 class _Ops:
@@ -572,6 +598,149 @@ class _Ops:
                                           _ptr(v_zero), int(v_cache.shape[0]), int(v_cache.stride(0)),
                                           int(v_scale.stride(0)) * 4, int(v_zero.stride(0)) * 4, _stream(dev))
         _check(rc, self._lib)
+
+    # -- reading the cache back ----------------------------------------------
+    def kv_load_paged(self, k_cache, k_scale, v_cache, v_scale, v_zero, block_table, seq_starts, row_starts,
+                      pages_per_block, k_out, v_out):
+        """The inverse of :meth:`kv_store_paged`: cached K/V rows of a ragged batch, dequantized.
+
+        Sequence b's tokens from ``seq_starts[b]`` (int32 ``[B]``; None: 0) on go to
+        rows ``row_starts[b] .. row_starts[b + 1] - 1`` (int32 ``[B + 1]``, not
+        decreasing) of ``k_out`` / ``v_out`` ``[N, HKV, D]`` (fp16, bf16 or fp32;
+        either may be None), its pages in ``block_table[b]``.  A token outside its
+        table row or on a page outside the cache gives zeros; rows that belong to
+        no sequence are left as they were."""
+        bound = self.bind_kv_load_paged(k_cache, k_scale, v_cache, v_scale, v_zero, block_table, seq_starts,
+                                        row_starts, pages_per_block, k_out, v_out)
+        if bound is not None:
+            bound()
+
+    def bind_kv_load_paged(self, k_cache, k_scale, v_cache, v_scale, v_zero, block_table, seq_starts, row_starts,
+                           pages_per_block, k_out, v_out):
+        """Validate a read once; returns a :class:`DeviceCall` (None when there are no rows)."""
+        outs = [x for x in (k_out, v_out) if x is not None]
+        _require(len(outs) > 0, "k_out or v_out")
+        _require(k_cache.dim() == 4 and v_cache.dim() == 4, "k_cache [num_blocks,64,HKV,D] NHD")
+        hkv, head_dim = _checked_hkv(int(k_cache.shape[2])), int(k_cache.shape[3])
+        _require(head_dim in (128, 256), "k_cache head dim must be 128 or 256")
+        check_paged_k(k_cache, k_scale, hkv, head_dim)
+        check_paged_v(v_cache, v_scale, v_zero, hkv, head_dim)
+        _require(k_cache.shape[0] == v_cache.shape[0], "k/v num_blocks")
+        _require(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1,
+                 "block_table must be int32 [B, W] with unit column stride")
+        batch = int(block_table.shape[0])
+        _require(row_starts.dtype == torch.int32 and row_starts.dim() == 1 and row_starts.shape[0] == batch + 1
+                 and row_starts.is_contiguous(), "row_starts must be a contiguous int32 [B + 1]")
+        if seq_starts is not None:
+            _require(seq_starts.dtype == torch.int32 and seq_starts.dim() == 1 and seq_starts.shape[0] == batch
+                     and seq_starts.is_contiguous(), "seq_starts must be a contiguous int32 [B]")
+        _require(int(pages_per_block) >= 1, "pages_per_block")
+        rows, dtype = int(outs[0].shape[0]) if outs[0].dim() else -1, outs[0].dtype
+        _require(dtype in (torch.float16, torch.bfloat16, torch.float32), "k/v_out float16, bfloat16 or float32")
+        for x in outs:
+            _require(x.dtype == dtype, "k/v_out dtypes differ")
+            _require(x.shape == (rows, hkv, head_dim), "k/v_out [N,%d,%d]" % (hkv, head_dim))
+            _require(x.stride(2) == 1 and x.stride(1) == head_dim, "k/v_out head/dim strides")
+        if rows == 0 or batch == 0:
+            return None
+        _require(int(block_table.shape[1]) > 0, "block_table width")
+        tensors = (k_cache, k_scale, v_cache, v_scale, v_zero, block_table, row_starts, *outs)
+        if seq_starts is not None:
+            tensors += (seq_starts,)
+        dev = _on_gpu(*tensors)
+        row = hkv * head_dim
+        args = [
+            *cache_args(k_cache, k_scale, v_cache, v_scale, v_zero),
+            _ptr(block_table), int(block_table.stride(0)), int(block_table.shape[1]), int(pages_per_block),
+            0 if seq_starts is None else _ptr(seq_starts), _ptr(row_starts), batch, hkv, head_dim,
+            0 if k_out is None else _ptr(k_out), 0 if v_out is None else _ptr(v_out), _DTYPE_CODE[dtype],
+            row if k_out is None or rows == 1 else int(k_out.stride(0)),
+            row if v_out is None or rows == 1 else int(v_out.stride(0)), rows,
+        ]
+        return DeviceCall(self._lib, self._lib.k8v4_kv_load_paged, args, dev, tensors)
+
+    # -- verification of drafted tokens ----------------------------------------
+    def verify_drafts_workspace_bytes(self, batch: int, vocab: int) -> int:
+        """Scratch bytes :meth:`verify_drafts` needs (any number of drafts)."""
+        n = int(self._lib.k8v4_verify_drafts_workspace_bytes(int(batch), int(vocab)))
+        _require(n >= 0, "bad shape for the verify workspace")
+        return n
+
+    def verify_drafts(self, target_probs, draft_probs, draft_tokens, num_drafts, accept_uniform, sample_uniform,
+                      seq_lens, workspace, out_tokens, accepted, next_lens):
+        """Accept or refuse a step's drafted tokens and sample the token after them.
+
+        ``target_probs`` ``[B, K + 1, V]`` and ``draft_probs`` ``[B, K, V]`` (None: the
+        drafts were chosen outright) of one dtype (fp16, bf16, fp32); ``draft_tokens``
+        int32 or int64 ``[B, K]``; ``num_drafts`` int32 ``[B]`` (None: K each);
+        ``accept_uniform`` fp32 ``[B, K]`` and ``sample_uniform`` fp32 ``[B]`` in [0, 1).
+        Draft i is accepted iff ``u_i q_i(x_i) < p_i(x_i)``; behind the first refusal
+        (or the last draft) one token is drawn from ``max(p - q, 0)`` (or ``p``).
+        ``out_tokens`` int64 ``[B, K + 1]``: the accepted drafts, the drawn token, then
+        -1; ``accepted`` int32 ``[B]``; ``next_lens`` int32 ``[B]`` (None: not wanted;
+        may be ``seq_lens``): ``seq_lens + accepted + 1``, what the next step's
+        attention takes.  A row without any positive probability draws -1."""
+        bound = self.bind_verify_drafts(target_probs, draft_probs, draft_tokens, num_drafts, accept_uniform,
+                                        sample_uniform, seq_lens, workspace, out_tokens, accepted, next_lens)
+        if bound is not None:
+            bound()
+
+    def bind_verify_drafts(self, target_probs, draft_probs, draft_tokens, num_drafts, accept_uniform,
+                           sample_uniform, seq_lens, workspace, out_tokens, accepted, next_lens):
+        """Validate a verification once; returns a :class:`DeviceCall` (None for an empty batch)."""
+        _require(target_probs.dim() == 3, "target_probs [B,K+1,V]")
+        _require(target_probs.dtype in (torch.float16, torch.bfloat16, torch.float32),
+                 "target_probs float16, bfloat16 or float32")
+        batch, drafts, vocab = int(target_probs.shape[0]), int(target_probs.shape[1]) - 1, int(target_probs.shape[2])
+        _require(drafts >= 0 and vocab >= 1, "target_probs [B,K+1,V]")
+        _require(target_probs.stride(2) == 1 or vocab == 1, "target_probs rows must be contiguous")
+        tensors = (target_probs, draft_tokens, accept_uniform, sample_uniform, workspace, out_tokens, accepted)
+        if draft_probs is not None:
+            _require(draft_probs.shape == (batch, drafts, vocab), "draft_probs [B,K,V]")
+            _require(draft_probs.dtype == target_probs.dtype, "target/draft_probs dtypes differ")
+            _require(draft_probs.stride(2) == 1 or vocab == 1, "draft_probs rows must be contiguous")
+            tensors += (draft_probs,)
+        _require(draft_tokens.dtype in (torch.int32, torch.int64) and draft_tokens.shape == (batch, drafts),
+                 "draft_tokens int32 or int64 [B,K]")
+        _require(drafts <= 1 or draft_tokens.stride(1) == 1, "draft_tokens rows must be contiguous")
+        _require(accept_uniform.dtype == torch.float32 and accept_uniform.shape == (batch, drafts),
+                 "accept_uniform float32 [B,K]")
+        _require(drafts <= 1 or accept_uniform.stride(1) == 1, "accept_uniform rows must be contiguous")
+        _require(sample_uniform.dtype == torch.float32 and sample_uniform.shape == (batch,)
+                 and sample_uniform.is_contiguous(), "sample_uniform must be a contiguous float32 [B]")
+        _require(out_tokens.dtype == torch.int64 and out_tokens.shape == (batch, drafts + 1)
+                 and (drafts == 0 or out_tokens.stride(1) == 1), "out_tokens int64 [B,K+1] with contiguous rows")
+        _require(next_lens is None or seq_lens is not None, "next_lens needs seq_lens")
+        for name, x in (("num_drafts", num_drafts), ("seq_lens", seq_lens), ("accepted", accepted),
+                        ("next_lens", next_lens)):
+            if x is not None or name == "accepted":
+                _require(x is not None and x.dtype == torch.int32 and x.shape == (batch,) and x.is_contiguous(),
+                         "%s must be a contiguous int32 [B]" % name)
+                if name != "accepted":
+                    tensors += (x,)
+        _require(workspace.is_contiguous(), "verify workspace must be a contiguous buffer")
+        if batch == 0:
+            return None
+        dev = _on_gpu(*tensors)
+        many = batch > 1
+        has_q = draft_probs is not None
+        args = [
+            _ptr(target_probs), _DTYPE_CODE[target_probs.dtype],
+            int(target_probs.stride(0)) if many else vocab * (drafts + 1),
+            int(target_probs.stride(1)) if drafts else vocab,
+            _ptr(draft_probs) if has_q else 0,
+            int(draft_probs.stride(0)) if has_q and many else vocab * max(drafts, 1),
+            int(draft_probs.stride(1)) if has_q and drafts > 1 else vocab,
+            _ptr(draft_tokens), int(draft_tokens.dtype == torch.int64),
+            int(draft_tokens.stride(0)) if many else drafts,
+            0 if num_drafts is None else _ptr(num_drafts),
+            _ptr(accept_uniform), int(accept_uniform.stride(0)) if many else drafts, _ptr(sample_uniform),
+            0 if seq_lens is None else _ptr(seq_lens), batch, drafts, vocab,
+            _ptr(out_tokens), int(out_tokens.stride(0)) if many else drafts + 1, _ptr(accepted),
+            0 if next_lens is None else _ptr(next_lens),
+            _ptr(workspace), int(workspace.numel()) * workspace.element_size(),
+        ]
+        return DeviceCall(self._lib, self._lib.k8v4_verify_drafts, args, dev, tensors)
 
     # -- the Q-once tile and the ops that read it ----------------------------
     def q_quant_once(self, q_fp16, q8, q_scale):
