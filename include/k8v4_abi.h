@@ -311,6 +311,35 @@ int64_t k8v4_attn_workspace_bytes(int64_t batch, int64_t table_width, int pages_
                                   int q_len, int hkv, int head_dim, int num_splits);
 
 /*
+ * k8v4_attn_batch for sequences that begin with the same cached pages, those
+ * read once for the whole batch (no counterpart in the reference, whose batch
+ * op attends to each sequence alone, k8v4_v030/native/xe2_kv_ops.cpp:1728-1775).
+ *
+ * prefix_table: int32 [prefix_width], the table entries of the first
+ * prefix_len tokens (NULL allowed where they fill no page).  Its prefix_len /
+ * 64 whole pages stand for the first pages of every sequence, whose own rows
+ * of block_table are not read there; the tokens behind them come from those
+ * rows.  seq_lens: int32 [batch] (device), all tokens of a sequence, the
+ * prefix and the step's own included; the causal end of token j is seq_len -
+ * q_len + j + 1.  A row whose end lies inside the prefix sees it up to there;
+ * one that sees no key outputs zeros, whatever its query holds.  Query rows,
+ * cache, table entries, out and the numerics as in k8v4_attn_batch.
+ * workspace: >= k8v4_attn_shared_workspace_bytes(batch, q_len, hkv, head_dim)
+ * bytes, 16-byte aligned: the quantized query rows and the states of the page
+ * runs.  Calls that may overlap (other streams, captured graphs) need one each.
+ */
+int k8v4_attn_shared(const void *q, int q_dtype, int64_t q_tok_stride, const int8_t *k_cache, const float *k_scale,
+                     const uint8_t *v_cache, const float *v_scale, const float *v_zero, int64_t num_pages,
+                     int64_t k_page_stride, int64_t ks_page_stride, int64_t v_page_stride, int64_t vs_page_stride,
+                     int64_t vz_page_stride, const int32_t *prefix_table, int64_t prefix_width, int64_t prefix_len,
+                     const int32_t *block_table, int64_t bt_stride, int64_t table_width, int pages_per_block,
+                     const int32_t *seq_lens, int64_t batch, int q_len, int hkv, int head_dim, void *out,
+                     int out_dtype, int64_t out_tok_stride, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Workspace bytes k8v4_attn_shared needs, whatever the lengths (-1 on bad arguments). */
+int64_t k8v4_attn_shared_workspace_bytes(int64_t batch, int q_len, int hkv, int head_dim);
+
+/*
  * Reading the cache back: K and V rows of a ragged batch of token ranges,
  * dequantized (the inverse of k8v4_kv_store_paged; the gather and
  * dequantization of k8v4_v030/dequant.py:96-106 as an entry of its own).

@@ -1,0 +1,864 @@
+// Paged decode / MTP-verify attention of a batch whose sequences begin with
+// the same cached pages, those read once for all of them.
+//
+// For every query row (token j of sequence b, query head) with visible end
+// e = seq_len_b - q_len + j + 1, softmax attention over the keys t < e as in
+// k8v4_attn_batch (int8-quantized query rows, exact integer scores, V as
+// (nibble - zero) * scale), where the keys below P (the prefix's whole pages)
+// are those of one table row and the others those of the sequence's own row.
+// With the (max m, sum l, output O / l) of disjoint key ranges i,
+//   out = sum_i 2^(m_i - M) l_i O_i / sum_i 2^(m_i - M) l_i,  M = max m_i,
+// so the prefix and each sequence's own keys are attended to apart, each cut
+// into page runs, and folded at the end.  Three launches: the query rows are
+// quantized (q_quant.hip), the page runs attended to, the states folded.
+//
+// The work is a list of segments: first the prefix once for every eight
+// consecutive tokens of the batch (48 rows of a KV head: three full 16-row
+// tiles, whichever sequences they belong to), then each sequence's own pages
+// for its tokens (nine or ten tokens: two segments).  Laid end to end, with a
+// fixed cost ahead of each segment's pages, they form one axis that is cut
+// into equal parts, one per work-group, so a work-group takes one or more
+// pieces of consecutive segments and all end together: a prefix of 2,000 pages
+// beside 200 sequences of two pages keeps the chip as busy as one of either
+// kind alone.  Every work-group derives the same cut from the lengths on the
+// device, so a captured call follows them.
+//
+// Inside a piece the kernel is the decode split kernel's: per KV head two
+// waves (head dim 256: the half-heads of a pair) over rings of LDS slots
+// filled by direct-to-LDS loads, see decode_chunk.h and decode.hip.
+#include "decode_chunk.h"
+
+namespace k8v4 {
+namespace {
+
+constexpr int kGroup = 8;  // tokens of one segment: 48 rows of a KV head
+// Fixed cost of a piece in pages of its pages' time.
+constexpr int kPieceCost = 6;
+constexpr int kFar = 1 << 30;
+
+struct SharedArgs {
+  const int8_t *q8;  // quantized query rows [hkv][head_rows][head_dim]
+  const float *q8_scale;
+  int64_t head_rows;
+  const int8_t *k_cache;
+  const float *k_scale;
+  const uint8_t *v_cache;
+  const float *v_scale;
+  const float *v_zero;
+  int64_t num_pages;
+  int64_t k_ps, ks_ps, v_ps, vs_ps, vz_ps;  // page strides, bytes
+  int planes_fast;                          // see DecodeArgs in decode.hip
+  int64_t d_kv, d_vz;
+  const int32_t *prefix_table;
+  int prefix_pages;
+  const int32_t *block_table;
+  int64_t bt_stride;
+  int table_pages;  // pages a table row covers
+  int ppb;
+  const int32_t *seq_lens;
+  int batch, q_len, hkv;
+  int tokens;      // batch * q_len
+  int groups;      // prefix segments (0 without a prefix)
+  int per_seq;     // own segments of a sequence: 1, or 2 for more than eight tokens
+  int grid;        // work-groups of the split launch
+  char *ws;        // states: prefix pieces, then the others
+  int prefix_rows, own_rows;        // state rows of a KV head in a piece of either kind
+  int64_t prefix_bytes, own_bytes;  // bytes of such a state
+  int merge_cs;    // column slices per output row in the merge
+  void *out;
+  int out_dtype;
+  int64_t out_tok_stride;  // elements
+};
+
+// Length of sequence b's own segments on the axis: its pages behind the
+// prefix and the fixed cost, or nothing.
+__device__ __forceinline__ int own_pages(const SharedArgs &a, int len) {
+  const int pages = len > 0 ? min(static_cast<int>((static_cast<int64_t>(len) + kPage - 1) / kPage), a.table_pages) : 0;
+  return max(pages - a.prefix_pages, 0);
+}
+__device__ __forceinline__ int own_cost(const SharedArgs &a, int len) {
+  const int n = own_pages(a, len);
+  return n > 0 ? n + kPieceCost : 0;
+}
+__device__ __forceinline__ int prefix_cost(const SharedArgs &a) { return a.prefix_pages + kPieceCost; }
+
+// Units of the axis that one work-group takes, and the units ahead of
+// sequence `b` among the own segments.
+struct Axis {
+  int unit;
+  int before;
+};
+__device__ Axis plan_axis(const SharedArgs &a, int lane, int b) {
+  int own = 0, before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kWave) {
+    const int i = b0 + lane;
+    const int c = i < a.batch ? own_cost(a, a.seq_lens[i]) * a.per_seq : 0;
+    own += c;
+    before += i < b ? c : 0;
+  }
+  Axis x;
+  const int total = a.groups * prefix_cost(a) + wave_sum(own);
+  x.unit = __builtin_amdgcn_readfirstlane(max(1, (total + a.grid - 1) / a.grid));
+  x.before = wave_sum(before);
+  return x;
+}
+
+// The segment that holds unit u of the axis (or the first one behind it) and
+// where that segment begins; segments 0 .. groups - 1 are the prefix's.
+struct Where {
+  int seg;
+  int base;
+};
+__device__ Where locate(const SharedArgs &a, int lane, int u) {
+  Where w;
+  const int pre = a.groups * prefix_cost(a);
+  if (u < pre) {
+    w.seg = u / prefix_cost(a);
+    w.base = w.seg * prefix_cost(a);
+    return w;
+  }
+  int base = pre;
+  for (int b0 = 0; b0 < a.batch; b0 += kWave) {
+    const int i = b0 + lane;
+    const int c = i < a.batch ? own_cost(a, a.seq_lens[i]) : 0;
+    const int incl = base + wave_inclusive_scan(c * a.per_seq);
+    const uint64_t past = __ballot(i < a.batch && incl > u);
+    if (past) {
+      const int src = __builtin_ctzll(past);
+      const int cost = __builtin_amdgcn_readlane(c, src);
+      const int first = __builtin_amdgcn_readlane(incl, src) - cost * a.per_seq;
+      const int sub = u >= first + cost ? 1 : 0;  // at most two segments a sequence
+      w.seg = __builtin_amdgcn_readfirstlane(a.groups + (b0 + src) * a.per_seq + sub);
+      w.base = __builtin_amdgcn_readfirstlane(first + sub * cost);
+      return w;
+    }
+    base = __builtin_amdgcn_readlane(incl, kWave - 1);
+  }
+  w.seg = a.groups + a.batch * a.per_seq;
+  w.base = base;
+  return w;
+}
+
+// State of the piece that work-group g makes of a segment.  A work-group's
+// pieces are of different segments and a segment's of different work-groups,
+// both in the order of the axis, so g + segment is a number of its own.
+__device__ __forceinline__ char *piece_state(const SharedArgs &a, int g, int seg) {
+  if (seg < a.groups) return a.ws + static_cast<int64_t>(g + seg) * a.prefix_bytes;
+  return a.ws + static_cast<int64_t>(a.groups ? a.grid + a.groups : 0) * a.prefix_bytes +
+         static_cast<int64_t>(g + seg - a.groups) * a.own_bytes;
+}
+
+// x of lane `src`.
+__device__ __forceinline__ float lane_value(float x, int src) {
+  return __int_as_float(__builtin_amdgcn_ds_bpermute(4 * src, __float_as_int(x)));
+}
+
+// The arguments again, through a pointer the compiler knows nothing of: read
+// where they are used, instead of being held in scalar registers (more than
+// there are) across the pieces of a work-group.
+typedef const __attribute__((address_space(4))) SharedArgs *args_ptr;
+__device__ __forceinline__ args_ptr reread(args_ptr p) {
+  asm volatile("" : "+s"(p));
+  return p;
+}
+
+template <int NT, int HKV, int NWH, bool PH>
+__global__ __attribute__((amdgpu_flat_work_group_size(64 * HKV * NWH, 64 * HKV * NWH),
+                          amdgpu_waves_per_eu(SplitConfig<128, NT, HKV, NWH, PH>::OCC,
+                                              SplitConfig<128, NT, HKV, NWH, PH>::OCC)))
+void shared_split_kernel(SharedArgs args) {
+  constexpr int D = 128;  // PH: dims of a half-head
+  using S = Slot<D>;
+  using CFG = SplitConfig<D, NT, HKV, NWH, PH>;
+  constexpr int RK = CFG::RK, RV = CFG::RV, DQ = CFG::DQ, KSQ = DQ / 64;
+  __shared__ __attribute__((aligned(16))) char lds_raw[CFG::LDS_BYTES];
+  lds_t *lds = (lds_t *)(lds_raw);
+
+  const int wg = static_cast<int>(blockIdx.x);
+  int u0, u1, seg, base;
+  {
+    const int lane = threadIdx.x & (kWave - 1);
+    const int unit = plan_axis(args, lane, 0).unit;
+    u0 = wg * unit;
+    u1 = u0 + unit;
+    const Where at = locate(args, lane, u0);
+    seg = at.seg;
+    base = at.base;
+  }
+
+  // The pieces of this work-group (uniform over it).
+  const int segments = args.groups + args.batch * args.per_seq;
+  for (; seg < segments && base < u1; ++seg) {
+    // Nothing derived from the lane or the arguments is kept from one piece to
+    // the next: hoisted out of this loop it would take the registers the
+    // piece needs (NT = 3: 63 of them spilled).
+    const SharedArgs &a = (const SharedArgs &)*reread((args_ptr)__builtin_amdgcn_kernarg_segment_ptr());
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int h = wave % HKV;  // KV head (PH: half-head)
+    const int w = wave / HKV;  // position among the NWH waves of this head
+    const int hq = PH ? h >> 1 : h;
+    const int half = PH ? h & 1 : 0;
+    const int n = lane & 15, g = lane >> 4;
+    lds_t *qlds = lds + CFG::Q_OFF + hq * CFG::Q_BYTES_PER_HEAD;
+    lds_t *kring = lds + wave * CFG::WAVE_BYTES;
+    lds_t *vring = kring + RK * S::K_BYTES;
+    lds_int *flags = reinterpret_cast<lds_int *>(lds + CFG::FLAG_OFF);
+    const LaneOffsets lo = lane_offsets<D, HKV, PH>(a, h, lane);
+    const const_i32_ptr lens = (const_i32_ptr)(a.seq_lens);
+
+    const bool shared = seg < a.groups;
+    const int os = seg - a.groups;  // own segment
+    const int b = shared ? 0 : os / a.per_seq;
+    const int sub = shared ? 0 : os - b * a.per_seq;
+    const int len = shared ? 0 : lens[b];
+    const int pages = shared ? a.prefix_pages : own_pages(a, len);
+    const int first = base + kPieceCost;  // of the segment's pages on the axis
+    base = pages > 0 ? first + pages : base;
+    const int s0 = max(u0 - first, 0), s1 = min(u1 - first, pages);
+    if (s1 <= s0) continue;
+    const int p0 = (shared ? 0 : a.prefix_pages) + s0, p1 = (shared ? 0 : a.prefix_pages) + s1;
+    const int L0 = shared ? a.prefix_pages * kPage : len;
+    const int tok0 = shared ? seg * kGroup : b * a.q_len + sub * kGroup;
+    const int ntok = shared ? min(kGroup, a.tokens - tok0) : min(kGroup, a.q_len - sub * kGroup);
+    const int rows = ntok * kGqa;
+    const int x0 = 2 * p0;
+    const int x1 = min(2 * p1, static_cast<int>((static_cast<int64_t>(L0) + 31) / 32));
+    const int32_t *bt_row = shared ? a.prefix_table : a.block_table + static_cast<int64_t>(b) * a.bt_stride;
+
+    // Causal ends of this lane's rows: row r is token tok0 + r / 6, of any
+    // sequence in a prefix segment.  A row that sees no key at all (a padding
+    // sequence) takes no part in the masking, which it would force on every
+    // chunk; its state is dropped below.
+    WaveState<D, NT> st;
+    int far = 0;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = 16 * nt + n;
+      int end = L0;
+      if (r < rows) {
+        const int tok = tok0 + r / kGqa;
+        const int sb = tok / a.q_len;
+        end = a.seq_lens[sb] - a.q_len + (tok - sb * a.q_len) + 1;
+      }
+      st.lim[nt] = min(end, L0);
+      if (end > 0) far = max(far, kFar - min(st.lim[nt], kFar));
+    }
+    const int min_end = kFar - wave_max(far);
+
+    const int my0 = x0 + w;
+    const int cnt = my0 < x1 ? (x1 - my0 + NWH - 1) / NWH : 0;
+    // The query rows' fragments go straight into their operand positions
+    // (lane L of fragment (nt, ks) is 16 bytes at 16 L: row 16 nt + n, dims 64
+    // ks + 16 g), the rows' scales into the factor words.  The rows behind a
+    // short segment's last are other rows of the buffer (it is padded at the
+    // end); they are zeroed below.
+    int issued = 0;  // DMA bookkeeping as in the decode split kernel
+    {
+      const int8_t *tile = a.q8 + (hq * a.head_rows + static_cast<int64_t>(tok0) * kGqa) * DQ;
+      const float *scales = a.q8_scale + hq * a.head_rows + static_cast<int64_t>(tok0) * kGqa;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if (nt % NWH != w) continue;
+#pragma unroll
+        for (int ks = 2 * half; ks < 2 * half + 2; ++ks) {
+          dma16s(tile, static_cast<uint32_t>((16 * nt + n) * DQ + 64 * ks + 16 * g), qlds + (nt * KSQ + ks) * kWave * 16);
+          ++issued;
+        }
+      }
+      if (w == 0 && half == 0) {
+        if (lane < NT * 16) dma4s(scales, static_cast<uint32_t>(lane * 4), qlds + CFG::Q_FRAG_BYTES);
+        ++issued;
+      }
+    }
+    const int q_done = issued;
+    // Physical pages of the piece, looked up once (runs of up to 128 pages).
+    const bool tab_vgpr = p1 - p0 <= 128;
+    int ptab[2] = {-1, -1};
+    if (tab_vgpr) {
+      int raw[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int p = min(p0 + 64 * i + lane, p1 - 1);
+        raw[i] = bt_row[a.ppb <= 1 ? p : p / a.ppb];
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int p = p0 + 64 * i + lane;
+        const int64_t ph = a.ppb <= 1 ? raw[i] : static_cast<int64_t>(raw[i]) * a.ppb + p % a.ppb;
+        ptab[i] = (p < p1 && ph >= 0 && ph < a.num_pages) ? static_cast<int>(ph) : -1;
+      }
+    }
+    auto page_of = [&](int x) -> int {  // x: chunk index in the sequence (wave-uniform)
+      const int p = x >> 1;
+      if (tab_vgpr) {
+        const int d = p - p0;
+        const int lo_pg = __builtin_amdgcn_readlane(ptab[0], d & 63);
+        const int hi_pg = __builtin_amdgcn_readlane(ptab[1], d & 63);
+        return d < 64 ? lo_pg : hi_pg;
+      }
+      const const_i32_ptr row = (const_i32_ptr)(bt_row);
+      const int64_t ph = a.ppb <= 1 ? row[p] : static_cast<int64_t>(row[p / a.ppb]) * a.ppb + p % a.ppb;
+      return (ph >= 0 && ph < a.num_pages) ? static_cast<int>(ph) : -1;
+    };
+    int mk[4] = {0, 0, 0, 0}, mv[4] = {0, 0, 0, 0};
+    uint32_t valid_mask = 0;  // bit s: K slot s holds a chunk of a valid page
+#pragma unroll
+    for (int s = 0; s < (RK > RV ? RK : RV); ++s) {
+      if (s >= cnt) break;
+      const int xs = my0 + s * NWH;
+      if (s < RK) {
+        valid_mask |= static_cast<uint32_t>(issue_k<D, HKV>(a, page_of(xs), xs, lo, kring + s * S::K_BYTES)) << s;
+        issued += S::NK;
+        mk[s] = issued;
+      }
+      if (s < RV) {
+        issue_v<D, HKV, PH>(a, page_of(xs), xs, lo, lane, vring + s * S::V_BYTES);
+        issued += S::NVS;
+        mv[s] = issued;
+      }
+    }
+    wait_vm(issued - q_done);  // the query rows are here
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      if (nt % NWH != w || 16 * nt + n < rows) continue;
+#pragma unroll
+      for (int ks = 2 * half; ks < 2 * half + 2; ++ks)
+        *reinterpret_cast<__attribute__((address_space(3))) v4i *>(qlds + ((nt * KSQ + ks) * kWave + lane) * 16) =
+            (v4i){0, 0, 0, 0};
+    }
+    if constexpr (PH) {
+      pair_flag_set(flags + wave, 0, lane);
+      pair_flag_set(flags + CFG::WAVES + wave, 0, lane);
+    } else if constexpr (CFG::BALANCE) {
+      pair_flag_set(flags + wave, 0, lane);
+    }
+    // Fragments and factors visible to both waves of the head (a bare barrier:
+    // __syncthreads() would also wait for every ring load in flight).
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float f =
+          reinterpret_cast<const __attribute__((address_space(3))) float *>(qlds + CFG::Q_FRAG_BYTES)[nt * 16 + n];
+      // Kept above zero so that a masked (-inf) score never meets a zero factor.
+      const double c = static_cast<double>(16 * nt + n < rows ? f : 0.f) *
+                       (static_cast<double>(kLog2e) / sqrt(static_cast<double>(DQ)));
+      st.crow[nt] = fmaxf(static_cast<float>(c), 1e-30f);
+      st.lsum[nt] = (v4f){0.f, 0.f, 0.f, 0.f};
+      st.corr[nt] = (v4f){0.f, 0.f, 0.f, 0.f};
+      st.m_run[nt] = -INFINITY;
+      st.thr[nt] = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) st.O[nt][0][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+    }
+
+    for (int k = 0; k < cnt; ++k) {
+      const int sk = k % RK, sv = k % RV;  // wave-uniform ring slots
+      if constexpr (CFG::BALANCE) {
+        // The two waves of a SIMD yield to each other (see the decode split kernel).
+        pair_flag_set(flags + wave, k, lane);
+        const int pk = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const volatile lds_int *>(flags + (wave ^ 4)));
+        if (k > pk)
+          __builtin_amdgcn_s_setprio(0);
+        else
+          __builtin_amdgcn_s_setprio(1);
+      }
+      lds_t *kslot = kring + sk * S::K_BYTES;
+      lds_t *vslot = vring + sv * S::V_BYTES;
+      int mks = mk[0], mvs = mv[0];
+#pragma unroll
+      for (int s = 1; s < RK; ++s)
+        if (sk == s) mks = mk[s];
+#pragma unroll
+      for (int s = 1; s < RV; ++s)
+        if (sv == s) mvs = mv[s];
+      {
+        const int left = issued - max(mks, mvs);
+        if (left == CFG::STEADY_AFTER)
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(CFG::STEADY_AFTER) : "memory");
+        else
+          wait_vm(left);
+      }
+      if constexpr (PH) {
+        pair_flag_set(flags + wave, k + 1, lane);
+        pair_flag_wait(flags + (wave ^ 1), k + 1, lane);
+      }
+      const bool valid = (valid_mask >> sk) & 1u;
+      const int tbase = 32 * (my0 + k * NWH);
+      v4i sc[2][NT];
+      if constexpr (PH) {
+        const lds_t *pslot = lds + (wave ^ 1) * CFG::WAVE_BYTES + sk * S::K_BYTES;
+        if (valid) chunk_qk_pair<NT>(half ? pslot : kslot, half ? kslot : pslot, qlds, lane, g, sc);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        pair_flag_set(flags + CFG::WAVES + wave, k + 1, lane);
+      } else {
+        if (valid) chunk_qk<D, NT>(kslot, qlds, lane, g, sc);
+      }
+      auto refill_k = [&]() {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        const int xr = my0 + (k + RK) * NWH;
+        const uint32_t v = static_cast<uint32_t>(issue_k<D, HKV>(a, page_of(xr), xr, lo, kslot));
+        valid_mask = (valid_mask & ~(1u << sk)) | (v << sk);
+        issued += S::NK;
+#pragma unroll
+        for (int s = 0; s < RK; ++s)
+          if (sk == s) mk[s] = issued;
+      };
+      if (CFG::K_EARLY && k + RK < cnt) refill_k();
+      if (valid) chunk_softmax_pv<D, NT, PH>(st, sc, vslot, tbase, L0, lane, g, tbase + 32 > min_end);
+      if (!CFG::K_EARLY && k + RK < cnt) {
+        if constexpr (PH) pair_flag_wait(flags + CFG::WAVES + (wave ^ 1), k + 1, lane);
+        refill_k();
+      }
+      if (k + RV < cnt) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        const int xr = my0 + (k + RV) * NWH;
+        issue_v<D, HKV, PH>(a, page_of(xr), xr, lo, lane, vslot);
+        issued += S::NVS;
+#pragma unroll
+        for (int s = 0; s < RV; ++s)
+          if (sv == s) mv[s] = issued;
+      }
+    }
+
+    finalize_output(st);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+      if (st.lim[nt] <= 0) st.m_run[nt] = -INFINITY;
+
+    // The state's form is the decode split kernel's: a quarter of O / l in fp16,
+    // then m and l.
+    auto write_state = [&]() {
+      const int srows = shared ? a.prefix_rows : a.own_rows;
+      char *state = piece_state(a, wg, seg);
+      _Float16 *obase = reinterpret_cast<_Float16 *>(state);
+      float2 *mlbase = reinterpret_cast<float2 *>(state + static_cast<int64_t>(CFG::QHEADS) * srows * DQ * 2);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 16 * nt + 4 * g + i;
+          const float m_r = lane_value(st.m_run[nt], 4 * g + i);
+          if (r < rows) {
+            // A row that saw nothing: zeros, whatever its lanes hold (a padding
+            // row's query may be anything).
+            const bool seen = m_r != -INFINITY;
+            const float l = seen ? st.lsum[nt][i] : 0.f;
+            const float f = l > 0.f ? 0.25f / l : 0.f;
+            _Float16 *dst = obase + static_cast<int64_t>(hq * srows + r) * DQ + half * 128 + 8 * n;
+            v8h o;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = static_cast<_Float16>(seen ? st.O[nt][0][j][i] * f : 0.f);
+            store_wt16(dst, o);
+            if (n == 0 && half == 0) store_wt8(mlbase + hq * srows + r, make_float2(m_r, l));
+          }
+        }
+      }
+    };
+    // Combine the two waves of each head, then write the state.
+    if constexpr (NWH > 1) {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __syncthreads();  // every ring is drained; the LDS serves the exchange
+      float *xb = reinterpret_cast<float *>(lds_raw) + h * (CFG::XCHG_FLOATS);
+      if (w == 1) {
+        int e = 0;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          xb[(e++) * kWave + lane] = st.m_run[nt];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) xb[(e++) * kWave + lane] = st.lsum[nt][i];
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) xb[(e++) * kWave + lane] = st.O[nt][0][j][i];
+        }
+      }
+      __syncthreads();
+      if (w == 0) {
+        int e = 0;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float m1 = xb[(e++) * kWave + lane];
+          const float m0 = st.m_run[nt];
+          const float M = fmaxf(m0, m1);
+          const float a0 = m0 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m0 - M);
+          const float a1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - M);
+          st.m_run[nt] = M;
+          float a0i[4], a1i[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            a0i[i] = lane_value(a0, 4 * g + i);
+            a1i[i] = lane_value(a1, 4 * g + i);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) st.lsum[nt][i] = st.lsum[nt][i] * a0i[i] + xb[(e++) * kWave + lane] * a1i[i];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              st.O[nt][0][j][i] = st.O[nt][0][j][i] * a0i[i] + xb[(e++) * kWave + lane] * a1i[i];
+            // Combined here, not where the rows are written: there the words
+            // of all columns would wait in registers (21 of them spilled).
+            asm volatile("" : "+v"(st.O[nt][0][j]));
+          }
+        }
+        write_state();
+      }
+    }
+    if constexpr (NWH == 1) write_state();
+    // The next piece's loads overwrite the LDS and count from zero.
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
+}
+
+// Folds the states of one column slice of one output row (token, query head):
+// the prefix's for its group, then its sequence's own.
+template <int D, int TPU>
+__global__ __launch_bounds__(TPU) void shared_merge_kernel(SharedArgs a) {
+  constexpr int NW = TPU / kWave;
+  __shared__ float red[NW * 32 * 10];  // per wave and column: M, l, o[8]
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = threadIdx.x / kWave;
+  const int hq = kGqa * a.hkv;
+  const int unit = static_cast<int>(blockIdx.x);
+  const int row_id = unit / a.merge_cs;
+  const int slice = unit - row_id * a.merge_cs;
+  const int tok = row_id / hq, qh = row_id - tok * hq;
+  const int h = qh / kGqa, i6 = qh - h * kGqa;
+  const int b = tok / a.q_len, j = tok - b * a.q_len;
+
+  const int VPR = (D / 8) / a.merge_cs;
+  const int SPI = TPU / VPR;
+  const int t = threadIdx.x, col = t % VPR, sg = t / VPR;
+
+  const Axis ax = plan_axis(a, lane, b);
+  // Pieces of the row's prefix segment and of its own one.
+  int pf = 0, pn = 0, of = 0, on = 0;
+  const int ps = tok / kGroup, sub = j / kGroup;
+  const int os = b * a.per_seq + sub;
+  if (a.groups) {
+    const int first = ps * prefix_cost(a) + kPieceCost;
+    pf = first / ax.unit;
+    pn = (first + a.prefix_pages - 1) / ax.unit - pf + 1;
+  }
+  const int len = a.seq_lens[b];
+  const int pages = own_pages(a, len);
+  if (pages > 0) {
+    const int first = a.groups * prefix_cost(a) + ax.before + sub * (pages + kPieceCost) + kPieceCost;
+    of = first / ax.unit;
+    on = (first + pages - 1) / ax.unit - of + 1;
+  }
+  const int dcol = 8 * (slice * VPR + col);
+  const int pr = h * a.prefix_rows + (tok - ps * kGroup) * kGqa + i6;
+  const int orow = h * a.own_rows + (j - sub * kGroup) * kGqa + i6;
+  const char *pbase = piece_state(a, pf, ps), *obase = piece_state(a, of, a.groups + os);
+  const int64_t p_o = (static_cast<int64_t>(pr) * D + dcol) * 2;
+  const int64_t p_ml = static_cast<int64_t>(a.hkv) * a.prefix_rows * D * 2 + pr * 8;
+  const int64_t o_o = (static_cast<int64_t>(orow) * D + dcol) * 2;
+  const int64_t o_ml = static_cast<int64_t>(a.hkv) * a.own_rows * D * 2 + orow * 8;
+
+  MergeAcc acc{-INFINITY, 0.f, (v8f){0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}};
+  const int count = pn + on;
+  for (int s0 = sg; s0 < count; s0 += kMergeMU * SPI) {
+    // All loads are issued before any is used; a state past the last reads
+    // the last one and is dropped.
+    MergeRound rd;
+    v8h raw[kMergeMU];
+    float2 ml[kMergeMU];
+#pragma unroll
+    for (int u = 0; u < kMergeMU; ++u) {
+      const int s = min(s0 + u * SPI, count - 1);
+      const bool pre = s < pn;
+      const char *state = pre ? pbase + s * a.prefix_bytes : obase + (s - pn) * a.own_bytes;
+      ml[u] = *reinterpret_cast<const float2 *>(state + (pre ? p_ml : o_ml));
+      raw[u] = *reinterpret_cast<const v8h *>(state + (pre ? p_o : o_o));
+    }
+#pragma unroll
+    for (int u = 0; u < kMergeMU; ++u) {
+      const bool live = s0 + u * SPI < count;
+      rd.ms[u] = live ? ml[u].x : -INFINITY;
+      rd.ls[u] = live ? ml[u].y : 0.f;
+      rd.os[u] = live ? __builtin_convertvector(raw[u], v8f) : (v8f){0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    }
+    merge_fold_round(acc, rd);
+  }
+  // The lanes of one column in a wave are col + VPR * k: combine them.
+  float Mw = acc.M;
+  for (int off = VPR; off < kWave; off <<= 1) Mw = fmaxf(Mw, __shfl_xor(Mw, off, kWave));
+  merge_rescale(acc, Mw);
+  for (int off = VPR; off < kWave; off <<= 1) {
+    acc.l += __shfl_xor(acc.l, off, kWave);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc.o[e] += __shfl_xor(acc.o[e], off, kWave);
+  }
+  // Then the waves: each publishes its columns, wave 0 folds them.
+  if (lane < VPR) {
+    float *x = red + (wave * 32 + lane) * 10;
+    x[0] = acc.M;
+    x[1] = acc.l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[2 + e] = acc.o[e];
+  }
+  __syncthreads();
+  if (wave != 0 || lane >= VPR) return;
+  float Mg = acc.M;
+#pragma unroll
+  for (int v = 1; v < NW; ++v) Mg = fmaxf(Mg, red[(v * 32 + lane) * 10]);
+  merge_rescale(acc, Mg);
+#pragma unroll
+  for (int v = 1; v < NW; ++v) {
+    const float *x = red + (v * 32 + lane) * 10;
+    MergeAcc y{x[0], x[1], (v8f){x[2], x[3], x[4], x[5], x[6], x[7], x[8], x[9]}};
+    merge_rescale(y, Mg);
+    acc.l += y.l;
+    acc.o += y.o;
+  }
+  const float inv = acc.l > 0.f ? 1.f / acc.l : 0.f;
+  const int64_t ob = static_cast<int64_t>(tok) * a.out_tok_stride + static_cast<int64_t>(qh) * D + dcol;
+  const v8f o = acc.o * inv;
+  const uintptr_t addr = reinterpret_cast<uintptr_t>(a.out) + static_cast<uintptr_t>(ob) * (a.out_dtype == K8V4_F32 ? 4 : 2);
+  if (a.out_dtype == K8V4_F16 && addr % 16 == 0) {
+    *reinterpret_cast<v8h *>(addr) = __builtin_convertvector(o, v8h);
+  } else if (a.out_dtype == K8V4_BF16 && addr % 16 == 0) {
+    *reinterpret_cast<v8bf *>(addr) = __builtin_convertvector(o, v8bf);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) store_out(a.out, a.out_dtype, ob + e, o[e]);
+  }
+}
+
+template <int HKV, int NWH, bool PH>
+void launch_split(const SharedArgs &a, int tiles, hipStream_t s) {
+  const dim3 grid(a.grid), block(64 * HKV * NWH);
+  if (tiles == 1)
+    shared_split_kernel<1, HKV, NWH, PH><<<grid, block, 0, s>>>(a);
+  else if (tiles == 2)
+    shared_split_kernel<2, HKV, NWH, PH><<<grid, block, 0, s>>>(a);
+  else
+    shared_split_kernel<3, HKV, NWH, PH><<<grid, block, 0, s>>>(a);
+}
+
+int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
+
+// What a call of this shape keeps in its workspace: the quantized query rows,
+// their scales, then the states.
+struct SharedShape {
+  int64_t tokens, groups, per_seq, head_rows, grid;
+  int prefix_rows, own_rows;
+  int64_t prefix_bytes, own_bytes;
+  int64_t q_bytes, scale_bytes, state_bytes;
+};
+SharedShape shape_of(int64_t batch, int q_len, int hkv, int head_dim) {
+  SharedShape s;
+  s.tokens = batch * q_len;
+  s.groups = (s.tokens + kGroup - 1) / kGroup;
+  s.per_seq = (q_len + kGroup - 1) / kGroup;
+  s.head_rows = s.tokens * kGqa + 3 * 16;  // a last segment's tiles read rows behind the last token's
+  // One work-group per CU, two with two 128-dim heads (half the waves).
+  s.grid = static_cast<int64_t>(device_cus()) * (hkv == 2 && head_dim == 128 ? 2 : 1);
+  s.prefix_rows = static_cast<int>(s.tokens < kGroup ? s.tokens : kGroup) * kGqa;
+  s.own_rows = (q_len < kGroup ? q_len : kGroup) * kGqa;
+  s.prefix_bytes = static_cast<int64_t>(hkv) * s.prefix_rows * (2 * head_dim + 8);
+  s.own_bytes = static_cast<int64_t>(hkv) * s.own_rows * (2 * head_dim + 8);
+  s.q_bytes = round256(hkv * s.head_rows * head_dim);
+  s.scale_bytes = round256(hkv * s.head_rows * 4);
+  s.state_bytes = (s.grid + s.groups) * s.prefix_bytes + (s.grid + batch * s.per_seq) * s.own_bytes;
+  return s;
+}
+
+constexpr int64_t kMaxBatch = int64_t(1) << 20;
+
+}  // namespace
+
+int64_t shared_wait_timeouts() {
+  int n = 0;
+  const hipError_t e = hipMemcpyFromSymbol(&n, HIP_SYMBOL(g_pair_wait_timeouts), sizeof(n));
+  if (e != hipSuccess) {
+    set_error("k8v4_decode_fault_count: %s", hipGetErrorString(e));
+    return -1;
+  }
+  return n;
+}
+
+}  // namespace k8v4
+
+extern "C" int64_t k8v4_attn_shared_workspace_bytes(int64_t batch, int q_len, int hkv, int head_dim) {
+  using namespace k8v4;
+  if (batch < 1 || batch > kMaxBatch || q_len < 1 || q_len * kGqa > kPage || !supported_heads(hkv) ||
+      !supported_dim(head_dim))
+    return -1;
+  const SharedShape s = shape_of(batch, q_len, hkv, head_dim);
+  return s.q_bytes + s.scale_bytes + s.state_bytes;
+}
+
+extern "C" int k8v4_attn_shared(const void *q, int q_dtype, int64_t q_tok_stride, const int8_t *k_cache,
+                                const float *k_scale, const uint8_t *v_cache, const float *v_scale,
+                                const float *v_zero, int64_t num_pages, int64_t k_page_stride,
+                                int64_t ks_page_stride, int64_t v_page_stride, int64_t vs_page_stride,
+                                int64_t vz_page_stride, const int32_t *prefix_table, int64_t prefix_width,
+                                int64_t prefix_len, const int32_t *block_table, int64_t bt_stride,
+                                int64_t table_width, int pages_per_block, const int32_t *seq_lens, int64_t batch,
+                                int q_len, int hkv, int head_dim, void *out, int out_dtype, int64_t out_tok_stride,
+                                void *workspace, int64_t workspace_bytes, void *stream) {
+  using namespace k8v4;
+  clear_error();
+  K8V4_REQUIRE(supported_heads(hkv), "unsupported per-GPU KV head count %d (this library serves 2 or 4)", hkv);
+  K8V4_REQUIRE(supported_dim(head_dim), "unsupported head dim %d (this library serves 128 or 256)", head_dim);
+  K8V4_REQUIRE(q_len >= 1 && q_len * kGqa <= kPage, "q_len*GQA exceeds BM (q_len=%d)", q_len);
+  K8V4_REQUIRE(pages_per_block >= 1, "pages_per_block");
+  K8V4_REQUIRE(num_pages >= 1 && num_pages <= INT32_MAX, "num_pages must be 1 .. 2^31 - 1");
+  K8V4_REQUIRE(batch >= 1 && batch <= kMaxBatch, "empty or too large batch");
+  K8V4_REQUIRE(table_width >= 1 && table_width <= (int64_t(1) << 24) / pages_per_block, "block_table width");
+  K8V4_REQUIRE(prefix_len >= 0, "negative prefix length");
+  const int64_t prefix_pages = prefix_len / kPage;  // whole pages are shared, a part of one is each sequence's own
+  K8V4_REQUIRE(prefix_pages <= (int64_t(1) << 24), "prefix too long");
+  K8V4_REQUIRE(prefix_pages == 0 || prefix_width >= (prefix_pages + pages_per_block - 1) / pages_per_block,
+               "prefix_table has %lld entries, the prefix of %lld tokens needs %lld",
+               static_cast<long long>(prefix_width), static_cast<long long>(prefix_len),
+               static_cast<long long>((prefix_pages + pages_per_block - 1) / pages_per_block));
+  K8V4_REQUIRE(q_dtype == K8V4_F16 || q_dtype == K8V4_BF16, "q dtype must be fp16 or bf16");
+  K8V4_REQUIRE(out_dtype == K8V4_F16 || out_dtype == K8V4_BF16 || out_dtype == K8V4_F32,
+               "out dtype must be fp16, bf16 or fp32");
+  K8V4_REQUIRE(q && k_cache && k_scale && v_cache && v_scale && v_zero && block_table && seq_lens && out && workspace &&
+                   (prefix_table || prefix_pages == 0),
+               "null pointer");
+  const auto aligned = [](const void *p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
+  K8V4_REQUIRE(aligned(q, 16) && q_tok_stride % 8 == 0,
+               "q must be 16-byte aligned with a token stride that is a multiple of 8 elements");
+  const int64_t row = static_cast<int64_t>(hkv) * kGqa * head_dim;
+  K8V4_REQUIRE(q_tok_stride >= row, "q token stride shorter than HQ*D");
+  K8V4_REQUIRE(out_tok_stride >= row, "out token stride shorter than HQ*D");
+  K8V4_REQUIRE(aligned(out, out_dtype == K8V4_F32 ? 4 : 2), "out misaligned");
+  K8V4_REQUIRE(bt_stride >= table_width, "block_table row stride shorter than its width");
+  K8V4_REQUIRE(aligned(block_table, 4) && aligned(prefix_table, 4) && aligned(seq_lens, 4), "index arrays misaligned");
+  K8V4_REQUIRE(aligned(k_cache, 16) && k_page_stride % 16 == 0, "k_cache must keep 16-byte aligned rows");
+  K8V4_REQUIRE(aligned(v_cache, 4) && v_page_stride % 4 == 0, "v_cache must keep 4-byte aligned rows");
+  K8V4_REQUIRE(aligned(k_scale, 8) && aligned(v_scale, 8) && aligned(v_zero, 8) && ks_page_stride % 8 == 0 &&
+                   vs_page_stride % 8 == 0 && vz_page_stride % 8 == 0,
+               "scale planes must be 8-byte aligned");
+  K8V4_REQUIRE(aligned(workspace, 16), "workspace must be 16-byte aligned");
+
+  const SharedShape sh = shape_of(batch, q_len, hkv, head_dim);
+  const int64_t need = sh.q_bytes + sh.scale_bytes + sh.state_bytes;
+  if (workspace_bytes < need) {
+    set_error("shared-prefix workspace holds %lld bytes, the batch needs %lld", static_cast<long long>(workspace_bytes),
+              static_cast<long long>(need));
+    return K8V4_ERR_WORKSPACE;
+  }
+  const int64_t table_pages = table_width * pages_per_block;
+  const int64_t groups = prefix_pages ? sh.groups : 0;
+  // The axis has at most this many units; a work-group's end may pass it by a
+  // work-group's share.
+  const int64_t units = groups * (prefix_pages + kPieceCost) +
+                        batch * sh.per_seq * ((table_pages > prefix_pages ? table_pages - prefix_pages : 0) + kPieceCost);
+  K8V4_REQUIRE(units < (int64_t(1) << 30), "batch too large for one call");
+
+  SharedArgs a;
+  char *ws = static_cast<char *>(workspace);
+  int8_t *q8 = reinterpret_cast<int8_t *>(ws);
+  float *scales = reinterpret_cast<float *>(ws + sh.q_bytes);
+  a.q8 = q8;
+  a.q8_scale = scales;
+  a.head_rows = sh.head_rows;
+  a.k_cache = k_cache;
+  a.k_scale = k_scale;
+  a.v_cache = v_cache;
+  a.v_scale = v_scale;
+  a.v_zero = v_zero;
+  a.num_pages = num_pages;
+  a.k_ps = k_page_stride;
+  a.ks_ps = ks_page_stride;
+  a.v_ps = v_page_stride;
+  a.vs_ps = vs_page_stride;
+  a.vz_ps = vz_page_stride;
+  {
+    const int64_t dkv = reinterpret_cast<intptr_t>(v_scale) - reinterpret_cast<intptr_t>(k_scale);
+    const int64_t dvz = reinterpret_cast<intptr_t>(v_zero) - reinterpret_cast<intptr_t>(v_scale);
+    const int64_t lim = int64_t(1) << 30;
+    a.planes_fast = ks_page_stride == vs_page_stride && vs_page_stride == vz_page_stride && dkv > -lim &&
+                    dkv < lim && dvz > -lim && dvz < lim;
+    a.d_kv = a.planes_fast ? dkv : 0;
+    a.d_vz = a.planes_fast ? dvz : 0;
+  }
+  a.prefix_table = prefix_table;
+  a.prefix_pages = static_cast<int>(prefix_pages);
+  a.block_table = block_table;
+  a.bt_stride = bt_stride;
+  a.table_pages = static_cast<int>(table_pages);
+  a.ppb = pages_per_block;
+  a.seq_lens = seq_lens;
+  a.batch = static_cast<int>(batch);
+  a.q_len = q_len;
+  a.hkv = hkv;
+  a.tokens = static_cast<int>(sh.tokens);
+  a.groups = static_cast<int>(groups);
+  a.per_seq = static_cast<int>(sh.per_seq);
+  a.grid = static_cast<int>(sh.grid);
+  a.ws = ws + sh.q_bytes + sh.scale_bytes;
+  a.prefix_rows = sh.prefix_rows;
+  a.own_rows = sh.own_rows;
+  a.prefix_bytes = sh.prefix_bytes;
+  a.own_bytes = sh.own_bytes;
+  a.out = out;
+  a.out_dtype = out_dtype;
+  a.out_tok_stride = out_tok_stride;
+  // The merge's column slices and threads, as for the decode merge: the fewest
+  // with which one round of loads covers a row's pieces on average.
+  int tpu = 256;
+  {
+    const int vpr_max = head_dim / 8;
+    const int64_t avg = groups ? (sh.grid + groups - 1) / groups + 1 : (sh.grid + batch - 1) / batch;
+    int cs = vpr_max / 8;
+    bool found = false;
+    for (int threads : {128, 256}) {
+      for (int c = 1; vpr_max / c >= 8 && !found; c *= 2) {
+        const int spi = threads / (vpr_max / c);
+        if ((avg + spi - 1) / spi <= kMergeMU) {
+          cs = c;
+          tpu = threads;
+          found = true;
+        }
+      }
+      if (found) break;
+    }
+    a.merge_cs = cs;
+  }
+  const int64_t merge_units = sh.tokens * kGqa * hkv * a.merge_cs;
+  K8V4_REQUIRE(merge_units <= INT32_MAX / 2, "batch too large for one merge launch");
+
+  auto s = static_cast<hipStream_t>(stream);
+  int rc = q_rows_launch(q, q_dtype == K8V4_BF16, q_tok_stride, sh.tokens, hkv, head_dim, sh.head_rows, q8, scales, s);
+  if (rc) return rc;
+  const int widest = groups && sh.prefix_rows > sh.own_rows ? sh.prefix_rows : sh.own_rows;
+  const int tiles = (widest + 15) / 16;
+  if (head_dim == 256) {
+    if (hkv == 4)
+      launch_split<8, 1, true>(a, tiles, s);
+    else
+      launch_split<4, 2, true>(a, tiles, s);
+  } else {
+    if (hkv == 4)
+      launch_split<4, 2, false>(a, tiles, s);
+    else
+      launch_split<2, 2, false>(a, tiles, s);
+  }
+  rc = launch_status("k8v4_attn_shared split");
+  if (rc) return rc;
+  const dim3 mgrid(static_cast<unsigned>(merge_units));
+  if (head_dim == 128) {
+    if (tpu == 128)
+      shared_merge_kernel<128, 128><<<mgrid, dim3(128), 0, s>>>(a);
+    else
+      shared_merge_kernel<128, 256><<<mgrid, dim3(256), 0, s>>>(a);
+  } else {
+    if (tpu == 128)
+      shared_merge_kernel<256, 128><<<mgrid, dim3(128), 0, s>>>(a);
+    else
+      shared_merge_kernel<256, 256><<<mgrid, dim3(256), 0, s>>>(a);
+  }
+  return launch_status("k8v4_attn_shared merge");
+}

@@ -47,6 +47,18 @@ inline bool supported_dim(int d) { return d == 128 || d == 256; }
 int q_quant_launch(const void *q, int bf16, int padded, int64_t q_tok_stride, int64_t batch, int q_len, int hkv,
                    int head_dim, int8_t *q8, float *q_scale, hipStream_t stream);
 
+// The same quantization of [tokens][6 * hkv][head_dim] rows into [hkv]
+// [head_rows][head_dim] codes and [hkv][head_rows] scales: row token * 6 + i of
+// head h is query head h * 6 + i of the token (rows from tokens * 6 on are not
+// written).  Arguments are not checked here.
+int q_rows_launch(const void *q, int bf16, int64_t q_tok_stride, int64_t tokens, int hkv, int head_dim,
+                  int64_t head_rows, int8_t *q8, float *q_scale, hipStream_t stream);
+
+// In-kernel waits of the shared-prefix kernels that gave up on the current
+// device (k8v4_decode_fault_count adds them to the decode kernels'); -1 on a
+// HIP error.
+int64_t shared_wait_timeouts();
+
 // Loads one element of a 16-bit float tensor as float (exact for fp16 and bf16).
 __device__ __forceinline__ float half_bits_to_float(uint16_t bits, bool is_bf16) {
   if (is_bf16) return __uint_as_float(static_cast<uint32_t>(bits) << 16);

@@ -29,23 +29,12 @@ struct QQuantArgs {
   float *q_scale;
 };
 
+// One row of D values (null: zeros) into its codes and scale, by one wave.
 template <int D>
-__global__ __launch_bounds__(256) void q_quant_kernel(QQuantArgs a) {
+__device__ __forceinline__ void quantize_row(const uint16_t *src, bool bf16, int lane, int8_t *dst_row,
+                                             float *dst_scale) {
 #pragma clang fp contract(off)
   constexpr int E = D / kWave;  // elements per lane
-  const int lane = threadIdx.x & (kWave - 1);
-  const int row = static_cast<int>(blockIdx.x) * 4 + static_cast<int>(threadIdx.x) / kWave;
-  if (row >= a.rows) return;  // whole waves
-  const int bh = row / kPage, r = row - bh * kPage;  // bh = b * hkv + h
-  const int b = bh / a.hkv, h = bh - b * a.hkv;
-  const uint16_t *src = nullptr;
-  if (a.padded) {
-    src = a.q + static_cast<int64_t>(row) * D;
-  } else if (r < a.q_len * kGqa) {
-    const int tok = r / kGqa;
-    src = a.q + (static_cast<int64_t>(b) * a.q_len + tok) * a.tok_stride +
-          static_cast<int64_t>(h * kGqa + (r - tok * kGqa)) * D;
-  }
   // One load per lane (rows start 16-byte aligned: both entry points require
   // it), under one condition: per-element selects become one branch and
   // one round trip each.
@@ -62,7 +51,7 @@ __global__ __launch_bounds__(256) void q_quant_kernel(QQuantArgs a) {
   float x[E];
 #pragma unroll
   for (int e = 0; e < E; ++e)
-    x[e] = half_bits_to_float(static_cast<uint16_t>(words[e >> 1] >> (16 * (e & 1))), a.bf16);
+    x[e] = half_bits_to_float(static_cast<uint16_t>(words[e >> 1] >> (16 * (e & 1))), bf16);
   float amax = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) amax = fmaxf(amax, fabsf(x[e]));
@@ -73,12 +62,46 @@ __global__ __launch_bounds__(256) void q_quant_kernel(QQuantArgs a) {
   uint32_t packed = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) packed |= (static_cast<uint32_t>(k_rule_code(x[e], inv)) & 0xFFu) << (8 * e);
-  int8_t *dst = a.q8 + static_cast<int64_t>(row) * D + lane * E;
+  int8_t *dst = dst_row + lane * E;
   if constexpr (E == 4)
     *reinterpret_cast<uint32_t *>(dst) = packed;
   else
     *reinterpret_cast<uint16_t *>(dst) = static_cast<uint16_t>(packed);
-  if (lane == 0) a.q_scale[row] = static_cast<float>(scale);
+  if (lane == 0) *dst_scale = static_cast<float>(scale);
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void q_quant_kernel(QQuantArgs a) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const int row = static_cast<int>(blockIdx.x) * 4 + static_cast<int>(threadIdx.x) / kWave;
+  if (row >= a.rows) return;  // whole waves
+  const int bh = row / kPage, r = row - bh * kPage;  // bh = b * hkv + h
+  const int b = bh / a.hkv, h = bh - b * a.hkv;
+  const uint16_t *src = nullptr;
+  if (a.padded) {
+    src = a.q + static_cast<int64_t>(row) * D;
+  } else if (r < a.q_len * kGqa) {
+    const int tok = r / kGqa;
+    src = a.q + (static_cast<int64_t>(b) * a.q_len + tok) * a.tok_stride +
+          static_cast<int64_t>(h * kGqa + (r - tok * kGqa)) * D;
+  }
+  quantize_row<D>(src, a.bf16, lane, a.q8 + static_cast<int64_t>(row) * D, a.q_scale + row);
+}
+
+// The rows of many tokens, head by head: row (h, token * 6 + i) is query head
+// h * 6 + i of that token, heads head_rows rows apart.  A run of tokens of one
+// head is then a run of rows, wherever it starts.
+template <int D>
+__global__ __launch_bounds__(256) void q_rows_kernel(QQuantArgs a, int64_t head_rows) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const int64_t src_row = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;  // token * 6 hkv + query head
+  if (src_row >= a.rows) return;  // whole waves
+  const int hq = kGqa * a.hkv;
+  const int64_t tok = src_row / hq;
+  const int qh = static_cast<int>(src_row - tok * hq);
+  const int h = qh / kGqa;
+  const int64_t row = h * head_rows + tok * kGqa + (qh - h * kGqa);
+  quantize_row<D>(a.q + tok * a.tok_stride + static_cast<int64_t>(qh) * D, a.bf16, lane, a.q8 + row * D, a.q_scale + row);
 }
 
 }  // namespace
@@ -100,6 +123,24 @@ int q_quant_launch(const void *q, int bf16, int padded, int64_t q_tok_stride, in
     q_quant_kernel<128><<<grid, dim3(256), 0, stream>>>(a);
   else
     q_quant_kernel<256><<<grid, dim3(256), 0, stream>>>(a);
+  return launch_status("k8v4 query quantization");
+}
+
+int q_rows_launch(const void *q, int bf16, int64_t q_tok_stride, int64_t tokens, int hkv, int head_dim,
+                  int64_t head_rows, int8_t *q8, float *q_scale, hipStream_t stream) {
+  QQuantArgs a{};
+  a.q = static_cast<const uint16_t *>(q);
+  a.bf16 = bf16;
+  a.tok_stride = q_tok_stride;
+  a.rows = tokens * kGqa * hkv;
+  a.hkv = hkv;
+  a.q8 = q8;
+  a.q_scale = q_scale;
+  const dim3 grid(static_cast<unsigned>((a.rows + 3) / 4));
+  if (head_dim == 128)
+    q_rows_kernel<128><<<grid, dim3(256), 0, stream>>>(a, head_rows);
+  else
+    q_rows_kernel<256><<<grid, dim3(256), 0, stream>>>(a, head_rows);
   return launch_status("k8v4 query quantization");
 }
 

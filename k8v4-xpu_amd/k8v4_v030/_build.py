@@ -35,7 +35,8 @@ COMMON_FLAGS = [
 # The decode kernels never produce or consume NaN (unwritten tails are masked
 # by selection before any arithmetic), so max/min need no NaN quieting.
 PER_FILE_FLAGS = {"kv_store.hip": ["-ffp-contract=off"], "q_quant.hip": ["-ffp-contract=off"],
-                  "decode.hip": ["-fno-honor-nans"], "prefill.hip": ["-fno-honor-nans"]}
+                  "decode.hip": ["-fno-honor-nans"], "decode_shared.hip": ["-fno-honor-nans"],
+                  "prefill.hip": ["-fno-honor-nans"]}
 
 
 def hipcc() -> str:

@@ -104,6 +104,13 @@ _EXTRA_SYMBOLS.append((
     _i32,
 ))
 _EXTRA_SYMBOLS.append((
+    "k8v4_attn_shared",
+    [_vp, _i32, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64,
+     _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _i32, _i32, _i32, _vp, _i32, _i64, _vp, _i64, _vp],
+    _i32,
+))
+_EXTRA_SYMBOLS.append(("k8v4_attn_shared_workspace_bytes", [_i64, _i32, _i32, _i32], _i64))
+_EXTRA_SYMBOLS.append((
     "k8v4_verify_drafts",
     [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _i64, _vp, _vp, _i64, _vp, _vp,
      _i64, _i32, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp],
@@ -429,6 +436,84 @@ class _Ops:
         keep = tensors + ((visible_lens,) if vis_ptr else ())
         return BoundCall(self._lib, self._lib.k8v4_attn_batch, args, dev, keep,
                          profiled=self._lib.k8v4_attn_batch_profiled)
+
+    # -- decode / MTP verify over a shared prefix -----------------------------
+    def attn_shared_workspace_bytes(self, batch: int, q_len: int, hkv: int, head_dim: int) -> int:
+        """Scratch bytes :meth:`int8k_int4v_attn_shared` needs (any prefix and lengths)."""
+        n = int(self._lib.k8v4_attn_shared_workspace_bytes(int(batch), int(q_len), int(hkv), int(head_dim)))
+        _require(n > 0, "bad shape for the shared-prefix workspace")
+        return n
+
+    def int8k_int4v_attn_shared(self, q_fp16, k_cache, k_scale, v_cache, v_scale, v_zero, prefix_table, prefix_len,
+                                block_table, seq_lens, workspace, out, q_len, pages_per_block):
+        """:meth:`int8k_int4v_attn_batch` for sequences that begin with the same cached
+        pages, those read once for all of them.
+
+        ``prefix_table`` (int32 ``[W']``, for instance ``block_table[0]``) names the
+        pages of the first ``prefix_len`` tokens; its whole pages (``prefix_len // 64``)
+        stand for those of every sequence, whatever the sequences' own rows of
+        ``block_table`` (int32 ``[B, W]``) hold there, and the tokens behind them come
+        from those rows.  ``seq_lens`` (int32 ``[B]``) counts all of a sequence's
+        tokens, the prefix included; a row whose causal end lies inside the prefix
+        sees the prefix up to there, one that sees nothing gives zeros.  The other
+        arguments and the numerics are the batch op's; ``workspace`` holds
+        :meth:`attn_shared_workspace_bytes` bytes."""
+        self.bind_int8k_int4v_attn_shared(q_fp16, k_cache, k_scale, v_cache, v_scale, v_zero, prefix_table,
+                                          prefix_len, block_table, seq_lens, workspace, out, q_len,
+                                          pages_per_block)()
+
+    def bind_int8k_int4v_attn_shared(self, q_fp16, k_cache, k_scale, v_cache, v_scale, v_zero, prefix_table,
+                                     prefix_len, block_table, seq_lens, workspace, out, q_len, pages_per_block):
+        """Validate one shared-prefix call; returns a :class:`DeviceCall` that launches it.
+
+        Lengths, tables and queries may change between launches, ``prefix_len`` may not."""
+        q_len, prefix_len, pages_per_block = int(q_len), int(prefix_len), int(pages_per_block)
+        _require(pages_per_block >= 1, "pages_per_block")
+        _require(prefix_len >= 0, "negative prefix length")
+        _require(q_len > 0 and q_len * GQA <= PAGE, "q_len*GQA exceeds BM")
+        _require(q_fp16.dim() == 3, "q_fp16 [T,HQ,D]")
+        tokens, heads, head_dim = (int(x) for x in q_fp16.shape)
+        _require(head_dim in (128, 256), "q_fp16 [T,HQ,D] with D in (128, 256)")
+        _require(heads % GQA == 0, "q_fp16 heads must be a multiple of GQA=6")
+        hkv = _checked_hkv(heads // GQA)
+        _require(q_fp16.dtype in (torch.float16, torch.bfloat16), "q_fp16 must be float16 or bfloat16")
+        _require(q_fp16.stride()[1:] == (head_dim, 1), "q_fp16 head/dim strides")
+        _require(out.shape == q_fp16.shape, "out shape")
+        _require(out.dtype in (torch.float16, torch.bfloat16, torch.float32), "out float16, bfloat16 or float32")
+        _require(out.stride()[1:] == (head_dim, 1), "out head/dim strides")
+        _require(tokens % q_len == 0, "T must be B*q_len")
+        batch = tokens // q_len
+        _require(batch >= 1, "empty batch")
+        check_paged_k(k_cache, k_scale, hkv, head_dim)
+        check_paged_v(v_cache, v_scale, v_zero, hkv, head_dim)
+        _require(k_cache.shape[0] == v_cache.shape[0], "k/v num_blocks")
+        _require(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == batch,
+                 "block_table int32 [B, splits]")
+        _require(int(block_table.shape[1]) > 0, "block_table n_splits")
+        _require(block_table.stride(1) == 1, "block_table rows must be contiguous")
+        _require(seq_lens.dtype == torch.int32 and seq_lens.numel() >= batch and seq_lens.is_contiguous(),
+                 "seq_lens must be a contiguous int32 [B]")
+        _require(workspace.is_contiguous(), "workspace must be a contiguous buffer")
+        tensors = (q_fp16, k_cache, k_scale, v_cache, v_scale, v_zero, block_table, seq_lens, out, workspace)
+        prefix_width = 0
+        if prefix_len >= PAGE:
+            _require(prefix_table.dtype == torch.int32 and prefix_table.dim() == 1
+                     and (prefix_table.shape[0] < 2 or prefix_table.stride(0) == 1),
+                     "prefix_table must be a contiguous int32 row")
+            prefix_width = int(prefix_table.shape[0])
+            tensors += (prefix_table,)
+        dev = _on_gpu(*tensors)
+        row = heads * head_dim
+        args = [
+            _ptr(q_fp16), _DTYPE_CODE[q_fp16.dtype], int(q_fp16.stride(0)) if tokens > 1 else row,
+            *cache_args(k_cache, k_scale, v_cache, v_scale, v_zero),
+            _ptr(prefix_table) if prefix_width else 0, prefix_width, prefix_len,
+            _ptr(block_table), int(block_table.stride(0)) if batch > 1 else int(block_table.shape[1]),
+            int(block_table.shape[1]), pages_per_block, _ptr(seq_lens), batch, q_len, hkv, head_dim,
+            _ptr(out), _DTYPE_CODE[out.dtype], int(out.stride(0)) if tokens > 1 else row,
+            _ptr(workspace), int(workspace.numel()) * workspace.element_size(),
+        ]
+        return DeviceCall(self._lib, self._lib.k8v4_attn_shared, args, dev, tensors)
 
     # -- chunked prefill ----------------------------------------------------
     def prefill_workspace_bytes(self, seq_len: int, q_len: int, hkv: int, head_dim: int) -> int:

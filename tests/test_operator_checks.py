@@ -1,4 +1,4 @@
-"""What kv_load_paged and verify_drafts refuse (host checks, no GPU)."""
+"""What int8k_int4v_attn_shared, kv_load_paged and verify_drafts refuse (host checks, no GPU)."""
 from __future__ import annotations
 
 from pathlib import Path
@@ -85,6 +85,48 @@ def test_verify_workspace(lib):
         assert lib.k8v4_verify_drafts_workspace_bytes(*bad) == -1
 
 
+def shared(lib, **over):
+    a = dict(q=P, q_dtype=0, q_stride=24 * 128, k=P, ks=P, v=P, vs=P, vz=P, pages=64, k_ps=52224, ks_ps=52224,
+             v_ps=52224, vs_ps=52224, vz_ps=52224, pre=P, pre_width=8, pre_len=512, bt=P, bt_stride=32, width=32, ppb=1,
+             lens=P, batch=4, q_len=2, hkv=4, d=128, out=P, out_dtype=0, out_stride=24 * 128, ws=P, ws_bytes=1 << 30,
+             stream=None)
+    a.update(over)
+    return lib.k8v4_attn_shared(*a.values())
+
+
+@pytest.mark.parametrize("over,text", [
+    (dict(hkv=3), "unsupported per-GPU KV head count 3"), (dict(d=64), "head dim"), (dict(q_len=11), "q_len*GQA"),
+    (dict(q_len=0), "q_len*GQA"), (dict(ppb=0), "pages_per_block"), (dict(pages=0), "num_pages"),
+    (dict(batch=0), "batch"), (dict(batch=2**21), "batch"), (dict(width=0), "width"), (dict(width=2**25), "width"),
+    (dict(pre_len=-1), "negative prefix"), (dict(pre_len=2**40), "prefix too long"),
+    (dict(pre_len=576), "prefix_table has 8 entries, the prefix of 576 tokens needs 9"),
+    (dict(pre=None), "null"), (dict(q=None), "null"), (dict(lens=None), "null"), (dict(ws=None), "null"),
+    (dict(q_dtype=2), "q dtype"), (dict(out_dtype=5), "out dtype"), (dict(q=P + 8), "16-byte"),
+    (dict(q_stride=24 * 128 + 4), "multiple of 8"), (dict(q_stride=128), "q token stride"),
+    (dict(out_stride=128), "out token stride"), (dict(out=P + 1), "out misaligned"), (dict(bt_stride=31), "row stride"),
+    (dict(bt=P + 2), "index arrays"), (dict(pre=P + 1), "index arrays"), (dict(k=P + 8), "k_cache"),
+    (dict(v_ps=52222), "v_cache"), (dict(vs=P + 4), "scale planes"), (dict(ws=P + 8), "workspace must be"),
+    (dict(batch=2**16, width=2**15, bt_stride=2**15), "too large"),
+])
+def test_shared_refuses(lib, over, text):
+    refused(lib, shared, text, **{"ws_bytes": 1 << 40, **over})
+
+
+@pytest.mark.parametrize("hkv,d", [(2, 128), (4, 128), (2, 256), (4, 256)])
+def test_shared_workspace(lib, hkv, d):
+    size = lib.k8v4_attn_shared_workspace_bytes
+    for bad in ((0, 1, hkv, d), (1, 0, hkv, d), (1, 11, hkv, d), (1, 1, 3, d), (1, 1, hkv, 64), (2**21, 1, hkv, d)):
+        assert size(*bad) == -1
+    last = 0
+    for batch in (1, 2, 7, 8, 9, 64, 1000):
+        need = size(batch, 3, hkv, d)
+        assert need > last
+        last = need
+    over = dict(hkv=hkv, d=d, q_stride=6 * hkv * d, out_stride=6 * hkv * d)
+    refused(lib, shared, "shared-prefix workspace holds 4096 bytes", code=2, ws_bytes=4096, **over)
+    refused(lib, shared, "the batch needs %d" % size(4, 2, hkv, d), code=2, ws_bytes=size(4, 2, hkv, d) - 1, **over)
+
+
 def test_op_table_checks_tensors(lib):
     o = ops_api.ops()
     lay = PageLayout(2, 128)
@@ -119,3 +161,22 @@ def test_op_table_checks_tensors(lib):
                        ("next_lens needs", dict(lens=None)), ("GPU tensors", dict())):
         with pytest.raises(RuntimeError, match=text):
             o.verify_drafts(*{**good, **over}.values())
+
+    q, lens = torch.zeros(4, 12, 128, dtype=torch.float16), torch.zeros(2, dtype=torch.int32)
+    pre, table = torch.zeros(2, dtype=torch.int32), torch.zeros((2, 3), dtype=torch.int32)
+    base = dict(q=q, pre=pre, n=100, table=table, lens=lens, ws=torch.zeros(64), out=q.clone(), q_len=2, ppb=1)
+
+    def shared(**over):
+        a = {**base, **over}
+        o.int8k_int4v_attn_shared(a["q"], *regions, a["pre"], a["n"], a["table"], a["lens"], a["ws"], a["out"],
+                                  a["q_len"], a["ppb"])
+
+    for text, over in (("pages_per_block", dict(ppb=0)), ("negative prefix", dict(n=-1)), ("exceeds BM", dict(q_len=11)),
+                       (r"q_fp16 \[T,HQ,D\]", dict(q=q[0])), ("float16 or bfloat16", dict(q=q.float())),
+                       ("out shape", dict(out=q[:2])), ("float16, bfloat16 or float32", dict(out=q.double())),
+                       ("B\\*q_len", dict(q_len=3)), ("block_table int32", dict(table=table.long())),
+                       ("block_table int32", dict(table=table[:1])), ("seq_lens", dict(lens=lens[:1])),
+                       ("prefix_table", dict(pre=pre.long())), ("prefix_table", dict(pre=table)),
+                       ("GPU tensors", dict())):
+        with pytest.raises(RuntimeError, match=text):
+            shared(**over)
