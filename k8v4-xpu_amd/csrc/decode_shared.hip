@@ -28,12 +28,21 @@
 // filled by direct-to-LDS loads, see decode_chunk.h and decode.hip.
 #include "decode_chunk.h"
 
+#include <type_traits>
+
 namespace k8v4 {
 namespace {
 
 constexpr int kGroup = 8;  // tokens of one segment: 48 rows of a KV head
 // Fixed cost of a piece in pages of its pages' time.
 constexpr int kPieceCost = 6;
+#ifndef K8V4_AHEAD
+#define K8V4_AHEAD (D == 128 ? 6 : 4)
+#endif
+#ifndef K8V4_WIDE_MIN
+#define K8V4_WIDE_MIN 200
+#endif
+constexpr int kWideCost = 6;  // the same for a piece of the many-rows kernel
 constexpr int kFar = 1 << 30;
 
 struct SharedArgs {
@@ -58,10 +67,12 @@ struct SharedArgs {
   const int32_t *seq_lens;
   int batch, q_len, hkv;
   int tokens;      // batch * q_len
-  int groups;      // prefix segments (0 without a prefix)
+  int groups;      // prefix segments (0 without a prefix, or where the many-rows kernel serves it)
+  int wide_segments, wide_blocks;  // many-rows kernel: KV heads x row blocks, row blocks (0: not used)
   int per_seq;     // own segments of a sequence: 1, or 2 for more than eight tokens
   int grid;        // work-groups of the split launch
-  char *ws;        // states: prefix pieces, then the others
+  int wide_grid;   // work-groups of the many-rows launch
+  char *ws, *own_ws;  // states of the prefix's pieces and of the sequences' own
   int prefix_rows, own_rows;        // state rows of a KV head in a piece of either kind
   int64_t prefix_bytes, own_bytes;  // bytes of such a state
   int merge_cs;    // column slices per output row in the merge
@@ -144,8 +155,7 @@ __device__ Where locate(const SharedArgs &a, int lane, int u) {
 // both in the order of the axis, so g + segment is a number of its own.
 __device__ __forceinline__ char *piece_state(const SharedArgs &a, int g, int seg) {
   if (seg < a.groups) return a.ws + static_cast<int64_t>(g + seg) * a.prefix_bytes;
-  return a.ws + static_cast<int64_t>(a.groups ? a.grid + a.groups : 0) * a.prefix_bytes +
-         static_cast<int64_t>(g + seg - a.groups) * a.own_bytes;
+  return a.own_ws + static_cast<int64_t>(g + seg - a.groups) * a.own_bytes;
 }
 
 // x of lane `src`.
@@ -515,6 +525,425 @@ void shared_split_kernel(SharedArgs args) {
   }
 }
 
+// ------------------------------------------------------------ many rows
+//
+// With many query rows the prefix is bound by issue, not by memory: a wave of
+// the kernel above spends as much on fetching, unpacking and addressing a
+// chunk as on multiplying it.  Here the eight waves of a work-group hold
+// consecutive rows of ONE KV head (NT 16-row tiles each) and share every page:
+// K stays int8 codes as they are in the cache; V is dequantized once per page
+// for all waves, (nibble - zero) * scale / 16 rounded once to fp16 (the 1/16
+// keeps rows of the whole fp16 range finite).
+//
+// Waves w and w + 4 share a SIMD.  They form two groups half a page apart,
+// separated by a barrier per phase: in phase A of page p a wave multiplies (O
+// += V(p - 1)^T P(p - 1), S = K(p) Q^T); in phase B it turns S into
+// probabilities, issues its share of a later page's loads and dequantizes its
+// share of V.  So each SIMD holds one wave that
+// feeds the matrix core and one that feeds the vector unit.  With t counting
+// phases, group 0 runs A(p) at t = 2p and B(p) at 2p + 1, group 1 one later:
+//   raw page p (K codes, V codes, planes): read from t = 2p (A of group 0) to
+//     2p + 2 (B of group 1); each wave issues its loads of page p + SLOTS - 1,
+//     into the slot of page p - 1, in B(p);
+//   V16(p): written at 2p (group 1's half) and 2p + 1, read at 2p + 2 and 2p + 3:
+//     two buffers.
+// Products are transposed (tokens x rows, dims x rows): a lane owns one row of
+// each tile, so the running max, sum and rescale need no exchange but the max
+// over the four lanes of a row.
+constexpr int kWideWaves = 8;
+
+template <int D>
+struct Wide {
+  static constexpr int NT = D == 128 ? 3 : 2;    // row tiles a wave holds in registers
+  static constexpr int ROWS = kWideWaves * 16 * NT;
+  static constexpr int SLOTS = D == 128 ? 4 : 3;
+  static constexpr int VROW = D / 2;
+  static constexpr int K_BYTES = kPage * D;
+  static constexpr int V_OFF = K_BYTES;
+  static constexpr int S_OFF = V_OFF + kPage * VROW;   // ks[64] | vs[64] | vz[64]
+  static constexpr int SLOT_BYTES = S_OFF + 3 * kPage * 4;
+  static constexpr int V16_BYTES = D * kPage * 2;      // [D rows][64 tokens]
+  static constexpr int V16_OFF = SLOTS * SLOT_BYTES;
+  static constexpr int PAD_OFF = V16_OFF + 2 * V16_BYTES;  // where loads nobody reads land
+  static constexpr int LDS_BYTES = PAD_OFF + 256;
+  static constexpr int KPW = K_BYTES / 1024 / kWideWaves;  // K loads of a wave: 1, 2
+  static constexpr int LOADS = KPW + 1 + (D == 128 ? 0 : 1);  // loads of a wave per page
+  static_assert(LDS_BYTES <= 163840, "ring exceeds the LDS");
+};
+
+// Position of 16-byte chunk c of a V16 row: rows are read 16 at a time at one
+// chunk and written 64 at a time at one chunk, both conflict-free.
+__device__ __forceinline__ int vswz(int row) { return (row & 7) ^ ((row >> 3) & 1); }
+
+template <int D, int HKV>
+__global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_per_eu(2, 2)))
+void shared_wide_kernel(SharedArgs args) {
+  using W = Wide<D>;
+  constexpr int NT = W::NT, KS = D / 64, DT = D / 16;
+  __shared__ __attribute__((aligned(16))) char lds_raw[W::LDS_BYTES];
+  lds_t *lds = (lds_t *)(lds_raw);
+
+  const int wg = static_cast<int>(blockIdx.x);
+  const int cost = args.prefix_pages + kWideCost;
+  const int unit = (args.wide_segments * cost + args.wide_grid - 1) / args.wide_grid;
+  const int u0 = wg * unit, u1 = u0 + unit;
+
+  for (int seg = u0 / cost; seg < args.wide_segments && seg * cost < u1; ++seg) {
+    const SharedArgs &a = (const SharedArgs &)*reread((args_ptr)__builtin_amdgcn_kernarg_segment_ptr());
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int grp = wave >> 2;
+    const int n = lane & 15, g = lane >> 4;
+
+    const int first = seg * cost + kWideCost;
+    const int p0 = max(u0 - first, 0), p1 = min(u1 - first, a.prefix_pages);
+    if (p1 <= p0) continue;
+    const int h = seg / a.wide_blocks, block = seg - h * a.wide_blocks;
+    const int row0 = block * W::ROWS + wave * 16 * NT;  // first row of this wave, of the head's tokens * 6
+    const int nrows = a.tokens * kGqa;
+    const bool active = row0 < nrows;
+    const int pages = p1 - p0;
+
+    // Query rows: lane (n, g) of tile nt holds row 16 nt + n, dims 64 ks + 16 g ...
+    v4i qf[NT][KS];
+    float crow[NT];
+    int lim[NT];
+    int far = 0;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = row0 + 16 * nt + n;
+      const int64_t at = h * a.head_rows + r;  // the buffer is padded to whole blocks
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) qf[nt][ks] = *reinterpret_cast<const v4i *>(a.q8 + at * D + 64 * ks + 16 * g);
+      int end = a.prefix_pages * kPage;
+      double f = 0.0;
+      if (r < nrows) {
+        f = a.q8_scale[at];
+        const int tok = r / kGqa, sb = tok / a.q_len;
+        end = a.seq_lens[sb] - a.q_len + (tok - sb * a.q_len) + 1;
+        if (end > 0) far = max(far, kFar - min(end, kFar));
+      }
+      lim[nt] = end;
+      crow[nt] = fmaxf(static_cast<float>(f * (static_cast<double>(kLog2e) / sqrt(static_cast<double>(D)))), 1e-30f);
+    }
+    const int min_end = kFar - wave_max(far);
+
+    // Lane offsets of this wave's loads of a page: K rows (swizzled as in
+    // lane_offsets), V rows, one cell of a plane.
+    uint32_t koff[W::KPW];
+#pragma unroll
+    for (int k = 0; k < W::KPW; ++k) {
+      constexpr int CPR = D / 16;  // 16-byte chunks of a K row
+      const int t = (wave * W::KPW + k) * (1024 / D) + lane / CPR;
+      koff[k] = static_cast<uint32_t>(t * (HKV * D) + h * D + 16 * ((lane % CPR) ^ kswz<D>(t)));
+    }
+    const int vj = wave & (kPage * W::VROW / 1024 - 1);  // 1 KB piece of V rows
+    const uint32_t voff = static_cast<uint32_t>((vj * (1024 / W::VROW) + lane * 16 / W::VROW) * (HKV * W::VROW) +
+                                                h * W::VROW + lane * 16 % W::VROW);
+    const uint32_t poff = static_cast<uint32_t>((lane * HKV + h) * 4);
+    // Physical pages, 64 at a time: lane l holds page p0 + 64 k + l.
+    int ptab = -1;
+    auto load_table = [&](int k) {
+      const int p = min(p0 + 64 * k + lane, p1 - 1);
+      const int raw = a.prefix_table[a.ppb <= 1 ? p : p / a.ppb];
+      const int64_t ph = a.ppb <= 1 ? raw : static_cast<int64_t>(raw) * a.ppb + p % a.ppb;
+      ptab = ph >= 0 && ph < a.num_pages ? static_cast<int>(ph) : -1;
+    };
+    // Whether page i of the piece is in the cache, for the last SLOTS pages issued.
+    uint32_t valid = 0;
+    // This wave's loads of page i of the piece (W::LOADS of them, also for a
+    // page behind the last or outside the cache, so every page costs the same
+    // count): its share of the K rows and of the V rows, and a plane.
+    const char *const kbase = reinterpret_cast<const char *>(a.k_cache);
+    const char *const vbase = reinterpret_cast<const char *>(a.v_cache);
+    const int plane = D == 128 ? wave - 4 : wave;  // 1: v_scale, 2: v_zero, others k_scale
+    const char *const pbase = plane == 1   ? reinterpret_cast<const char *>(a.v_scale)
+                              : plane == 2 ? reinterpret_cast<const char *>(a.v_zero)
+                                           : reinterpret_cast<const char *>(a.k_scale);
+    const int64_t k_ps = a.k_ps, v_ps = a.v_ps, p_ps = plane == 1 ? a.vs_ps : plane == 2 ? a.vz_ps : a.ks_ps;
+    lds_t *const pdst0 = lds + W::S_OFF + (plane == 1 || plane == 2 ? plane : 0) * kPage * 4;
+    auto issue = [&](int i) {
+      if ((i & 63) == 0 && i < pages) load_table(i >> 6);
+      const int phys = i < pages ? __builtin_amdgcn_readlane(ptab, i & 63) : -1;
+      const int slot = i % W::SLOTS;
+      valid = (valid & ~(1u << slot)) | (phys >= 0 ? 1u << slot : 0u);
+      const int64_t ph = phys >= 0 ? phys : 0;
+      lds_t *dst = lds + slot * W::SLOT_BYTES;
+#pragma unroll
+      for (int k = 0; k < W::KPW; ++k) dma16s(kbase + ph * k_ps, koff[k], dst + (wave * W::KPW + k) * 1024);
+      if (D == 256 || wave < 4) dma16s(vbase + ph * v_ps, voff, dst + W::V_OFF + vj * 1024);
+      if (D == 256 || wave >= 4) {
+        // D = 128: waves 4 and 7 both fetch k_scale; D = 256: 0 and 3 .. 7.  A page
+        // outside the cache holds no keys: its scores are masked in B, and its
+        // planes are zeros here, so that its V is zeros whatever page 0 holds.
+        lds_t *pdst = pdst0 + slot * W::SLOT_BYTES;
+        dma4s(pbase + ph * p_ps, poff, phys >= 0 ? pdst : lds + W::PAD_OFF);
+        if (phys < 0) *reinterpret_cast<__attribute__((address_space(3))) float *>(pdst + 4 * lane) = 0.f;
+      }
+    };
+
+    v4f O[NT][DT];
+    v4f lsum[NT];
+    float m_run[NT], thr[NT];
+    v4i S[NT][4];
+    v8h P[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      lsum[nt] = (v4f){0.f, 0.f, 0.f, 0.f};
+      m_run[nt] = -INFINITY;
+      thr[nt] = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < DT; ++j) O[nt][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+    }
+    const v4i bias = {kScoreBias, kScoreBias, kScoreBias, kScoreBias};
+    const v8h ones = {1, 1, 1, 1, 1, 1, 1, 1};
+
+    // This wave's share of V16(i): its group's 32-token half of the page, tokens
+    // 32 grp + 4 (wave & 3) + {0..3, 16..19}, byte columns `lane` (D = 256: and
+    // 64 + lane).  A byte holds two dims; as fp16 its low nibble is n 2^-24 and
+    // its high one n 2^-20 (subnormal, exact), so one fma each, rounded once to
+    // fp16, gives (n - zero) scale / 16.  V16 rows are parity * D / 2 + byte
+    // column, a lane's eight tokens a 16-byte chunk.
+    auto convert = [&](int i) {
+      const lds_t *raw = lds + (i % W::SLOTS) * W::SLOT_BYTES;
+      lds_t *dst = lds + W::V16_OFF + (i & 1) * W::V16_BYTES;
+      const int t0 = 32 * grp + 4 * (wave & 3), chunk = 4 * grp + (wave & 3);
+      typedef __attribute__((address_space(3))) const v4f *lv4f;
+      v4f vs[2], vz[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        vs[e] = *reinterpret_cast<lv4f>(raw + W::S_OFF + (kPage + t0 + 16 * e) * 4);
+        vz[e] = *reinterpret_cast<lv4f>(raw + W::S_OFF + (2 * kPage + t0 + 16 * e) * 4);
+      }
+#pragma unroll
+      for (int c0 = 0; c0 < W::VROW; c0 += kWave) {
+        const int col = c0 + lane;
+        uint32_t byte[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+          byte[t] = *reinterpret_cast<__attribute__((address_space(3))) const uint8_t *>(
+              raw + W::V_OFF + (t0 + (t < 4 ? t : 12 + t)) * W::VROW + col);
+        v8h even, odd;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          const float s = vs[t >> 2][t & 3], c = vz[t >> 2][t & 3] * (s * -0.0625f);
+          const _Float16 lo = __builtin_bit_cast(_Float16, static_cast<uint16_t>(byte[t] & 0x0Fu));
+          const _Float16 hi = __builtin_bit_cast(_Float16, static_cast<uint16_t>(byte[t] & 0xF0u));
+          even[t] = static_cast<_Float16>(fmaf(static_cast<float>(lo), s * 0x1p20f, c));
+          odd[t] = static_cast<_Float16>(fmaf(static_cast<float>(hi), s * 0x1p16f, c));
+        }
+        const int pos = 16 * (chunk ^ vswz(col));
+        *reinterpret_cast<__attribute__((address_space(3))) v8h *>(dst + col * 128 + pos) = even;
+        *reinterpret_cast<__attribute__((address_space(3))) v8h *>(dst + (W::VROW + col) * 128 + pos) = odd;
+      }
+    };
+
+    // Phase A: O += V(i)^T P and the row sums with it, S = K(i + 1) Q^T, in steps
+    // of one operand (16 bytes a lane) and the NT products that use it.  Operands
+    // are read AHEAD steps before their use (an LDS round trip takes about as
+    // long as eight products), one step's code fenced off from the next.
+    constexpr int NV = 2 * DT, NK = 4 * KS, AHEAD = K8V4_AHEAD;
+    auto phase_a = [&](int i, auto with_v) {
+      constexpr int FIRST = decltype(with_v)::value ? 0 : NV, LAST = NV + NK;
+      const lds_t *vsrc = lds + W::V16_OFF + (i & 1) * W::V16_BYTES;
+      const lds_t *raw = lds + ((i + 1) % W::SLOTS) * W::SLOT_BYTES;
+      auto operand = [&](int x) -> v4i {
+        if (x < NV) {
+          // Tile j: dims 32 (j / 2) + 2 n' + j % 2 for n' = 0..15, tokens 32 s + ...
+          const int s = x / DT, j = x % DT, c = 16 * (j >> 1) + n;
+          return *reinterpret_cast<__attribute__((address_space(3))) const v4i *>(
+              vsrc + ((j & 1) * W::VROW + c) * 128 + 16 * ((4 * s + g) ^ vswz(c)));
+        }
+        const int ml = (x - NV) / KS, ks = (x - NV) % KS, t = 16 * ml + n;
+        return *reinterpret_cast<__attribute__((address_space(3))) const v4i *>(raw + t * D + 16 * ((4 * ks + g) ^ kswz<D>(t)));
+      };
+      v4i ring[AHEAD];
+#pragma unroll
+      for (int x = 0; x < AHEAD; ++x) ring[x] = operand(FIRST + x);
+#pragma unroll
+      for (int x = FIRST; x < LAST; ++x) {
+        const int k = x - FIRST;
+        const v4i f = ring[k % AHEAD];
+        if (x + AHEAD < LAST) ring[k % AHEAD] = operand(x + AHEAD);
+        if (x < NV) {
+          const int s = x / DT, j = x % DT;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            O[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, f), P[nt][s], O[nt][j], 0, 0, 0);
+          if (j == DT - 1) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) lsum[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, P[nt][s], lsum[nt], 0, 0, 0);
+          }
+        } else {
+          const int ml = (x - NV) / KS, ks = (x - NV) % KS;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            S[nt][ml] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, qf[nt][ks], ks ? S[nt][ml] : bias, 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    // P = exp2(score - m - 2) of page i, see chunk_softmax_pv in decode_chunk.h.
+    auto softmax = [&](int i, bool there) {
+      const lds_t *src = lds + (i % W::SLOTS) * W::SLOT_BYTES + W::S_OFF;
+      typedef __attribute__((address_space(3))) const v4f *lv4f;
+      float t[NT][4][4], mx[NT];
+      const int tbase = (p0 + i) * kPage;
+      const bool masked = !there || tbase + kPage > min_end;
+      const int seen_to = there ? INT32_MAX : 0;
+#pragma unroll
+      for (int ml = 0; ml < 4; ++ml) {
+        const v4f ks = *reinterpret_cast<lv4f>(src + (16 * ml + 4 * g) * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float kb = -12582912.0f * ks[e];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) t[nt][ml][e] = fmaf(__int_as_float(S[nt][ml][e]), ks[e], kb);
+        }
+      }
+      if (__builtin_expect(masked, 0)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int ml = 0; ml < 4; ++ml)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (tbase + 16 * ml + 4 * g + e >= min(lim[nt], seen_to)) t[nt][ml][e] = -INFINITY;
+      }
+      bool grow = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float x = -INFINITY;
+#pragma unroll
+        for (int ml = 0; ml < 4; ++ml)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x = fmaxf(x, t[nt][ml][e]);
+        mx[nt] = x;
+        grow |= x > thr[nt];
+      }
+      if (__ballot(grow)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float mnew = fmaxf(m_run[nt], xlane_max16_32(mx[nt]) * crow[nt]);
+          const float alpha = m_run[nt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[nt] - mnew);
+          m_run[nt] = mnew;
+          thr[nt] = (mnew + kRescaleThreshold) / crow[nt];
+          lsum[nt] *= alpha;
+#pragma unroll
+          for (int j = 0; j < DT; ++j) O[nt][j] *= alpha;
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float nm = -fmaxf(m_run[nt], -FLT_MAX) - kPLog2Offset;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          float p[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            p[e] = __builtin_amdgcn_exp2f(fmaf(t[nt][2 * s + (e >> 2)][e & 3], crow[nt], nm));
+          const v2h a0 = pack_h2(p[0], p[1]), a1 = pack_h2(p[2], p[3]), a2 = pack_h2(p[4], p[5]), a3 = pack_h2(p[6], p[7]);
+          P[nt][s] = (v8h){a0[0], a0[1], a1[0], a1[1], a2[0], a2[1], a3[0], a3[1]};
+        }
+      }
+    };
+    // Ends a phase.  Before an even phase t = 2q the raw page q has to be there:
+    // `left` of this wave's loads may still be under way.
+    auto end_phase = [&](bool before_even, int left) {
+      if (before_even) {
+        if (left == 2)
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * W::LOADS) : "memory");
+        else if (left == 1)
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(W::LOADS) : "memory");
+        else
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");  // no LDS access moves over the barrier
+      __builtin_amdgcn_sched_barrier(0);
+    };
+
+    // The query words are used here, so that the compiler's wait for them does
+    // not fall behind the page loads it does not count.
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) asm volatile("" ::"v"(qf[nt][ks]));
+#pragma unroll
+    for (int i = 0; i < W::SLOTS - 1; ++i) issue(i);
+    end_phase(true, W::SLOTS - 2);
+    if (grp) {  // group 1 sits out phase 0
+      convert(0);
+      end_phase(false, 0);
+    }
+    // Before phase 2q group 0 has issued up to page q + SLOTS - 2 (in B(q - 1))
+    // and group 1 up to the one before.
+    auto run = [&](auto compute) {
+      constexpr bool C = decltype(compute)::value;
+      if constexpr (C) phase_a(-1, std::false_type{});
+      end_phase(grp, W::SLOTS - 3);
+      for (int i = 0; i < pages; ++i) {
+        // Phase B(i): group 0 is one page behind group 1 in dequantizing.
+        const bool there = (valid >> (i % W::SLOTS)) & 1u;
+        issue(i + W::SLOTS - 1);
+        if constexpr (C) softmax(i, there);
+        if constexpr (C && D == 256) {
+          // The probabilities first: beside the dequantization's words their
+          // scores are more than the registers hold.
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) asm volatile("" : "+v"(P[nt][0]), "+v"(P[nt][1]));
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        convert(i + grp);
+        end_phase(!grp, W::SLOTS - 2);
+        // Phase A(i + 1); behind the last page its scores are of no page and not used.
+        if constexpr (C) phase_a(i, std::true_type{});
+        end_phase(grp, W::SLOTS - 3);
+      }
+    };
+    // Waves whose rows lie behind the batch's only move and dequantize pages.
+    if (active)
+      run(std::true_type{});
+    else
+      run(std::false_type{});
+    if (!grp) end_phase(false, 0);
+
+    // The state, as in the kernel above: a quarter of O / l (O is a sixteenth),
+    // then m and l; lane (n, g) holds dims 32 q + 8 g .. + 7 of row n.
+    if (active) {
+      char *state = a.ws + static_cast<int64_t>(wg + seg) * a.prefix_bytes;
+      float2 *ml = reinterpret_cast<float2 *>(state + static_cast<int64_t>(W::ROWS) * D * 2);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int lr = wave * 16 * NT + 16 * nt + n;
+        if (row0 + 16 * nt + n < nrows) {
+          const bool seen = lim[nt] > 0 && m_run[nt] != -INFINITY;
+          const float l = seen ? lsum[nt][0] : 0.f;
+          const float f = l > 0.f ? 4.f / l : 0.f;
+          _Float16 *dst = reinterpret_cast<_Float16 *>(state) + static_cast<int64_t>(lr) * D + 8 * g;
+#pragma unroll
+          for (int q = 0; q < DT / 2; ++q) {
+            v8h o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              o[2 * e] = static_cast<_Float16>(seen ? O[nt][2 * q][e] * f : 0.f);
+              o[2 * e + 1] = static_cast<_Float16>(seen ? O[nt][2 * q + 1][e] * f : 0.f);
+            }
+            store_wt16(dst + 32 * q, o);
+          }
+          if (g == 0) store_wt8(ml + lr, make_float2(seen ? m_run[nt] : -INFINITY, l));
+        }
+      }
+    }
+    // The next piece's loads overwrite the LDS and count from zero.
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
+}
+
 // Folds the states of one column slice of one output row (token, query head):
 // the prefix's for its group, then its sequence's own.
 template <int D, int TPU>
@@ -553,11 +982,23 @@ __global__ __launch_bounds__(TPU) void shared_merge_kernel(SharedArgs a) {
     on = (first + pages - 1) / ax.unit - of + 1;
   }
   const int dcol = 8 * (slice * VPR + col);
-  const int pr = h * a.prefix_rows + (tok - ps * kGroup) * kGqa + i6;
-  const int orow = h * a.own_rows + (j - sub * kGroup) * kGqa + i6;
+  int pr = h * a.prefix_rows + (tok - ps * kGroup) * kGqa + i6;
+  int64_t pml = static_cast<int64_t>(a.hkv) * a.prefix_rows * D * 2;
   const char *pbase = piece_state(a, pf, ps), *obase = piece_state(a, of, a.groups + os);
+  if (a.wide_segments) {
+    const int cost = a.prefix_pages + kWideCost;
+    const int unit_pages = (a.wide_segments * cost + a.wide_grid - 1) / a.wide_grid;
+    const int r = tok * kGqa + i6, block = r / Wide<D>::ROWS, seg = h * a.wide_blocks + block;
+    const int first = seg * cost + kWideCost;
+    pf = first / unit_pages;
+    pn = (first + a.prefix_pages - 1) / unit_pages - pf + 1;
+    pr = r - block * Wide<D>::ROWS;
+    pml = static_cast<int64_t>(Wide<D>::ROWS) * D * 2;
+    pbase = a.ws + static_cast<int64_t>(pf + seg) * a.prefix_bytes;
+  }
+  const int orow = h * a.own_rows + (j - sub * kGroup) * kGqa + i6;
   const int64_t p_o = (static_cast<int64_t>(pr) * D + dcol) * 2;
-  const int64_t p_ml = static_cast<int64_t>(a.hkv) * a.prefix_rows * D * 2 + pr * 8;
+  const int64_t p_ml = pml + pr * 8;
   const int64_t o_o = (static_cast<int64_t>(orow) * D + dcol) * 2;
   const int64_t o_ml = static_cast<int64_t>(a.hkv) * a.own_rows * D * 2 + orow * 8;
 
@@ -644,31 +1085,60 @@ void launch_split(const SharedArgs &a, int tiles, hipStream_t s) {
 
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 
+template <int HKV>
+void launch_wide(const SharedArgs &a, int head_dim, hipStream_t s) {
+  const dim3 grid(a.wide_grid), block(512);
+  if (head_dim == 128)
+    shared_wide_kernel<128, HKV><<<grid, block, 0, s>>>(a);
+  else
+    shared_wide_kernel<256, HKV><<<grid, block, 0, s>>>(a);
+}
+
+// Whether the many-rows kernel serves the prefix for this many query rows.
+bool wide_pays(int64_t rows, int head_dim) {
+  (void)head_dim;
+  return rows >= K8V4_WIDE_MIN;
+}
+
 // What a call of this shape keeps in its workspace: the quantized query rows,
-// their scales, then the states.
+// their scales, then the states of the prefix's pieces and of the others.
 struct SharedShape {
-  int64_t tokens, groups, per_seq, head_rows, grid;
+  int64_t tokens, groups, per_seq, head_rows, grid, wide_grid;
+  int64_t blocks;  // row blocks of the many-rows kernel (0: not used)
   int prefix_rows, own_rows;
   int64_t prefix_bytes, own_bytes;
-  int64_t q_bytes, scale_bytes, state_bytes;
+  int64_t q_bytes, scale_bytes, prefix_state_bytes, own_state_bytes;
 };
 SharedShape shape_of(int64_t batch, int q_len, int hkv, int head_dim) {
   SharedShape s;
   s.tokens = batch * q_len;
   s.groups = (s.tokens + kGroup - 1) / kGroup;
   s.per_seq = (q_len + kGroup - 1) / kGroup;
-  s.head_rows = s.tokens * kGqa + 3 * 16;  // a last segment's tiles read rows behind the last token's
+  const int64_t rows = s.tokens * kGqa;
   // One work-group per CU, two with two 128-dim heads (half the waves).
   s.grid = static_cast<int64_t>(device_cus()) * (hkv == 2 && head_dim == 128 ? 2 : 1);
-  s.prefix_rows = static_cast<int>(s.tokens < kGroup ? s.tokens : kGroup) * kGqa;
+  s.wide_grid = device_cus();
+  const int wide_rows = head_dim == 128 ? Wide<128>::ROWS : Wide<256>::ROWS;
+  s.blocks = wide_pays(rows, head_dim) ? (rows + wide_rows - 1) / wide_rows : 0;
+  // A last segment's tiles (a last block's rows) read rows behind the last token's.
+  s.head_rows = s.blocks * wide_rows > rows + 3 * 16 ? s.blocks * wide_rows : rows + 3 * 16;
   s.own_rows = (q_len < kGroup ? q_len : kGroup) * kGqa;
-  s.prefix_bytes = static_cast<int64_t>(hkv) * s.prefix_rows * (2 * head_dim + 8);
   s.own_bytes = static_cast<int64_t>(hkv) * s.own_rows * (2 * head_dim + 8);
+  if (s.blocks) {
+    s.prefix_rows = wide_rows;
+    s.prefix_bytes = static_cast<int64_t>(wide_rows) * (2 * head_dim + 8);
+    s.prefix_state_bytes = (s.wide_grid + hkv * s.blocks) * s.prefix_bytes;
+  } else {
+    s.prefix_rows = static_cast<int>(s.tokens < kGroup ? s.tokens : kGroup) * kGqa;
+    s.prefix_bytes = static_cast<int64_t>(hkv) * s.prefix_rows * (2 * head_dim + 8);
+    s.prefix_state_bytes = (s.grid + s.groups) * s.prefix_bytes;
+  }
   s.q_bytes = round256(hkv * s.head_rows * head_dim);
   s.scale_bytes = round256(hkv * s.head_rows * 4);
-  s.state_bytes = (s.grid + s.groups) * s.prefix_bytes + (s.grid + batch * s.per_seq) * s.own_bytes;
+  s.own_state_bytes = (s.grid + batch * s.per_seq) * s.own_bytes;
   return s;
 }
+int64_t bytes_of(const SharedShape &s) { return s.q_bytes + s.scale_bytes + s.prefix_state_bytes + s.own_state_bytes; }
 
 constexpr int64_t kMaxBatch = int64_t(1) << 20;
 
@@ -692,7 +1162,7 @@ extern "C" int64_t k8v4_attn_shared_workspace_bytes(int64_t batch, int q_len, in
       !supported_dim(head_dim))
     return -1;
   const SharedShape s = shape_of(batch, q_len, hkv, head_dim);
-  return s.q_bytes + s.scale_bytes + s.state_bytes;
+  return bytes_of(s);
 }
 
 extern "C" int k8v4_attn_shared(const void *q, int q_dtype, int64_t q_tok_stride, const int8_t *k_cache,
@@ -743,19 +1213,21 @@ extern "C" int k8v4_attn_shared(const void *q, int q_dtype, int64_t q_tok_stride
   K8V4_REQUIRE(aligned(workspace, 16), "workspace must be 16-byte aligned");
 
   const SharedShape sh = shape_of(batch, q_len, hkv, head_dim);
-  const int64_t need = sh.q_bytes + sh.scale_bytes + sh.state_bytes;
+  const int64_t need = bytes_of(sh);
   if (workspace_bytes < need) {
     set_error("shared-prefix workspace holds %lld bytes, the batch needs %lld", static_cast<long long>(workspace_bytes),
               static_cast<long long>(need));
     return K8V4_ERR_WORKSPACE;
   }
   const int64_t table_pages = table_width * pages_per_block;
-  const int64_t groups = prefix_pages ? sh.groups : 0;
+  const int64_t blocks = prefix_pages ? sh.blocks : 0;
+  const int64_t groups = prefix_pages && !blocks ? sh.groups : 0;
   // The axis has at most this many units; a work-group's end may pass it by a
   // work-group's share.
   const int64_t units = groups * (prefix_pages + kPieceCost) +
                         batch * sh.per_seq * ((table_pages > prefix_pages ? table_pages - prefix_pages : 0) + kPieceCost);
-  K8V4_REQUIRE(units < (int64_t(1) << 30), "batch too large for one call");
+  K8V4_REQUIRE(units < (int64_t(1) << 30) && hkv * blocks * (prefix_pages + kWideCost) < (int64_t(1) << 30),
+               "batch too large for one call");
 
   SharedArgs a;
   char *ws = static_cast<char *>(workspace);
@@ -797,8 +1269,12 @@ extern "C" int k8v4_attn_shared(const void *q, int q_dtype, int64_t q_tok_stride
   a.tokens = static_cast<int>(sh.tokens);
   a.groups = static_cast<int>(groups);
   a.per_seq = static_cast<int>(sh.per_seq);
+  a.wide_blocks = static_cast<int>(blocks);
+  a.wide_segments = static_cast<int>(hkv * blocks);
   a.grid = static_cast<int>(sh.grid);
+  a.wide_grid = static_cast<int>(sh.wide_grid);
   a.ws = ws + sh.q_bytes + sh.scale_bytes;
+  a.own_ws = a.ws + sh.prefix_state_bytes;
   a.prefix_rows = sh.prefix_rows;
   a.own_rows = sh.own_rows;
   a.prefix_bytes = sh.prefix_bytes;
@@ -811,7 +1287,7 @@ extern "C" int k8v4_attn_shared(const void *q, int q_dtype, int64_t q_tok_stride
   int tpu = 256;
   {
     const int vpr_max = head_dim / 8;
-    const int64_t avg = groups ? (sh.grid + groups - 1) / groups + 1 : (sh.grid + batch - 1) / batch;
+    const int64_t avg = blocks ? (sh.wide_grid + hkv * blocks - 1) / (hkv * blocks) + 1 : groups ? (sh.grid + groups - 1) / groups + 1 : (sh.grid + batch - 1) / batch;
     int cs = vpr_max / 8;
     bool found = false;
     for (int threads : {128, 256}) {
@@ -833,6 +1309,14 @@ extern "C" int k8v4_attn_shared(const void *q, int q_dtype, int64_t q_tok_stride
   auto s = static_cast<hipStream_t>(stream);
   int rc = q_rows_launch(q, q_dtype == K8V4_BF16, q_tok_stride, sh.tokens, hkv, head_dim, sh.head_rows, q8, scales, s);
   if (rc) return rc;
+  if (blocks) {
+    if (hkv == 4)
+      launch_wide<4>(a, head_dim, s);
+    else
+      launch_wide<2>(a, head_dim, s);
+    rc = launch_status("k8v4_attn_shared prefix");
+    if (rc) return rc;
+  }
   const int widest = groups && sh.prefix_rows > sh.own_rows ? sh.prefix_rows : sh.own_rows;
   const int tiles = (widest + 15) / 16;
   if (head_dim == 256) {
