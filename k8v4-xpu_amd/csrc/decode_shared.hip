@@ -36,13 +36,6 @@ namespace {
 constexpr int kGroup = 8;  // tokens of one segment: 48 rows of a KV head
 // Fixed cost of a piece in pages of its pages' time.
 constexpr int kPieceCost = 6;
-#ifndef K8V4_AHEAD
-#define K8V4_AHEAD (D == 128 ? 6 : 4)
-#endif
-#ifndef K8V4_WIDE_MIN
-#define K8V4_WIDE_MIN 200
-#endif
-constexpr int kWideCost = 6;  // the same for a piece of the many-rows kernel
 constexpr int kFar = 1 << 30;
 
 struct SharedArgs {
@@ -67,11 +60,10 @@ struct SharedArgs {
   const int32_t *seq_lens;
   int batch, q_len, hkv;
   int tokens;      // batch * q_len
-  int groups;      // prefix segments (0 without a prefix, or where the many-rows kernel serves it)
-  int wide_segments, wide_blocks;  // many-rows kernel: KV heads x row blocks, row blocks (0: not used)
+  int groups;      // prefix segments (0 without a prefix)
+  int wide_blocks; // many-rows kernel: row blocks of a KV head, groups = hkv * wide_blocks (0: not used)
   int per_seq;     // own segments of a sequence: 1, or 2 for more than eight tokens
   int grid;        // work-groups of the split launch
-  int wide_grid;   // work-groups of the many-rows launch
   char *ws, *own_ws;  // states of the prefix's pieces and of the sequences' own
   int prefix_rows, own_rows;        // state rows of a KV head in a piece of either kind
   int64_t prefix_bytes, own_bytes;  // bytes of such a state
@@ -172,357 +164,380 @@ __device__ __forceinline__ args_ptr reread(args_ptr p) {
   return p;
 }
 
+// Calls piece(args, thread, segment, first page, last page + 1) for the pieces of
+// work-group wg, pages counted from the segment's first (uniform over it).
+template <typename Piece>
+__device__ __forceinline__ void walk_pieces(const SharedArgs &args, int wg, Piece piece) {
+  int unit, seg, base;
+  {
+    const int lane = threadIdx.x & (kWave - 1);
+    unit = plan_axis(args, lane, 0).unit;
+    const Where at = locate(args, lane, wg * unit);
+    seg = at.seg;
+    base = at.base;
+  }
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  for (;; ++seg) {
+    // Nothing derived from the lane or the arguments is kept from one piece to
+    // the next: hoisted out of this loop it would take the registers the
+    // pieces need (three row tiles: 63 of them spilled).
+    const SharedArgs &a = (const SharedArgs &)*reread((args_ptr)__builtin_amdgcn_kernarg_segment_ptr());
+    const int u0 = wg * unit, u1 = u0 + unit;
+    if (seg >= a.groups + a.batch * a.per_seq || base >= u1) return;
+    int zero = 0;
+    asm volatile("" : "+v"(zero));
+    const int tid = wave * kWave + __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, zero));
+    const const_i32_ptr lens = (const_i32_ptr)(a.seq_lens);
+    const int pages = seg < a.groups ? a.prefix_pages : own_pages(a, lens[(seg - a.groups) / a.per_seq]);
+    const int first = base + kPieceCost;  // of the segment's pages on the axis
+    base = pages > 0 ? first + pages : base;
+    const int s0 = max(u0 - first, 0), s1 = min(u1 - first, pages);
+    if (s1 > s0) piece(a, tid, seg, s0, s1);
+  }
+}
+
+// Pages s0 .. s1 - 1 of segment `seg` (counted from the segment's first page), by
+// a work-group of WG_WAVES waves (those behind the first HKV * NWH only keep its barriers).
+template <int NT, int HKV, int NWH, bool PH, bool PREFIX, int WG_WAVES = HKV * NWH>
+__device__ __forceinline__ void attend_piece(const SharedArgs &a, char *lds_raw, int tid, int wg, int seg, int s0, int s1) {
+  constexpr int D = 128;  // PH: dims of a half-head
+  using S = Slot<D>;
+  using CFG = SplitConfig<D, NT, HKV, NWH, PH>;
+  constexpr int RK = CFG::RK, RV = CFG::RV, DQ = CFG::DQ, KSQ = DQ / 64;
+  lds_t *lds = (lds_t *)(lds_raw);
+  const int lane = tid & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  if (WG_WAVES > HKV * NWH && wave >= HKV * NWH) {
+    __builtin_amdgcn_s_barrier();
+    if constexpr (NWH > 1) {
+      __syncthreads();
+      __syncthreads();
+    }
+    __syncthreads();
+    return;
+  }
+  const int h = wave % HKV;  // KV head (PH: half-head)
+  const int w = wave / HKV;  // position among the NWH waves of this head
+  const int hq = PH ? h >> 1 : h;
+  const int half = PH ? h & 1 : 0;
+  const int n = lane & 15, g = lane >> 4;
+  lds_t *qlds = lds + CFG::Q_OFF + hq * CFG::Q_BYTES_PER_HEAD;
+  lds_t *kring = lds + wave * CFG::WAVE_BYTES;
+  lds_t *vring = kring + RK * S::K_BYTES;
+  lds_int *flags = reinterpret_cast<lds_int *>(lds + CFG::FLAG_OFF);
+  const LaneOffsets lo = lane_offsets<D, HKV, PH>(a, h, lane);
+  const const_i32_ptr lens = (const_i32_ptr)(a.seq_lens);
+
+  const bool shared = PREFIX && seg < a.groups;
+  const int os = seg - a.groups;  // own segment
+  const int b = shared ? 0 : os / a.per_seq;
+  const int sub = shared ? 0 : os - b * a.per_seq;
+  const int len = shared ? 0 : lens[b];
+  const int p0 = (shared ? 0 : a.prefix_pages) + s0, p1 = (shared ? 0 : a.prefix_pages) + s1;
+  const int L0 = shared ? a.prefix_pages * kPage : len;
+  const int tok0 = shared ? seg * kGroup : b * a.q_len + sub * kGroup;
+  const int ntok = shared ? min(kGroup, a.tokens - tok0) : min(kGroup, a.q_len - sub * kGroup);
+  const int rows = ntok * kGqa;
+  const int x0 = 2 * p0;
+  const int x1 = min(2 * p1, static_cast<int>((static_cast<int64_t>(L0) + 31) / 32));
+  const int32_t *bt_row = shared ? a.prefix_table : a.block_table + static_cast<int64_t>(b) * a.bt_stride;
+
+  // Causal ends of this lane's rows: row r is token tok0 + r / 6, of any
+  // sequence in a prefix segment.  A row that sees no key at all (a padding
+  // sequence) takes no part in the masking, which it would force on every
+  // chunk; its state is dropped below.
+  WaveState<D, NT> st;
+  int far = 0;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = 16 * nt + n;
+    int end = L0;
+    if (r < rows) {
+      const int tok = tok0 + r / kGqa;
+      const int sb = tok / a.q_len;
+      end = a.seq_lens[sb] - a.q_len + (tok - sb * a.q_len) + 1;
+    }
+    st.lim[nt] = min(end, L0);
+    if (end > 0) far = max(far, kFar - min(st.lim[nt], kFar));
+  }
+  const int min_end = kFar - wave_max(far);
+
+  const int my0 = x0 + w;
+  const int cnt = my0 < x1 ? (x1 - my0 + NWH - 1) / NWH : 0;
+  // The query rows' fragments go straight into their operand positions
+  // (lane L of fragment (nt, ks) is 16 bytes at 16 L: row 16 nt + n, dims 64
+  // ks + 16 g), the rows' scales into the factor words.  The rows behind a
+  // short segment's last are other rows of the buffer (it is padded at the
+  // end); they are zeroed below.
+  int issued = 0;  // DMA bookkeeping as in the decode split kernel
+  {
+    const int8_t *tile = a.q8 + (hq * a.head_rows + static_cast<int64_t>(tok0) * kGqa) * DQ;
+    const float *scales = a.q8_scale + hq * a.head_rows + static_cast<int64_t>(tok0) * kGqa;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      if (nt % NWH != w) continue;
+#pragma unroll
+      for (int ks = 2 * half; ks < 2 * half + 2; ++ks) {
+        dma16s(tile, static_cast<uint32_t>((16 * nt + n) * DQ + 64 * ks + 16 * g), qlds + (nt * KSQ + ks) * kWave * 16);
+        ++issued;
+      }
+    }
+    if (w == 0 && half == 0) {
+      if (lane < NT * 16) dma4s(scales, static_cast<uint32_t>(lane * 4), qlds + CFG::Q_FRAG_BYTES);
+      ++issued;
+    }
+  }
+  const int q_done = issued;
+  // Physical pages of the piece, looked up once (runs of up to 128 pages).
+  const bool tab_vgpr = p1 - p0 <= 128;
+  int ptab[2] = {-1, -1};
+  if (tab_vgpr) {
+    int raw[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int p = min(p0 + 64 * i + lane, p1 - 1);
+      raw[i] = bt_row[a.ppb <= 1 ? p : p / a.ppb];
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int p = p0 + 64 * i + lane;
+      const int64_t ph = a.ppb <= 1 ? raw[i] : static_cast<int64_t>(raw[i]) * a.ppb + p % a.ppb;
+      ptab[i] = (p < p1 && ph >= 0 && ph < a.num_pages) ? static_cast<int>(ph) : -1;
+    }
+  }
+  auto page_of = [&](int x) -> int {  // x: chunk index in the sequence (wave-uniform)
+    const int p = x >> 1;
+    if (tab_vgpr) {
+      const int d = p - p0;
+      const int lo_pg = __builtin_amdgcn_readlane(ptab[0], d & 63);
+      const int hi_pg = __builtin_amdgcn_readlane(ptab[1], d & 63);
+      return d < 64 ? lo_pg : hi_pg;
+    }
+    const const_i32_ptr row = (const_i32_ptr)(bt_row);
+    const int64_t ph = a.ppb <= 1 ? row[p] : static_cast<int64_t>(row[p / a.ppb]) * a.ppb + p % a.ppb;
+    return (ph >= 0 && ph < a.num_pages) ? static_cast<int>(ph) : -1;
+  };
+  int mk[4] = {0, 0, 0, 0}, mv[4] = {0, 0, 0, 0};
+  uint32_t valid_mask = 0;  // bit s: K slot s holds a chunk of a valid page
+#pragma unroll
+  for (int s = 0; s < (RK > RV ? RK : RV); ++s) {
+    if (s >= cnt) break;
+    const int xs = my0 + s * NWH;
+    if (s < RK) {
+      valid_mask |= static_cast<uint32_t>(issue_k<D, HKV>(a, page_of(xs), xs, lo, kring + s * S::K_BYTES)) << s;
+      issued += S::NK;
+      mk[s] = issued;
+    }
+    if (s < RV) {
+      issue_v<D, HKV, PH>(a, page_of(xs), xs, lo, lane, vring + s * S::V_BYTES);
+      issued += S::NVS;
+      mv[s] = issued;
+    }
+  }
+  wait_vm(issued - q_done);  // the query rows are here
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    if (nt % NWH != w || 16 * nt + n < rows) continue;
+#pragma unroll
+    for (int ks = 2 * half; ks < 2 * half + 2; ++ks)
+      *reinterpret_cast<__attribute__((address_space(3))) v4i *>(qlds + ((nt * KSQ + ks) * kWave + lane) * 16) =
+          (v4i){0, 0, 0, 0};
+  }
+  if constexpr (PH) {
+    pair_flag_set(flags + wave, 0, lane);
+    pair_flag_set(flags + CFG::WAVES + wave, 0, lane);
+  } else if constexpr (CFG::BALANCE) {
+    pair_flag_set(flags + wave, 0, lane);
+  }
+  // Fragments and factors visible to both waves of the head (a bare barrier:
+  // __syncthreads() would also wait for every ring load in flight).
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const float f =
+        reinterpret_cast<const __attribute__((address_space(3))) float *>(qlds + CFG::Q_FRAG_BYTES)[nt * 16 + n];
+    // Kept above zero so that a masked (-inf) score never meets a zero factor.
+    const double c = static_cast<double>(16 * nt + n < rows ? f : 0.f) *
+                     (static_cast<double>(kLog2e) / sqrt(static_cast<double>(DQ)));
+    st.crow[nt] = fmaxf(static_cast<float>(c), 1e-30f);
+    st.lsum[nt] = (v4f){0.f, 0.f, 0.f, 0.f};
+    st.corr[nt] = (v4f){0.f, 0.f, 0.f, 0.f};
+    st.m_run[nt] = -INFINITY;
+    st.thr[nt] = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) st.O[nt][0][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+  }
+
+  for (int k = 0; k < cnt; ++k) {
+    const int sk = k % RK, sv = k % RV;  // wave-uniform ring slots
+    if constexpr (CFG::BALANCE) {
+      // The two waves of a SIMD yield to each other (see the decode split kernel).
+      pair_flag_set(flags + wave, k, lane);
+      const int pk = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const volatile lds_int *>(flags + (wave ^ 4)));
+      if (k > pk)
+        __builtin_amdgcn_s_setprio(0);
+      else
+        __builtin_amdgcn_s_setprio(1);
+    }
+    lds_t *kslot = kring + sk * S::K_BYTES;
+    lds_t *vslot = vring + sv * S::V_BYTES;
+    int mks = mk[0], mvs = mv[0];
+#pragma unroll
+    for (int s = 1; s < RK; ++s)
+      if (sk == s) mks = mk[s];
+#pragma unroll
+    for (int s = 1; s < RV; ++s)
+      if (sv == s) mvs = mv[s];
+    {
+      const int left = issued - max(mks, mvs);
+      if (left == CFG::STEADY_AFTER)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(CFG::STEADY_AFTER) : "memory");
+      else
+        wait_vm(left);
+    }
+    if constexpr (PH) {
+      pair_flag_set(flags + wave, k + 1, lane);
+      pair_flag_wait(flags + (wave ^ 1), k + 1, lane);
+    }
+    const bool valid = (valid_mask >> sk) & 1u;
+    const int tbase = 32 * (my0 + k * NWH);
+    v4i sc[2][NT];
+    if constexpr (PH) {
+      const lds_t *pslot = lds + (wave ^ 1) * CFG::WAVE_BYTES + sk * S::K_BYTES;
+      if (valid) chunk_qk_pair<NT>(half ? pslot : kslot, half ? kslot : pslot, qlds, lane, g, sc);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      pair_flag_set(flags + CFG::WAVES + wave, k + 1, lane);
+    } else {
+      if (valid) chunk_qk<D, NT>(kslot, qlds, lane, g, sc);
+    }
+    auto refill_k = [&]() {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      const int xr = my0 + (k + RK) * NWH;
+      const uint32_t v = static_cast<uint32_t>(issue_k<D, HKV>(a, page_of(xr), xr, lo, kslot));
+      valid_mask = (valid_mask & ~(1u << sk)) | (v << sk);
+      issued += S::NK;
+#pragma unroll
+      for (int s = 0; s < RK; ++s)
+        if (sk == s) mk[s] = issued;
+    };
+    if (CFG::K_EARLY && k + RK < cnt) refill_k();
+    if (valid) chunk_softmax_pv<D, NT, PH>(st, sc, vslot, tbase, L0, lane, g, tbase + 32 > min_end);
+    if (!CFG::K_EARLY && k + RK < cnt) {
+      if constexpr (PH) pair_flag_wait(flags + CFG::WAVES + (wave ^ 1), k + 1, lane);
+      refill_k();
+    }
+    if (k + RV < cnt) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      const int xr = my0 + (k + RV) * NWH;
+      issue_v<D, HKV, PH>(a, page_of(xr), xr, lo, lane, vslot);
+      issued += S::NVS;
+#pragma unroll
+      for (int s = 0; s < RV; ++s)
+        if (sv == s) mv[s] = issued;
+    }
+  }
+
+  finalize_output(st);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+    if (st.lim[nt] <= 0) st.m_run[nt] = -INFINITY;
+
+  // The state's form is the decode split kernel's: a quarter of O / l in fp16,
+  // then m and l.
+  auto write_state = [&]() {
+    const int srows = shared ? a.prefix_rows : a.own_rows;
+    char *state = piece_state(a, wg, seg);
+    _Float16 *obase = reinterpret_cast<_Float16 *>(state);
+    float2 *mlbase = reinterpret_cast<float2 *>(state + static_cast<int64_t>(CFG::QHEADS) * srows * DQ * 2);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 16 * nt + 4 * g + i;
+        const float m_r = lane_value(st.m_run[nt], 4 * g + i);
+        if (r < rows) {
+          // A row that saw nothing: zeros, whatever its lanes hold (a padding
+          // row's query may be anything).
+          const bool seen = m_r != -INFINITY;
+          const float l = seen ? st.lsum[nt][i] : 0.f;
+          const float f = l > 0.f ? 0.25f / l : 0.f;
+          _Float16 *dst = obase + static_cast<int64_t>(hq * srows + r) * DQ + half * 128 + 8 * n;
+          v8h o;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o[j] = static_cast<_Float16>(seen ? st.O[nt][0][j][i] * f : 0.f);
+          store_wt16(dst, o);
+          if (n == 0 && half == 0) store_wt8(mlbase + hq * srows + r, make_float2(m_r, l));
+        }
+      }
+    }
+  };
+  // Combine the two waves of each head, then write the state.
+  if constexpr (NWH > 1) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __syncthreads();  // every ring is drained; the LDS serves the exchange
+    float *xb = reinterpret_cast<float *>(lds_raw) + h * (CFG::XCHG_FLOATS);
+    if (w == 1) {
+      int e = 0;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        xb[(e++) * kWave + lane] = st.m_run[nt];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) xb[(e++) * kWave + lane] = st.lsum[nt][i];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) xb[(e++) * kWave + lane] = st.O[nt][0][j][i];
+      }
+    }
+    __syncthreads();
+    if (w == 0) {
+      int e = 0;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float m1 = xb[(e++) * kWave + lane];
+        const float m0 = st.m_run[nt];
+        const float M = fmaxf(m0, m1);
+        const float a0 = m0 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m0 - M);
+        const float a1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - M);
+        st.m_run[nt] = M;
+        float a0i[4], a1i[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          a0i[i] = lane_value(a0, 4 * g + i);
+          a1i[i] = lane_value(a1, 4 * g + i);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st.lsum[nt][i] = st.lsum[nt][i] * a0i[i] + xb[(e++) * kWave + lane] * a1i[i];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            st.O[nt][0][j][i] = st.O[nt][0][j][i] * a0i[i] + xb[(e++) * kWave + lane] * a1i[i];
+          // Combined here, not where the rows are written: there the words
+          // of all columns would wait in registers (21 of them spilled).
+          asm volatile("" : "+v"(st.O[nt][0][j]));
+        }
+      }
+      write_state();
+    }
+  }
+  if constexpr (NWH == 1) write_state();
+  // The next piece's loads overwrite the LDS and count from zero.
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
 template <int NT, int HKV, int NWH, bool PH>
 __global__ __attribute__((amdgpu_flat_work_group_size(64 * HKV * NWH, 64 * HKV * NWH),
                           amdgpu_waves_per_eu(SplitConfig<128, NT, HKV, NWH, PH>::OCC,
                                               SplitConfig<128, NT, HKV, NWH, PH>::OCC)))
 void shared_split_kernel(SharedArgs args) {
-  constexpr int D = 128;  // PH: dims of a half-head
-  using S = Slot<D>;
-  using CFG = SplitConfig<D, NT, HKV, NWH, PH>;
-  constexpr int RK = CFG::RK, RV = CFG::RV, DQ = CFG::DQ, KSQ = DQ / 64;
-  __shared__ __attribute__((aligned(16))) char lds_raw[CFG::LDS_BYTES];
-  lds_t *lds = (lds_t *)(lds_raw);
-
+  __shared__ __attribute__((aligned(16))) char lds[SplitConfig<128, NT, HKV, NWH, PH>::LDS_BYTES];
   const int wg = static_cast<int>(blockIdx.x);
-  int u0, u1, seg, base;
-  {
-    const int lane = threadIdx.x & (kWave - 1);
-    const int unit = plan_axis(args, lane, 0).unit;
-    u0 = wg * unit;
-    u1 = u0 + unit;
-    const Where at = locate(args, lane, u0);
-    seg = at.seg;
-    base = at.base;
-  }
-
-  // The pieces of this work-group (uniform over it).
-  const int segments = args.groups + args.batch * args.per_seq;
-  for (; seg < segments && base < u1; ++seg) {
-    // Nothing derived from the lane or the arguments is kept from one piece to
-    // the next: hoisted out of this loop it would take the registers the
-    // piece needs (NT = 3: 63 of them spilled).
-    const SharedArgs &a = (const SharedArgs &)*reread((args_ptr)__builtin_amdgcn_kernarg_segment_ptr());
-    int tid = threadIdx.x;
-    asm volatile("" : "+v"(tid));
-    const int lane = tid & (kWave - 1);
-    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-    const int h = wave % HKV;  // KV head (PH: half-head)
-    const int w = wave / HKV;  // position among the NWH waves of this head
-    const int hq = PH ? h >> 1 : h;
-    const int half = PH ? h & 1 : 0;
-    const int n = lane & 15, g = lane >> 4;
-    lds_t *qlds = lds + CFG::Q_OFF + hq * CFG::Q_BYTES_PER_HEAD;
-    lds_t *kring = lds + wave * CFG::WAVE_BYTES;
-    lds_t *vring = kring + RK * S::K_BYTES;
-    lds_int *flags = reinterpret_cast<lds_int *>(lds + CFG::FLAG_OFF);
-    const LaneOffsets lo = lane_offsets<D, HKV, PH>(a, h, lane);
-    const const_i32_ptr lens = (const_i32_ptr)(a.seq_lens);
-
-    const bool shared = seg < a.groups;
-    const int os = seg - a.groups;  // own segment
-    const int b = shared ? 0 : os / a.per_seq;
-    const int sub = shared ? 0 : os - b * a.per_seq;
-    const int len = shared ? 0 : lens[b];
-    const int pages = shared ? a.prefix_pages : own_pages(a, len);
-    const int first = base + kPieceCost;  // of the segment's pages on the axis
-    base = pages > 0 ? first + pages : base;
-    const int s0 = max(u0 - first, 0), s1 = min(u1 - first, pages);
-    if (s1 <= s0) continue;
-    const int p0 = (shared ? 0 : a.prefix_pages) + s0, p1 = (shared ? 0 : a.prefix_pages) + s1;
-    const int L0 = shared ? a.prefix_pages * kPage : len;
-    const int tok0 = shared ? seg * kGroup : b * a.q_len + sub * kGroup;
-    const int ntok = shared ? min(kGroup, a.tokens - tok0) : min(kGroup, a.q_len - sub * kGroup);
-    const int rows = ntok * kGqa;
-    const int x0 = 2 * p0;
-    const int x1 = min(2 * p1, static_cast<int>((static_cast<int64_t>(L0) + 31) / 32));
-    const int32_t *bt_row = shared ? a.prefix_table : a.block_table + static_cast<int64_t>(b) * a.bt_stride;
-
-    // Causal ends of this lane's rows: row r is token tok0 + r / 6, of any
-    // sequence in a prefix segment.  A row that sees no key at all (a padding
-    // sequence) takes no part in the masking, which it would force on every
-    // chunk; its state is dropped below.
-    WaveState<D, NT> st;
-    int far = 0;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int r = 16 * nt + n;
-      int end = L0;
-      if (r < rows) {
-        const int tok = tok0 + r / kGqa;
-        const int sb = tok / a.q_len;
-        end = a.seq_lens[sb] - a.q_len + (tok - sb * a.q_len) + 1;
-      }
-      st.lim[nt] = min(end, L0);
-      if (end > 0) far = max(far, kFar - min(st.lim[nt], kFar));
-    }
-    const int min_end = kFar - wave_max(far);
-
-    const int my0 = x0 + w;
-    const int cnt = my0 < x1 ? (x1 - my0 + NWH - 1) / NWH : 0;
-    // The query rows' fragments go straight into their operand positions
-    // (lane L of fragment (nt, ks) is 16 bytes at 16 L: row 16 nt + n, dims 64
-    // ks + 16 g), the rows' scales into the factor words.  The rows behind a
-    // short segment's last are other rows of the buffer (it is padded at the
-    // end); they are zeroed below.
-    int issued = 0;  // DMA bookkeeping as in the decode split kernel
-    {
-      const int8_t *tile = a.q8 + (hq * a.head_rows + static_cast<int64_t>(tok0) * kGqa) * DQ;
-      const float *scales = a.q8_scale + hq * a.head_rows + static_cast<int64_t>(tok0) * kGqa;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        if (nt % NWH != w) continue;
-#pragma unroll
-        for (int ks = 2 * half; ks < 2 * half + 2; ++ks) {
-          dma16s(tile, static_cast<uint32_t>((16 * nt + n) * DQ + 64 * ks + 16 * g), qlds + (nt * KSQ + ks) * kWave * 16);
-          ++issued;
-        }
-      }
-      if (w == 0 && half == 0) {
-        if (lane < NT * 16) dma4s(scales, static_cast<uint32_t>(lane * 4), qlds + CFG::Q_FRAG_BYTES);
-        ++issued;
-      }
-    }
-    const int q_done = issued;
-    // Physical pages of the piece, looked up once (runs of up to 128 pages).
-    const bool tab_vgpr = p1 - p0 <= 128;
-    int ptab[2] = {-1, -1};
-    if (tab_vgpr) {
-      int raw[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int p = min(p0 + 64 * i + lane, p1 - 1);
-        raw[i] = bt_row[a.ppb <= 1 ? p : p / a.ppb];
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int p = p0 + 64 * i + lane;
-        const int64_t ph = a.ppb <= 1 ? raw[i] : static_cast<int64_t>(raw[i]) * a.ppb + p % a.ppb;
-        ptab[i] = (p < p1 && ph >= 0 && ph < a.num_pages) ? static_cast<int>(ph) : -1;
-      }
-    }
-    auto page_of = [&](int x) -> int {  // x: chunk index in the sequence (wave-uniform)
-      const int p = x >> 1;
-      if (tab_vgpr) {
-        const int d = p - p0;
-        const int lo_pg = __builtin_amdgcn_readlane(ptab[0], d & 63);
-        const int hi_pg = __builtin_amdgcn_readlane(ptab[1], d & 63);
-        return d < 64 ? lo_pg : hi_pg;
-      }
-      const const_i32_ptr row = (const_i32_ptr)(bt_row);
-      const int64_t ph = a.ppb <= 1 ? row[p] : static_cast<int64_t>(row[p / a.ppb]) * a.ppb + p % a.ppb;
-      return (ph >= 0 && ph < a.num_pages) ? static_cast<int>(ph) : -1;
-    };
-    int mk[4] = {0, 0, 0, 0}, mv[4] = {0, 0, 0, 0};
-    uint32_t valid_mask = 0;  // bit s: K slot s holds a chunk of a valid page
-#pragma unroll
-    for (int s = 0; s < (RK > RV ? RK : RV); ++s) {
-      if (s >= cnt) break;
-      const int xs = my0 + s * NWH;
-      if (s < RK) {
-        valid_mask |= static_cast<uint32_t>(issue_k<D, HKV>(a, page_of(xs), xs, lo, kring + s * S::K_BYTES)) << s;
-        issued += S::NK;
-        mk[s] = issued;
-      }
-      if (s < RV) {
-        issue_v<D, HKV, PH>(a, page_of(xs), xs, lo, lane, vring + s * S::V_BYTES);
-        issued += S::NVS;
-        mv[s] = issued;
-      }
-    }
-    wait_vm(issued - q_done);  // the query rows are here
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      if (nt % NWH != w || 16 * nt + n < rows) continue;
-#pragma unroll
-      for (int ks = 2 * half; ks < 2 * half + 2; ++ks)
-        *reinterpret_cast<__attribute__((address_space(3))) v4i *>(qlds + ((nt * KSQ + ks) * kWave + lane) * 16) =
-            (v4i){0, 0, 0, 0};
-    }
-    if constexpr (PH) {
-      pair_flag_set(flags + wave, 0, lane);
-      pair_flag_set(flags + CFG::WAVES + wave, 0, lane);
-    } else if constexpr (CFG::BALANCE) {
-      pair_flag_set(flags + wave, 0, lane);
-    }
-    // Fragments and factors visible to both waves of the head (a bare barrier:
-    // __syncthreads() would also wait for every ring load in flight).
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const float f =
-          reinterpret_cast<const __attribute__((address_space(3))) float *>(qlds + CFG::Q_FRAG_BYTES)[nt * 16 + n];
-      // Kept above zero so that a masked (-inf) score never meets a zero factor.
-      const double c = static_cast<double>(16 * nt + n < rows ? f : 0.f) *
-                       (static_cast<double>(kLog2e) / sqrt(static_cast<double>(DQ)));
-      st.crow[nt] = fmaxf(static_cast<float>(c), 1e-30f);
-      st.lsum[nt] = (v4f){0.f, 0.f, 0.f, 0.f};
-      st.corr[nt] = (v4f){0.f, 0.f, 0.f, 0.f};
-      st.m_run[nt] = -INFINITY;
-      st.thr[nt] = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) st.O[nt][0][j] = (v4f){0.f, 0.f, 0.f, 0.f};
-    }
-
-    for (int k = 0; k < cnt; ++k) {
-      const int sk = k % RK, sv = k % RV;  // wave-uniform ring slots
-      if constexpr (CFG::BALANCE) {
-        // The two waves of a SIMD yield to each other (see the decode split kernel).
-        pair_flag_set(flags + wave, k, lane);
-        const int pk = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const volatile lds_int *>(flags + (wave ^ 4)));
-        if (k > pk)
-          __builtin_amdgcn_s_setprio(0);
-        else
-          __builtin_amdgcn_s_setprio(1);
-      }
-      lds_t *kslot = kring + sk * S::K_BYTES;
-      lds_t *vslot = vring + sv * S::V_BYTES;
-      int mks = mk[0], mvs = mv[0];
-#pragma unroll
-      for (int s = 1; s < RK; ++s)
-        if (sk == s) mks = mk[s];
-#pragma unroll
-      for (int s = 1; s < RV; ++s)
-        if (sv == s) mvs = mv[s];
-      {
-        const int left = issued - max(mks, mvs);
-        if (left == CFG::STEADY_AFTER)
-          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(CFG::STEADY_AFTER) : "memory");
-        else
-          wait_vm(left);
-      }
-      if constexpr (PH) {
-        pair_flag_set(flags + wave, k + 1, lane);
-        pair_flag_wait(flags + (wave ^ 1), k + 1, lane);
-      }
-      const bool valid = (valid_mask >> sk) & 1u;
-      const int tbase = 32 * (my0 + k * NWH);
-      v4i sc[2][NT];
-      if constexpr (PH) {
-        const lds_t *pslot = lds + (wave ^ 1) * CFG::WAVE_BYTES + sk * S::K_BYTES;
-        if (valid) chunk_qk_pair<NT>(half ? pslot : kslot, half ? kslot : pslot, qlds, lane, g, sc);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        pair_flag_set(flags + CFG::WAVES + wave, k + 1, lane);
-      } else {
-        if (valid) chunk_qk<D, NT>(kslot, qlds, lane, g, sc);
-      }
-      auto refill_k = [&]() {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        const int xr = my0 + (k + RK) * NWH;
-        const uint32_t v = static_cast<uint32_t>(issue_k<D, HKV>(a, page_of(xr), xr, lo, kslot));
-        valid_mask = (valid_mask & ~(1u << sk)) | (v << sk);
-        issued += S::NK;
-#pragma unroll
-        for (int s = 0; s < RK; ++s)
-          if (sk == s) mk[s] = issued;
-      };
-      if (CFG::K_EARLY && k + RK < cnt) refill_k();
-      if (valid) chunk_softmax_pv<D, NT, PH>(st, sc, vslot, tbase, L0, lane, g, tbase + 32 > min_end);
-      if (!CFG::K_EARLY && k + RK < cnt) {
-        if constexpr (PH) pair_flag_wait(flags + CFG::WAVES + (wave ^ 1), k + 1, lane);
-        refill_k();
-      }
-      if (k + RV < cnt) {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        const int xr = my0 + (k + RV) * NWH;
-        issue_v<D, HKV, PH>(a, page_of(xr), xr, lo, lane, vslot);
-        issued += S::NVS;
-#pragma unroll
-        for (int s = 0; s < RV; ++s)
-          if (sv == s) mv[s] = issued;
-      }
-    }
-
-    finalize_output(st);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-      if (st.lim[nt] <= 0) st.m_run[nt] = -INFINITY;
-
-    // The state's form is the decode split kernel's: a quarter of O / l in fp16,
-    // then m and l.
-    auto write_state = [&]() {
-      const int srows = shared ? a.prefix_rows : a.own_rows;
-      char *state = piece_state(a, wg, seg);
-      _Float16 *obase = reinterpret_cast<_Float16 *>(state);
-      float2 *mlbase = reinterpret_cast<float2 *>(state + static_cast<int64_t>(CFG::QHEADS) * srows * DQ * 2);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 16 * nt + 4 * g + i;
-          const float m_r = lane_value(st.m_run[nt], 4 * g + i);
-          if (r < rows) {
-            // A row that saw nothing: zeros, whatever its lanes hold (a padding
-            // row's query may be anything).
-            const bool seen = m_r != -INFINITY;
-            const float l = seen ? st.lsum[nt][i] : 0.f;
-            const float f = l > 0.f ? 0.25f / l : 0.f;
-            _Float16 *dst = obase + static_cast<int64_t>(hq * srows + r) * DQ + half * 128 + 8 * n;
-            v8h o;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) o[j] = static_cast<_Float16>(seen ? st.O[nt][0][j][i] * f : 0.f);
-            store_wt16(dst, o);
-            if (n == 0 && half == 0) store_wt8(mlbase + hq * srows + r, make_float2(m_r, l));
-          }
-        }
-      }
-    };
-    // Combine the two waves of each head, then write the state.
-    if constexpr (NWH > 1) {
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-      __syncthreads();  // every ring is drained; the LDS serves the exchange
-      float *xb = reinterpret_cast<float *>(lds_raw) + h * (CFG::XCHG_FLOATS);
-      if (w == 1) {
-        int e = 0;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          xb[(e++) * kWave + lane] = st.m_run[nt];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) xb[(e++) * kWave + lane] = st.lsum[nt][i];
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) xb[(e++) * kWave + lane] = st.O[nt][0][j][i];
-        }
-      }
-      __syncthreads();
-      if (w == 0) {
-        int e = 0;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const float m1 = xb[(e++) * kWave + lane];
-          const float m0 = st.m_run[nt];
-          const float M = fmaxf(m0, m1);
-          const float a0 = m0 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m0 - M);
-          const float a1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - M);
-          st.m_run[nt] = M;
-          float a0i[4], a1i[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            a0i[i] = lane_value(a0, 4 * g + i);
-            a1i[i] = lane_value(a1, 4 * g + i);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) st.lsum[nt][i] = st.lsum[nt][i] * a0i[i] + xb[(e++) * kWave + lane] * a1i[i];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              st.O[nt][0][j][i] = st.O[nt][0][j][i] * a0i[i] + xb[(e++) * kWave + lane] * a1i[i];
-            // Combined here, not where the rows are written: there the words
-            // of all columns would wait in registers (21 of them spilled).
-            asm volatile("" : "+v"(st.O[nt][0][j]));
-          }
-        }
-        write_state();
-      }
-    }
-    if constexpr (NWH == 1) write_state();
-    // The next piece's loads overwrite the LDS and count from zero.
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __syncthreads();
-  }
+  walk_pieces(args, wg, [&](const SharedArgs &a, int tid, int seg, int s0, int s1) {
+    attend_piece<NT, HKV, NWH, PH, true>(a, lds, tid, wg, seg, s0, s1);
+  });
 }
 
 // ------------------------------------------------------------ many rows
@@ -575,373 +590,392 @@ struct Wide {
 // chunk and written 64 at a time at one chunk, both conflict-free.
 __device__ __forceinline__ int vswz(int row) { return (row & 7) ^ ((row >> 3) & 1); }
 
+// Pages p0 .. p1 - 1 of the prefix for one row block of one KV head.
 template <int D, int HKV>
-__global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_per_eu(2, 2)))
-void shared_wide_kernel(SharedArgs args) {
+__device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, int tid, int wg, int seg, int p0, int p1) {
   using W = Wide<D>;
   constexpr int NT = W::NT, KS = D / 64, DT = D / 16;
-  __shared__ __attribute__((aligned(16))) char lds_raw[W::LDS_BYTES];
   lds_t *lds = (lds_t *)(lds_raw);
+  const int lane = tid & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int grp = wave >> 2;
+  const int n = lane & 15, g = lane >> 4;
 
-  const int wg = static_cast<int>(blockIdx.x);
-  const int cost = args.prefix_pages + kWideCost;
-  const int unit = (args.wide_segments * cost + args.wide_grid - 1) / args.wide_grid;
-  const int u0 = wg * unit, u1 = u0 + unit;
+  const int h = seg / a.wide_blocks, block = seg - h * a.wide_blocks;
+  const int row0 = block * W::ROWS + wave * 16 * NT;  // first row of this wave, of the head's tokens * 6
+  const int nrows = a.tokens * kGqa;
+  const bool active = row0 < nrows;
+  const int pages = p1 - p0;
 
-  for (int seg = u0 / cost; seg < args.wide_segments && seg * cost < u1; ++seg) {
-    const SharedArgs &a = (const SharedArgs &)*reread((args_ptr)__builtin_amdgcn_kernarg_segment_ptr());
-    int tid = threadIdx.x;
-    asm volatile("" : "+v"(tid));
-    const int lane = tid & (kWave - 1);
-    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-    const int grp = wave >> 2;
-    const int n = lane & 15, g = lane >> 4;
-
-    const int first = seg * cost + kWideCost;
-    const int p0 = max(u0 - first, 0), p1 = min(u1 - first, a.prefix_pages);
-    if (p1 <= p0) continue;
-    const int h = seg / a.wide_blocks, block = seg - h * a.wide_blocks;
-    const int row0 = block * W::ROWS + wave * 16 * NT;  // first row of this wave, of the head's tokens * 6
-    const int nrows = a.tokens * kGqa;
-    const bool active = row0 < nrows;
-    const int pages = p1 - p0;
-
-    // Query rows: lane (n, g) of tile nt holds row 16 nt + n, dims 64 ks + 16 g ...
-    v4i qf[NT][KS];
-    float crow[NT];
-    int lim[NT];
-    int far = 0;
+  // Query rows: lane (n, g) of tile nt holds row 16 nt + n, dims 64 ks + 16 g ...
+  v4i qf[NT][KS];
+  float crow[NT];
+  int lim[NT];
+  int far = 0;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int r = row0 + 16 * nt + n;
-      const int64_t at = h * a.head_rows + r;  // the buffer is padded to whole blocks
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = row0 + 16 * nt + n;
+    const int64_t at = h * a.head_rows + r;  // the buffer is padded to whole blocks
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) qf[nt][ks] = *reinterpret_cast<const v4i *>(a.q8 + at * D + 64 * ks + 16 * g);
-      int end = a.prefix_pages * kPage;
-      double f = 0.0;
-      if (r < nrows) {
-        f = a.q8_scale[at];
-        const int tok = r / kGqa, sb = tok / a.q_len;
-        end = a.seq_lens[sb] - a.q_len + (tok - sb * a.q_len) + 1;
-        if (end > 0) far = max(far, kFar - min(end, kFar));
-      }
-      lim[nt] = end;
-      crow[nt] = fmaxf(static_cast<float>(f * (static_cast<double>(kLog2e) / sqrt(static_cast<double>(D)))), 1e-30f);
+    for (int ks = 0; ks < KS; ++ks) qf[nt][ks] = *reinterpret_cast<const v4i *>(a.q8 + at * D + 64 * ks + 16 * g);
+    int end = a.prefix_pages * kPage;
+    double f = 0.0;
+    if (r < nrows) {
+      f = a.q8_scale[at];
+      const int tok = r / kGqa, sb = tok / a.q_len;
+      end = a.seq_lens[sb] - a.q_len + (tok - sb * a.q_len) + 1;
+      if (end > 0) far = max(far, kFar - min(end, kFar));
     }
-    const int min_end = kFar - wave_max(far);
+    lim[nt] = end;
+    crow[nt] = fmaxf(static_cast<float>(f * (static_cast<double>(kLog2e) / sqrt(static_cast<double>(D)))), 1e-30f);
+  }
+  const int min_end = kFar - wave_max(far);
 
-    // Lane offsets of this wave's loads of a page: K rows (swizzled as in
-    // lane_offsets), V rows, one cell of a plane.
-    uint32_t koff[W::KPW];
+  // Lane offsets of this wave's loads of a page: K rows (swizzled as in
+  // lane_offsets), V rows, one cell of a plane.
+  const int vj = wave & (kPage * W::VROW / 1024 - 1);  // 1 KB piece of V rows
+  struct Offsets {
+    uint32_t k[W::KPW], v, p;
+  };
+  auto offsets = [&](int l) {
+    Offsets o;
 #pragma unroll
     for (int k = 0; k < W::KPW; ++k) {
       constexpr int CPR = D / 16;  // 16-byte chunks of a K row
-      const int t = (wave * W::KPW + k) * (1024 / D) + lane / CPR;
-      koff[k] = static_cast<uint32_t>(t * (HKV * D) + h * D + 16 * ((lane % CPR) ^ kswz<D>(t)));
+      const int t = (wave * W::KPW + k) * (1024 / D) + l / CPR;
+      o.k[k] = static_cast<uint32_t>(t * (HKV * D) + h * D + 16 * ((l % CPR) ^ kswz<D>(t)));
     }
-    const int vj = wave & (kPage * W::VROW / 1024 - 1);  // 1 KB piece of V rows
-    const uint32_t voff = static_cast<uint32_t>((vj * (1024 / W::VROW) + lane * 16 / W::VROW) * (HKV * W::VROW) +
-                                                h * W::VROW + lane * 16 % W::VROW);
-    const uint32_t poff = static_cast<uint32_t>((lane * HKV + h) * 4);
-    // Physical pages, 64 at a time: lane l holds page p0 + 64 k + l.
-    int ptab = -1;
-    auto load_table = [&](int k) {
-      const int p = min(p0 + 64 * k + lane, p1 - 1);
-      const int raw = a.prefix_table[a.ppb <= 1 ? p : p / a.ppb];
-      const int64_t ph = a.ppb <= 1 ? raw : static_cast<int64_t>(raw) * a.ppb + p % a.ppb;
-      ptab = ph >= 0 && ph < a.num_pages ? static_cast<int>(ph) : -1;
-    };
-    // Whether page i of the piece is in the cache, for the last SLOTS pages issued.
-    uint32_t valid = 0;
-    // This wave's loads of page i of the piece (W::LOADS of them, also for a
-    // page behind the last or outside the cache, so every page costs the same
-    // count): its share of the K rows and of the V rows, and a plane.
-    const char *const kbase = reinterpret_cast<const char *>(a.k_cache);
-    const char *const vbase = reinterpret_cast<const char *>(a.v_cache);
-    const int plane = D == 128 ? wave - 4 : wave;  // 1: v_scale, 2: v_zero, others k_scale
-    const char *const pbase = plane == 1   ? reinterpret_cast<const char *>(a.v_scale)
-                              : plane == 2 ? reinterpret_cast<const char *>(a.v_zero)
-                                           : reinterpret_cast<const char *>(a.k_scale);
-    const int64_t k_ps = a.k_ps, v_ps = a.v_ps, p_ps = plane == 1 ? a.vs_ps : plane == 2 ? a.vz_ps : a.ks_ps;
-    lds_t *const pdst0 = lds + W::S_OFF + (plane == 1 || plane == 2 ? plane : 0) * kPage * 4;
-    auto issue = [&](int i) {
-      if ((i & 63) == 0 && i < pages) load_table(i >> 6);
-      const int phys = i < pages ? __builtin_amdgcn_readlane(ptab, i & 63) : -1;
-      const int slot = i % W::SLOTS;
-      valid = (valid & ~(1u << slot)) | (phys >= 0 ? 1u << slot : 0u);
-      const int64_t ph = phys >= 0 ? phys : 0;
-      lds_t *dst = lds + slot * W::SLOT_BYTES;
-#pragma unroll
-      for (int k = 0; k < W::KPW; ++k) dma16s(kbase + ph * k_ps, koff[k], dst + (wave * W::KPW + k) * 1024);
-      if (D == 256 || wave < 4) dma16s(vbase + ph * v_ps, voff, dst + W::V_OFF + vj * 1024);
-      if (D == 256 || wave >= 4) {
-        // D = 128: waves 4 and 7 both fetch k_scale; D = 256: 0 and 3 .. 7.  A page
-        // outside the cache holds no keys: its scores are masked in B, and its
-        // planes are zeros here, so that its V is zeros whatever page 0 holds.
-        lds_t *pdst = pdst0 + slot * W::SLOT_BYTES;
-        dma4s(pbase + ph * p_ps, poff, phys >= 0 ? pdst : lds + W::PAD_OFF);
-        if (phys < 0) *reinterpret_cast<__attribute__((address_space(3))) float *>(pdst + 4 * lane) = 0.f;
-      }
-    };
-
-    v4f O[NT][DT];
-    v4f lsum[NT];
-    float m_run[NT], thr[NT];
-    v4i S[NT][4];
-    v8h P[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      lsum[nt] = (v4f){0.f, 0.f, 0.f, 0.f};
-      m_run[nt] = -INFINITY;
-      thr[nt] = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < DT; ++j) O[nt][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+    o.v = static_cast<uint32_t>((vj * (1024 / W::VROW) + l * 16 / W::VROW) * (HKV * W::VROW) + h * W::VROW + l * 16 % W::VROW);
+    o.p = static_cast<uint32_t>((l * HKV + h) * 4);
+    return o;
+  };
+  const Offsets off0 = offsets(lane);
+  // Physical pages, 64 at a time: lane l holds page p0 + 64 k + l.
+  int ptab = -1;
+  auto load_table = [&](int k) {
+    const int p = min(p0 + 64 * k + lane, p1 - 1);
+    const int raw = a.prefix_table[a.ppb <= 1 ? p : p / a.ppb];
+    const int64_t ph = a.ppb <= 1 ? raw : static_cast<int64_t>(raw) * a.ppb + p % a.ppb;
+    ptab = ph >= 0 && ph < a.num_pages ? static_cast<int>(ph) : -1;
+  };
+  // Whether page i of the piece is in the cache, for the last SLOTS pages issued.
+  uint32_t valid = 0;
+  // This wave's loads of page i of the piece (W::LOADS of them, also for a
+  // page behind the last or outside the cache, so every page costs the same
+  // count): its share of the K rows and of the V rows, and a plane.
+  const char *const kbase = reinterpret_cast<const char *>(a.k_cache);
+  const char *const vbase = reinterpret_cast<const char *>(a.v_cache);
+  const int plane = D == 128 ? wave - 4 : wave;  // 1: v_scale, 2: v_zero, others k_scale
+  const char *const pbase = plane == 1   ? reinterpret_cast<const char *>(a.v_scale)
+                            : plane == 2 ? reinterpret_cast<const char *>(a.v_zero)
+                                         : reinterpret_cast<const char *>(a.k_scale);
+  // Page strides are below 2^31 bytes, page numbers below 2^31.
+  const uint32_t k_ps = static_cast<uint32_t>(a.k_ps), v_ps = static_cast<uint32_t>(a.v_ps);
+  const uint32_t p_ps = static_cast<uint32_t>(plane == 1 ? a.vs_ps : plane == 2 ? a.vz_ps : a.ks_ps);
+  lds_t *const pdst0 = lds + W::S_OFF + (plane == 1 || plane == 2 ? plane : 0) * kPage * 4;
+  auto issue = [&](int i) {
+    if ((i & 63) == 0 && i < pages) load_table(i >> 6);
+    const int phys = i < pages ? __builtin_amdgcn_readlane(ptab, i & 63) : -1;
+    const int slot = i % W::SLOTS;
+    valid = (valid & ~(1u << slot)) | (phys >= 0 ? 1u << slot : 0u);
+    const uint64_t ph = static_cast<uint32_t>(phys >= 0 ? phys : 0);
+    lds_t *dst = lds + slot * W::SLOT_BYTES;
+    Offsets off = off0;
+    if constexpr (D == 256) {
+      // Formed anew for each page: kept, these four are what is too many for
+      // the registers.
+      int l = lane;
+      asm volatile("" : "+v"(l));
+      off = offsets(l);
     }
-    const v4i bias = {kScoreBias, kScoreBias, kScoreBias, kScoreBias};
-    const v8h ones = {1, 1, 1, 1, 1, 1, 1, 1};
+#pragma unroll
+    for (int k = 0; k < W::KPW; ++k) dma16s(kbase + ph * k_ps, off.k[k], dst + (wave * W::KPW + k) * 1024);
+    if (D == 256 || wave < 4) dma16s(vbase + ph * v_ps, off.v, dst + W::V_OFF + vj * 1024);
+    if (D == 256 || wave >= 4) {
+      // D = 128: waves 4 and 7 both fetch k_scale; D = 256: 0 and 3 .. 7.  A page
+      // outside the cache holds no keys: its scores are masked in B, and its
+      // planes are zeros here, so that its V is zeros whatever page 0 holds.
+      lds_t *pdst = pdst0 + slot * W::SLOT_BYTES;
+      dma4s(pbase + ph * p_ps, off.p, phys >= 0 ? pdst : lds + W::PAD_OFF);
+      if (phys < 0) *reinterpret_cast<__attribute__((address_space(3))) float *>(pdst + 4 * lane) = 0.f;
+    }
+  };
 
-    // This wave's share of V16(i): its group's 32-token half of the page, tokens
-    // 32 grp + 4 (wave & 3) + {0..3, 16..19}, byte columns `lane` (D = 256: and
-    // 64 + lane).  A byte holds two dims; as fp16 its low nibble is n 2^-24 and
-    // its high one n 2^-20 (subnormal, exact), so one fma each, rounded once to
-    // fp16, gives (n - zero) scale / 16.  V16 rows are parity * D / 2 + byte
-    // column, a lane's eight tokens a 16-byte chunk.
-    auto convert = [&](int i) {
-      const lds_t *raw = lds + (i % W::SLOTS) * W::SLOT_BYTES;
-      lds_t *dst = lds + W::V16_OFF + (i & 1) * W::V16_BYTES;
-      const int t0 = 32 * grp + 4 * (wave & 3), chunk = 4 * grp + (wave & 3);
-      typedef __attribute__((address_space(3))) const v4f *lv4f;
-      v4f vs[2], vz[2];
+  v4f O[NT][DT];
+  v4f lsum[NT];
+  float m_run[NT], thr[NT];
+  v4i S[NT][4];
+  v8h P[NT][2];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        vs[e] = *reinterpret_cast<lv4f>(raw + W::S_OFF + (kPage + t0 + 16 * e) * 4);
-        vz[e] = *reinterpret_cast<lv4f>(raw + W::S_OFF + (2 * kPage + t0 + 16 * e) * 4);
-      }
+  for (int nt = 0; nt < NT; ++nt) {
+    lsum[nt] = (v4f){0.f, 0.f, 0.f, 0.f};
+    m_run[nt] = -INFINITY;
+    thr[nt] = -INFINITY;
 #pragma unroll
-      for (int c0 = 0; c0 < W::VROW; c0 += kWave) {
-        const int col = c0 + lane;
-        uint32_t byte[8];
-#pragma unroll
-        for (int t = 0; t < 8; ++t)
-          byte[t] = *reinterpret_cast<__attribute__((address_space(3))) const uint8_t *>(
-              raw + W::V_OFF + (t0 + (t < 4 ? t : 12 + t)) * W::VROW + col);
-        v8h even, odd;
-#pragma unroll
-        for (int t = 0; t < 8; ++t) {
-          const float s = vs[t >> 2][t & 3], c = vz[t >> 2][t & 3] * (s * -0.0625f);
-          const _Float16 lo = __builtin_bit_cast(_Float16, static_cast<uint16_t>(byte[t] & 0x0Fu));
-          const _Float16 hi = __builtin_bit_cast(_Float16, static_cast<uint16_t>(byte[t] & 0xF0u));
-          even[t] = static_cast<_Float16>(fmaf(static_cast<float>(lo), s * 0x1p20f, c));
-          odd[t] = static_cast<_Float16>(fmaf(static_cast<float>(hi), s * 0x1p16f, c));
-        }
-        const int pos = 16 * (chunk ^ vswz(col));
-        *reinterpret_cast<__attribute__((address_space(3))) v8h *>(dst + col * 128 + pos) = even;
-        *reinterpret_cast<__attribute__((address_space(3))) v8h *>(dst + (W::VROW + col) * 128 + pos) = odd;
-      }
-    };
+    for (int j = 0; j < DT; ++j) O[nt][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+  }
+  const v4i bias = {kScoreBias, kScoreBias, kScoreBias, kScoreBias};
+  const v8h ones = {1, 1, 1, 1, 1, 1, 1, 1};
 
-    // Phase A: O += V(i)^T P and the row sums with it, S = K(i + 1) Q^T, in steps
-    // of one operand (16 bytes a lane) and the NT products that use it.  Operands
-    // are read AHEAD steps before their use (an LDS round trip takes about as
-    // long as eight products), one step's code fenced off from the next.
-    constexpr int NV = 2 * DT, NK = 4 * KS, AHEAD = K8V4_AHEAD;
-    auto phase_a = [&](int i, auto with_v) {
-      constexpr int FIRST = decltype(with_v)::value ? 0 : NV, LAST = NV + NK;
-      const lds_t *vsrc = lds + W::V16_OFF + (i & 1) * W::V16_BYTES;
-      const lds_t *raw = lds + ((i + 1) % W::SLOTS) * W::SLOT_BYTES;
-      auto operand = [&](int x) -> v4i {
-        if (x < NV) {
-          // Tile j: dims 32 (j / 2) + 2 n' + j % 2 for n' = 0..15, tokens 32 s + ...
-          const int s = x / DT, j = x % DT, c = 16 * (j >> 1) + n;
-          return *reinterpret_cast<__attribute__((address_space(3))) const v4i *>(
-              vsrc + ((j & 1) * W::VROW + c) * 128 + 16 * ((4 * s + g) ^ vswz(c)));
-        }
-        const int ml = (x - NV) / KS, ks = (x - NV) % KS, t = 16 * ml + n;
-        return *reinterpret_cast<__attribute__((address_space(3))) const v4i *>(raw + t * D + 16 * ((4 * ks + g) ^ kswz<D>(t)));
-      };
-      v4i ring[AHEAD];
+  // This wave's share of V16(i): its group's 32-token half of the page, tokens
+  // 32 grp + 4 (wave & 3) + {0..3, 16..19}, byte columns `lane` (D = 256: and
+  // 64 + lane).  A byte holds two dims; as fp16 its low nibble is n 2^-24 and
+  // its high one n 2^-20 (subnormal, exact), so one fma each, rounded once to
+  // fp16, gives (n - zero) scale / 16.  V16 rows are parity * D / 2 + byte
+  // column, a lane's eight tokens a 16-byte chunk.
+  auto convert = [&](int i) {
+    const lds_t *raw = lds + (i % W::SLOTS) * W::SLOT_BYTES;
+    lds_t *dst = lds + W::V16_OFF + (i & 1) * W::V16_BYTES;
+    const int t0 = 32 * grp + 4 * (wave & 3), chunk = 4 * grp + (wave & 3);
+    typedef __attribute__((address_space(3))) const v4f *lv4f;
+    v4f vs[2], vz[2];
 #pragma unroll
-      for (int x = 0; x < AHEAD; ++x) ring[x] = operand(FIRST + x);
+    for (int e = 0; e < 2; ++e) {
+      vs[e] = *reinterpret_cast<lv4f>(raw + W::S_OFF + (kPage + t0 + 16 * e) * 4);
+      vz[e] = *reinterpret_cast<lv4f>(raw + W::S_OFF + (2 * kPage + t0 + 16 * e) * 4);
+    }
 #pragma unroll
-      for (int x = FIRST; x < LAST; ++x) {
-        const int k = x - FIRST;
-        const v4i f = ring[k % AHEAD];
-        if (x + AHEAD < LAST) ring[k % AHEAD] = operand(x + AHEAD);
-        if (x < NV) {
-          const int s = x / DT, j = x % DT;
+    for (int c0 = 0; c0 < W::VROW; c0 += kWave) {
+      const int col = c0 + lane;
+      uint32_t byte[8];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            O[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, f), P[nt][s], O[nt][j], 0, 0, 0);
-          if (j == DT - 1) {
+      for (int t = 0; t < 8; ++t)
+        byte[t] = *reinterpret_cast<__attribute__((address_space(3))) const uint8_t *>(
+            raw + W::V_OFF + (t0 + (t < 4 ? t : 12 + t)) * W::VROW + col);
+      v8h even, odd;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) lsum[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, P[nt][s], lsum[nt], 0, 0, 0);
-          }
-        } else {
-          const int ml = (x - NV) / KS, ks = (x - NV) % KS;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            S[nt][ml] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, qf[nt][ks], ks ? S[nt][ml] : bias, 0, 0, 0);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+      for (int t = 0; t < 8; ++t) {
+        const float s = vs[t >> 2][t & 3], c = vz[t >> 2][t & 3] * (s * -0.0625f);
+        const _Float16 lo = __builtin_bit_cast(_Float16, static_cast<uint16_t>(byte[t] & 0x0Fu));
+        const _Float16 hi = __builtin_bit_cast(_Float16, static_cast<uint16_t>(byte[t] & 0xF0u));
+        even[t] = static_cast<_Float16>(fmaf(static_cast<float>(lo), s * 0x1p20f, c));
+        odd[t] = static_cast<_Float16>(fmaf(static_cast<float>(hi), s * 0x1p16f, c));
       }
+      const int pos = 16 * (chunk ^ vswz(col));
+      *reinterpret_cast<__attribute__((address_space(3))) v8h *>(dst + col * 128 + pos) = even;
+      *reinterpret_cast<__attribute__((address_space(3))) v8h *>(dst + (W::VROW + col) * 128 + pos) = odd;
+    }
+  };
+
+  // Phase A: O += V(i)^T P and the row sums with it, S = K(i + 1) Q^T, in steps
+  // of one operand (16 bytes a lane) and the NT products that use it.  Operands
+  // are read AHEAD steps before their use (an LDS round trip takes about as
+  // long as eight products), one step's code fenced off from the next.
+  constexpr int NV = 2 * DT, NK = 4 * KS, AHEAD = D == 128 ? 6 : 4;
+  auto phase_a = [&](int i, auto with_v) {
+    constexpr int FIRST = decltype(with_v)::value ? 0 : NV, LAST = NV + NK;
+    const lds_t *vsrc = lds + W::V16_OFF + (i & 1) * W::V16_BYTES;
+    const lds_t *raw = lds + ((i + 1) % W::SLOTS) * W::SLOT_BYTES;
+    auto operand = [&](int x) -> v4i {
+      if (x < NV) {
+        // Tile j: dims 32 (j / 2) + 2 n' + j % 2 for n' = 0..15, tokens 32 s + ...
+        const int s = x / DT, j = x % DT, c = 16 * (j >> 1) + n;
+        return *reinterpret_cast<__attribute__((address_space(3))) const v4i *>(
+            vsrc + ((j & 1) * W::VROW + c) * 128 + 16 * ((4 * s + g) ^ vswz(c)));
+      }
+      const int ml = (x - NV) / KS, ks = (x - NV) % KS, t = 16 * ml + n;
+      return *reinterpret_cast<__attribute__((address_space(3))) const v4i *>(raw + t * D + 16 * ((4 * ks + g) ^ kswz<D>(t)));
     };
-    // P = exp2(score - m - 2) of page i, see chunk_softmax_pv in decode_chunk.h.
-    auto softmax = [&](int i, bool there) {
-      const lds_t *src = lds + (i % W::SLOTS) * W::SLOT_BYTES + W::S_OFF;
-      typedef __attribute__((address_space(3))) const v4f *lv4f;
-      float t[NT][4][4], mx[NT];
-      const int tbase = (p0 + i) * kPage;
-      const bool masked = !there || tbase + kPage > min_end;
-      const int seen_to = there ? INT32_MAX : 0;
+    v4i ring[AHEAD];
 #pragma unroll
-      for (int ml = 0; ml < 4; ++ml) {
-        const v4f ks = *reinterpret_cast<lv4f>(src + (16 * ml + 4 * g) * 4);
+    for (int x = 0; x < AHEAD; ++x) ring[x] = operand(FIRST + x);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float kb = -12582912.0f * ks[e];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) t[nt][ml][e] = fmaf(__int_as_float(S[nt][ml][e]), ks[e], kb);
-        }
-      }
-      if (__builtin_expect(masked, 0)) {
+    for (int x = FIRST; x < LAST; ++x) {
+      const int k = x - FIRST;
+      const v4i f = ring[k % AHEAD];
+      if (x + AHEAD < LAST) ring[k % AHEAD] = operand(x + AHEAD);
+      if (x < NV) {
+        const int s = x / DT, j = x % DT;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
+          O[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, f), P[nt][s], O[nt][j], 0, 0, 0);
+        if (j == DT - 1) {
 #pragma unroll
-          for (int ml = 0; ml < 4; ++ml)
+          for (int nt = 0; nt < NT; ++nt) lsum[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, P[nt][s], lsum[nt], 0, 0, 0);
+        }
+      } else {
+        const int ml = (x - NV) / KS, ks = (x - NV) % KS;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (tbase + 16 * ml + 4 * g + e >= min(lim[nt], seen_to)) t[nt][ml][e] = -INFINITY;
+        for (int nt = 0; nt < NT; ++nt)
+          S[nt][ml] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, qf[nt][ks], ks ? S[nt][ml] : bias, 0, 0, 0);
       }
-      bool grow = false;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // P = exp2(score - m - 2) of page i, see chunk_softmax_pv in decode_chunk.h.
+  auto softmax = [&](int i, bool there) {
+    const lds_t *src = lds + (i % W::SLOTS) * W::SLOT_BYTES + W::S_OFF;
+    typedef __attribute__((address_space(3))) const v4f *lv4f;
+    float t[NT][4][4], mx[NT];
+    const int tbase = (p0 + i) * kPage;
+    const bool masked = !there || tbase + kPage > min_end;
+    const int seen_to = there ? INT32_MAX : 0;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float x = -INFINITY;
+    for (int ml = 0; ml < 4; ++ml) {
+      const v4f ks = *reinterpret_cast<lv4f>(src + (16 * ml + 4 * g) * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float kb = -12582912.0f * ks[e];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) t[nt][ml][e] = fmaf(__int_as_float(S[nt][ml][e]), ks[e], kb);
+      }
+    }
+    if (__builtin_expect(masked, 0)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int ml = 0; ml < 4; ++ml)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x = fmaxf(x, t[nt][ml][e]);
-        mx[nt] = x;
-        grow |= x > thr[nt];
-      }
-      if (__ballot(grow)) {
+          for (int e = 0; e < 4; ++e)
+            if (tbase + 16 * ml + 4 * g + e >= min(lim[nt], seen_to)) t[nt][ml][e] = -INFINITY;
+    }
+    bool grow = false;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const float mnew = fmaxf(m_run[nt], xlane_max16_32(mx[nt]) * crow[nt]);
-          const float alpha = m_run[nt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[nt] - mnew);
-          m_run[nt] = mnew;
-          thr[nt] = (mnew + kRescaleThreshold) / crow[nt];
-          lsum[nt] *= alpha;
+    for (int nt = 0; nt < NT; ++nt) {
+      float x = -INFINITY;
 #pragma unroll
-          for (int j = 0; j < DT; ++j) O[nt][j] *= alpha;
-        }
-      }
+      for (int ml = 0; ml < 4; ++ml)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x = fmaxf(x, t[nt][ml][e]);
+      mx[nt] = x;
+      grow |= x > thr[nt];
+    }
+    if (__ballot(grow)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float nm = -fmaxf(m_run[nt], -FLT_MAX) - kPLog2Offset;
+        const float mnew = fmaxf(m_run[nt], xlane_max16_32(mx[nt]) * crow[nt]);
+        const float alpha = m_run[nt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[nt] - mnew);
+        m_run[nt] = mnew;
+        thr[nt] = (mnew + kRescaleThreshold) / crow[nt];
+        lsum[nt] *= alpha;
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          float p[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            p[e] = __builtin_amdgcn_exp2f(fmaf(t[nt][2 * s + (e >> 2)][e & 3], crow[nt], nm));
-          const v2h a0 = pack_h2(p[0], p[1]), a1 = pack_h2(p[2], p[3]), a2 = pack_h2(p[4], p[5]), a3 = pack_h2(p[6], p[7]);
-          P[nt][s] = (v8h){a0[0], a0[1], a1[0], a1[1], a2[0], a2[1], a3[0], a3[1]};
-        }
-      }
-    };
-    // Ends a phase.  Before an even phase t = 2q the raw page q has to be there:
-    // `left` of this wave's loads may still be under way.
-    auto end_phase = [&](bool before_even, int left) {
-      if (before_even) {
-        if (left == 2)
-          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * W::LOADS) : "memory");
-        else if (left == 1)
-          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(W::LOADS) : "memory");
-        else
-          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");  // no LDS access moves over the barrier
-      __builtin_amdgcn_sched_barrier(0);
-    };
-
-    // The query words are used here, so that the compiler's wait for them does
-    // not fall behind the page loads it does not count.
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) asm volatile("" ::"v"(qf[nt][ks]));
-#pragma unroll
-    for (int i = 0; i < W::SLOTS - 1; ++i) issue(i);
-    end_phase(true, W::SLOTS - 2);
-    if (grp) {  // group 1 sits out phase 0
-      convert(0);
-      end_phase(false, 0);
-    }
-    // Before phase 2q group 0 has issued up to page q + SLOTS - 2 (in B(q - 1))
-    // and group 1 up to the one before.
-    auto run = [&](auto compute) {
-      constexpr bool C = decltype(compute)::value;
-      if constexpr (C) phase_a(-1, std::false_type{});
-      end_phase(grp, W::SLOTS - 3);
-      for (int i = 0; i < pages; ++i) {
-        // Phase B(i): group 0 is one page behind group 1 in dequantizing.
-        const bool there = (valid >> (i % W::SLOTS)) & 1u;
-        issue(i + W::SLOTS - 1);
-        if constexpr (C) softmax(i, there);
-        if constexpr (C && D == 256) {
-          // The probabilities first: beside the dequantization's words their
-          // scores are more than the registers hold.
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) asm volatile("" : "+v"(P[nt][0]), "+v"(P[nt][1]));
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        convert(i + grp);
-        end_phase(!grp, W::SLOTS - 2);
-        // Phase A(i + 1); behind the last page its scores are of no page and not used.
-        if constexpr (C) phase_a(i, std::true_type{});
-        end_phase(grp, W::SLOTS - 3);
-      }
-    };
-    // Waves whose rows lie behind the batch's only move and dequantize pages.
-    if (active)
-      run(std::true_type{});
-    else
-      run(std::false_type{});
-    if (!grp) end_phase(false, 0);
-
-    // The state, as in the kernel above: a quarter of O / l (O is a sixteenth),
-    // then m and l; lane (n, g) holds dims 32 q + 8 g .. + 7 of row n.
-    if (active) {
-      char *state = a.ws + static_cast<int64_t>(wg + seg) * a.prefix_bytes;
-      float2 *ml = reinterpret_cast<float2 *>(state + static_cast<int64_t>(W::ROWS) * D * 2);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int lr = wave * 16 * NT + 16 * nt + n;
-        if (row0 + 16 * nt + n < nrows) {
-          const bool seen = lim[nt] > 0 && m_run[nt] != -INFINITY;
-          const float l = seen ? lsum[nt][0] : 0.f;
-          const float f = l > 0.f ? 4.f / l : 0.f;
-          _Float16 *dst = reinterpret_cast<_Float16 *>(state) + static_cast<int64_t>(lr) * D + 8 * g;
-#pragma unroll
-          for (int q = 0; q < DT / 2; ++q) {
-            v8h o;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              o[2 * e] = static_cast<_Float16>(seen ? O[nt][2 * q][e] * f : 0.f);
-              o[2 * e + 1] = static_cast<_Float16>(seen ? O[nt][2 * q + 1][e] * f : 0.f);
-            }
-            store_wt16(dst + 32 * q, o);
-          }
-          if (g == 0) store_wt8(ml + lr, make_float2(seen ? m_run[nt] : -INFINITY, l));
-        }
+        for (int j = 0; j < DT; ++j) O[nt][j] *= alpha;
       }
     }
-    // The next piece's loads overwrite the LDS and count from zero.
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __syncthreads();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float nm = -fmaxf(m_run[nt], -FLT_MAX) - kPLog2Offset;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          p[e] = __builtin_amdgcn_exp2f(fmaf(t[nt][2 * s + (e >> 2)][e & 3], crow[nt], nm));
+        const v2h a0 = pack_h2(p[0], p[1]), a1 = pack_h2(p[2], p[3]), a2 = pack_h2(p[4], p[5]), a3 = pack_h2(p[6], p[7]);
+        P[nt][s] = (v8h){a0[0], a0[1], a1[0], a1[1], a2[0], a2[1], a3[0], a3[1]};
+      }
+    }
+  };
+  // Ends a phase.  Before an even phase t = 2q the raw page q has to be there:
+  // `left` of this wave's loads may still be under way.
+  auto end_phase = [&](bool before_even, int left) {
+    if (before_even) {
+      if (left == 2)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * W::LOADS) : "memory");
+      else if (left == 1)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(W::LOADS) : "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");  // no LDS access moves over the barrier
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  // The query words are used here, so that the compiler's wait for them does
+  // not fall behind the page loads it does not count.
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" ::"v"(qf[nt][ks]));
+#pragma unroll
+  for (int i = 0; i < W::SLOTS - 1; ++i) issue(i);
+  end_phase(true, W::SLOTS - 2);
+  if (grp) {  // group 1 sits out phase 0
+    convert(0);
+    end_phase(false, 0);
   }
+  // Before phase 2q group 0 has issued up to page q + SLOTS - 2 (in B(q - 1))
+  // and group 1 up to the one before.
+  auto run = [&](auto compute) {
+    constexpr bool C = decltype(compute)::value;
+    if constexpr (C) phase_a(-1, std::false_type{});
+    end_phase(grp, W::SLOTS - 3);
+    for (int i = 0; i < pages; ++i) {
+      // Phase B(i): group 0 is one page behind group 1 in dequantizing.
+      const bool there = (valid >> (i % W::SLOTS)) & 1u;
+      issue(i + W::SLOTS - 1);
+      if constexpr (C) softmax(i, there);
+      if constexpr (C && D == 256) {
+        // The probabilities first: beside the dequantization's words their
+        // scores are more than the registers hold.
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) asm volatile("" : "+v"(P[nt][0]), "+v"(P[nt][1]));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      convert(i + grp);
+      end_phase(!grp, W::SLOTS - 2);
+      // Phase A(i + 1); behind the last page its scores are of no page and not used.
+      if constexpr (C) phase_a(i, std::true_type{});
+      end_phase(grp, W::SLOTS - 3);
+    }
+  };
+  // Waves whose rows lie behind the batch's only move and dequantize pages.
+  if (active)
+    run(std::true_type{});
+  else
+    run(std::false_type{});
+  if (!grp) end_phase(false, 0);
+
+  // The state, as in the kernel above: a quarter of O / l (O is a sixteenth),
+  // then m and l; lane (n, g) holds dims 32 q + 8 g .. + 7 of row n.
+  if (active) {
+    char *state = a.ws + static_cast<int64_t>(wg + seg) * a.prefix_bytes;
+    float2 *ml = reinterpret_cast<float2 *>(state + static_cast<int64_t>(W::ROWS) * D * 2);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int lr = wave * 16 * NT + 16 * nt + n;
+      if (row0 + 16 * nt + n < nrows) {
+        const bool seen = lim[nt] > 0 && m_run[nt] != -INFINITY;
+        const float l = seen ? lsum[nt][0] : 0.f;
+        const float f = l > 0.f ? 4.f / l : 0.f;
+        _Float16 *dst = reinterpret_cast<_Float16 *>(state) + static_cast<int64_t>(lr) * D + 8 * g;
+#pragma unroll
+        for (int q = 0; q < DT / 2; ++q) {
+          v8h o;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            o[2 * e] = static_cast<_Float16>(seen ? O[nt][2 * q][e] * f : 0.f);
+            o[2 * e + 1] = static_cast<_Float16>(seen ? O[nt][2 * q + 1][e] * f : 0.f);
+          }
+          store_wt16(dst + 32 * q, o);
+        }
+        if (g == 0) store_wt8(ml + lr, make_float2(seen ? m_run[nt] : -INFINITY, l));
+      }
+    }
+  }
+  // The next piece's loads overwrite the LDS and count from zero.
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
+// The many-rows form of the whole launch: the prefix's segments (KV heads x row
+// blocks) by wide_piece, the sequences' own by attend_piece on the same axis.
+template <int D, int HKV, int NT>
+__global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_per_eu(2, 2)))
+void shared_wide_kernel(SharedArgs args) {
+  constexpr bool PH = D == 256;
+  constexpr int WAVE_HEADS = PH ? 2 * HKV : HKV, NWH = WAVE_HEADS == 8 ? 1 : 2;
+  constexpr int OWN_LDS = SplitConfig<128, NT, WAVE_HEADS, NWH, PH>::LDS_BYTES;
+  __shared__ __attribute__((aligned(16))) char lds[OWN_LDS > Wide<D>::LDS_BYTES ? OWN_LDS : Wide<D>::LDS_BYTES];
+  const int wg = static_cast<int>(blockIdx.x);
+  walk_pieces(args, wg, [&](const SharedArgs &a, int tid, int seg, int s0, int s1) {
+    if (seg < a.groups)
+      wide_piece<D, HKV>(a, lds, tid, wg, seg, s0, s1);
+    else
+      attend_piece<NT, WAVE_HEADS, NWH, PH, false, kWideWaves>(a, lds, tid, wg, seg, s0, s1);
+  });
 }
 
 // Folds the states of one column slice of one output row (token, query head):
@@ -967,7 +1001,14 @@ __global__ __launch_bounds__(TPU) void shared_merge_kernel(SharedArgs a) {
   const Axis ax = plan_axis(a, lane, b);
   // Pieces of the row's prefix segment and of its own one.
   int pf = 0, pn = 0, of = 0, on = 0;
-  const int ps = tok / kGroup, sub = j / kGroup;
+  const int sub = j / kGroup;
+  int ps = tok / kGroup;                                      // prefix segment
+  int pr = h * a.prefix_rows + (tok - ps * kGroup) * kGqa + i6;  // the row in its states
+  if (a.wide_blocks) {
+    const int r = tok * kGqa + i6, block = r / Wide<D>::ROWS;
+    ps = h * a.wide_blocks + block;
+    pr = r - block * Wide<D>::ROWS;
+  }
   const int os = b * a.per_seq + sub;
   if (a.groups) {
     const int first = ps * prefix_cost(a) + kPieceCost;
@@ -982,23 +1023,10 @@ __global__ __launch_bounds__(TPU) void shared_merge_kernel(SharedArgs a) {
     on = (first + pages - 1) / ax.unit - of + 1;
   }
   const int dcol = 8 * (slice * VPR + col);
-  int pr = h * a.prefix_rows + (tok - ps * kGroup) * kGqa + i6;
-  int64_t pml = static_cast<int64_t>(a.hkv) * a.prefix_rows * D * 2;
-  const char *pbase = piece_state(a, pf, ps), *obase = piece_state(a, of, a.groups + os);
-  if (a.wide_segments) {
-    const int cost = a.prefix_pages + kWideCost;
-    const int unit_pages = (a.wide_segments * cost + a.wide_grid - 1) / a.wide_grid;
-    const int r = tok * kGqa + i6, block = r / Wide<D>::ROWS, seg = h * a.wide_blocks + block;
-    const int first = seg * cost + kWideCost;
-    pf = first / unit_pages;
-    pn = (first + a.prefix_pages - 1) / unit_pages - pf + 1;
-    pr = r - block * Wide<D>::ROWS;
-    pml = static_cast<int64_t>(Wide<D>::ROWS) * D * 2;
-    pbase = a.ws + static_cast<int64_t>(pf + seg) * a.prefix_bytes;
-  }
   const int orow = h * a.own_rows + (j - sub * kGroup) * kGqa + i6;
+  const char *pbase = piece_state(a, pf, ps), *obase = piece_state(a, of, a.groups + os);
   const int64_t p_o = (static_cast<int64_t>(pr) * D + dcol) * 2;
-  const int64_t p_ml = pml + pr * 8;
+  const int64_t p_ml = static_cast<int64_t>(a.wide_blocks ? 1 : a.hkv) * a.prefix_rows * D * 2 + pr * 8;
   const int64_t o_o = (static_cast<int64_t>(orow) * D + dcol) * 2;
   const int64_t o_ml = static_cast<int64_t>(a.hkv) * a.own_rows * D * 2 + orow * 8;
 
@@ -1083,62 +1111,79 @@ void launch_split(const SharedArgs &a, int tiles, hipStream_t s) {
     shared_split_kernel<3, HKV, NWH, PH><<<grid, block, 0, s>>>(a);
 }
 
+template <int D, int HKV>
+void launch_wide(const SharedArgs &a, int tiles, hipStream_t s) {
+  const dim3 grid(a.grid), block(64 * kWideWaves);
+  if (tiles == 1)
+    shared_wide_kernel<D, HKV, 1><<<grid, block, 0, s>>>(a);
+  else if (tiles == 2)
+    shared_wide_kernel<D, HKV, 2><<<grid, block, 0, s>>>(a);
+  else
+    shared_wide_kernel<D, HKV, 3><<<grid, block, 0, s>>>(a);
+}
+
+// Which form serves a prefix of `pages` pages for `rows` query rows of a KV head:
+// the many-rows kernel, or the one that takes eight tokens at a time.  Measured
+// (us, eight tokens at a time / many rows, one token a sequence):
+//   D    heads  pages   8 tokens   16         32         64         128
+//   128  4      8       21 / 17    22 / 17    24 / 21    26 / 30    34 / 36
+//   128  4      2,048   41 / 71    56 / 74    87 / 83    148 / 121  325 / 214
+//   128  2      8       19 / 16    19 / 17    20 / 19    23 / 29    24 / 35
+//   128  2      2,048   33 / 43    41 / 46    55 / 52    86 / 75    148 / 127
+//   256  2      8       23 / 18    21 / 20    24 / 28    27 / 33    34 / 39
+//   256  2      2,048   43 / 54    62 / 58    98 / 79    178 / 132  364 / 204
+//   256  4      8       23 / 19    27 / 21    30 / 29    37 / 34    46 / 40
+//   256  4      2,048   63 / 88    101 / 94   176 / 126  343 / 220  678 / 351
+// Over a long prefix many rows pay as soon as they fill about half the waves;
+// over a short one the many-rows piece is the shorter chain while there are few
+// of them, and with more rows it is each sequence's own pages that count, which
+// it serves with one work-group per CU.
+bool wide_pays(int64_t rows, int64_t pages, int hkv, int head_dim) {
+  if (pages >= 256) return rows >= (head_dim == 128 ? 192 : 96);
+  if (hkv == 4 && head_dim == 256) return true;
+  return rows <= (head_dim == 256 ? 96 : 192);
+}
+
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 
-template <int HKV>
-void launch_wide(const SharedArgs &a, int head_dim, hipStream_t s) {
-  const dim3 grid(a.wide_grid), block(512);
-  if (head_dim == 128)
-    shared_wide_kernel<128, HKV><<<grid, block, 0, s>>>(a);
-  else
-    shared_wide_kernel<256, HKV><<<grid, block, 0, s>>>(a);
-}
-
-// Whether the many-rows kernel serves the prefix for this many query rows.
-bool wide_pays(int64_t rows, int head_dim) {
-  (void)head_dim;
-  return rows >= K8V4_WIDE_MIN;
-}
-
-// What a call of this shape keeps in its workspace: the quantized query rows,
-// their scales, then the states of the prefix's pieces and of the others.
+// What a call keeps in its workspace in one of the two forms: the quantized
+// query rows, their scales, the states of the prefix's pieces and the others'.
 struct SharedShape {
-  int64_t tokens, groups, per_seq, head_rows, grid, wide_grid;
-  int64_t blocks;  // row blocks of the many-rows kernel (0: not used)
+  int64_t tokens, groups, per_seq, head_rows, grid;
+  int64_t blocks;  // row blocks of the many-rows form (0: eight tokens at a time)
   int prefix_rows, own_rows;
   int64_t prefix_bytes, own_bytes;
   int64_t q_bytes, scale_bytes, prefix_state_bytes, own_state_bytes;
+  int64_t bytes() const { return q_bytes + scale_bytes + prefix_state_bytes + own_state_bytes; }
 };
-SharedShape shape_of(int64_t batch, int q_len, int hkv, int head_dim) {
+SharedShape shape_of(bool wide, int64_t batch, int q_len, int hkv, int head_dim) {
   SharedShape s;
   s.tokens = batch * q_len;
-  s.groups = (s.tokens + kGroup - 1) / kGroup;
   s.per_seq = (q_len + kGroup - 1) / kGroup;
-  const int64_t rows = s.tokens * kGqa;
-  // One work-group per CU, two with two 128-dim heads (half the waves).
-  s.grid = static_cast<int64_t>(device_cus()) * (hkv == 2 && head_dim == 128 ? 2 : 1);
-  s.wide_grid = device_cus();
-  const int wide_rows = head_dim == 128 ? Wide<128>::ROWS : Wide<256>::ROWS;
-  s.blocks = wide_pays(rows, head_dim) ? (rows + wide_rows - 1) / wide_rows : 0;
-  // A last segment's tiles (a last block's rows) read rows behind the last token's.
-  s.head_rows = s.blocks * wide_rows > rows + 3 * 16 ? s.blocks * wide_rows : rows + 3 * 16;
+  const int64_t rows = s.tokens * kGqa, state = 2 * head_dim + 8;
+  const int block_rows = head_dim == 128 ? Wide<128>::ROWS : Wide<256>::ROWS;
+  s.blocks = wide ? (rows + block_rows - 1) / block_rows : 0;
+  // One work-group per CU, two of the half-sized ones of two 128-dim heads.
+  s.grid = static_cast<int64_t>(device_cus()) * (hkv == 2 && head_dim == 128 && !wide ? 2 : 1);
   s.own_rows = (q_len < kGroup ? q_len : kGroup) * kGqa;
-  s.own_bytes = static_cast<int64_t>(hkv) * s.own_rows * (2 * head_dim + 8);
-  if (s.blocks) {
-    s.prefix_rows = wide_rows;
-    s.prefix_bytes = static_cast<int64_t>(wide_rows) * (2 * head_dim + 8);
-    s.prefix_state_bytes = (s.wide_grid + hkv * s.blocks) * s.prefix_bytes;
+  s.own_bytes = hkv * s.own_rows * state;
+  if (wide) {
+    s.groups = hkv * s.blocks;
+    s.prefix_rows = block_rows;
+    s.prefix_bytes = block_rows * state;
   } else {
+    s.groups = (s.tokens + kGroup - 1) / kGroup;
     s.prefix_rows = static_cast<int>(s.tokens < kGroup ? s.tokens : kGroup) * kGqa;
-    s.prefix_bytes = static_cast<int64_t>(hkv) * s.prefix_rows * (2 * head_dim + 8);
-    s.prefix_state_bytes = (s.grid + s.groups) * s.prefix_bytes;
+    s.prefix_bytes = hkv * s.prefix_rows * state;
   }
+  // A last segment's tiles, or a last block's rows, read rows behind the last token's.
+  s.head_rows = s.blocks * block_rows > rows + 3 * 16 ? s.blocks * block_rows : rows + 3 * 16;
   s.q_bytes = round256(hkv * s.head_rows * head_dim);
   s.scale_bytes = round256(hkv * s.head_rows * 4);
+  s.prefix_state_bytes = (s.grid + s.groups) * s.prefix_bytes;
   s.own_state_bytes = (s.grid + batch * s.per_seq) * s.own_bytes;
   return s;
 }
-int64_t bytes_of(const SharedShape &s) { return s.q_bytes + s.scale_bytes + s.prefix_state_bytes + s.own_state_bytes; }
 
 constexpr int64_t kMaxBatch = int64_t(1) << 20;
 
@@ -1161,8 +1206,10 @@ extern "C" int64_t k8v4_attn_shared_workspace_bytes(int64_t batch, int q_len, in
   if (batch < 1 || batch > kMaxBatch || q_len < 1 || q_len * kGqa > kPage || !supported_heads(hkv) ||
       !supported_dim(head_dim))
     return -1;
-  const SharedShape s = shape_of(batch, q_len, hkv, head_dim);
-  return bytes_of(s);
+  // Either form, whatever the prefix.
+  const int64_t narrow = shape_of(false, batch, q_len, hkv, head_dim).bytes();
+  const int64_t wide = shape_of(true, batch, q_len, hkv, head_dim).bytes();
+  return narrow > wide ? narrow : wide;
 }
 
 extern "C" int k8v4_attn_shared(const void *q, int q_dtype, int64_t q_tok_stride, const int8_t *k_cache,
@@ -1210,24 +1257,25 @@ extern "C" int k8v4_attn_shared(const void *q, int q_dtype, int64_t q_tok_stride
   K8V4_REQUIRE(aligned(k_scale, 8) && aligned(v_scale, 8) && aligned(v_zero, 8) && ks_page_stride % 8 == 0 &&
                    vs_page_stride % 8 == 0 && vz_page_stride % 8 == 0,
                "scale planes must be 8-byte aligned");
+  for (const int64_t stride : {k_page_stride, ks_page_stride, v_page_stride, vs_page_stride, vz_page_stride})
+    K8V4_REQUIRE(stride >= 0 && stride < (int64_t(1) << 31), "cache page strides must be 0 .. 2^31 - 1 bytes");
   K8V4_REQUIRE(aligned(workspace, 16), "workspace must be 16-byte aligned");
 
-  const SharedShape sh = shape_of(batch, q_len, hkv, head_dim);
-  const int64_t need = bytes_of(sh);
+  const int64_t need = k8v4_attn_shared_workspace_bytes(batch, q_len, hkv, head_dim);
   if (workspace_bytes < need) {
     set_error("shared-prefix workspace holds %lld bytes, the batch needs %lld", static_cast<long long>(workspace_bytes),
               static_cast<long long>(need));
     return K8V4_ERR_WORKSPACE;
   }
+  const bool wide = prefix_pages > 0 && wide_pays(batch * q_len * kGqa, prefix_pages, hkv, head_dim);
+  const SharedShape sh = shape_of(wide, batch, q_len, hkv, head_dim);
   const int64_t table_pages = table_width * pages_per_block;
-  const int64_t blocks = prefix_pages ? sh.blocks : 0;
-  const int64_t groups = prefix_pages && !blocks ? sh.groups : 0;
+  const int64_t groups = prefix_pages ? sh.groups : 0;
   // The axis has at most this many units; a work-group's end may pass it by a
   // work-group's share.
   const int64_t units = groups * (prefix_pages + kPieceCost) +
                         batch * sh.per_seq * ((table_pages > prefix_pages ? table_pages - prefix_pages : 0) + kPieceCost);
-  K8V4_REQUIRE(units < (int64_t(1) << 30) && hkv * blocks * (prefix_pages + kWideCost) < (int64_t(1) << 30),
-               "batch too large for one call");
+  K8V4_REQUIRE(units < (int64_t(1) << 30), "batch too large for one call");
 
   SharedArgs a;
   char *ws = static_cast<char *>(workspace);
@@ -1269,10 +1317,8 @@ extern "C" int k8v4_attn_shared(const void *q, int q_dtype, int64_t q_tok_stride
   a.tokens = static_cast<int>(sh.tokens);
   a.groups = static_cast<int>(groups);
   a.per_seq = static_cast<int>(sh.per_seq);
-  a.wide_blocks = static_cast<int>(blocks);
-  a.wide_segments = static_cast<int>(hkv * blocks);
+  a.wide_blocks = static_cast<int>(sh.blocks);
   a.grid = static_cast<int>(sh.grid);
-  a.wide_grid = static_cast<int>(sh.wide_grid);
   a.ws = ws + sh.q_bytes + sh.scale_bytes;
   a.own_ws = a.ws + sh.prefix_state_bytes;
   a.prefix_rows = sh.prefix_rows;
@@ -1287,7 +1333,7 @@ extern "C" int k8v4_attn_shared(const void *q, int q_dtype, int64_t q_tok_stride
   int tpu = 256;
   {
     const int vpr_max = head_dim / 8;
-    const int64_t avg = blocks ? (sh.wide_grid + hkv * blocks - 1) / (hkv * blocks) + 1 : groups ? (sh.grid + groups - 1) / groups + 1 : (sh.grid + batch - 1) / batch;
+    const int64_t avg = groups ? (sh.grid + groups - 1) / groups + 1 : (sh.grid + batch - 1) / batch;
     int cs = vpr_max / 8;
     bool found = false;
     for (int threads : {128, 256}) {
@@ -1309,17 +1355,21 @@ extern "C" int k8v4_attn_shared(const void *q, int q_dtype, int64_t q_tok_stride
   auto s = static_cast<hipStream_t>(stream);
   int rc = q_rows_launch(q, q_dtype == K8V4_BF16, q_tok_stride, sh.tokens, hkv, head_dim, sh.head_rows, q8, scales, s);
   if (rc) return rc;
-  if (blocks) {
-    if (hkv == 4)
-      launch_wide<4>(a, head_dim, s);
-    else
-      launch_wide<2>(a, head_dim, s);
-    rc = launch_status("k8v4_attn_shared prefix");
-    if (rc) return rc;
-  }
-  const int widest = groups && sh.prefix_rows > sh.own_rows ? sh.prefix_rows : sh.own_rows;
+  const int widest = groups && !sh.blocks && sh.prefix_rows > sh.own_rows ? sh.prefix_rows : sh.own_rows;
   const int tiles = (widest + 15) / 16;
-  if (head_dim == 256) {
+  if (sh.blocks) {
+    if (head_dim == 256) {
+      if (hkv == 4)
+        launch_wide<256, 4>(a, tiles, s);
+      else
+        launch_wide<256, 2>(a, tiles, s);
+    } else {
+      if (hkv == 4)
+        launch_wide<128, 4>(a, tiles, s);
+      else
+        launch_wide<128, 2>(a, tiles, s);
+    }
+  } else if (head_dim == 256) {
     if (hkv == 4)
       launch_split<8, 1, true>(a, tiles, s);
     else
