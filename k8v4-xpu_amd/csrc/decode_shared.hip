@@ -552,14 +552,14 @@ void shared_split_kernel(SharedArgs args) {
 //
 // Waves w and w + 4 share a SIMD.  They form two groups half a page apart,
 // separated by a barrier per phase: in phase A of page p a wave multiplies (O
-// += V(p - 1)^T P(p - 1), S = K(p) Q^T); in phase B it turns S into
-// probabilities, issues its share of a later page's loads and dequantizes its
-// share of V.  So each SIMD holds one wave that
+// += V(p - 1)^T P(p - 1), S = K(p) Q^T) and issues its share of a later page's
+// loads; in phase B it turns S into probabilities and dequantizes its share of V.  So each SIMD holds one wave that
 // feeds the matrix core and one that feeds the vector unit.  With t counting
 // phases, group 0 runs A(p) at t = 2p and B(p) at 2p + 1, group 1 one later:
 //   raw page p (K codes, V codes, planes): read from t = 2p (A of group 0) to
-//     2p + 2 (B of group 1); each wave issues its loads of page p + SLOTS - 1,
-//     into the slot of page p - 1, in B(p);
+//     2p + 1 (B of group 0 dequantizes its half; the key scales, to 2p + 2, lie
+//     apart); a wave issues its loads of page
+//     p + SLOTS - 1, into the slot of page p - 1, in A(p);
 //   V16(p): written at 2p (group 1's half) and 2p + 1, read at 2p + 2 and 2p + 3:
 //     two buffers.
 // Products are transposed (tokens x rows, dims x rows): a lane owns one row of
@@ -575,12 +575,14 @@ struct Wide {
   static constexpr int VROW = D / 2;
   static constexpr int K_BYTES = kPage * D;
   static constexpr int V_OFF = K_BYTES;
-  static constexpr int S_OFF = V_OFF + kPage * VROW;   // ks[64] | vs[64] | vz[64]
-  static constexpr int SLOT_BYTES = S_OFF + 3 * kPage * 4;
+  static constexpr int S_OFF = V_OFF + kPage * VROW;   // vs[64] | vz[64]
+  static constexpr int SLOT_BYTES = S_OFF + 2 * kPage * 4;
   static constexpr int V16_BYTES = D * kPage * 2;      // [D rows][64 tokens]
   static constexpr int V16_OFF = SLOTS * SLOT_BYTES;
   static constexpr int PAD_OFF = V16_OFF + 2 * V16_BYTES;  // where loads nobody reads land
-  static constexpr int LDS_BYTES = PAD_OFF + 256;
+  // Key scales are read last of a page (D = 256: in B): a ring of their own.
+  static constexpr int KS_OFF = PAD_OFF + 256;
+  static constexpr int LDS_BYTES = KS_OFF + 4 * kPage * 4;
   static constexpr int KPW = K_BYTES / 1024 / kWideWaves;  // K loads of a wave: 1, 2
   static constexpr int LOADS = KPW + 1 + (D == 128 ? 0 : 1);  // loads of a wave per page
   static_assert(LDS_BYTES <= 163840, "ring exceeds the LDS");
@@ -672,7 +674,6 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
   // Page strides are below 2^31 bytes, page numbers below 2^31.
   const uint32_t k_ps = static_cast<uint32_t>(a.k_ps), v_ps = static_cast<uint32_t>(a.v_ps);
   const uint32_t p_ps = static_cast<uint32_t>(plane == 1 ? a.vs_ps : plane == 2 ? a.vz_ps : a.ks_ps);
-  lds_t *const pdst0 = lds + W::S_OFF + (plane == 1 || plane == 2 ? plane : 0) * kPage * 4;
   auto issue = [&](int i) {
     if ((i & 63) == 0 && i < pages) load_table(i >> 6);
     const int phys = i < pages ? __builtin_amdgcn_readlane(ptab, i & 63) : -1;
@@ -695,7 +696,7 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
       // D = 128: waves 4 and 7 both fetch k_scale; D = 256: 0 and 3 .. 7.  A page
       // outside the cache holds no keys: its scores are masked in B, and its
       // planes are zeros here, so that its V is zeros whatever page 0 holds.
-      lds_t *pdst = pdst0 + slot * W::SLOT_BYTES;
+      lds_t *pdst = plane == 1 || plane == 2 ? dst + W::S_OFF + (plane - 1) * kPage * 4 : lds + W::KS_OFF + (i & 3) * kPage * 4;
       dma4s(pbase + ph * p_ps, off.p, phys >= 0 ? pdst : lds + W::PAD_OFF);
       if (phys < 0) *reinterpret_cast<__attribute__((address_space(3))) float *>(pdst + 4 * lane) = 0.f;
     }
@@ -723,38 +724,41 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
   // its high one n 2^-20 (subnormal, exact), so one fma each, rounded once to
   // fp16, gives (n - zero) scale / 16.  V16 rows are parity * D / 2 + byte
   // column, a lane's eight tokens a 16-byte chunk.
-  auto convert = [&](int i) {
+  constexpr int COLS = W::VROW / kWave;
+  struct Packed {
+    uint32_t byte[8];
+  };
+  auto fetch = [&](int i, int c) {
     const lds_t *raw = lds + (i % W::SLOTS) * W::SLOT_BYTES;
+    const int t0 = 32 * grp + 4 * (wave & 3);
+    Packed p;
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+      p.byte[t] = *reinterpret_cast<__attribute__((address_space(3))) const uint8_t *>(
+          raw + W::V_OFF + (t0 + (t < 4 ? t : 12 + t)) * W::VROW + c * kWave + lane);
+    return p;
+  };
+  auto convert = [&](int i, int c, const Packed &p) {
+    const lds_t *planes = lds + (i % W::SLOTS) * W::SLOT_BYTES + W::S_OFF + (32 * grp + 4 * (wave & 3)) * 4;
     lds_t *dst = lds + W::V16_OFF + (i & 1) * W::V16_BYTES;
-    const int t0 = 32 * grp + 4 * (wave & 3), chunk = 4 * grp + (wave & 3);
-    typedef __attribute__((address_space(3))) const v4f *lv4f;
-    v4f vs[2], vz[2];
+    v8h even, odd;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      vs[e] = *reinterpret_cast<lv4f>(raw + W::S_OFF + (kPage + t0 + 16 * e) * 4);
-      vz[e] = *reinterpret_cast<lv4f>(raw + W::S_OFF + (2 * kPage + t0 + 16 * e) * 4);
-    }
+      const v4f vs = *reinterpret_cast<__attribute__((address_space(3))) const v4f *>(planes + 64 * e);
+      const v4f vz = *reinterpret_cast<__attribute__((address_space(3))) const v4f *>(planes + kPage * 4 + 64 * e);
 #pragma unroll
-    for (int c0 = 0; c0 < W::VROW; c0 += kWave) {
-      const int col = c0 + lane;
-      uint32_t byte[8];
-#pragma unroll
-      for (int t = 0; t < 8; ++t)
-        byte[t] = *reinterpret_cast<__attribute__((address_space(3))) const uint8_t *>(
-            raw + W::V_OFF + (t0 + (t < 4 ? t : 12 + t)) * W::VROW + col);
-      v8h even, odd;
-#pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        const float s = vs[t >> 2][t & 3], c = vz[t >> 2][t & 3] * (s * -0.0625f);
-        const _Float16 lo = __builtin_bit_cast(_Float16, static_cast<uint16_t>(byte[t] & 0x0Fu));
-        const _Float16 hi = __builtin_bit_cast(_Float16, static_cast<uint16_t>(byte[t] & 0xF0u));
-        even[t] = static_cast<_Float16>(fmaf(static_cast<float>(lo), s * 0x1p20f, c));
-        odd[t] = static_cast<_Float16>(fmaf(static_cast<float>(hi), s * 0x1p16f, c));
+      for (int t = 0; t < 4; ++t) {
+        const uint32_t byte = p.byte[4 * e + t];
+        const float z = vz[t] * (vs[t] * -0.0625f);
+        const _Float16 lo = __builtin_bit_cast(_Float16, static_cast<uint16_t>(byte & 0x0Fu));
+        const _Float16 hi = __builtin_bit_cast(_Float16, static_cast<uint16_t>(byte & 0xF0u));
+        even[4 * e + t] = static_cast<_Float16>(fmaf(static_cast<float>(lo), vs[t] * 0x1p20f, z));
+        odd[4 * e + t] = static_cast<_Float16>(fmaf(static_cast<float>(hi), vs[t] * 0x1p16f, z));
       }
-      const int pos = 16 * (chunk ^ vswz(col));
-      *reinterpret_cast<__attribute__((address_space(3))) v8h *>(dst + col * 128 + pos) = even;
-      *reinterpret_cast<__attribute__((address_space(3))) v8h *>(dst + (W::VROW + col) * 128 + pos) = odd;
     }
+    const int col = c * kWave + lane, pos = 16 * ((4 * grp + (wave & 3)) ^ vswz(col));
+    *reinterpret_cast<__attribute__((address_space(3))) v8h *>(dst + col * 128 + pos) = even;
+    *reinterpret_cast<__attribute__((address_space(3))) v8h *>(dst + (W::VROW + col) * 128 + pos) = odd;
   };
 
   // Phase A: O += V(i)^T P and the row sums with it, S = K(i + 1) Q^T, in steps
@@ -762,6 +766,13 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
   // are read AHEAD steps before their use (an LDS round trip takes about as
   // long as eight products), one step's code fenced off from the next.
   constexpr int NV = 2 * DT, NK = 4 * KS, AHEAD = D == 128 ? 6 : 4;
+  v4f kscale[4];  // of the page whose scores S holds: tokens 16 ml + 4 g ..
+  auto read_kscale = [&](int i) {
+#pragma unroll
+    for (int ml = 0; ml < 4; ++ml)
+      kscale[ml] = *reinterpret_cast<__attribute__((address_space(3))) const v4f *>(
+          lds + W::KS_OFF + ((i & 3) * kPage + 16 * ml + 4 * g) * 4);
+  };
   auto phase_a = [&](int i, auto with_v) {
     constexpr int FIRST = decltype(with_v)::value ? 0 : NV, LAST = NV + NK;
     const lds_t *vsrc = lds + W::V16_OFF + (i & 1) * W::V16_BYTES;
@@ -782,6 +793,10 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
 #pragma unroll
     for (int x = FIRST; x < LAST; ++x) {
       const int k = x - FIRST;
+      // Behind the first products: the loads of a later page, and towards the
+      // end (P's registers are free by then) what phase B needs first.
+      if (k == 1) issue(i + W::SLOTS);
+      if (D == 128 && x == LAST - 6) read_kscale(i + 1);
       const v4i f = ring[k % AHEAD];
       if (x + AHEAD < LAST) ring[k % AHEAD] = operand(x + AHEAD);
       if (x < NV) {
@@ -804,15 +819,14 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
   };
   // P = exp2(score - m - 2) of page i, see chunk_softmax_pv in decode_chunk.h.
   auto softmax = [&](int i, bool there) {
-    const lds_t *src = lds + (i % W::SLOTS) * W::SLOT_BYTES + W::S_OFF;
-    typedef __attribute__((address_space(3))) const v4f *lv4f;
+    if constexpr (D == 256) read_kscale(i);
     float t[NT][4][4], mx[NT];
     const int tbase = (p0 + i) * kPage;
     const bool masked = !there || tbase + kPage > min_end;
     const int seen_to = there ? INT32_MAX : 0;
 #pragma unroll
     for (int ml = 0; ml < 4; ++ml) {
-      const v4f ks = *reinterpret_cast<lv4f>(src + (16 * ml + 4 * g) * 4);
+      const v4f ks = kscale[ml];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float kb = -12582912.0f * ks[e];
@@ -889,36 +903,49 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) asm volatile("" ::"v"(qf[nt][ks]));
+  // Before phase 2q both groups have issued up to page q + SLOTS - 2, in A(q - 1).
 #pragma unroll
   for (int i = 0; i < W::SLOTS - 1; ++i) issue(i);
   end_phase(true, W::SLOTS - 2);
   if (grp) {  // group 1 sits out phase 0
-    convert(0);
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) convert(0, c, fetch(0, c));
     end_phase(false, 0);
   }
-  // Before phase 2q group 0 has issued up to page q + SLOTS - 2 (in B(q - 1))
-  // and group 1 up to the one before.
   auto run = [&](auto compute) {
     constexpr bool C = decltype(compute)::value;
-    if constexpr (C) phase_a(-1, std::false_type{});
-    end_phase(grp, W::SLOTS - 3);
+    if constexpr (C)
+      phase_a(-1, std::false_type{});
+    else
+      issue(W::SLOTS - 1);
+    end_phase(grp, W::SLOTS - 2);
     for (int i = 0; i < pages; ++i) {
       // Phase B(i): group 0 is one page behind group 1 in dequantizing.
       const bool there = (valid >> (i % W::SLOTS)) & 1u;
-      issue(i + W::SLOTS - 1);
-      if constexpr (C) softmax(i, there);
-      if constexpr (C && D == 256) {
-        // The probabilities first: beside the dequantization's words their
-        // scores are more than the registers hold.
+      // What is dequantized is read ahead of the softmax, which hides it (D =
+      // 256: after it, the registers do not hold both).
+      Packed packed;
+      if constexpr (COLS == 1) packed = fetch(i + grp, 0);
+      if constexpr (C) {
+        __builtin_amdgcn_sched_barrier(0);
+        softmax(i, there);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) asm volatile("" : "+v"(P[nt][0]), "+v"(P[nt][1]));
         __builtin_amdgcn_sched_barrier(0);
       }
-      convert(i + grp);
+      if constexpr (COLS == 1) {
+        convert(i + grp, 0, packed);
+      } else {
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) convert(i + grp, c, fetch(i + grp, c));
+      }
       end_phase(!grp, W::SLOTS - 2);
       // Phase A(i + 1); behind the last page its scores are of no page and not used.
-      if constexpr (C) phase_a(i, std::true_type{});
-      end_phase(grp, W::SLOTS - 3);
+      if constexpr (C)
+        phase_a(i, std::true_type{});
+      else
+        issue(i + W::SLOTS);
+      end_phase(grp, W::SLOTS - 2);
     }
   };
   // Waves whose rows lie behind the batch's only move and dequantize pages.
