@@ -1,12 +1,13 @@
 """vLLM attention backend for the K8/V4 cache on MI355X (2 or 4 local KV heads).
 
 This is the caller of the hot path: vLLM owns the block table and the slot
-map; the backend turns one engine step's metadata into the library's three
-entry points (quantize-and-write, batched decode / MTP verify, chunked
-prefill).  The vLLM-facing surface follows the reference backend
-(k8v4_v030/backend.py:56-486): the class names, the metadata fields, the
-constructor and forward signatures, the capture support and the error
-messages callers and tests match.  The implementation is this package's own:
+map; the backend turns one engine step's metadata into the library's entry
+points (quantize-and-write, batched decode / MTP verify, the same over a
+prefix that all requests share, chunked prefill).  The vLLM-facing surface
+follows the reference backend (k8v4_v030/backend.py:56-486): the class names,
+the metadata fields, the constructor and forward signatures, the capture
+support and the error messages callers and tests match.  The implementation is
+this package's own:
 
 * the metadata builder turns ``query_start_loc`` into a step plan once per
   step (decode runs of equal query length, and the prefill sequences), which
@@ -17,6 +18,9 @@ messages callers and tests match.  The implementation is this package's own:
 * decode runs use the scratch's decode workspace and prefill sequences its
   prefill workspace, both allocated before capture (``scratch.py``), so no
   call allocates;
+* where every running request begins with the same cached blocks (vLLM's
+  prefix cache), the builder says when that pays and decode runs read those
+  blocks once for all their requests;
 * a step made only of decode runs of one query length is one launch pair and
   can be captured in a HIP graph; a step with prefill refuses capture.
 """
@@ -43,7 +47,15 @@ from vllm.v1.kv_cache_interface import AttentionSpec
 from .cache_views import bind_regions
 from .layout import CACHE_DTYPE, DECODE_MAX_T, PAGE, PageLayout, attention_pages_per_block
 from .ops_api import ops
-from .plan import layout_for_heads, query_segments, require_decoder, scratch_capacity, token_span, uniform_packed_q_len
+from .plan import (
+    layout_for_heads,
+    query_segments,
+    require_decoder,
+    scratch_capacity,
+    shared_prefix_pays,
+    token_span,
+    uniform_packed_q_len,
+)
 from .scratch import Scratch, ensure_scratch, get_scratch, scratch_ready
 
 logger = init_logger(__name__)
@@ -112,6 +124,7 @@ class Xe2K8V4Metadata(AttentionMetadata):
         pages_per_block: int,
         packed_q_len: int,
         layout: PageLayout,
+        common_prefix_len: int = 0,
     ):
         for name, value in list(locals().items()):
             if name != "self":
@@ -161,18 +174,43 @@ class Xe2K8V4MetadataBuilder(AttentionMetadataBuilder[Xe2K8V4Metadata]):
         )
         return ensure_scratch(self.device, self.layout, *capacity, max_seqs=int(cfg.scheduler_config.max_num_seqs))
 
+    def use_cascade_attention(
+        self,
+        common_prefix_len: int,
+        query_lens,
+        num_query_heads: int = 0,
+        num_kv_heads: int = 0,
+        use_alibi: bool = False,
+        use_sliding_window: bool = False,
+        use_local_attention: bool = False,
+        num_sms: int = 0,
+        dcp_world_size: int = 1,
+        **_: object,
+    ) -> bool:
+        """Whether this step gains from reading the common prefix once: one of its
+        decode runs saves enough of the cache (plan.shared_prefix_pays).  The engine
+        runs such a step outside its captured graphs and passes the prefix to
+        :meth:`build`, 0 otherwise."""
+        if use_alibi or use_sliding_window or use_local_attention or dcp_world_size > 1:
+            return False
+        starts = [0]
+        for n in query_lens:
+            starts.append(starts[-1] + int(n))
+        runs, _seqs = plan_step(tuple(starts)) if len(starts) > 1 else ((), ())
+        return any(shared_prefix_pays(run.count, common_prefix_len, self.layout) for run in runs)
+
     def build(
         self,
         common_prefix_len: int,
         common_attn_metadata: CommonAttentionMetadata,
         fast_build: bool = False,
     ) -> Xe2K8V4Metadata:
-        del common_prefix_len, fast_build
+        del fast_build
         if not scratch_ready(self.device, self.layout):
             self._ensure_scratch()
         cam = common_attn_metadata
         starts = tuple(int(x) for x in cam.query_start_loc_cpu.tolist())
-        return Xe2K8V4Metadata(
+        meta = Xe2K8V4Metadata(
             seq_lens=cam.seq_lens,
             slot_mapping=cam.slot_mapping,
             block_table=cam.block_table_tensor,
@@ -185,7 +223,11 @@ class Xe2K8V4MetadataBuilder(AttentionMetadataBuilder[Xe2K8V4Metadata]):
             pages_per_block=self._pages_per_entry(),
             packed_q_len=uniform_packed_q_len(starts),
             layout=self.layout,
+            common_prefix_len=int(common_prefix_len),
         )
+        if any(_reads_prefix_once(meta, run) for run in meta.decode_runs):
+            get_scratch(self.device, self.layout).shared_ws()  # before the layers run
+        return meta
 
 
 # --------------------------------------------------------------- the layer
@@ -313,6 +355,10 @@ class Xe2K8V4Impl(AttentionImpl[Xe2K8V4Metadata]):
                                % (lens.dtype, tuple(lens.stride())))
         lens = lens.reshape(-1)[run.first : run.first + run.count]
         rows = slice(run.tok0, run.tok0 + width)
+        if _reads_prefix_once(meta, run):
+            ops().int8k_int4v_attn_shared(q[rows], *regions, table[0], meta.common_prefix_len, table, lens,
+                                          scratch.shared_ws(), out[rows], run.q_len, meta.pages_per_block)
+            return
         ops().int8k_int4v_attn_batch(q[rows], None, None, *regions, table, lens, None, scratch.decode_ws,
                                      None, None, None, out[rows], run.q_len, meta.pages_per_block)
 
@@ -350,6 +396,13 @@ class Xe2K8V4Impl(AttentionImpl[Xe2K8V4Metadata]):
 def _runs_alone(width: int, seq_len: int, layout) -> bool:
     _check_covers(seq_len, width)
     return ops().prefill_uses_tiles(seq_len, width, layout.hkv, layout.head_dim)
+
+
+def _reads_prefix_once(meta: Xe2K8V4Metadata, run: DecodeRun) -> bool:
+    """Whether ``run`` reads the step's common prefix once for its requests.  Not
+    while a graph is captured: its replays may be of steps with another prefix,
+    while the tables every request has of its own are right for any step."""
+    return shared_prefix_pays(run.count, meta.common_prefix_len, meta.layout) and not _graph_capturing()
 
 
 def _check_covers(seq_len: int, width: int) -> None:

@@ -73,6 +73,26 @@ def token_span(starts: Sequence[int], first_request: int, count: int, q_len: int
     return t0, t1 - t0
 
 
+# The bytes of cache a batch has to save before a launch over a shared prefix is
+# used.  It costs 2 to 20 us more than the batch op where it saves nothing (a
+# launch more, the sequences' states joined with the prefix's); both ops were
+# timed for 2 .. 64 sequences of 1 and 4 query tokens over prefixes of 4 .. 1024
+# pages, and broke even between 25 MB saved (8 sequences, one query token, head
+# dim 256) and 200 MB (64 sequences of 4, head dim 128, 4 KV heads, 64 pages:
+# 56 us against 58).  From there on the shared form was the faster one at every
+# shape, by up to 8.5 times (64 sequences, 1024 pages, head dim 256: 129 us
+# against 1094).
+SHARED_PREFIX_MIN_SAVED = 192 << 20
+
+
+def shared_prefix_pays(sequences: int, prefix_len: int, layout: PageLayout) -> bool:
+    """Whether ``sequences`` that begin with the same ``prefix_len`` cached tokens are
+    decoded faster by ``int8k_int4v_attn_shared`` than by ``int8k_int4v_attn_batch``
+    (which reads the prefix once for each; the other serves any shape too)."""
+    pages = max(0, int(prefix_len)) // PAGE
+    return (int(sequences) - 1) * pages * layout.page_bytes >= SHARED_PREFIX_MIN_SAVED
+
+
 def scratch_capacity(
     max_model_len: int,
     manager_block: int,

@@ -1,6 +1,6 @@
 """Device buffers the K8/V4 kernels write besides the cache, one set per (device, layout).
 
-The HIP library needs exactly two scratch buffers, both caller-owned so that
+The HIP library needs two scratch buffers, both caller-owned so that
 a captured HIP graph keeps stable addresses and no call allocates:
 
 * the decode workspace -- split-K states of ``k8v4_attn_batch`` (fp16 partial
@@ -12,6 +12,10 @@ a captured HIP graph keeps stable addresses and no call allocates:
   (``k8v4_prefill_workspace_bytes``) for the longest chunk over the longest
   context, and at least what one launch of ``k8v4_prefill_paged_batch``
   (a step's short chunks together) needs.
+
+A third one, the workspace of ``k8v4_attn_shared``, is made the first time a
+step's requests share a prefix worth reading once (engines without prefix
+caching never pay for it).
 
 Capacity is given in the reference's terms (k8v4_v030/scratch.py:17-115):
 ``nprog_max`` = kernel pages of the longest sequence times the KV head count,
@@ -54,6 +58,19 @@ def decode_workspace_bytes(layout: PageLayout, max_pages: int, max_out_tokens: i
     return need
 
 
+def shared_workspace_bytes(layout: PageLayout, max_out_tokens: int, max_seqs: int | None = None) -> int:
+    """Largest workspace of a decode call over a shared prefix, as
+    :func:`decode_workspace_bytes` (the prefix's length does not matter)."""
+    lib = _library_ops()
+    need = 0
+    for q_len in range(1, DECODE_MAX_T + 1):
+        batch = max(1, int(max_out_tokens) // q_len)
+        if max_seqs is not None:
+            batch = max(1, min(batch, int(max_seqs)))
+        need = max(need, lib.attn_shared_workspace_bytes(batch, q_len, layout.hkv, layout.head_dim))
+    return need
+
+
 def prefill_workspace_bytes(layout: PageLayout, max_pages: int, max_chunk: int) -> int:
     """Prefill workspace for a ``max_chunk``-token query over ``max_pages`` pages of
     context, and for a batch of a step's short chunks in one call."""
@@ -93,12 +110,23 @@ class Scratch:
         self.prefill_ws = torch.empty(_words(self.prefill_bytes), dtype=torch.int32, device=self.device)
         # An empty visible_lens tells the decode op to derive causal ends from seq_lens.
         self.visible = torch.empty((0,), dtype=torch.int32, device=self.device)
+        self._shared_ws: torch.Tensor | None = None
         self._legacy: dict[str, torch.Tensor] = {}
 
     @property
     def nbytes(self) -> int:
-        """Device bytes this scratch holds (the two workspaces)."""
-        return 4 * (self.decode_ws.numel() + self.prefill_ws.numel())
+        """Device bytes this scratch holds (the workspaces)."""
+        shared = 0 if self._shared_ws is None else self._shared_ws.numel()
+        return 4 * (self.decode_ws.numel() + self.prefill_ws.numel() + shared)
+
+    def shared_ws(self) -> torch.Tensor:
+        """The workspace of decode calls over a shared prefix, made on the first call."""
+        if self._shared_ws is None:
+            if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("K8/V4 shared-prefix workspace was not allocated before capture")
+            need = shared_workspace_bytes(self.layout, self.max_out_tokens, self.max_seqs)
+            self._shared_ws = torch.empty(_words(need), dtype=torch.int32, device=self.device)
+        return self._shared_ws
 
     def workspace(self, nprog: int) -> tuple[torch.Tensor, None, None, None]:
         """The decode workspace in the reference's ``(partials, m, l, merged)`` slot order.
@@ -201,4 +229,4 @@ def clear_scratch() -> None:
 
 
 __all__ = ["Scratch", "clear_scratch", "decode_workspace_bytes", "ensure_scratch", "get_scratch",
-           "prefill_workspace_bytes", "scratch_key", "scratch_ready"]
+           "prefill_workspace_bytes", "scratch_key", "scratch_ready", "shared_workspace_bytes"]
