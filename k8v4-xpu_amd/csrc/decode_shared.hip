@@ -633,6 +633,13 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
   }
   const int min_end = kFar - wave_max(far);
 
+  // The lane for addresses that, kept over the loop, would be what is too many
+  // for the registers at head dim 256: formed anew where they are used.
+  auto fresh_lane = [&] {
+    int l = lane;
+    if constexpr (D == 256) asm volatile("" : "+v"(l));
+    return l;
+  };
   // Lane offsets of this wave's loads of a page: K rows (swizzled as in
   // lane_offsets), V rows, one cell of a plane.
   const int vj = wave & (kPage * W::VROW / 1024 - 1);  // 1 KB piece of V rows
@@ -681,14 +688,7 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
     valid = (valid & ~(1u << slot)) | (phys >= 0 ? 1u << slot : 0u);
     const uint64_t ph = static_cast<uint32_t>(phys >= 0 ? phys : 0);
     lds_t *dst = lds + slot * W::SLOT_BYTES;
-    Offsets off = off0;
-    if constexpr (D == 256) {
-      // Formed anew for each page: kept, these four are what is too many for
-      // the registers.
-      int l = lane;
-      asm volatile("" : "+v"(l));
-      off = offsets(l);
-    }
+    const Offsets off = D == 128 ? off0 : offsets(fresh_lane());
 #pragma unroll
     for (int k = 0; k < W::KPW; ++k) dma16s(kbase + ph * k_ps, off.k[k], dst + (wave * W::KPW + k) * 1024);
     if (D == 256 || wave < 4) dma16s(vbase + ph * v_ps, off.v, dst + W::V_OFF + vj * 1024);
@@ -718,47 +718,56 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
   const v4i bias = {kScoreBias, kScoreBias, kScoreBias, kScoreBias};
   const v8h ones = {1, 1, 1, 1, 1, 1, 1, 1};
 
-  // This wave's share of V16(i): its group's 32-token half of the page, tokens
-  // 32 grp + 4 (wave & 3) + {0..3, 16..19}, byte columns `lane` (D = 256: and
-  // 64 + lane).  A byte holds two dims; as fp16 its low nibble is n 2^-24 and
-  // its high one n 2^-20 (subnormal, exact), so one fma each, rounded once to
-  // fp16, gives (n - zero) scale / 16.  V16 rows are parity * D / 2 + byte
-  // column, a lane's eight tokens a 16-byte chunk.
-  constexpr int COLS = W::VROW / kWave;
-  struct Packed {
-    uint32_t byte[8];
-  };
-  auto fetch = [&](int i, int c) {
+  // This wave's share of V16(i): tokens 4 wave' + {0..3, 16..19} of its group's
+  // 32-token half of the page, byte columns `lane` (D = 256: and 64 + lane).  A
+  // byte holds two dims; as fp16 its low nibble is n 2^-24 and its high one n
+  // 2^-20 (subnormal, exact), so one fma each, rounded once to fp16, gives (n -
+  // zero) scale / 16.  V16 rows are parity * D / 2 + byte column, a lane's eight
+  // tokens a 16-byte chunk.
+  // In units of one byte column (D = 256: and four tokens, for the registers).
+  // Balanced between the phases: all of it in A, at head dim 256 one unit of four.
+  constexpr int COLS = W::VROW / kWave, TOK = D == 128 ? 8 : 4, UNITS = COLS * 8 / TOK, IN_A = 1;
+  typedef _Float16 vth __attribute__((ext_vector_type(TOK)));
+  uint32_t byte[TOK];
+  v4f vs[TOK / 4], vz[TOK / 4];
+  vth even, odd;
+  auto fetch = [&](int i, int u) __attribute__((always_inline)) {
     const lds_t *raw = lds + (i % W::SLOTS) * W::SLOT_BYTES;
-    const int t0 = 32 * grp + 4 * (wave & 3);
-    Packed p;
+    const int c = u * TOK / 8, e0 = u * TOK % 8 / 4, t0 = 32 * grp + 4 * (wave & 3) + 16 * e0;
+    const int l = fresh_lane();
 #pragma unroll
-    for (int t = 0; t < 8; ++t)
-      p.byte[t] = *reinterpret_cast<__attribute__((address_space(3))) const uint8_t *>(
-          raw + W::V_OFF + (t0 + (t < 4 ? t : 12 + t)) * W::VROW + c * kWave + lane);
-    return p;
-  };
-  auto convert = [&](int i, int c, const Packed &p) {
-    const lds_t *planes = lds + (i % W::SLOTS) * W::SLOT_BYTES + W::S_OFF + (32 * grp + 4 * (wave & 3)) * 4;
-    lds_t *dst = lds + W::V16_OFF + (i & 1) * W::V16_BYTES;
-    v8h even, odd;
+    for (int t = 0; t < TOK; ++t)
+      byte[t] = *reinterpret_cast<__attribute__((address_space(3))) const uint8_t *>(
+          raw + W::V_OFF + (t0 + (t < 4 ? t : 12 + t)) * W::VROW + c * kWave + l);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const v4f vs = *reinterpret_cast<__attribute__((address_space(3))) const v4f *>(planes + 64 * e);
-      const v4f vz = *reinterpret_cast<__attribute__((address_space(3))) const v4f *>(planes + kPage * 4 + 64 * e);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const uint32_t byte = p.byte[4 * e + t];
-        const float z = vz[t] * (vs[t] * -0.0625f);
-        const _Float16 lo = __builtin_bit_cast(_Float16, static_cast<uint16_t>(byte & 0x0Fu));
-        const _Float16 hi = __builtin_bit_cast(_Float16, static_cast<uint16_t>(byte & 0xF0u));
-        even[4 * e + t] = static_cast<_Float16>(fmaf(static_cast<float>(lo), vs[t] * 0x1p20f, z));
-        odd[4 * e + t] = static_cast<_Float16>(fmaf(static_cast<float>(hi), vs[t] * 0x1p16f, z));
-      }
+    for (int e = 0; e < TOK / 4; ++e) {
+      vs[e] = *reinterpret_cast<__attribute__((address_space(3))) const v4f *>(raw + W::S_OFF + (t0 + 16 * e) * 4);
+      vz[e] = *reinterpret_cast<__attribute__((address_space(3))) const v4f *>(raw + W::S_OFF + (kPage + t0 + 16 * e) * 4);
     }
-    const int col = c * kWave + lane, pos = 16 * ((4 * grp + (wave & 3)) ^ vswz(col));
-    *reinterpret_cast<__attribute__((address_space(3))) v8h *>(dst + col * 128 + pos) = even;
-    *reinterpret_cast<__attribute__((address_space(3))) v8h *>(dst + (W::VROW + col) * 128 + pos) = odd;
+  };
+  auto dequantize = [&](int t) __attribute__((always_inline)) {
+    const float s = vs[t >> 2][t & 3], z = vz[t >> 2][t & 3] * (s * -0.0625f);
+    const _Float16 lo = __builtin_bit_cast(_Float16, static_cast<uint16_t>(byte[t] & 0x0Fu));
+    const _Float16 hi = __builtin_bit_cast(_Float16, static_cast<uint16_t>(byte[t] & 0xF0u));
+    even[t] = static_cast<_Float16>(fmaf(static_cast<float>(lo), s * 0x1p20f, z));
+    odd[t] = static_cast<_Float16>(fmaf(static_cast<float>(hi), s * 0x1p16f, z));
+  };
+  auto put = [&](int i, int u) __attribute__((always_inline)) {
+    lds_t *dst = lds + W::V16_OFF + (i & 1) * W::V16_BYTES;
+    const int col = u * TOK / 8 * kWave + fresh_lane();
+    const int pos = 16 * ((4 * grp + (wave & 3)) ^ vswz(col)) + 2 * (u * TOK % 8);
+    *reinterpret_cast<__attribute__((address_space(3))) vth *>(dst + col * 128 + pos) = even;
+    *reinterpret_cast<__attribute__((address_space(3))) vth *>(dst + (W::VROW + col) * 128 + pos) = odd;
+  };
+  auto convert = [&](int i, auto in_a) __attribute__((always_inline)) {
+    constexpr int U0 = decltype(in_a)::value ? 0 : IN_A, U1 = decltype(in_a)::value ? IN_A : UNITS;
+#pragma unroll
+    for (int u = U0; u < U1; ++u) {
+      fetch(i, u);
+#pragma unroll
+      for (int t = 0; t < TOK; ++t) dequantize(t);
+      put(i, u);
+    }
   };
 
   // Phase A: O += V(i)^T P and the row sums with it, S = K(i + 1) Q^T, in steps
@@ -773,7 +782,8 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
       kscale[ml] = *reinterpret_cast<__attribute__((address_space(3))) const v4f *>(
           lds + W::KS_OFF + ((i & 3) * kPage + 16 * ml + 4 * g) * 4);
   };
-  auto phase_a = [&](int i, auto with_v) {
+  auto phase_a = [&](int i, auto with_v) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_setprio(1);  // the products first, phase B in their gaps
     constexpr int FIRST = decltype(with_v)::value ? 0 : NV, LAST = NV + NK;
     const lds_t *vsrc = lds + W::V16_OFF + (i & 1) * W::V16_BYTES;
     const lds_t *raw = lds + ((i + 1) % W::SLOTS) * W::SLOT_BYTES;
@@ -790,12 +800,21 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
     v4i ring[AHEAD];
 #pragma unroll
     for (int x = 0; x < AHEAD; ++x) ring[x] = operand(FIRST + x);
+    __builtin_amdgcn_sched_barrier(0);
+    issue(i + W::SLOTS);
+    if constexpr (FIRST != 0) convert(i + 1, std::true_type{});
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int x = FIRST; x < LAST; ++x) {
       const int k = x - FIRST;
-      // Behind the first products: the loads of a later page, and towards the
-      // end (P's registers are free by then) what phase B needs first.
-      if (k == 1) issue(i + W::SLOTS);
+      // Between the products, while S is not yet needed: page i + 1 dequantized;
+      // towards the end (P's registers are free by then) what phase B needs first.
+      if constexpr (FIRST == 0) {
+        constexpr int FROM = 3;
+        if (k == 1) fetch(i + 1, 0);
+        if (k >= FROM && k < FROM + TOK) dequantize(k - FROM);
+        if (k == FROM + TOK) put(i + 1, 0);
+      }
       if (D == 128 && x == LAST - 6) read_kscale(i + 1);
       const v4i f = ring[k % AHEAD];
       if (x + AHEAD < LAST) ring[k % AHEAD] = operand(x + AHEAD);
@@ -816,9 +835,10 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
   };
   // P = exp2(score - m - 2) of page i, see chunk_softmax_pv in decode_chunk.h.
-  auto softmax = [&](int i, bool there) {
+  auto softmax = [&](int i, bool there) __attribute__((always_inline)) {
     if constexpr (D == 256) read_kscale(i);
     float t[NT][4][4], mx[NT];
     const int tbase = (p0 + i) * kPage;
@@ -908,44 +928,33 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
   for (int i = 0; i < W::SLOTS - 1; ++i) issue(i);
   end_phase(true, W::SLOTS - 2);
   if (grp) {  // group 1 sits out phase 0
-#pragma unroll
-    for (int c = 0; c < COLS; ++c) convert(0, c, fetch(0, c));
+    convert(0, std::false_type{});
     end_phase(false, 0);
   }
   auto run = [&](auto compute) {
     constexpr bool C = decltype(compute)::value;
-    if constexpr (C)
-      phase_a(-1, std::false_type{});
-    else
-      issue(W::SLOTS - 1);
-    end_phase(grp, W::SLOTS - 2);
-    for (int i = 0; i < pages; ++i) {
-      // Phase B(i): group 0 is one page behind group 1 in dequantizing.
-      const bool there = (valid >> (i % W::SLOTS)) & 1u;
-      // What is dequantized is read ahead of the softmax, which hides it (D =
-      // 256: after it, the registers do not hold both).
-      Packed packed;
-      if constexpr (COLS == 1) packed = fetch(i + grp, 0);
+    auto phase = [&](int i, auto with_v) {
       if constexpr (C) {
-        __builtin_amdgcn_sched_barrier(0);
-        softmax(i, there);
+        phase_a(i, with_v);
+      } else {
+        issue(i + W::SLOTS);
+        convert(i + 1, std::true_type{});
+      }
+      end_phase(grp, W::SLOTS - 2);
+    };
+    phase(-1, std::false_type{});
+    for (int i = 0; i < pages; ++i) {
+      if constexpr (C) {
+        softmax(i, (valid >> (i % W::SLOTS)) & 1u);
+        // Used here: its last steps would otherwise be moved over the barrier.
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) asm volatile("" : "+v"(P[nt][0]), "+v"(P[nt][1]));
         __builtin_amdgcn_sched_barrier(0);
       }
-      if constexpr (COLS == 1) {
-        convert(i + grp, 0, packed);
-      } else {
-#pragma unroll
-        for (int c = 0; c < COLS; ++c) convert(i + grp, c, fetch(i + grp, c));
-      }
+      convert(i + grp, std::false_type{});
       end_phase(!grp, W::SLOTS - 2);
-      // Phase A(i + 1); behind the last page its scores are of no page and not used.
-      if constexpr (C)
-        phase_a(i, std::true_type{});
-      else
-        issue(i + W::SLOTS);
-      end_phase(grp, W::SLOTS - 2);
+      // A(i + 1); behind the last page its scores are of no page and not used.
+      phase(i, std::true_type{});
     }
   };
   // Waves whose rows lie behind the batch's only move and dequantize pages.
