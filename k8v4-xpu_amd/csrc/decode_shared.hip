@@ -610,6 +610,8 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
   const int pages = p1 - p0;
 
   // Query rows: lane (n, g) of tile nt holds row 16 nt + n, dims 64 ks + 16 g ...
+  // A row behind the batch's last reads the last's length and scale and uses
+  // neither, so that all tiles' loads are one round trip.
   v4i qf[NT][KS];
   float crow[NT];
   int lim[NT];
@@ -618,17 +620,27 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
   for (int nt = 0; nt < NT; ++nt) {
     const int r = row0 + 16 * nt + n;
     const int64_t at = h * a.head_rows + r;  // the buffer is padded to whole blocks
+    const int rl = min(r, nrows - 1), tok = rl / kGqa, sb = tok / a.q_len;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[nt][ks] = *reinterpret_cast<const v4i *>(a.q8 + at * D + 64 * ks + 16 * g);
-    int end = a.prefix_pages * kPage;
-    double f = 0.0;
-    if (r < nrows) {
-      f = a.q8_scale[at];
-      const int tok = r / kGqa, sb = tok / a.q_len;
-      end = a.seq_lens[sb] - a.q_len + (tok - sb * a.q_len) + 1;
-      if (end > 0) far = max(far, kFar - min(end, kFar));
-    }
-    lim[nt] = end;
+    crow[nt] = a.q8_scale[h * a.head_rows + rl];
+    lim[nt] = a.seq_lens[sb] - a.q_len + (tok - sb * a.q_len) + 1;
+  }
+  // Physical pages, 64 at a time: lane l holds page p0 + 64 k + l.
+  int ptab = -1;
+  auto load_table = [&](int k) {
+    const int p = min(p0 + 64 * k + lane, p1 - 1);
+    const int raw = a.prefix_table[a.ppb <= 1 ? p : p / a.ppb];
+    const int64_t ph = a.ppb <= 1 ? raw : static_cast<int64_t>(raw) * a.ppb + p % a.ppb;
+    ptab = ph >= 0 && ph < a.num_pages ? static_cast<int>(ph) : -1;
+  };
+  load_table(0);  // in the query rows' round trip
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const bool live = row0 + 16 * nt + n < nrows;
+    if (live && lim[nt] > 0) far = max(far, kFar - min(lim[nt], kFar));
+    if (!live) lim[nt] = a.prefix_pages * kPage;
+    const double f = live ? static_cast<double>(crow[nt]) : 0.0;
     crow[nt] = fmaxf(static_cast<float>(f * (static_cast<double>(kLog2e) / sqrt(static_cast<double>(D)))), 1e-30f);
   }
   const int min_end = kFar - wave_max(far);
@@ -659,14 +671,6 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
     return o;
   };
   const Offsets off0 = offsets(lane);
-  // Physical pages, 64 at a time: lane l holds page p0 + 64 k + l.
-  int ptab = -1;
-  auto load_table = [&](int k) {
-    const int p = min(p0 + 64 * k + lane, p1 - 1);
-    const int raw = a.prefix_table[a.ppb <= 1 ? p : p / a.ppb];
-    const int64_t ph = a.ppb <= 1 ? raw : static_cast<int64_t>(raw) * a.ppb + p % a.ppb;
-    ptab = ph >= 0 && ph < a.num_pages ? static_cast<int>(ph) : -1;
-  };
   // Whether page i of the piece is in the cache, for the last SLOTS pages issued.
   uint32_t valid = 0;
   // This wave's loads of page i of the piece (W::LOADS of them, also for a
@@ -682,7 +686,7 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
   const uint32_t k_ps = static_cast<uint32_t>(a.k_ps), v_ps = static_cast<uint32_t>(a.v_ps);
   const uint32_t p_ps = static_cast<uint32_t>(plane == 1 ? a.vs_ps : plane == 2 ? a.vz_ps : a.ks_ps);
   auto issue = [&](int i) {
-    if ((i & 63) == 0 && i < pages) load_table(i >> 6);
+    if ((i & 63) == 0 && i > 0 && i < pages) load_table(i >> 6);
     const int phys = i < pages ? __builtin_amdgcn_readlane(ptab, i & 63) : -1;
     const int slot = i % W::SLOTS;
     valid = (valid & ~(1u << slot)) | (phys >= 0 ? 1u << slot : 0u);
