@@ -1166,14 +1166,14 @@ void launch_wide(const SharedArgs &a, int tiles, hipStream_t s) {
 // the many-rows kernel, or the one that takes eight tokens at a time.  Measured
 // (us, eight tokens at a time / many rows, one token a sequence):
 //   D    heads  pages   8 tokens   16         32         64         128
-//   128  4      8       21 / 17    22 / 17    24 / 21    26 / 30    34 / 36
-//   128  4      2,048   41 / 71    56 / 74    87 / 83    148 / 121  325 / 214
-//   128  2      8       19 / 16    19 / 17    20 / 19    23 / 29    24 / 35
-//   128  2      2,048   33 / 43    41 / 46    55 / 52    86 / 75    148 / 127
-//   256  2      8       23 / 18    21 / 20    24 / 28    27 / 33    34 / 39
-//   256  2      2,048   43 / 54    62 / 58    98 / 79    178 / 132  364 / 204
-//   256  4      8       23 / 19    27 / 21    30 / 29    37 / 34    46 / 40
-//   256  4      2,048   63 / 88    101 / 94   176 / 126  343 / 220  678 / 351
+//   128  4      8       21 / 17    21 / 17    25 / 21    27 / 29    35 / 34
+//   128  4      2,048   41 / 73    56 / 76    89 / 85    154 / 109  331 / 196
+//   128  2      8       19 / 17    19 / 17    20 / 20    22 / 28    25 / 33
+//   128  2      2,048   33 / 44    41 / 47    56 / 54    90 / 69    154 / 114
+//   256  2      8       24 / 19    21 / 20    25 / 28    28 / 33    33 / 39
+//   256  2      2,048   44 / 58    63 / 60    102 / 78   181 / 133  383 / 201
+//   256  4      8       23 / 19    26 / 21    31 / 29    36 / 34    46 / 40
+//   256  4      2,048   64 / 94    101 / 98   186 / 127  351 / 228  693 / 369
 // Over a long prefix many rows pay as soon as they fill about half the waves;
 // over a short one the many-rows piece is the shorter chain while there are few
 // of them, and with more rows it is each sequence's own pages that count, which
@@ -1376,7 +1376,7 @@ extern "C" int k8v4_attn_shared(const void *q, int q_dtype, int64_t q_tok_stride
     const int64_t avg = groups ? (sh.grid + groups - 1) / groups + 1 : (sh.grid + batch - 1) / batch;
     int cs = vpr_max / 8;
     bool found = false;
-    for (int threads : {128, 256}) {
+    for (int threads : {64, 128, 256}) {
       for (int c = 1; vpr_max / c >= 8 && !found; c *= 2) {
         const int spi = threads / (vpr_max / c);
         if ((avg + spi - 1) / spi <= kMergeMU) {
@@ -1424,12 +1424,16 @@ extern "C" int k8v4_attn_shared(const void *q, int q_dtype, int64_t q_tok_stride
   if (rc) return rc;
   const dim3 mgrid(static_cast<unsigned>(merge_units));
   if (head_dim == 128) {
-    if (tpu == 128)
+    if (tpu == 64)
+      shared_merge_kernel<128, 64><<<mgrid, dim3(64), 0, s>>>(a);
+    else if (tpu == 128)
       shared_merge_kernel<128, 128><<<mgrid, dim3(128), 0, s>>>(a);
     else
       shared_merge_kernel<128, 256><<<mgrid, dim3(256), 0, s>>>(a);
   } else {
-    if (tpu == 128)
+    if (tpu == 64)
+      shared_merge_kernel<256, 64><<<mgrid, dim3(64), 0, s>>>(a);
+    else if (tpu == 128)
       shared_merge_kernel<256, 128><<<mgrid, dim3(128), 0, s>>>(a);
     else
       shared_merge_kernel<256, 256><<<mgrid, dim3(256), 0, s>>>(a);
