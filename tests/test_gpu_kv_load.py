@@ -279,3 +279,33 @@ def test_offsets_past_32_bits(gpu_ops):
     want = views["k"][page, t % PAGE].double() * views["k_scale"][page, t % PAGE].double()[..., None]
     assert_rounded(k[-100:], want, 1)
     assert not bool(k[-101].any()) and not bool(k[:1000].any())
+
+
+@pytest.mark.parametrize("batch", [1, 2, 255, 256, 257, 512, 513, 1000])
+def test_every_row_finds_its_sequence(gpu_ops, batch):
+    """Ragged and empty sequences around the number the kernel's first search covers
+    (256): every row holds its own sequence's token, found by the codes alone."""
+    hkv, d = 2, 128
+    counts = [(7 * i + i // 5) % 4 for i in range(batch)]
+    counts[-1] = 3
+    cache = Cache(batch, PageLayout(hkv, d))
+    cache.views["k_scale"].fill_(1.0)
+    cache.views["v_scale"].fill_(1.0)
+    # Page p's token r: K codes hold p % 100 and r, V nibbles p // 100.
+    page = torch.arange(batch, device=DEV, dtype=torch.int8) if batch < 100 else (
+        torch.arange(batch, device=DEV) % 100).to(torch.int8)
+    cache.views["k"][..., 0] = page[:, None, None]
+    cache.views["k"][..., 1] = torch.arange(PAGE, device=DEV, dtype=torch.int8)[None, :, None]
+    cache.views["v"][..., 0] = (torch.arange(batch, device=DEV) // 100).to(torch.uint8)[:, None, None]
+    table = torch.randperm(batch, generator=torch.Generator().manual_seed(batch)).to(torch.int32)
+    firsts = [(3 * i) % 60 for i in range(batch)]
+    k = torch.full((sum(counts) + 2, hkv, d), SENTINEL, device=DEV)
+    v = torch.full_like(k, SENTINEL)
+    gpu_ops.kv_load_paged(*cache.region_args(), table[:, None].to(DEV), index(firsts), starts_of(counts, 1), 1, k, v)
+    torch.cuda.synchronize()
+    want = torch.tensor([(int(table[b]) % 100, firsts[b] + j, int(table[b]) // 100)
+                         for b, n in enumerate(counts) for j in range(n)], dtype=torch.float32)
+    got = torch.cat((k[1:-1, 0, :2], v[1:-1, 0, :1]), 1).cpu()
+    assert torch.equal(got, want)
+    for x in (k, v):
+        assert bool((x[0] == SENTINEL).all()) and bool((x[-1] == SENTINEL).all())
