@@ -285,8 +285,8 @@ int64_t k8v4_attn_noalloc_max_bytes(void);
 
 /*
  * Diagnostics, no counterpart in the reference: how many in-kernel waits of
- * the decode kernels on the current device gave up since the library was
- * loaded (the paired-halves handshake of head dim 256 caps
+ * the decode kernels (k8v4_attn_shared's too) on the current device gave up
+ * since the library was loaded (the paired-halves handshake of head dim 256 caps
  * each wait; a give-up means a wrong output).  Synchronizes with the device
  * (a copy from device memory); -1 on a HIP error.  Zero in a correct run.
  */
@@ -316,14 +316,16 @@ int64_t k8v4_attn_workspace_bytes(int64_t batch, int64_t table_width, int pages_
  * op attends to each sequence alone, k8v4_v030/native/xe2_kv_ops.cpp:1728-1775).
  *
  * prefix_table: int32 [prefix_width], the table entries of the first
- * prefix_len tokens (NULL allowed where they fill no page).  Its prefix_len /
+ * prefix_len tokens (NULL allowed where they fill no page), all of which have
+ * been stored, whether or not a sequence reaches so far.  Its prefix_len /
  * 64 whole pages stand for the first pages of every sequence, whose own rows
  * of block_table are not read there; the tokens behind them come from those
  * rows.  seq_lens: int32 [batch] (device), all tokens of a sequence, the
  * prefix and the step's own included; the causal end of token j is seq_len -
  * q_len + j + 1.  A row whose end lies inside the prefix sees it up to there;
  * one that sees no key outputs zeros, whatever its query holds.  Query rows,
- * cache, table entries, out and the numerics as in k8v4_attn_batch.
+ * cache, table entries, out and the numerics as in k8v4_attn_batch; page
+ * strides below 2^31 bytes.
  * workspace: >= k8v4_attn_shared_workspace_bytes(batch, q_len, hkv, head_dim)
  * bytes, 16-byte aligned: the quantized query rows and the states of the page
  * runs.  Calls that may overlap (other streams, captured graphs) need one each.

@@ -552,16 +552,28 @@ void shared_split_kernel(SharedArgs args) {
 //
 // Waves w and w + 4 share a SIMD.  They form two groups half a page apart,
 // separated by a barrier per phase: in phase A of page p a wave multiplies (O
-// += V(p - 1)^T P(p - 1), S = K(p) Q^T) and issues its share of a later page's
-// loads; in phase B it turns S into probabilities and dequantizes its share of V.  So each SIMD holds one wave that
-// feeds the matrix core and one that feeds the vector unit.  With t counting
+// += V(p - 1)^T P(p - 1), S = K(p) Q^T), issues its share of a later page's
+// loads and dequantizes its share of V(p) (head dim 256: a quarter of it)
+// between the products; in phase B it turns S into probabilities and, at head
+// dim 256, dequantizes the rest.  So each SIMD holds one wave that feeds the
+// matrix core and one that feeds the vector unit; the former issues first
+// (s_setprio), as the latter has an instruction for every gap.  With t counting
 // phases, group 0 runs A(p) at t = 2p and B(p) at 2p + 1, group 1 one later:
-//   raw page p (K codes, V codes, planes): read from t = 2p (A of group 0) to
-//     2p + 1 (B of group 0 dequantizes its half; the key scales, to 2p + 2, lie
-//     apart); a wave issues its loads of page
+//   raw page p (K codes, V codes, planes): read from t = 2p (A of group 0; at
+//     head dim 256 group 1, a page ahead in its B, reads its V) to 2p + 1; the
+//     key scales, read to 2p + 2, lie apart.  A wave issues its loads of page
 //     p + SLOTS - 1, into the slot of page p - 1, in A(p);
-//   V16(p): written at 2p (group 1's half) and 2p + 1, read at 2p + 2 and 2p + 3:
-//     two buffers.
+//   V16(p): written at 2p and 2p + 1, read at 2p + 2 and 2p + 3: two buffers.
+//
+// Bound by issue: at head dim 128 a page of a SIMD's two waves takes 4,900
+// cycles, in which its matrix core multiplies for 2,500 and its vector unit
+// works for about 3,600 (48 exponentials and 270 other instructions a wave).
+// Measured: 64 sequences of 4 tokens over 1,562 pages, 4 KV heads, 250 us of a
+// 261 us call (the batch op 835): 1,258 TFLOP/s; at a large fp16 product's
+// 1,312, and twice that for the int8 one, the two products take 180 us.
+// Head dim 256 470 us, 2 KV heads 137 and 258.  Tried and not better: the
+// vector phase first (310 us), no priority (290), row blocks of two tiles a wave
+// (5 % at 200 to 256 rows, slower at head dim 256).
 // Products are transposed (tokens x rows, dims x rows): a lane owns one row of
 // each tile, so the running max, sum and rescale need no exchange but the max
 // over the four lanes of a row.
@@ -729,7 +741,7 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
   // zero) scale / 16.  V16 rows are parity * D / 2 + byte column, a lane's eight
   // tokens a 16-byte chunk.
   // In units of one byte column (D = 256: and four tokens, for the registers).
-  // Balanced between the phases: all of it in A, at head dim 256 one unit of four.
+  // All of it in A, at head dim 256 one unit of four (none: 470 us, two: 470).
   constexpr int COLS = W::VROW / kWave, TOK = D == 128 ? 8 : 4, UNITS = COLS * 8 / TOK, IN_A = 1;
   typedef _Float16 vth __attribute__((ext_vector_type(TOK)));
   uint32_t byte[TOK];

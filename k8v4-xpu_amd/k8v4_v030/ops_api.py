@@ -450,10 +450,10 @@ class _Ops:
         pages, those read once for all of them.
 
         ``prefix_table`` (int32 ``[W']``, for instance ``block_table[0]``) names the
-        pages of the first ``prefix_len`` tokens; its whole pages (``prefix_len // 64``)
-        stand for those of every sequence, whatever the sequences' own rows of
-        ``block_table`` (int32 ``[B, W]``) hold there, and the tokens behind them come
-        from those rows.  ``seq_lens`` (int32 ``[B]``) counts all of a sequence's
+        pages of the first ``prefix_len`` tokens, all of them stored; its whole pages
+        (``prefix_len // 64``) stand for those of every sequence, whatever the
+        sequences' own rows of ``block_table`` (int32 ``[B, W]``) hold there, and the
+        tokens behind them come from those rows.  ``seq_lens`` (int32 ``[B]``) counts all of a sequence's
         tokens, the prefix included; a row whose causal end lies inside the prefix
         sees the prefix up to there, one that sees nothing gives zeros.  The other
         arguments and the numerics are the batch op's; ``workspace`` holds

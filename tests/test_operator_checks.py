@@ -107,6 +107,7 @@ def shared(lib, **over):
     (dict(bt=P + 2), "index arrays"), (dict(pre=P + 1), "index arrays"), (dict(k=P + 8), "k_cache"),
     (dict(v_ps=52222), "v_cache"), (dict(vs=P + 4), "scale planes"), (dict(ws=P + 8), "workspace must be"),
     (dict(batch=2**16, width=2**15, bt_stride=2**15), "too large"),
+    (dict(k_ps=2**31), "page strides"), (dict(vz_ps=-52224), "page strides"), (dict(ks_ps=2**32), "page strides"),
 ])
 def test_shared_refuses(lib, over, text):
     refused(lib, shared, text, **{"ws_bytes": 1 << 40, **over})
