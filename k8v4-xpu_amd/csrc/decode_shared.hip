@@ -552,28 +552,30 @@ void shared_split_kernel(SharedArgs args) {
 //
 // Waves w and w + 4 share a SIMD.  They form two groups half a page apart,
 // separated by a barrier per phase: in phase A of page p a wave multiplies (O
-// += V(p - 1)^T P(p - 1), S = K(p) Q^T), issues its share of a later page's
-// loads and dequantizes its share of V(p) (head dim 256: a quarter of it)
-// between the products; in phase B it turns S into probabilities and, at head
-// dim 256, dequantizes the rest.  So each SIMD holds one wave that feeds the
-// matrix core and one that feeds the vector unit; the former issues first
-// (s_setprio), as the latter has an instruction for every gap.  With t counting
-// phases, group 0 runs A(p) at t = 2p and B(p) at 2p + 1, group 1 one later:
-//   raw page p (K codes, V codes, planes): read from t = 2p (A of group 0; at
-//     head dim 256 group 1, a page ahead in its B, reads its V) to 2p + 1; the
-//     key scales, read to 2p + 2, lie apart.  A wave issues its loads of page
-//     p + SLOTS - 1, into the slot of page p - 1, in A(p);
+// += V(p - 1)^T P(p - 1), S = K(p) Q^T) and, between the products, dequantizes
+// its share of V(p) (head dim 256: a quarter of it) and issues its share of a
+// later page's loads; in phase B it turns S into probabilities and, at head dim
+// 256, dequantizes the rest.  So each SIMD holds one wave that feeds the matrix
+// core and one that feeds the vector unit; the former issues first (s_setprio),
+// as the latter has an instruction for every gap.  With t counting phases, group
+// 0 runs A(p) at t = 2p and B(p) at 2p + 1, group 1 one later:
+//   raw page p (K codes, V codes): read from t = 2p (A of group 0; at head dim 256
+//     group 1, a page ahead in its B, reads its V) to 2p + 1; its V planes, which
+//     group 0 loads, are scaled by one wave at t = 2p - 1; the key scales, read
+//     to 2p + 2, lie apart.  A wave issues its loads of page p + SLOTS - 1, into
+//     the slot of page p - 1, in A(p);
 //   V16(p): written at 2p and 2p + 1, read at 2p + 2 and 2p + 3: two buffers.
 //
-// Bound by issue: at head dim 128 a page of a SIMD's two waves takes 4,900
-// cycles, in which its matrix core multiplies for 2,500 and its vector unit
-// works for about 3,600 (48 exponentials and 270 other instructions a wave).
-// Measured: 64 sequences of 4 tokens over 1,562 pages, 4 KV heads, 250 us of a
-// 261 us call (the batch op 835): 1,258 TFLOP/s; at a large fp16 product's
-// 1,312, and twice that for the int8 one, the two products take 180 us.
-// Head dim 256 470 us, 2 KV heads 137 and 258.  Tried and not better: the
-// vector phase first (310 us), no priority (290), row blocks of two tiles a wave
-// (5 % at 200 to 256 rows, slower at head dim 256).
+// Bound by issue, the largest calls by power: at head dim 128 a page of a SIMD's
+// two waves takes 4,700 cycles, in which its matrix core multiplies for 2,870 (78
+// products of 18.4 cycles a wave) and its vector unit works for about 3,300 (48
+// exponentials and 240 other instructions a wave).  64 sequences of 4 tokens over
+// 1,562 pages run at 2.1 GHz where smaller calls hold 2.4.
+// Measured: that call, 4 KV heads, 259 us (the batch op 835): 1,215 TFLOP/s; at a
+// large fp16 product's 1,312, and twice that for the int8 one, the two products
+// take 180 us.  Head dim 256 459 us, 2 KV heads 137 and 259.  Tried and not
+// better: the vector phase first (310 us), no priority (290), row blocks of two
+// tiles a wave (4 % at 200 to 256 rows, slower at head dim 256).
 // Products are transposed (tokens x rows, dims x rows): a lane owns one row of
 // each tile, so the running max, sum and rescale need no exchange but the max
 // over the four lanes of a row.
@@ -690,32 +692,48 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
   // count): its share of the K rows and of the V rows, and a plane.
   const char *const kbase = reinterpret_cast<const char *>(a.k_cache);
   const char *const vbase = reinterpret_cast<const char *>(a.v_cache);
-  const int plane = D == 128 ? wave - 4 : wave;  // 1: v_scale, 2: v_zero, others k_scale
+  // The V planes are loaded by waves of group 0, which waits for a page first.
+  const int plane = wave;  // 1: v_scale, 2: v_zero, others k_scale
   const char *const pbase = plane == 1   ? reinterpret_cast<const char *>(a.v_scale)
                             : plane == 2 ? reinterpret_cast<const char *>(a.v_zero)
                                          : reinterpret_cast<const char *>(a.k_scale);
   // Page strides are below 2^31 bytes, page numbers below 2^31.
   const uint32_t k_ps = static_cast<uint32_t>(a.k_ps), v_ps = static_cast<uint32_t>(a.v_ps);
   const uint32_t p_ps = static_cast<uint32_t>(plane == 1 ? a.vs_ps : plane == 2 ? a.vz_ps : a.ks_ps);
-  auto issue = [&](int i) {
+  // In three parts, which phase A runs between its products.
+  int phys = -1;
+  uint32_t ph = 0;
+  auto issue_page = [&](int i) __attribute__((always_inline)) {
     if ((i & 63) == 0 && i > 0 && i < pages) load_table(i >> 6);
-    const int phys = i < pages ? __builtin_amdgcn_readlane(ptab, i & 63) : -1;
-    const int slot = i % W::SLOTS;
-    valid = (valid & ~(1u << slot)) | (phys >= 0 ? 1u << slot : 0u);
-    const uint64_t ph = static_cast<uint32_t>(phys >= 0 ? phys : 0);
-    lds_t *dst = lds + slot * W::SLOT_BYTES;
+    phys = i < pages ? __builtin_amdgcn_readlane(ptab, i & 63) : -1;
+    const uint32_t bit = 1u << (i % W::SLOTS);
+    valid = phys >= 0 ? valid | bit : valid & ~bit;
+    ph = static_cast<uint32_t>(max(phys, 0));
+  };
+  auto issue_k = [&](int i) __attribute__((always_inline)) {
+    lds_t *dst = lds + (i % W::SLOTS) * W::SLOT_BYTES;
     const Offsets off = D == 128 ? off0 : offsets(fresh_lane());
 #pragma unroll
-    for (int k = 0; k < W::KPW; ++k) dma16s(kbase + ph * k_ps, off.k[k], dst + (wave * W::KPW + k) * 1024);
-    if (D == 256 || wave < 4) dma16s(vbase + ph * v_ps, off.v, dst + W::V_OFF + vj * 1024);
-    if (D == 256 || wave >= 4) {
-      // D = 128: waves 4 and 7 both fetch k_scale; D = 256: 0 and 3 .. 7.  A page
+    for (int k = 0; k < W::KPW; ++k)
+      dma16s(kbase + static_cast<uint64_t>(ph) * k_ps, off.k[k], dst + (wave * W::KPW + k) * 1024);
+  };
+  auto issue_rest = [&](int i) __attribute__((always_inline)) {
+    lds_t *dst = lds + (i % W::SLOTS) * W::SLOT_BYTES;
+    const Offsets off = D == 128 ? off0 : offsets(fresh_lane());
+    if (D == 256 || wave >= 4) dma16s(vbase + static_cast<uint64_t>(ph) * v_ps, off.v, dst + W::V_OFF + vj * 1024);
+    if (D == 256 || wave < 4) {
+      // D = 128: waves 0 and 3 both fetch k_scale; D = 256: 0 and 3 .. 7.  A page
       // outside the cache holds no keys: its scores are masked in B, and its
       // planes are zeros here, so that its V is zeros whatever page 0 holds.
       lds_t *pdst = plane == 1 || plane == 2 ? dst + W::S_OFF + (plane - 1) * kPage * 4 : lds + W::KS_OFF + (i & 3) * kPage * 4;
-      dma4s(pbase + ph * p_ps, off.p, phys >= 0 ? pdst : lds + W::PAD_OFF);
+      dma4s(pbase + static_cast<uint64_t>(ph) * p_ps, off.p, phys >= 0 ? pdst : lds + W::PAD_OFF);
       if (phys < 0) *reinterpret_cast<__attribute__((address_space(3))) float *>(pdst + 4 * lane) = 0.f;
     }
+  };
+  auto issue = [&](int i) __attribute__((always_inline)) {
+    issue_page(i);
+    issue_k(i);
+    issue_rest(i);
   };
 
   v4f O[NT][DT];
@@ -734,14 +752,29 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
   const v4i bias = {kScoreBias, kScoreBias, kScoreBias, kScoreBias};
   const v8h ones = {1, 1, 1, 1, 1, 1, 1, 1};
 
+  // The V planes of page i made into what its dequantization takes, by one wave
+  // for all: a byte holds two dims, each as fp16 bits n 2^-24 (subnormal, exact),
+  // so with s' = 2^20 scale and z' = -zero scale / 16 one fma, rounded once to
+  // fp16, gives (n - zero) scale / 16.
+  float plane_s, plane_z;
+  auto read_planes = [&](int i) __attribute__((always_inline)) {
+    const lds_t *planes = lds + (i % W::SLOTS) * W::SLOT_BYTES + W::S_OFF + 4 * lane;
+    plane_s = *reinterpret_cast<__attribute__((address_space(3))) const float *>(planes);
+    plane_z = *reinterpret_cast<__attribute__((address_space(3))) const float *>(planes + kPage * 4);
+  };
+  auto scale_planes = [&](int i) __attribute__((always_inline)) {
+    if (wave != 0) return;
+    lds_t *planes = lds + (i % W::SLOTS) * W::SLOT_BYTES + W::S_OFF + 4 * lane;
+    *reinterpret_cast<__attribute__((address_space(3))) float *>(planes) = plane_s * 0x1p20f;
+    *reinterpret_cast<__attribute__((address_space(3))) float *>(planes + kPage * 4) = plane_z * (plane_s * -0.0625f);
+  };
+
   // This wave's share of V16(i): tokens 4 wave' + {0..3, 16..19} of its group's
-  // 32-token half of the page, byte columns `lane` (D = 256: and 64 + lane).  A
-  // byte holds two dims; as fp16 its low nibble is n 2^-24 and its high one n
-  // 2^-20 (subnormal, exact), so one fma each, rounded once to fp16, gives (n -
-  // zero) scale / 16.  V16 rows are parity * D / 2 + byte column, a lane's eight
-  // tokens a 16-byte chunk.
+  // 32-token half of the page, byte columns `lane` (D = 256: and 64 + lane).
+  // V16 rows are parity * D / 2 + byte column, a lane's eight tokens a 16-byte
+  // chunk.
   // In units of one byte column (D = 256: and four tokens, for the registers).
-  // All of it in A, at head dim 256 one unit of four (none: 470 us, two: 470).
+  // All of it in A, at head dim 256 one unit of four (none or two: the same time).
   constexpr int COLS = W::VROW / kWave, TOK = D == 128 ? 8 : 4, UNITS = COLS * 8 / TOK, IN_A = 1;
   typedef _Float16 vth __attribute__((ext_vector_type(TOK)));
   uint32_t byte[TOK];
@@ -762,11 +795,10 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
     }
   };
   auto dequantize = [&](int t) __attribute__((always_inline)) {
-    const float s = vs[t >> 2][t & 3], z = vz[t >> 2][t & 3] * (s * -0.0625f);
     const _Float16 lo = __builtin_bit_cast(_Float16, static_cast<uint16_t>(byte[t] & 0x0Fu));
-    const _Float16 hi = __builtin_bit_cast(_Float16, static_cast<uint16_t>(byte[t] & 0xF0u));
-    even[t] = static_cast<_Float16>(fmaf(static_cast<float>(lo), s * 0x1p20f, z));
-    odd[t] = static_cast<_Float16>(fmaf(static_cast<float>(hi), s * 0x1p16f, z));
+    const _Float16 hi = __builtin_bit_cast(_Float16, static_cast<uint16_t>(byte[t] >> 4));
+    even[t] = static_cast<_Float16>(fmaf(static_cast<float>(lo), vs[t >> 2][t & 3], vz[t >> 2][t & 3]));
+    odd[t] = static_cast<_Float16>(fmaf(static_cast<float>(hi), vs[t >> 2][t & 3], vz[t >> 2][t & 3]));
   };
   auto put = [&](int i, int u) __attribute__((always_inline)) {
     lds_t *dst = lds + W::V16_OFF + (i & 1) * W::V16_BYTES;
@@ -816,26 +848,19 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
     v4i ring[AHEAD];
 #pragma unroll
     for (int x = 0; x < AHEAD; ++x) ring[x] = operand(FIRST + x);
-    __builtin_amdgcn_sched_barrier(0);
-    issue(i + W::SLOTS);
     if constexpr (FIRST != 0) convert(i + 1, std::true_type{});
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (FIRST == 0) {
 #pragma unroll
-    for (int x = FIRST; x < LAST; ++x) {
-      const int k = x - FIRST;
-      // Between the products, while S is not yet needed: page i + 1 dequantized;
-      // towards the end (P's registers are free by then) what phase B needs first.
-      if constexpr (FIRST == 0) {
+      for (int x = 0; x < NV; ++x) {
+        // Between the products, while S is not yet needed: page i + 1 dequantized.
         constexpr int FROM = 3;
-        if (k == 1) fetch(i + 1, 0);
-        if (k >= FROM && k < FROM + TOK) dequantize(k - FROM);
-        if (k == FROM + TOK) put(i + 1, 0);
-      }
-      if (D == 128 && x == LAST - 6) read_kscale(i + 1);
-      const v4i f = ring[k % AHEAD];
-      if (x + AHEAD < LAST) ring[k % AHEAD] = operand(x + AHEAD);
-      if (x < NV) {
+        if (x == 1) fetch(i + 1, 0);
+        if (x >= FROM && x < FROM + TOK) dequantize(x - FROM);
+        if (x == FROM + TOK) put(i + 1, 0);
         const int s = x / DT, j = x % DT;
+        const v4i f = ring[x % AHEAD];
+        ring[x % AHEAD] = operand(x + AHEAD);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
           O[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, f), P[nt][s], O[nt][j], 0, 0, 0);
@@ -843,12 +868,23 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) lsum[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, P[nt][s], lsum[nt], 0, 0, 0);
         }
-      } else {
-        const int ml = (x - NV) / KS, ks = (x - NV) % KS;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          S[nt][ml] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, qf[nt][ks], ks ? S[nt][ml] : bias, 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
       }
+    }
+#pragma unroll
+    for (int x = NV; x < LAST; ++x) {
+      // P's registers are free: a later page's loads, which ahead of the products
+      // were 300 (D = 256: 650) cycles without one, and what B needs first.
+      if (x == NV) issue_page(i + W::SLOTS);
+      if (x == NV + NK / 4) issue_k(i + W::SLOTS);
+      if (x == NV + NK / 2) issue_rest(i + W::SLOTS);
+      if (D == 128 && x == LAST - 5) read_kscale(i + 1);
+      const int k = x - FIRST, ml = (x - NV) / KS, ks = (x - NV) % KS;
+      const v4i f = ring[k % AHEAD];
+      if (x + AHEAD < LAST) ring[k % AHEAD] = operand(x + AHEAD);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        S[nt][ml] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, qf[nt][ks], ks ? S[nt][ml] : bias, 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_s_setprio(0);
@@ -916,16 +952,13 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
       }
     }
   };
-  // Ends a phase.  Before an even phase t = 2q the raw page q has to be there:
-  // `left` of this wave's loads may still be under way.
-  auto end_phase = [&](bool before_even, int left) {
-    if (before_even) {
+  // Ends a phase; with `wait`, `left` pages of this wave's loads may be under way.
+  auto end_phase = [&](bool wait, int left) {
+    if (wait) {
       if (left == 2)
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * W::LOADS) : "memory");
-      else if (left == 1)
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(W::LOADS) : "memory");
       else
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(W::LOADS) : "memory");
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
@@ -939,10 +972,15 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) asm volatile("" ::"v"(qf[nt][ks]));
-  // Before phase 2q both groups have issued up to page q + SLOTS - 2, in A(q - 1).
+  // After A(i), in which it issued page i + SLOTS, a wave waits for page i + 2: group
+  // 0 (t = 2i + 2) a phase before its V planes are scaled, group 1 (t = 2i + 3) as
+  // the page is about to be read.
 #pragma unroll
   for (int i = 0; i < W::SLOTS - 1; ++i) issue(i);
   end_phase(true, W::SLOTS - 2);
+  read_planes(0);
+  scale_planes(0);
+  end_phase(false, 0);
   if (grp) {  // group 1 sits out phase 0
     convert(0, std::false_type{});
     end_phase(false, 0);
@@ -956,10 +994,11 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
         issue(i + W::SLOTS);
         convert(i + 1, std::true_type{});
       }
-      end_phase(grp, W::SLOTS - 2);
+      end_phase(true, W::SLOTS - 2);
     };
     phase(-1, std::false_type{});
     for (int i = 0; i < pages; ++i) {
+      read_planes(i + 1);  // group 0's wave 0 scales them; the others read nothing of use
       if constexpr (C) {
         softmax(i, (valid >> (i % W::SLOTS)) & 1u);
         // Used here: its last steps would otherwise be moved over the barrier.
@@ -967,8 +1006,9 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
         for (int nt = 0; nt < NT; ++nt) asm volatile("" : "+v"(P[nt][0]), "+v"(P[nt][1]));
         __builtin_amdgcn_sched_barrier(0);
       }
+      scale_planes(i + 1);
       convert(i + grp, std::false_type{});
-      end_phase(!grp, W::SLOTS - 2);
+      end_phase(false, 0);
       // A(i + 1); behind the last page its scores are of no page and not used.
       phase(i, std::true_type{});
     }
