@@ -567,7 +567,7 @@ void shared_split_kernel(SharedArgs args) {
 //   V16(p): written at 2p and 2p + 1, read at 2p + 2 and 2p + 3: two buffers.
 //
 // Bound by issue, the largest calls by power: at head dim 128 a page of a SIMD's
-// two waves takes 4,700 cycles, in which its matrix core multiplies for 2,870 (78
+// two waves takes 4,800 cycles, in which its matrix core multiplies for 2,870 (78
 // products of 18.4 cycles a wave) and its vector unit works for about 3,300 (48
 // exponentials and 240 other instructions a wave).  64 sequences of 4 tokens over
 // 1,562 pages run at 2.1 GHz where smaller calls hold 2.4.
