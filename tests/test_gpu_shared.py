@@ -104,7 +104,9 @@ class Batch:
     def want(self):
         """(o, a, r): the result, the sums of p |v| and the fp32 sums' roundings, float64."""
         q = self.q.double()
-        scale = q.abs().amax(-1, keepdim=True) / 127.0
+        # By a tensor: torch multiplies by the reciprocal of a Python number, an ulp off, and a
+        # query value on a rounding tie (bf16 with amax 127 / 64, say) gets the other code.
+        scale = q.abs().amax(-1, keepdim=True) / torch.full((), 127.0, dtype=torch.float64, device=DEV)
         inv = torch.where(scale == 0, torch.zeros_like(scale), 1.0 / scale)
         q = torch.sign(q) * torch.floor(q.abs() * inv + 0.5) * scale
         o, a = torch.zeros_like(q), torch.zeros_like(q)
@@ -347,6 +349,18 @@ def test_random_shapes(gpu_ops, case):
     x = Batch(gpu_ops, hkv, d, q_len, prefix, own, ppb, rng.choice([torch.float16, torch.bfloat16]), seed=case,
               fused=rng.random() < 0.5)
     x.check(x.run(rng.choice([torch.float16, torch.bfloat16, torch.float32])))
+
+
+@pytest.mark.parametrize("hkv,d,batch,prefix", [(4, 128, 3, 130), (2, 256, 5, 64), (4, 128, 40, 17000), (4, 256, 30, 640)])
+def test_query_values_on_rounding_ties(gpu_ops, hkv, d, batch, prefix):
+    """Every query value halfway between two codes of its row (bf16, the largest 127 / 64): the rule's codes, in both forms."""
+    x = Batch(gpu_ops, hkv, d, 2, prefix, [2 + 3 * i for i in range(batch)], dtype=torch.bfloat16, seed=batch)
+    gen = torch.Generator().manual_seed(batch)
+    rows = (torch.randint(-127, 127, x.q.shape, generator=gen) + 0.5) / 64
+    rows[..., 5] = 127 / 64
+    x.q = rows.to(torch.bfloat16).to(DEV)
+    assert torch.equal(x.q.float().cpu(), rows)
+    x.check(x.run(torch.float32))
 
 
 def test_wide_value_range(gpu_ops):
