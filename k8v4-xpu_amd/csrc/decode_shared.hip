@@ -777,17 +777,20 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
   // All of it in A, at head dim 256 one unit of four (none or two: the same time).
   constexpr int COLS = W::VROW / kWave, TOK = D == 128 ? 8 : 4, UNITS = COLS * 8 / TOK, IN_A = 1;
   typedef _Float16 vth __attribute__((ext_vector_type(TOK)));
-  uint32_t byte[TOK];
+  typedef int v2i __attribute__((ext_vector_type(2)));
+  v2i bytes;  // of tokens 0 .. 3 | 4 .. 7 of a lane's column
   v4f vs[TOK / 4], vz[TOK / 4];
   vth even, odd;
   auto fetch = [&](int i, int u) __attribute__((always_inline)) {
     const lds_t *raw = lds + (i % W::SLOTS) * W::SLOT_BYTES;
     const int c = u * TOK / 8, e0 = u * TOK % 8 / 4, t0 = 32 * grp + 4 * (wave & 3) + 16 * e0;
-    const int l = fresh_lane();
-#pragma unroll
-    for (int t = 0; t < TOK; ++t)
-      byte[t] = *reinterpret_cast<__attribute__((address_space(3))) const uint8_t *>(
-          raw + W::V_OFF + (t0 + (t < 4 ? t : 12 + t)) * W::VROW + c * kWave + l);
+    // The transposing read: of 16 lanes, lane 2 j + h reads bytes 8 h .. 8 h + 7 of
+    // the sixteen columns in token j, and lane l receives column l of tokens 0 .. 7.
+    const int l = fresh_lane(), j = (l & 15) >> 1;
+    const int row = 32 * grp + 4 * (wave & 3) + (j & 3) + 16 * (j >> 2);
+    bytes = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i *)(
+        raw + W::V_OFF + row * W::VROW + c * kWave + 16 * (l >> 4) + 8 * (l & 1)));
+    if (e0) bytes[0] = bytes[1];
 #pragma unroll
     for (int e = 0; e < TOK / 4; ++e) {
       vs[e] = *reinterpret_cast<__attribute__((address_space(3))) const v4f *>(raw + W::S_OFF + (t0 + 16 * e) * 4);
@@ -795,10 +798,12 @@ __device__ __forceinline__ void wide_piece(const SharedArgs &a, char *lds_raw, i
     }
   };
   auto dequantize = [&](int t) __attribute__((always_inline)) {
-    const _Float16 lo = __builtin_bit_cast(_Float16, static_cast<uint16_t>(byte[t] & 0x0Fu));
-    const _Float16 hi = __builtin_bit_cast(_Float16, static_cast<uint16_t>(byte[t] >> 4));
-    even[t] = static_cast<_Float16>(fmaf(static_cast<float>(lo), vs[t >> 2][t & 3], vz[t >> 2][t & 3]));
-    odd[t] = static_cast<_Float16>(fmaf(static_cast<float>(hi), vs[t >> 2][t & 3], vz[t >> 2][t & 3]));
+    // Tokens t and t + 2 of four share a word: the compiler forms each once.
+    const uint32_t w = static_cast<uint32_t>(bytes[t >> 2]) >> (8 * (t & 1));
+    const v2h lo = __builtin_bit_cast(v2h, w & 0x000F000Fu), hi = __builtin_bit_cast(v2h, (w >> 4) & 0x000F000Fu);
+    const float s = vs[t >> 2][t & 3], z = vz[t >> 2][t & 3];
+    even[t] = static_cast<_Float16>(fmaf(static_cast<float>(lo[(t >> 1) & 1]), s, z));
+    odd[t] = static_cast<_Float16>(fmaf(static_cast<float>(hi[(t >> 1) & 1]), s, z));
   };
   auto put = [&](int i, int u) __attribute__((always_inline)) {
     lds_t *dst = lds + W::V16_OFF + (i & 1) * W::V16_BYTES;
