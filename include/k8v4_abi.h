@@ -341,6 +341,12 @@ int k8v4_attn_shared(const void *q, int q_dtype, int64_t q_tok_stride, const int
 /* Workspace bytes k8v4_attn_shared needs, whatever the lengths (-1 on bad arguments). */
 int64_t k8v4_attn_shared_workspace_bytes(int64_t batch, int q_len, int hkv, int head_dim);
 
+/* Which of its two forms k8v4_attn_shared takes for this shape: 1 where the
+ * prefix is attended to by the kernel that holds many query rows, 0 where eight
+ * tokens at a time (or no page is shared); -1 on bad arguments.  Results of
+ * either lie within the same tolerance; a caller never has to ask. */
+int k8v4_attn_shared_many_rows(int64_t batch, int q_len, int hkv, int head_dim, int64_t prefix_len);
+
 /*
  * Reading the cache back: K and V rows of a ragged batch of token ranges,
  * dequantized (the inverse of k8v4_kv_store_paged; the gather and

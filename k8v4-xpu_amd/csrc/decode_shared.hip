@@ -1219,26 +1219,48 @@ void launch_wide(const SharedArgs &a, int tiles, hipStream_t s) {
     shared_wide_kernel<D, HKV, 3><<<grid, block, 0, s>>>(a);
 }
 
-// Which form serves a prefix of `pages` pages for `rows` query rows of a KV head:
-// the many-rows kernel, or the one that takes eight tokens at a time.  Measured
-// (us, eight tokens at a time / many rows, one token a sequence):
-//   D    heads  pages   8 tokens   16         32         64         128
-//   128  4      8       21 / 17    21 / 17    25 / 21    27 / 29    35 / 34
-//   128  4      2,048   41 / 73    56 / 76    89 / 85    154 / 109  331 / 196
-//   128  2      8       19 / 17    19 / 17    20 / 20    22 / 28    25 / 33
-//   128  2      2,048   33 / 44    41 / 47    56 / 54    90 / 69    154 / 114
-//   256  2      8       24 / 19    21 / 20    25 / 28    28 / 33    33 / 39
-//   256  2      2,048   44 / 58    63 / 60    102 / 78   181 / 133  383 / 201
-//   256  4      8       23 / 19    26 / 21    31 / 29    36 / 34    46 / 40
-//   256  4      2,048   64 / 94    101 / 98   186 / 127  351 / 228  693 / 369
-// Over a long prefix many rows pay as soon as they fill about half the waves;
-// over a short one the many-rows piece is the shorter chain while there are few
-// of them, and with more rows it is each sequence's own pages that count, which
-// it serves with one work-group per CU.
-bool wide_pays(int64_t rows, int64_t pages, int hkv, int head_dim) {
-  if (pages >= 256) return rows >= (head_dim == 128 ? 192 : 96);
-  if (hkv == 4 && head_dim == 256) return true;
-  return rows <= (head_dim == 256 ? 96 : 192);
+// Which form serves a prefix of `pages` pages for `rows` query rows of a KV head,
+// of `batch` sequences: the many-rows kernel, or the one that takes eight tokens
+// at a time.  Up to half a block of rows (a quarter at head dim 256) the former is
+// the shorter chain unless the prefix is long beside them; beyond, it pays once the
+// pages that each group of eight tokens would read again outweigh the waves it
+// leaves idle, and with two 128-dim heads also what it loses on each sequence's own
+// pages, which it serves with half as many work-groups.  Measured on both sides of
+// every line, us, eight tokens at a time / many rows, at so many pages (sequences x
+// query tokens, 100 tokens of each sequence's own):
+//   D 128, 4 heads   8 x 1   256: 23.8 / 23.5   384: 25.9 / 26.6   625: 29.3 / 33.9
+//                    5 x 7   192: 30.4 / 29.9   256: 32.4 / 31.3   384: 36.7 / 34.9
+//                    64 x 1  128: 35.0 / 35.7   192: 38.3 / 37.9   256: 41.8 / 40.1
+//                    128 x 1  32: 34.5 / 36.7    64: 38.2 / 39.4    96: 42.2 / 41.6
+//                    48 x 4    8: 28.9 / 29.1    16: 31.3 / 29.7    32: 35.9 / 32.4
+//   D 128, 2 heads   8 x 1   384: 22.7 / 21.5   625: 24.6 / 24.6
+//                    64 x 1  256: 34.2 / 34.9   384: 37.9 / 37.7   625: 44.7 / 40.0
+//                    32 x 4  192: 35.9 / 37.9   256: 39.7 / 39.0   384: 45.1 / 42.3
+//                    256 x 1 192: 54.7 / 56.4   256: 63.0 / 61.2   384: 78.7 / 69.3
+//                    64 x 4   96: 37.2 / 37.9   128: 41.1 / 39.6   192: 48.4 / 43.4
+//   D 256, 2 heads   8 x 1   256: 24.3 / 23.8   384: 26.1 / 26.0   625: 29.1 / 30.3
+//                    24 x 1  256: 31.5 / 33.5   384: 35.4 / 35.4   625: 42.1 / 39.4
+//                    64 x 1  192: 41.3 / 43.4   256: 46.0 / 45.8
+//                    128 x 1  64: 42.1 / 43.9    96: 46.7 / 47.1   128: 51.5 / 49.2
+//                    64 x 4   32: 37.9 / 38.2    64: 47.5 / 43.4
+//   D 256, 4 heads   8 x 1   256: 29.8 / 27.9   384: 31.6 / 32.4   625: 34.9 / 40.8
+//                    5 x 7     8: 24.5 / 29.2   128: 35.2 / 37.3   192: 42.5 / 39.0
+//                    64 x 4    8: 42.8 / 37.9    64: 73.1 / 53.9
+// Over 1,392 shapes (48 to 2,304 rows, 8 to 2,048 pages, 1 to 10 query tokens) the
+// form chosen is 0.2 % slower than the faster one on average and over 10 % slower at
+// eight of them (five sequences of seven tokens over a few pages, four 256-dim heads:
+// 19 %).  With 1,000 own tokens the lines lie at about the same pages (0.7 % on
+// average; two sequences over long prefixes, four 256-dim heads: up to 32 %).
+bool wide_pays(int64_t batch, int64_t rows, int64_t pages, int hkv, int head_dim) {
+  if (rows <= (head_dim == 128 ? 192 : 96)) return rows >= (head_dim == 128 ? 144 : 84) || pages <= 8 * rows;
+  if (head_dim == 256) return hkv == 4 || pages >= 384 || rows * pages >= 80000;
+  if (hkv == 4) return 3 * pages + rows >= 960;
+  return 4 * (pages - batch) + rows >= 1900;
+}
+
+// The form of a call (false where nothing is shared).
+bool takes_many_rows(int64_t batch, int q_len, int hkv, int head_dim, int64_t prefix_pages) {
+  return prefix_pages > 0 && wide_pays(batch, batch * q_len * kGqa, prefix_pages, hkv, head_dim);
 }
 
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -1283,6 +1305,12 @@ SharedShape shape_of(bool wide, int64_t batch, int q_len, int hkv, int head_dim)
 }
 
 constexpr int64_t kMaxBatch = int64_t(1) << 20;
+constexpr int64_t kMaxPrefixPages = int64_t(1) << 24;
+
+bool valid_shape(int64_t batch, int q_len, int hkv, int head_dim) {
+  return batch >= 1 && batch <= kMaxBatch && q_len >= 1 && q_len <= kPage / kGqa && supported_heads(hkv) &&
+         supported_dim(head_dim);
+}
 
 }  // namespace
 
@@ -1298,11 +1326,15 @@ int64_t shared_wait_timeouts() {
 
 }  // namespace k8v4
 
+extern "C" int k8v4_attn_shared_many_rows(int64_t batch, int q_len, int hkv, int head_dim, int64_t prefix_len) {
+  using namespace k8v4;
+  if (!valid_shape(batch, q_len, hkv, head_dim) || prefix_len < 0 || prefix_len / kPage > kMaxPrefixPages) return -1;
+  return takes_many_rows(batch, q_len, hkv, head_dim, prefix_len / kPage) ? 1 : 0;
+}
+
 extern "C" int64_t k8v4_attn_shared_workspace_bytes(int64_t batch, int q_len, int hkv, int head_dim) {
   using namespace k8v4;
-  if (batch < 1 || batch > kMaxBatch || q_len < 1 || q_len * kGqa > kPage || !supported_heads(hkv) ||
-      !supported_dim(head_dim))
-    return -1;
+  if (!valid_shape(batch, q_len, hkv, head_dim)) return -1;
   // Either form, whatever the prefix.
   const int64_t narrow = shape_of(false, batch, q_len, hkv, head_dim).bytes();
   const int64_t wide = shape_of(true, batch, q_len, hkv, head_dim).bytes();
@@ -1329,7 +1361,7 @@ extern "C" int k8v4_attn_shared(const void *q, int q_dtype, int64_t q_tok_stride
   K8V4_REQUIRE(table_width >= 1 && table_width <= (int64_t(1) << 24) / pages_per_block, "block_table width");
   K8V4_REQUIRE(prefix_len >= 0, "negative prefix length");
   const int64_t prefix_pages = prefix_len / kPage;  // whole pages are shared, a part of one is each sequence's own
-  K8V4_REQUIRE(prefix_pages <= (int64_t(1) << 24), "prefix too long");
+  K8V4_REQUIRE(prefix_pages <= kMaxPrefixPages, "prefix too long");
   K8V4_REQUIRE(prefix_pages == 0 || prefix_width >= (prefix_pages + pages_per_block - 1) / pages_per_block,
                "prefix_table has %lld entries, the prefix of %lld tokens needs %lld",
                static_cast<long long>(prefix_width), static_cast<long long>(prefix_len),
@@ -1364,7 +1396,7 @@ extern "C" int k8v4_attn_shared(const void *q, int q_dtype, int64_t q_tok_stride
               static_cast<long long>(need));
     return K8V4_ERR_WORKSPACE;
   }
-  const bool wide = prefix_pages > 0 && wide_pays(batch * q_len * kGqa, prefix_pages, hkv, head_dim);
+  const bool wide = takes_many_rows(batch, q_len, hkv, head_dim, prefix_pages);
   const SharedShape sh = shape_of(wide, batch, q_len, hkv, head_dim);
   const int64_t table_pages = table_width * pages_per_block;
   const int64_t groups = prefix_pages ? sh.groups : 0;

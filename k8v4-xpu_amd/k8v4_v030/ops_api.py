@@ -110,6 +110,7 @@ _EXTRA_SYMBOLS.append((
     _i32,
 ))
 _EXTRA_SYMBOLS.append(("k8v4_attn_shared_workspace_bytes", [_i64, _i32, _i32, _i32], _i64))
+_EXTRA_SYMBOLS.append(("k8v4_attn_shared_many_rows", [_i64, _i32, _i32, _i32, _i64], _i32))
 _EXTRA_SYMBOLS.append((
     "k8v4_verify_drafts",
     [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _i64, _vp, _vp, _i64, _vp, _vp,
@@ -443,6 +444,13 @@ class _Ops:
         n = int(self._lib.k8v4_attn_shared_workspace_bytes(int(batch), int(q_len), int(hkv), int(head_dim)))
         _require(n > 0, "bad shape for the shared-prefix workspace")
         return n
+
+    def attn_shared_many_rows(self, batch: int, q_len: int, hkv: int, head_dim: int, prefix_len: int) -> bool:
+        """Whether :meth:`int8k_int4v_attn_shared` attends to this prefix by the kernel that
+        holds many query rows (False: eight tokens at a time, or no page is shared)."""
+        n = int(self._lib.k8v4_attn_shared_many_rows(int(batch), int(q_len), int(hkv), int(head_dim), int(prefix_len)))
+        _require(n >= 0, "bad shape for the shared-prefix plan")
+        return n == 1
 
     def int8k_int4v_attn_shared(self, q_fp16, k_cache, k_scale, v_cache, v_scale, v_zero, prefix_table, prefix_len,
                                 block_table, seq_lens, workspace, out, q_len, pages_per_block):
