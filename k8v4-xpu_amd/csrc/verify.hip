@@ -22,9 +22,11 @@
 //
 // Two launches.  The first spreads the rows over the chip: one wave sums one
 // piece of kPiece weights (16 a lane), which is enough loads in flight, and
-// writes the sum.  The second takes one work-group per sequence, finds the
-// piece the sample falls in from the V / kPiece sums, rereads that piece
-// alone (it is still in cache) and finds the token.
+// writes the sum, and that of p alone where a refusal leaves the piece no weight.
+// The second takes one work-group per sequence, finds the piece the sample falls
+// in from the V / kPiece sums, rereads that piece alone (it is still in cache) and
+// finds the token; where the weights' sums are all zero it does so once more with
+// p's, so a row without weight costs a search and not a pass.
 #include "k8v4_common.h"
 
 namespace k8v4 {
@@ -52,7 +54,7 @@ struct VerifyArgs {
   int64_t out_stride;
   int32_t *accepted;
   int32_t *next_lens;  // nullable
-  double *sums;        // [batch][pieces]
+  double *sums;        // [batch][2][pieces]: of the weights, and of p alone (see verify_sum_kernel)
   int32_t *chain;      // [batch]: accepted drafts
   int batch, drafts, vocab, pieces;
 };
@@ -160,6 +162,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void verify_sum_kernel(VerifyArgs 
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) load_run<T, VEC>(w.q, at0 + s * kWave * VEC, a.vocab, q[s]);
   }
+  double *sums = a.sums + static_cast<int64_t>(b) * 2 * a.pieces + piece;
   double sum = 0.0;
 #pragma unroll
   for (int s = 0; s < STEPS; ++s)
@@ -169,7 +172,17 @@ __global__ __launch_bounds__(64 * kScanWaves) void verify_sum_kernel(VerifyArgs 
       sum += at0 + s * kWave * VEC + i == w.out ? 0.0 : x;
     }
   sum = wave_sum_f64(sum);
-  if (lane == 0) a.sums[static_cast<int64_t>(b) * a.pieces + piece] = sum;
+  if (lane == 0) sums[0] = sum;
+  if (acc < n && !(sum > 0.0)) {
+    // Read by the second launch only if no piece has any weight left.
+    sum = 0.0;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) sum += weight(p[s][i], 0.f);
+    sum = wave_sum_f64(sum);
+    if (lane == 0) sums[a.pieces] = sum;
+  }
 }
 
 constexpr int kPickThreads = 256;
@@ -251,13 +264,13 @@ __device__ int pick_in_piece(const VerifyArgs &a, const Weights<T> &w, int64_t a
 }
 
 // The sampled token from the per-piece sums, or -1 where no element weighs anything.
-template <typename T, typename Sum>
-__device__ int pick(const VerifyArgs &a, const Weights<T> &w, float u, PickShared *sh, Sum piece_sum) {
+template <typename T>
+__device__ int pick(const VerifyArgs &a, const Weights<T> &w, float u, PickShared *sh, const double *sums) {
   // Thread t holds the consecutive pieces t * per .. t * per + per - 1.
   const int per = (a.pieces + kPickThreads - 1) / kPickThreads;
   const int p0 = static_cast<int>(threadIdx.x) * per, p1 = min(p0 + per, a.pieces);
   double mine = 0.0;
-  for (int i = p0; i < p1; ++i) mine += piece_sum(i);
+  for (int i = p0; i < p1; ++i) mine += sums[i];
   double total;
   const double before = block_scan(mine, sh->scan, &total) - mine;
   if (!(total > 0.0)) return -1;
@@ -265,7 +278,7 @@ __device__ int pick(const VerifyArgs &a, const Weights<T> &w, float u, PickShare
   int first = INT32_MAX, last = -1;
   double run = before;
   for (int i = p0; i < p1; ++i) {
-    const double x = piece_sum(i);
+    const double x = sums[i];
     run += x;
     if (x > 0.0) {
       if (run > target && first == INT32_MAX) first = i;
@@ -276,7 +289,7 @@ __device__ int pick(const VerifyArgs &a, const Weights<T> &w, float u, PickShare
   if (chosen == INT32_MAX) chosen = block_max(last, sh->red);
   if (chosen >= p0 && chosen < p1) {
     double base = before;
-    for (int i = p0; i < chosen; ++i) base += piece_sum(i);
+    for (int i = p0; i < chosen; ++i) base += sums[i];
     sh->base = base;
   }
   __syncthreads();
@@ -290,19 +303,14 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a)
   const int n = draft_count(a, b);
   const int acc = a.chain[b];
   const float u = a.sample_u[b];
-  const double *sums = a.sums + static_cast<int64_t>(b) * a.pieces;
+  const double *sums = a.sums + static_cast<int64_t>(b) * 2 * a.pieces;
   Weights<T> w = weights_of<T>(a, b, n, acc);
-  int token = pick<T>(a, w, u, &sh, [&](int i) { return sums[i]; });
+  int token = pick<T>(a, w, u, &sh, sums);
   if (token < 0 && acc < n) {
     // Refused, and nothing is left of the row: the target's own probabilities.
     w.q = nullptr;
     w.out = -1;
-    token = pick<T>(a, w, u, &sh, [&](int i) {
-      double s = 0.0;
-      const int64_t end = min(static_cast<int64_t>(a.vocab), static_cast<int64_t>(i + 1) * kPiece);
-      for (int64_t v = static_cast<int64_t>(i) * kPiece; v < end; ++v) s += weight(to_float(w.p[v]), 0.f);
-      return s;
-    });
+    token = pick<T>(a, w, u, &sh, sums + a.pieces);
   }
   for (int j = threadIdx.x; j <= a.drafts; j += kPickThreads)
     a.out_tokens[b * a.out_stride + j] = j < acc ? token_at(a, b, j) : j == acc ? token : -1;
@@ -330,7 +338,7 @@ int64_t chain_bytes(int64_t batch) { return (batch * 4 + 255) / 256 * 256; }
 extern "C" int64_t k8v4_verify_drafts_workspace_bytes(int64_t batch, int64_t vocab) {
   using namespace k8v4;
   if (batch < 0 || batch > kMaxBatch || vocab < 1 || vocab > kMaxVocab) return -1;
-  return chain_bytes(batch) + batch * ((vocab + kPiece - 1) / kPiece) * 8;
+  return chain_bytes(batch) + batch * 2 * ((vocab + kPiece - 1) / kPiece) * 8;
 }
 
 extern "C" int k8v4_verify_drafts(const void *target_probs, int dtype, int64_t target_seq_stride,
