@@ -172,7 +172,10 @@ class Xe2K8V4MetadataBuilder(AttentionMetadataBuilder[Xe2K8V4Metadata]):
             list(capture),
             self.layout,
         )
-        return ensure_scratch(self.device, self.layout, *capacity, max_seqs=int(cfg.scheduler_config.max_num_seqs))
+        scratch = ensure_scratch(self.device, self.layout, *capacity, max_seqs=int(cfg.scheduler_config.max_num_seqs))
+        if _engine_shares_prefixes(cfg):
+            scratch.shared_ws()  # with the other workspaces: a step in mid-service must not run out of memory over it
+        return scratch
 
     def use_cascade_attention(
         self,
@@ -396,6 +399,13 @@ class Xe2K8V4Impl(AttentionImpl[Xe2K8V4Metadata]):
 def _runs_alone(width: int, seq_len: int, layout) -> bool:
     _check_covers(seq_len, width)
     return ops().prefill_uses_tiles(seq_len, width, layout.hkv, layout.head_dim)
+
+
+def _engine_shares_prefixes(cfg) -> bool:
+    """Whether the engine may hand :meth:`Xe2K8V4MetadataBuilder.build` a common prefix:
+    prefix caching is on and cascade attention not disabled."""
+    caching = getattr(getattr(cfg, "cache_config", None), "enable_prefix_caching", False)
+    return bool(caching) and not getattr(cfg.model_config, "disable_cascade_attn", False)
 
 
 def _reads_prefix_once(meta: Xe2K8V4Metadata, run: DecodeRun) -> bool:

@@ -13,9 +13,10 @@ a captured HIP graph keeps stable addresses and no call allocates:
   context, and at least what one launch of ``k8v4_prefill_paged_batch``
   (a step's short chunks together) needs.
 
-A third one, the workspace of ``k8v4_attn_shared``, is made the first time a
-step's requests share a prefix worth reading once (engines without prefix
-caching never pay for it).
+A third one, the workspace of ``k8v4_attn_shared``, is made beside them where
+the engine may report a common prefix (the backend's builder asks for it then),
+else by the first step that reads one: engines without prefix caching never pay
+for it.
 
 Capacity is given in the reference's terms (k8v4_v030/scratch.py:17-115):
 ``nprog_max`` = kernel pages of the longest sequence times the KV head count,
