@@ -52,6 +52,7 @@ from .plan import (
     query_segments,
     require_decoder,
     scratch_capacity,
+    shared_prefix_line,
     shared_prefix_pays,
     token_span,
     uniform_packed_q_len,
@@ -191,16 +192,22 @@ class Xe2K8V4MetadataBuilder(AttentionMetadataBuilder[Xe2K8V4Metadata]):
         **_: object,
     ) -> bool:
         """Whether this step gains from reading the common prefix once: one of its
-        decode runs saves enough of the cache (plan.shared_prefix_pays).  The engine
-        runs such a step outside its captured graphs and passes the prefix to
-        :meth:`build`, 0 otherwise."""
+        decode runs saves enough of the cache (plan.shared_prefix_line; the engine
+        runs such a step outside a captured graph of the whole model, which a step
+        that would have replayed one has to make up for).  The engine passes the
+        prefix to :meth:`build` then, 0 otherwise."""
         if use_alibi or use_sliding_window or use_local_attention or dcp_world_size > 1:
             return False
+        if not shared_prefix_pays(len(query_lens), common_prefix_len, self.layout):
+            return False  # not even if all requests were one run
         starts = [0]
         for n in query_lens:
             starts.append(starts[-1] + int(n))
-        runs, _seqs = plan_step(tuple(starts)) if len(starts) > 1 else ((), ())
-        return any(shared_prefix_pays(run.count, common_prefix_len, self.layout) for run in runs)
+        config = getattr(self.vllm_config, "compilation_config", None)
+        line = shared_prefix_line(starts, getattr(config, "cudagraph_capture_sizes", None) or (),
+                                  getattr(getattr(config, "cudagraph_mode", None), "name", None))
+        runs, _seqs = plan_step(tuple(starts))
+        return any(shared_prefix_pays(run.count, common_prefix_len, self.layout, line) for run in runs)
 
     def build(
         self,

@@ -74,23 +74,50 @@ def token_span(starts: Sequence[int], first_request: int, count: int, q_len: int
 
 
 # The bytes of cache a batch has to save before a launch over a shared prefix is
-# used.  It costs 2 to 20 us more than the batch op where it saves nothing (a
-# launch more, the sequences' states joined with the prefix's); both ops were
-# timed for 2 .. 64 sequences of 1 and 4 query tokens over prefixes of 4 .. 1024
-# pages, and broke even between 25 MB saved (8 sequences, one query token, head
-# dim 256) and 200 MB (64 sequences of 4, head dim 128, 4 KV heads, 64 pages:
-# 56 us against 58).  From there on the shared form was the faster one at every
-# shape, by up to 8.5 times (64 sequences, 1024 pages, head dim 256: 129 us
-# against 1094).
+# used in a step whose attention is called eagerly either way.  The launch costs 2 to
+# 20 us more than the batch op where it saves nothing (a launch more, the sequences'
+# states joined with the prefix's).  Both ops were timed at 128, 192 and 256 MiB saved
+# for 2 .. 384 sequences of 1, 4, 7 and 10 query tokens, both head counts and dims, 20
+# and 300 tokens of each sequence's own: at 192 MiB the shared form was 1.0 to 2.0
+# times as fast at every shape but two (sequences of seven tokens: two of them 0.94,
+# four 0.98); at 128 MiB down to 0.93, 0.96 for 256 sequences.
 SHARED_PREFIX_MIN_SAVED = 192 << 20
+# What it has to save where the step would otherwise replay one graph of the whole
+# model: outside it every layer's store and attention are called from Python (80 us a
+# layer), and the other operations too unless graphs of the pieces between are
+# replayed.  Steps of six small layers (2,048 wide, 90 to 120 us beside the attention)
+# were timed whole, the replayed graph with the batch op against the shared op in
+# pieces and in an eager step, 8 .. 256 sequences of 1, 4, 7 and 10 tokens; us a layer,
+# graph / pieces / eager, the least and the largest gain at each size:
+#   192 MiB  256 x 1 178 / 190 / 204   32 x 10 234 / 210 / 207
+#   384 MiB  256 x 1 196 / 192 / 205   32 x 10 287 / 233 / 225
+#   768 MiB   32 x 1 201 / 145 / 198   32 x 10 396 / 273 / 266
+# Over wider layers the calls hide behind the GPU's work and less would do.
+SHARED_PREFIX_MIN_SAVED_PIECES = 384 << 20
+SHARED_PREFIX_MIN_SAVED_EAGER = 768 << 20
 
 
-def shared_prefix_pays(sequences: int, prefix_len: int, layout: PageLayout) -> bool:
+def shared_prefix_pays(sequences: int, prefix_len: int, layout: PageLayout, min_saved: int | None = None) -> bool:
     """Whether ``sequences`` that begin with the same ``prefix_len`` cached tokens are
     decoded faster by ``int8k_int4v_attn_shared`` than by ``int8k_int4v_attn_batch``
-    (which reads the prefix once for each; the other serves any shape too)."""
+    (which reads the prefix once for each; the other serves any shape too): the bytes
+    it does not read again reach ``min_saved`` (None: SHARED_PREFIX_MIN_SAVED)."""
     pages = max(0, int(prefix_len)) // PAGE
-    return (int(sequences) - 1) * pages * layout.page_bytes >= SHARED_PREFIX_MIN_SAVED
+    saved = (int(sequences) - 1) * pages * layout.page_bytes
+    return saved >= (SHARED_PREFIX_MIN_SAVED if min_saved is None else int(min_saved))
+
+
+def shared_prefix_line(query_starts: Sequence[int], capture_sizes: Sequence[int], graph_mode: str | None) -> int:
+    """The bytes a step has to save for its engine to read the common prefix once,
+    which runs the step outside a graph of the whole model.
+
+    Such a graph would have been replayed for a step of one query length and of no
+    more tokens than the largest of ``capture_sizes``, unless ``graph_mode`` (the
+    name of the engine's graph mode, None: not known) has none."""
+    captured = uniform_packed_q_len(query_starts) and int(query_starts[-1]) <= max(capture_sizes, default=0)
+    if not captured or graph_mode in ("NONE", "PIECEWISE"):
+        return SHARED_PREFIX_MIN_SAVED
+    return SHARED_PREFIX_MIN_SAVED_PIECES if graph_mode == "FULL_AND_PIECEWISE" else SHARED_PREFIX_MIN_SAVED_EAGER
 
 
 def scratch_capacity(
