@@ -505,7 +505,7 @@ class _Ops:
         tensors = (q_fp16, k_cache, k_scale, v_cache, v_scale, v_zero, block_table, seq_lens, out, workspace)
         prefix_width = 0
         if prefix_len >= PAGE:
-            _require(prefix_table.dtype == torch.int32 and prefix_table.dim() == 1
+            _require(prefix_table is not None and prefix_table.dtype == torch.int32 and prefix_table.dim() == 1
                      and (prefix_table.shape[0] < 2 or prefix_table.stride(0) == 1),
                      "prefix_table must be a contiguous int32 row")
             prefix_width = int(prefix_table.shape[0])
