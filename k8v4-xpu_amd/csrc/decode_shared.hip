@@ -1354,7 +1354,7 @@ extern "C" int k8v4_attn_shared(const void *q, int q_dtype, int64_t q_tok_stride
   clear_error();
   K8V4_REQUIRE(supported_heads(hkv), "unsupported per-GPU KV head count %d (this library serves 2 or 4)", hkv);
   K8V4_REQUIRE(supported_dim(head_dim), "unsupported head dim %d (this library serves 128 or 256)", head_dim);
-  K8V4_REQUIRE(q_len >= 1 && q_len * kGqa <= kPage, "q_len*GQA exceeds BM (q_len=%d)", q_len);
+  K8V4_REQUIRE(q_len >= 1 && q_len <= kPage / kGqa, "q_len*GQA exceeds BM (q_len=%d)", q_len);
   K8V4_REQUIRE(pages_per_block >= 1, "pages_per_block");
   K8V4_REQUIRE(num_pages >= 1 && num_pages <= INT32_MAX, "num_pages must be 1 .. 2^31 - 1");
   K8V4_REQUIRE(batch >= 1 && batch <= kMaxBatch, "empty or too large batch");

@@ -7,6 +7,15 @@ import torch
 from k8v4_v030.cache_views import bind_regions
 from k8v4_v030.layout import PageLayout
 from k8v4_v030.ops_api import ops
+from test_operator_checks import lib, refused, shared  # noqa: F401
+
+
+@pytest.mark.parametrize("q_len", [2**30, 715827883, 2**31 - 1, -2**31])
+def test_query_lengths_whose_rows_overflow(lib, q_len):  # noqa: F811
+    """6 x 715,827,883 is 2 in 32 bits."""
+    refused(lib, shared, "q_len*GQA exceeds BM", q_len=q_len)
+    assert lib.k8v4_attn_shared_workspace_bytes(4, q_len, 4, 128) == -1
+    assert lib.k8v4_attn_shared_many_rows(4, q_len, 4, 128, 640) == -1
 
 
 def test_a_prefix_without_its_table():
