@@ -3,9 +3,10 @@
 //
 // For every query row (token j of sequence b, query head) with visible end
 // e = seq_len_b - q_len + j + 1, softmax attention over the keys t < e as in
-// k8v4_attn_batch (int8-quantized query rows, exact integer scores, V as
-// (nibble - zero) * scale), where the keys below P (the prefix's whole pages)
-// are those of one table row and the others those of the sequence's own row.
+// k8v4_attn_batch (int8-quantized query rows; exact integer dot products, whose
+// scaling by k_scale is off by at most 0.75 of a unit of the dot; V as (nibble -
+// zero) * scale), where the keys below P (the prefix's whole pages) are those of one
+// table row and the others those of the sequence's own row.
 // With the (max m, sum l, output O / l) of disjoint key ranges i,
 //   out = sum_i 2^(m_i - M) l_i O_i / sum_i 2^(m_i - M) l_i,  M = max m_i,
 // so the prefix and each sequence's own keys are attended to apart, each cut

@@ -12,19 +12,24 @@
 // eight dims.  A work-group takes kRows consecutive rows: its first kRows lanes
 // look up each row's sequence and cache cell once, into LDS; then every thread
 // converts eight dims of one (row, head) at a time, so the 64 lanes of a wave
-// read contiguous codes and write a contiguous kilobyte.
+// read contiguous codes and write a contiguous kilobyte (fp32: two kilobytes by
+// two stores of every other 16 bytes each).
 //
-// A small call is a chain of round trips (starts, table entry, codes).  The
-// search for a row's sequence runs over 256 of row_starts in LDS, read in one
-// of them (a binary search of the array itself is one for each halving); only
-// batches of more than 256 sequences search the array for the rest.  Sixteen
-// rows a work-group: two to eight passes whose loads go out together.
+// A small call is a chain of round trips: starts, first token, table entry, then
+// the passes.  The search for a row's sequence runs over 256 of row_starts in LDS,
+// read in one of them (a binary search of the array itself is one for each
+// halving); only batches of more than 256 sequences search the array for the rest.
+// Sixteen rows a work-group are two to eight passes, one after the other: their
+// branches keep a pass's K loads, K stores, V loads and V stores in that order,
+// each load waited for before the store behind it, so a wave makes two round trips
+// a pass and only the other waves of the CU fill them (in large calls they do).
 //
 // Measured on cold pages in random order, 16-bit outputs, by 16 rows a
 // work-group (by 8, by 32): 500 rows of 4 heads 5.3 us (5.3, 7.3), 19,800 rows of
 // 2 heads at head dim 256 from twelve sequences 12.8 (13.0, 13.5), 262,144 rows of
 // 4 heads 154.6, 4.86 TB/s of codes read and rows written (164.1, 154.6); a copy
-// of 1 GiB moves 5.0 TB/s.
+// of 1 GiB moves 5.0 TB/s.  fp32 outputs: 131,072 rows of 4 heads 179.8 us, 3.58
+// TB/s (half-line stores), 500 rows 6.6.
 #include "k8v4_common.h"
 
 namespace k8v4 {
