@@ -209,6 +209,12 @@ def _call(st, name, bind, op, args):
 
 
 # ---------------------------------------------------------------------- plain forms
+def _over(x, n):
+    """x / n, each quotient rounded once (by a Python number torch multiplies by its
+    reciprocal, an ulp off, which moves codes that lie on a border)."""
+    return x / torch.full_like(x, float(n))
+
+
 def _dequantized(st, slots):
     """fp32 K and V ``[..., hkv, D]`` of the given cache slots."""
     k, ks, v, vs, vz = st["regions"]
@@ -256,12 +262,12 @@ def _plain_rope(st):
     q_out = _rotated(q.float(), cos.float(), sin.float(), case["neox"]).to(q.dtype)
     # The cache's rules in 64 bits: K symmetric int8, half away from zero; V affine uint4.
     k = _rotated(st["k"].double(), cos.double(), sin.double(), case["neox"])
-    ks = k.abs().amax(-1) / 127.0
+    ks = _over(k.abs().amax(-1), 127)
     inv = torch.where(ks == 0, torch.zeros_like(ks), 1.0 / ks)[..., None]
     kc = (torch.sign(k) * torch.floor(k.abs() * inv + 0.5)).clamp(-127, 127).to(torch.int8)
     v = st["v"].double()
     lo = v.amin(-1)
-    vs = ((v.amax(-1) - lo) / 15.0).clamp_min(1.0e-8)
+    vs = _over(v.amax(-1) - lo, 15).clamp_min(1.0e-8)
     vz = torch.floor(-lo / vs + 0.5).clamp(0.0, 15.0)
     vc = torch.floor(v / vs[..., None] + vz[..., None] + 0.5).clamp(0.0, 15.0).to(torch.uint8)
     # Padding goes to a page that no sequence holds.
@@ -283,7 +289,7 @@ def _plain_tree(st):
     batch, dev = lens.shape[0], q.device
     # The query row's int8 rule (half away from zero, in 64 bits).
     x = q.double()
-    scale = x.abs().amax(-1, keepdim=True) / 127.0
+    scale = _over(x.abs().amax(-1, keepdim=True), 127)
     inv = torch.where(scale == 0, torch.zeros_like(scale), 1.0 / scale)
     code = torch.sign(x) * torch.floor(x.abs() * inv + 0.5)
     rows = (code.float() * (scale.float() / math.sqrt(d))).view(batch, n, hkv, GQA, d)
@@ -428,12 +434,12 @@ def _exact_rope(case, st):
     angles = st["cos_sin"][st["positions"]]
     q = _turned(st["q"], angles, case["neox"])
     k = _turned(st["k"], angles, case["neox"])[:n]  # padding lies behind the step's tokens
-    step = k.abs().amax(-1, keepdim=True) / 127.0
+    step = _over(k.abs().amax(-1, keepdim=True), 127)
     y = k * torch.where(step == 0, torch.zeros_like(step), 1.0 / step)
     code = torch.where(y >= 0, torch.floor(y + 0.5), torch.ceil(y - 0.5))
     v = st["v"][:n].double()
     low, high = v.amin(-1, keepdim=True), v.amax(-1, keepdim=True)
-    unit = torch.clamp((high - low) / 15.0, min=1.0e-8)
+    unit = torch.clamp(_over(high - low, 15), min=1.0e-8)
     zero = torch.clamp(torch.floor(-low / unit + 0.5), 0, 15)
     nib = torch.clamp(torch.floor(v / unit + zero + 0.5), 0, 15)
     return q, code * step.float().double(), (nib - zero) * unit.float().double()
@@ -443,7 +449,7 @@ def _exact_tree(case, st):
     hkv, d, n, ppb = case["hkv"], case["head_dim"], case["nodes"], case["ppb"]
     q = st["q"].double()
     amax = q.abs().amax(-1)
-    step = torch.where(amax == 0, torch.ones_like(amax), amax / 127.0)
+    step = torch.where(amax == 0, torch.ones_like(amax), _over(amax, 127))
     y = q * (1.0 / step)[..., None]
     q = torch.where(y >= 0, torch.floor(y + 0.5), torch.ceil(y - 0.5)) * step[..., None]
     out = torch.zeros_like(q)
