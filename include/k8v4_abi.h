@@ -411,6 +411,134 @@ int k8v4_verify_drafts(const void *target_probs, int dtype, int64_t target_seq_s
 /* Workspace bytes k8v4_verify_drafts needs (-1 on bad arguments). */
 int64_t k8v4_verify_drafts_workspace_bytes(int64_t batch, int64_t vocab);
 
+/*
+ * k8v4_kv_store_paged with the keys rotated by their positions on the way, and
+ * the step's queries rotated (no counterpart in the reference, whose model
+ * rotates in kernels of its own before the store).
+ *
+ * k, v, src_dtype, strides, slot_mapping, ntok and cache as in
+ * k8v4_kv_store_paged.  positions: int32, or int64 where positions_are_int64,
+ * [ntok].  cos_sin: [table_rows] rows of `table_dtype` (fp16, bf16 or fp32),
+ * table_stride ELEMENTS apart, each rotary_dim / 2 cosines, then as many
+ * sines.  rotary_dim: a multiple of 16 up to head_dim; dims from it on are not
+ * rotated.  neox: pair i is dims (i, i + rotary_dim / 2), else (2 i, 2 i + 1);
+ * a pair (x, y) becomes (x c - y s, y c + x s).
+ * Keys: the rotated row in float64, unrounded, goes through the K rule; a
+ * token without a slot stores nothing.  Values as in k8v4_kv_store_paged.
+ * q: [ntok, 6*hkv, head_dim] of src_dtype (NULL with q_out NULL: none), head
+ * stride head_dim; q_out: the rotated rows, computed in fp32 and rounded once;
+ * may be q itself (same strides), must not overlap it otherwise.  All tokens'
+ * queries are rotated, those without a slot too.  A position outside the table
+ * stores nothing and gives zero query rows.
+ */
+int k8v4_rope_kv_store_paged(const void *q, const void *k, const void *v, int src_dtype, int64_t q_tok_stride,
+                             int64_t k_tok_stride, int64_t v_tok_stride, const void *positions,
+                             int positions_are_int64, const void *cos_sin, int table_dtype, int64_t table_rows,
+                             int64_t table_stride, int rotary_dim, int neox, const int64_t *slot_mapping,
+                             int64_t ntok, int hkv, int head_dim, int8_t *k_cache, float *k_scale, uint8_t *v_cache,
+                             float *v_scale, float *v_zero, int64_t num_pages, int64_t k_page_stride,
+                             int64_t ks_page_stride, int64_t v_page_stride, int64_t vs_page_stride,
+                             int64_t vz_page_stride, void *q_out, int64_t q_out_stride, void *stream);
+
+/*
+ * k8v4_attn_batch for trees of drafted tokens (no counterpart in the
+ * reference, whose drafts are chains).
+ *
+ * Every sequence has `nodes` (1 .. 64) query tokens, the nodes of its tree,
+ * stored behind its context as its last tokens: node j is the token at position
+ * seq_len - nodes + j.  It attends to the seq_len - nodes tokens ahead of the
+ * tree and to every node i whose bit i is set in tree_masks[b][j] (int64
+ * [batch], rows mask_stride apart, 0: one tree for all), itself only if its own
+ * bit is; bits from `nodes` on, and nodes of a sequence shorter than its tree
+ * that lie before its first token, are ignored.  A row that sees no key outputs zeros.
+ * The chain's mask, 2^(j+1) - 1, gives what k8v4_attn_batch does.  Query
+ * rows, cache, table, seq_lens (the tree's tokens counted), out and numerics as
+ * in k8v4_attn_batch; page strides below 2^31 bytes.
+ * workspace: >= k8v4_attn_tree_workspace_bytes(batch, nodes, hkv, head_dim)
+ * bytes, 16-byte aligned.  Calls that may overlap (other streams, captured
+ * graphs) need one each.
+ */
+int k8v4_attn_tree(const void *q, int q_dtype, int64_t q_tok_stride, const int8_t *k_cache, const float *k_scale,
+                   const uint8_t *v_cache, const float *v_scale, const float *v_zero, int64_t num_pages,
+                   int64_t k_page_stride, int64_t ks_page_stride, int64_t v_page_stride, int64_t vs_page_stride,
+                   int64_t vz_page_stride, const int32_t *block_table, int64_t bt_stride, int64_t table_width,
+                   int pages_per_block, const int32_t *seq_lens, const int64_t *tree_masks, int64_t mask_stride,
+                   int64_t batch, int nodes, int hkv, int head_dim, void *out, int out_dtype, int64_t out_tok_stride,
+                   void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Workspace bytes k8v4_attn_tree needs, whatever the lengths (-1 on bad arguments). */
+int64_t k8v4_attn_tree_workspace_bytes(int64_t batch, int nodes, int hkv, int head_dim);
+
+/*
+ * The branch of a drafted tree that the target's tokens confirm (no
+ * counterpart in the reference, whose engine samples).
+ *
+ * Node 0 of a sequence is its last token, node i > 0 a drafted token
+ * (draft_tokens: int32, or int64 where drafts_are_int64, [batch][nodes]) that
+ * continues node parents[b][i] < i (int32, rows parent_stride apart, 0: one tree for
+ * all); other parents leave the node out of the tree.  target_tokens: int64
+ * [batch][nodes], the token the target chose (greedily or by sampling) after
+ * each node's branch; a negative one confirms nothing.  num_nodes: int32
+ * [batch] (clamped to 0 .. nodes) or NULL for `nodes`.
+ * From node 0 the walk goes to the lowest child whose draft is the token chosen
+ * at the node, over at most `width` (1 .. nodes) nodes.  path: int32
+ * [batch][width], the walk's nodes, then -1.  out_tokens: int64 [batch][width],
+ * the token chosen at each of them, the last one new, then -1.  accepted:
+ * int32 [batch], the walk's nodes behind node 0 (-1 for a sequence without
+ * nodes).  next_lens (NULL: not wanted; may be seq_lens): int32 [batch],
+ * seq_lens + accepted + 1, see k8v4_verify_drafts.
+ */
+int k8v4_accept_tree(const void *draft_tokens, int drafts_are_int64, int64_t draft_stride, const int32_t *parents,
+                     int64_t parent_stride, const int32_t *num_nodes, const int64_t *target_tokens,
+                     int64_t target_stride, const int32_t *seq_lens, int64_t batch, int nodes, int width,
+                     int32_t *path, int64_t path_stride, int64_t *out_tokens, int64_t out_stride, int32_t *accepted,
+                     int32_t *next_lens, void *stream);
+
+/*
+ * The cache rows of an accepted branch moved together (no counterpart in the
+ * reference, whose drafts are chains).
+ *
+ * Sequence b's tree lies in the cache from token seq_starts[b] (int32 [batch])
+ * on.  For i = 0 .. accepted[b] (int32 [batch]; -1: none), i < width, the token
+ * seq_starts[b] + path[b][i] (int32, rows path_stride apart) is copied to token
+ * seq_starts[b] + i, codes and planes unchanged, as if all were read before any is
+ * written.  An entry path[b][i] <= i, or one whose token (or target) lies outside
+ * the table row or on a page outside the cache, moves nothing.  Sequences
+ * must not share the pages of their trees.  block_table as in k8v4_attn_batch.
+ */
+int k8v4_kv_keep_paged(int8_t *k_cache, float *k_scale, uint8_t *v_cache, float *v_scale, float *v_zero,
+                       int64_t num_pages, int64_t k_page_stride, int64_t ks_page_stride, int64_t v_page_stride,
+                       int64_t vs_page_stride, int64_t vz_page_stride, const int32_t *block_table,
+                       int64_t bt_stride, int64_t table_width, int pages_per_block, const int32_t *seq_starts,
+                       const int32_t *path, int64_t path_stride, int width, const int32_t *accepted, int64_t batch,
+                       int hkv, int head_dim, void *stream);
+
+/*
+ * Log probabilities of given tokens with ranks, entropies and likeliest tokens
+ * (no counterpart in the reference, whose engine computes them).
+ *
+ * logits: [rows][vocab] of `dtype`, rows row_stride elements apart.  tokens: int32,
+ * or int64 where tokens_are_int64, [rows], or NULL with logprobs and ranks
+ * unused.  logprobs: fp32 [rows], the natural log of the token's softmax probability;
+ * ranks: int32 [rows], 1 + the number of tokens of larger logit, or of equal logit
+ * and lower index.  A token outside the vocabulary or without probability: minus
+ * infinity and rank 0.  entropy (NULL: not wanted): fp32 [rows], in nats.
+ * top_ids: int64 and top_logprobs: fp32 [rows][top], rows ids_stride and
+ * lps_stride apart, the tokens of rank 1 .. top; -1 and minus infinity where fewer
+ * have any probability.  A logit that is minus infinity or NaN has none; plus
+ * infinities share all of it.  A row without any gives minus infinity, entropy 0.
+ * Sums and logs in fp32 or more.
+ * workspace: >= k8v4_token_logprobs_workspace_bytes(rows, vocab, top) bytes (may be 0),
+ * 16-byte aligned; calls that may overlap need one each.  top <= 64, vocab <= 2^24.
+ */
+int k8v4_token_logprobs(const void *logits, int dtype, int64_t row_stride, const void *tokens, int tokens_are_int64,
+                        int64_t rows, int64_t vocab, int top, float *logprobs, int32_t *ranks, float *entropy,
+                        int64_t *top_ids, int64_t ids_stride, float *top_logprobs, int64_t lps_stride,
+                        void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Workspace bytes k8v4_token_logprobs needs (-1 on bad arguments). */
+int64_t k8v4_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1382,8 +1382,8 @@ extern "C" int64_t k8v4_decode_fault_count(void) {
     set_error("k8v4_decode_fault_count: %s", hipGetErrorString(e));
     return -1;
   }
-  const int64_t shared = shared_wait_timeouts();
-  return shared < 0 ? -1 : n + shared;
+  const int64_t shared = shared_wait_timeouts(), tree = tree_wait_timeouts();
+  return shared < 0 || tree < 0 ? -1 : n + shared + tree;
 }
 
 extern "C" int k8v4_attn_batch_noalloc(const void *q, int q_dtype, int64_t q_tok_stride, const int8_t *k_cache,

@@ -400,12 +400,20 @@ __device__ __forceinline__ void pair_flag_wait(const lds_int *f, int target, int
   if (lane == 0) __hip_atomic_fetch_add(&g_pair_wait_timeouts, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// What rows of a drafted tree see: the tokens ahead of `context`, and of the tree's
+// tokens behind them those whose bit is set in the row's word (row r's is words[r / 6]).
+struct TreeRows {
+  const __attribute__((address_space(3))) uint64_t *words;
+  int context;
+};
+
 // Softmax and P.V of one chunk whose scores chunk_qk produced; reads the V
-// rows and scale planes of the chunk's V slot.
-template <int D, int NT, bool RAISE = false>
+// rows and scale planes of the chunk's V slot.  A row sees the tokens ahead of
+// its st.lim, or (TREE) what `tree` says.
+template <int D, int NT, bool RAISE = false, bool TREE = false>
 __device__ __forceinline__ void chunk_softmax_pv(WaveState<D, NT> &st, const v4i (&sc)[2][NT],
                                                  const lds_t *vslot, int tbase, int L0, int lane, int g,
-                                                 bool masked) {
+                                                 bool masked, TreeRows tree = {}) {
   using S = Slot<D>;
   constexpr int DG = S::DG;
   // Phase fences keep the scheduler from hoisting later LDS reads into this
@@ -457,11 +465,22 @@ __device__ __forceinline__ void chunk_softmax_pv(WaveState<D, NT> &st, const v4i
         t[ml][nt][i] = v;
       }
     if (__builtin_expect(masked, 0)) {
+      if constexpr (TREE) {
+        const uint64_t word = tree.words[(16 * nt + (lane & 15)) / kGqa];
 #pragma unroll
-      for (int ml = 0; ml < 2; ++ml)
+        for (int ml = 0; ml < 2; ++ml)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (tbase + 16 * ml + 4 * g + i >= st.lim[nt]) t[ml][nt][i] = -INFINITY;
+          for (int i = 0; i < 4; ++i) {
+            const int tok = tbase + 16 * ml + 4 * g + i, node = tok - tree.context;
+            if (tok >= L0 || (node >= 0 && !((word >> (node & 63)) & 1))) t[ml][nt][i] = -INFINITY;
+          }
+      } else {
+#pragma unroll
+        for (int ml = 0; ml < 2; ++ml)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (tbase + 16 * ml + 4 * g + i >= st.lim[nt]) t[ml][nt][i] = -INFINITY;
+      }
     }
 #pragma unroll
     for (int ml = 0; ml < 2; ++ml)

@@ -54,6 +54,8 @@ struct PieceArgs {
   void *out;
   int out_dtype;
   int64_t out_tok_stride;  // elements
+  const int64_t *tree_masks;  // drafted trees: a word a query token (else unused)
+  int64_t mask_stride;        // words between sequences
 };
 
 // Length of sequence b's own segments on the axis: its pages behind the
@@ -95,6 +97,8 @@ struct Where {
   int seg;
   int base;
 };
+// MANY: any number of segments a sequence, else at most two.
+template <bool MANY>
 __device__ Where locate(const PieceArgs &a, int lane, int u) {
   Where w;
   const int pre = a.groups * prefix_cost(a);
@@ -113,7 +117,7 @@ __device__ Where locate(const PieceArgs &a, int lane, int u) {
       const int src = __builtin_ctzll(past);
       const int cost = __builtin_amdgcn_readlane(c, src);
       const int first = __builtin_amdgcn_readlane(incl, src) - cost * a.per_seq;
-      const int sub = u >= first + cost ? 1 : 0;  // at most two segments a sequence
+      const int sub = MANY ? (u - first) / cost : u >= first + cost ? 1 : 0;
       w.seg = __builtin_amdgcn_readfirstlane(a.groups + (b0 + src) * a.per_seq + sub);
       w.base = __builtin_amdgcn_readfirstlane(first + sub * cost);
       return w;
@@ -149,13 +153,13 @@ __device__ __forceinline__ args_ptr reread(args_ptr p) {
 
 // Calls piece(args, thread, segment, first page, last page + 1) for the pieces of
 // work-group wg, pages counted from the segment's first (uniform over it).
-template <typename Piece>
+template <bool MANY = false, typename Piece>
 __device__ __forceinline__ void walk_pieces(const PieceArgs &args, int wg, Piece piece) {
   int unit, seg, base;
   {
     const int lane = threadIdx.x & (kWave - 1);
     unit = plan_axis(args, lane, 0).unit;
-    const Where at = locate(args, lane, wg * unit);
+    const Where at = locate<MANY>(args, lane, wg * unit);
     seg = at.seg;
     base = at.base;
   }
@@ -181,7 +185,10 @@ __device__ __forceinline__ void walk_pieces(const PieceArgs &args, int wg, Piece
 
 // Pages s0 .. s1 - 1 of segment `seg` (counted from the segment's first page), by
 // a work-group of WG_WAVES waves (those behind the first HKV * NWH only keep its barriers).
-template <int NT, int HKV, int NWH, bool PH, bool PREFIX, int WG_WAVES = HKV * NWH>
+// TREE: the tokens are a drafted tree's, the words of a segment's eight lie in the
+// LDS behind everything else (kTreeWordBytes).
+constexpr int kTreeWordBytes = kGroup * 8;
+template <int NT, int HKV, int NWH, bool PH, bool PREFIX, int WG_WAVES = HKV * NWH, bool TREE = false>
 __device__ __forceinline__ void attend_piece(const PieceArgs &a, char *lds_raw, int tid, int wg, int seg, int s0, int s1) {
   constexpr int D = 128;  // PH: dims of a half-head
   using S = Slot<D>;
@@ -240,10 +247,17 @@ __device__ __forceinline__ void attend_piece(const PieceArgs &a, char *lds_raw, 
       const int sb = tok / a.q_len;
       end = a.seq_lens[sb] - a.q_len + (tok - sb * a.q_len) + 1;
     }
-    st.lim[nt] = min(end, L0);
+    st.lim[nt] = TREE ? L0 : min(end, L0);
     if (end > 0) far = max(far, kFar - min(st.lim[nt], kFar));
   }
-  const int min_end = kFar - wave_max(far);
+  const int min_end = TREE ? max(L0 - a.q_len, 0) : kFar - wave_max(far);
+  TreeRows tree{};
+  if constexpr (TREE) {
+    auto *words = reinterpret_cast<__attribute__((address_space(3))) uint64_t *>(lds + CFG::LDS_BYTES);
+    if (tid < kGroup) words[tid] = tid < ntok ? static_cast<uint64_t>(a.tree_masks[b * a.mask_stride + sub * kGroup + tid]) : 0;
+    tree.words = words;
+    tree.context = L0 - a.q_len;
+  }
 
   const int my0 = x0 + w;
   const int cnt = my0 < x1 ? (x1 - my0 + NWH - 1) / NWH : 0;
@@ -405,7 +419,7 @@ __device__ __forceinline__ void attend_piece(const PieceArgs &a, char *lds_raw, 
         if (sk == s) mk[s] = issued;
     };
     if (CFG::K_EARLY && k + RK < cnt) refill_k();
-    if (valid) chunk_softmax_pv<D, NT, PH>(st, sc, vslot, tbase, L0, lane, g, tbase + 32 > min_end);
+    if (valid) chunk_softmax_pv<D, NT, PH, TREE>(st, sc, vslot, tbase, L0, lane, g, tbase + 32 > min_end, tree);
     if (!CFG::K_EARLY && k + RK < cnt) {
       if constexpr (PH) pair_flag_wait(flags + CFG::WAVES + (wave ^ 1), k + 1, lane);
       refill_k();

@@ -54,10 +54,11 @@ int q_quant_launch(const void *q, int bf16, int padded, int64_t q_tok_stride, in
 int q_rows_launch(const void *q, int bf16, int64_t q_tok_stride, int64_t tokens, int hkv, int head_dim,
                   int64_t head_rows, int8_t *q8, float *q_scale, hipStream_t stream);
 
-// In-kernel waits of the shared-prefix kernels that gave up on the current
-// device (k8v4_decode_fault_count adds them to the decode kernels'); -1 on a
-// HIP error.
+// In-kernel waits of the shared-prefix and of the tree kernels that gave up on
+// the current device (k8v4_decode_fault_count adds them to the decode kernels');
+// -1 on a HIP error.
 int64_t shared_wait_timeouts();
+int64_t tree_wait_timeouts();
 
 // Loads one element of a 16-bit float tensor as float (exact for fp16 and bf16).
 __device__ __forceinline__ float half_bits_to_float(uint16_t bits, bool is_bf16) {

@@ -36,6 +36,7 @@ COMMON_FLAGS = [
 # by selection before any arithmetic), so max/min need no NaN quieting.
 PER_FILE_FLAGS = {"kv_store.hip": ["-ffp-contract=off"], "q_quant.hip": ["-ffp-contract=off"],
                   "decode.hip": ["-fno-honor-nans"], "decode_shared.hip": ["-fno-honor-nans"],
+                  "decode_tree.hip": ["-fno-honor-nans"],
                   "prefill.hip": ["-fno-honor-nans"]}
 
 

@@ -118,6 +118,36 @@ _EXTRA_SYMBOLS.append((
     _i32,
 ))
 _EXTRA_SYMBOLS.append(("k8v4_verify_drafts_workspace_bytes", [_i64, _i64], _i64))
+_CACHE = [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64]
+_EXTRA_SYMBOLS.append((
+    "k8v4_rope_kv_store_paged",
+    [_vp, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _i32, _vp, _i32, _i64, _i64, _i32, _i32, _vp, _i64, _i32, _i32,
+     *_CACHE, _vp, _i64, _vp],
+    _i32,
+))
+_EXTRA_SYMBOLS.append((
+    "k8v4_attn_tree",
+    [_vp, _i32, _i64, *_CACHE, _vp, _i64, _i64, _i32, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _vp, _i32, _i64,
+     _vp, _i64, _vp],
+    _i32,
+))
+_EXTRA_SYMBOLS.append(("k8v4_attn_tree_workspace_bytes", [_i64, _i32, _i32, _i32], _i64))
+_EXTRA_SYMBOLS.append((
+    "k8v4_accept_tree",
+    [_vp, _i32, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _vp],
+    _i32,
+))
+_EXTRA_SYMBOLS.append((
+    "k8v4_kv_keep_paged",
+    [*_CACHE, _vp, _i64, _i64, _i32, _vp, _vp, _i64, _i32, _vp, _i64, _i32, _i32, _vp],
+    _i32,
+))
+_EXTRA_SYMBOLS.append((
+    "k8v4_token_logprobs",
+    [_vp, _i32, _i64, _vp, _i32, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp],
+    _i32,
+))
+_EXTRA_SYMBOLS.append(("k8v4_token_logprobs_workspace_bytes", [_i64, _i64, _i32], _i64))
 Q_TOKENS, Q_PADDED = 0, 1
 
 
@@ -346,6 +376,70 @@ class _Ops:
         ]
         return BoundCall(self._lib, self._lib.k8v4_kv_store_paged, args, dev, tensors)
 
+    # -- quantize-and-write with the rotation ----------------------------------
+    def rope_kv_store_paged(self, q_fp16, k_fp16, v_fp16, positions, cos_sin, neox, slot_mapping, k_cache, k_scale,
+                            v_cache, v_scale, v_zero, q_out):
+        """:meth:`kv_store_paged` with the keys rotated by their positions on the way, and
+        the queries rotated.
+
+        ``q_fp16`` ``[T, HQ, D]`` and ``q_out`` of its shape and dtype (may be ``q_fp16``;
+        both None: no queries); ``positions`` int32 or int64 ``[T]``; ``cos_sin``
+        ``[P, R]`` (fp16, bf16 or fp32), row p the R / 2 cosines, then the sines of
+        position p, R a multiple of 16 up to D; ``neox``: pairs are dims (i, i + R / 2),
+        else (2 i, 2 i + 1).  Keys are quantized from the unrounded rotation.  A token
+        without a slot stores nothing; one whose position lies outside the table neither,
+        and its query rows become zeros."""
+        bound = self.bind_rope_kv_store_paged(q_fp16, k_fp16, v_fp16, positions, cos_sin, neox, slot_mapping, k_cache,
+                                              k_scale, v_cache, v_scale, v_zero, q_out)
+        if bound is not None:
+            bound()
+
+    def bind_rope_kv_store_paged(self, q_fp16, k_fp16, v_fp16, positions, cos_sin, neox, slot_mapping, k_cache,
+                                 k_scale, v_cache, v_scale, v_zero, q_out):
+        """Validate a rotated store once; returns a :class:`DeviceCall` (None when there are no tokens)."""
+        _require(k_fp16.dim() == 3, "k_fp16 [T,HKV,D]")
+        ntok, hkv, head_dim = (int(x) for x in k_fp16.shape)
+        _require(head_dim in (128, 256), "k_fp16 [T,HKV,D] with D in (128, 256)")
+        _checked_hkv(hkv)
+        _require(k_fp16.dtype == v_fp16.dtype, "k/v_fp16 dtypes differ")
+        _require(v_fp16.shape == k_fp16.shape, "v_fp16 must match k_fp16")
+        _require(slot_mapping.dtype == torch.int64 and slot_mapping.is_contiguous(), "slot_mapping int64")
+        check_paged_k(k_cache, k_scale, hkv, head_dim)
+        check_paged_v(v_cache, v_scale, v_zero, hkv, head_dim)
+        _require(k_cache.shape[0] == v_cache.shape[0], "k/v num_blocks")
+        _require(slot_mapping.shape == (ntok,), "slot_mapping [T]")
+        _require(positions.dtype in (torch.int32, torch.int64) and positions.shape == (ntok,)
+                 and positions.is_contiguous(), "positions must be a contiguous int32 or int64 [T]")
+        _require(cos_sin.dtype in _DTYPE_CODE and cos_sin.dim() == 2, "cos_sin float16, bfloat16 or float32 [P,R]")
+        table_rows, rot = (int(x) for x in cos_sin.shape)
+        _require(rot % 16 == 0 and 16 <= rot <= head_dim and table_rows >= 1,
+                 "cos_sin [P,R] with R a multiple of 16 up to %d" % head_dim)
+        _require(cos_sin.stride(1) == 1, "cos_sin rows must be contiguous")
+        ks = _src_rows(k_fp16, "k_fp16", hkv, head_dim)
+        vs = _src_rows(v_fp16, "v_fp16", hkv, head_dim)
+        _require((q_fp16 is None) == (q_out is None), "q_fp16 and q_out go together")
+        tensors = (k_fp16, v_fp16, positions, cos_sin, slot_mapping, k_cache, k_scale, v_cache, v_scale, v_zero)
+        qs = qos = GQA * hkv * head_dim
+        if q_fp16 is not None:
+            _require(q_fp16.shape == (ntok, GQA * hkv, head_dim), "q_fp16 [T,%d,%d]" % (GQA * hkv, head_dim))
+            _require(q_fp16.dtype == k_fp16.dtype, "q/k_fp16 dtypes differ")
+            _require(q_out.shape == q_fp16.shape and q_out.dtype == q_fp16.dtype, "q_out must match q_fp16")
+            qs = _src_rows(q_fp16, "q_fp16", GQA * hkv, head_dim)
+            qos = _src_rows(q_out, "q_out", GQA * hkv, head_dim)
+            tensors += (q_fp16, q_out)
+        if ntok == 0:
+            return None
+        dev = _on_gpu(*tensors)
+        args = [
+            0 if q_fp16 is None else _ptr(q_fp16), _ptr(k_fp16), _ptr(v_fp16), _DTYPE_CODE[k_fp16.dtype], qs, ks, vs,
+            _ptr(positions), int(positions.dtype == torch.int64), _ptr(cos_sin), _DTYPE_CODE[cos_sin.dtype],
+            table_rows, int(cos_sin.stride(0)) if table_rows > 1 else rot, rot, int(bool(neox)),
+            _ptr(slot_mapping), ntok, hkv, head_dim,
+            *cache_args(k_cache, k_scale, v_cache, v_scale, v_zero),
+            0 if q_out is None else _ptr(q_out), qos,
+        ]
+        return DeviceCall(self._lib, self._lib.k8v4_rope_kv_store_paged, args, dev, tensors)
+
     # -- decode / MTP verify ----------------------------------------------
     def attn_workspace_bytes(self, batch: int, table_width: int, pages_per_block: int, q_len: int,
                              hkv: int, head_dim: int, num_splits: int = 0) -> int:
@@ -522,6 +616,74 @@ class _Ops:
             _ptr(workspace), int(workspace.numel()) * workspace.element_size(),
         ]
         return DeviceCall(self._lib, self._lib.k8v4_attn_shared, args, dev, tensors)
+
+    # -- decode of drafted trees ------------------------------------------------
+    def attn_tree_workspace_bytes(self, batch: int, nodes: int, hkv: int, head_dim: int) -> int:
+        """Scratch bytes :meth:`int8k_int4v_attn_tree` needs (any lengths)."""
+        n = int(self._lib.k8v4_attn_tree_workspace_bytes(int(batch), int(nodes), int(hkv), int(head_dim)))
+        _require(n > 0, "bad shape for the tree workspace")
+        return n
+
+    def int8k_int4v_attn_tree(self, q_fp16, k_cache, k_scale, v_cache, v_scale, v_zero, block_table, seq_lens,
+                              tree_masks, workspace, out, nodes, pages_per_block):
+        """:meth:`int8k_int4v_attn_batch` for trees of drafted tokens.
+
+        Each sequence has ``nodes`` (up to 64) query tokens, stored as its last tokens
+        (``seq_lens`` counts them): node j lies at position ``seq_len - nodes + j`` and
+        attends to the tokens ahead of the tree and to every node i whose bit i is set in
+        ``tree_masks[b, j]`` (int64 ``[B, nodes]``; a row expanded over the batch is one
+        tree for all; :func:`k8v4_v030.plan.tree_masks` makes them from parents).  The
+        other arguments and the numerics are the batch op's; ``workspace`` holds
+        :meth:`attn_tree_workspace_bytes` bytes."""
+        self.bind_int8k_int4v_attn_tree(q_fp16, k_cache, k_scale, v_cache, v_scale, v_zero, block_table, seq_lens,
+                                        tree_masks, workspace, out, nodes, pages_per_block)()
+
+    def bind_int8k_int4v_attn_tree(self, q_fp16, k_cache, k_scale, v_cache, v_scale, v_zero, block_table, seq_lens,
+                                   tree_masks, workspace, out, nodes, pages_per_block):
+        """Validate one tree call; returns a :class:`DeviceCall` that launches it.
+
+        Lengths, tables, masks and queries may change between launches."""
+        nodes, pages_per_block = int(nodes), int(pages_per_block)
+        _require(pages_per_block >= 1, "pages_per_block")
+        _require(1 <= nodes <= 64, "1 to 64 nodes a tree")
+        _require(q_fp16.dim() == 3, "q_fp16 [T,HQ,D]")
+        tokens, heads, head_dim = (int(x) for x in q_fp16.shape)
+        _require(head_dim in (128, 256), "q_fp16 [T,HQ,D] with D in (128, 256)")
+        _require(heads % GQA == 0, "q_fp16 heads must be a multiple of GQA=6")
+        hkv = _checked_hkv(heads // GQA)
+        _require(q_fp16.dtype in (torch.float16, torch.bfloat16), "q_fp16 must be float16 or bfloat16")
+        _require(q_fp16.stride()[1:] == (head_dim, 1), "q_fp16 head/dim strides")
+        _require(out.shape == q_fp16.shape, "out shape")
+        _require(out.dtype in (torch.float16, torch.bfloat16, torch.float32), "out float16, bfloat16 or float32")
+        _require(out.stride()[1:] == (head_dim, 1), "out head/dim strides")
+        _require(tokens % nodes == 0, "T must be B*nodes")
+        batch = tokens // nodes
+        _require(batch >= 1, "empty batch")
+        check_paged_k(k_cache, k_scale, hkv, head_dim)
+        check_paged_v(v_cache, v_scale, v_zero, hkv, head_dim)
+        _require(k_cache.shape[0] == v_cache.shape[0], "k/v num_blocks")
+        _require(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == batch,
+                 "block_table int32 [B, splits]")
+        _require(int(block_table.shape[1]) > 0, "block_table n_splits")
+        _require(block_table.stride(1) == 1, "block_table rows must be contiguous")
+        _require(seq_lens.dtype == torch.int32 and seq_lens.numel() >= batch and seq_lens.is_contiguous(),
+                 "seq_lens must be a contiguous int32 [B]")
+        _require(tree_masks.dtype == torch.int64 and tree_masks.shape == (batch, nodes)
+                 and (nodes == 1 or tree_masks.stride(1) == 1), "tree_masks int64 [B,nodes] with contiguous rows")
+        _require(workspace.is_contiguous(), "workspace must be a contiguous buffer")
+        tensors = (q_fp16, k_cache, k_scale, v_cache, v_scale, v_zero, block_table, seq_lens, tree_masks, out, workspace)
+        dev = _on_gpu(*tensors)
+        row = heads * head_dim
+        args = [
+            _ptr(q_fp16), _DTYPE_CODE[q_fp16.dtype], int(q_fp16.stride(0)) if tokens > 1 else row,
+            *cache_args(k_cache, k_scale, v_cache, v_scale, v_zero),
+            _ptr(block_table), int(block_table.stride(0)) if batch > 1 else int(block_table.shape[1]),
+            int(block_table.shape[1]), pages_per_block, _ptr(seq_lens),
+            _ptr(tree_masks), int(tree_masks.stride(0)) if batch > 1 else nodes, batch, nodes, hkv, head_dim,
+            _ptr(out), _DTYPE_CODE[out.dtype], int(out.stride(0)) if tokens > 1 else row,
+            _ptr(workspace), int(workspace.numel()) * workspace.element_size(),
+        ]
+        return DeviceCall(self._lib, self._lib.k8v4_attn_tree, args, dev, tensors)
 
     # -- chunked prefill ----------------------------------------------------
     def prefill_workspace_bytes(self, seq_len: int, q_len: int, hkv: int, head_dim: int) -> int:
@@ -834,6 +996,184 @@ class _Ops:
             _ptr(workspace), int(workspace.numel()) * workspace.element_size(),
         ]
         return DeviceCall(self._lib, self._lib.k8v4_verify_drafts, args, dev, tensors)
+
+    # -- the accepted branch of a drafted tree ------------------------------------
+    def accept_tree(self, draft_tokens, parents, target_tokens, seq_lens, path, out_tokens, accepted, next_lens,
+                    num_nodes=None):
+        """The branch of each drafted tree that the target's tokens confirm.
+
+        ``draft_tokens`` int32 or int64 ``[B, N]`` (N up to 64; node 0 is the sequence's
+        last token, its draft is not read); ``parents`` int32 ``[B, N]`` (a row expanded
+        over the batch: one tree for all), ``parents[i] < i``; ``target_tokens`` int64
+        ``[B, N]``: what the target chose after each node; ``num_nodes`` int32 ``[B]``
+        (None: N each).  From node 0 the walk goes to the lowest child whose draft is the
+        token chosen at its parent, over at most ``path.shape[1]`` nodes.  ``path`` int32
+        ``[B, W]``: its nodes, then -1; ``out_tokens`` int64 ``[B, W]``: the token chosen at
+        each, then -1; ``accepted`` int32 ``[B]``: its nodes behind node 0; ``next_lens``
+        int32 ``[B]`` (None: not wanted; may be ``seq_lens``): ``seq_lens + accepted + 1``."""
+        bound = self.bind_accept_tree(draft_tokens, parents, target_tokens, seq_lens, path, out_tokens, accepted,
+                                      next_lens, num_nodes)
+        if bound is not None:
+            bound()
+
+    def bind_accept_tree(self, draft_tokens, parents, target_tokens, seq_lens, path, out_tokens, accepted, next_lens,
+                         num_nodes=None):
+        """Validate one acceptance; returns a :class:`DeviceCall` (None for an empty batch)."""
+        _require(draft_tokens.dim() == 2 and draft_tokens.dtype in (torch.int32, torch.int64),
+                 "draft_tokens int32 or int64 [B,N]")
+        batch, nodes = (int(x) for x in draft_tokens.shape)
+        _require(1 <= nodes <= 64, "1 to 64 nodes a tree")
+        _require(parents.dtype == torch.int32 and parents.shape == (batch, nodes), "parents int32 [B,N]")
+        _require(target_tokens.dtype == torch.int64 and target_tokens.shape == (batch, nodes), "target_tokens int64 [B,N]")
+        _require(path.dtype == torch.int32 and path.dim() == 2 and path.shape[0] == batch, "path int32 [B,W]")
+        width = int(path.shape[1])
+        _require(1 <= width <= nodes, "path [B,W] with W of 1 .. N")
+        _require(out_tokens.dtype == torch.int64 and out_tokens.shape == (batch, width), "out_tokens int64 [B,W]")
+        for name, x in (("draft_tokens", draft_tokens), ("parents", parents), ("target_tokens", target_tokens),
+                        ("path", path), ("out_tokens", out_tokens)):
+            _require(x.shape[1] == 1 or x.stride(1) == 1, "%s rows must be contiguous" % name)
+        _require(next_lens is None or seq_lens is not None, "next_lens needs seq_lens")
+        tensors = (draft_tokens, parents, target_tokens, path, out_tokens, accepted)
+        for name, x in (("accepted", accepted), ("seq_lens", seq_lens), ("next_lens", next_lens),
+                        ("num_nodes", num_nodes)):
+            if x is not None or name == "accepted":
+                _require(x is not None and x.dtype == torch.int32 and x.shape == (batch,) and x.is_contiguous(),
+                         "%s must be a contiguous int32 [B]" % name)
+                if name != "accepted":
+                    tensors += (x,)
+        if batch == 0:
+            return None
+        dev = _on_gpu(*tensors)
+        many = batch > 1
+        args = [
+            _ptr(draft_tokens), int(draft_tokens.dtype == torch.int64), int(draft_tokens.stride(0)) if many else nodes,
+            _ptr(parents), int(parents.stride(0)) if many else nodes, 0 if num_nodes is None else _ptr(num_nodes),
+            _ptr(target_tokens), int(target_tokens.stride(0)) if many else nodes,
+            0 if seq_lens is None else _ptr(seq_lens), batch, nodes, width,
+            _ptr(path), int(path.stride(0)) if many else width, _ptr(out_tokens),
+            int(out_tokens.stride(0)) if many else width, _ptr(accepted), 0 if next_lens is None else _ptr(next_lens),
+        ]
+        return DeviceCall(self._lib, self._lib.k8v4_accept_tree, args, dev, tensors)
+
+    def kv_keep_paged(self, k_cache, k_scale, v_cache, v_scale, v_zero, block_table, seq_starts, path, accepted,
+                      pages_per_block):
+        """The cache rows of each accepted branch moved to the places of a linear sequence.
+
+        The tree of sequence b lies in the cache from token ``seq_starts[b]`` (int32
+        ``[B]``) on; token ``seq_starts[b] + path[b, i]`` is copied to ``seq_starts[b] + i``
+        for i up to ``accepted[b]`` (:meth:`accept_tree` gives ``path`` int32 ``[B, W]`` and
+        ``accepted`` int32 ``[B]``), codes and planes unchanged.  Once per layer.  Entries
+        ``path[b, i] <= i`` or outside the table or cache move nothing; sequences must not
+        share the pages that their trees lie on."""
+        bound = self.bind_kv_keep_paged(k_cache, k_scale, v_cache, v_scale, v_zero, block_table, seq_starts, path,
+                                        accepted, pages_per_block)
+        if bound is not None:
+            bound()
+
+    def bind_kv_keep_paged(self, k_cache, k_scale, v_cache, v_scale, v_zero, block_table, seq_starts, path, accepted,
+                           pages_per_block):
+        """Validate one move; returns a :class:`DeviceCall` (None where there is nothing to move)."""
+        _require(k_cache.dim() == 4 and v_cache.dim() == 4, "k_cache [num_blocks,64,HKV,D] NHD")
+        hkv, head_dim = _checked_hkv(int(k_cache.shape[2])), int(k_cache.shape[3])
+        _require(head_dim in (128, 256), "k_cache head dim must be 128 or 256")
+        check_paged_k(k_cache, k_scale, hkv, head_dim)
+        check_paged_v(v_cache, v_scale, v_zero, hkv, head_dim)
+        _require(k_cache.shape[0] == v_cache.shape[0], "k/v num_blocks")
+        _require(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1,
+                 "block_table must be int32 [B, W] with unit column stride")
+        batch = int(block_table.shape[0])
+        for name, x in (("seq_starts", seq_starts), ("accepted", accepted)):
+            _require(x.dtype == torch.int32 and x.shape == (batch,) and x.is_contiguous(),
+                     "%s must be a contiguous int32 [B]" % name)
+        _require(path.dtype == torch.int32 and path.dim() == 2 and path.shape[0] == batch, "path int32 [B,W]")
+        width = int(path.shape[1])
+        _require(width <= 1 or path.stride(1) == 1, "path rows must be contiguous")
+        _require(int(pages_per_block) >= 1, "pages_per_block")
+        if batch == 0 or width == 0:
+            return None
+        _require(int(block_table.shape[1]) > 0, "block_table width")
+        tensors = (k_cache, k_scale, v_cache, v_scale, v_zero, block_table, seq_starts, path, accepted)
+        dev = _on_gpu(*tensors)
+        many = batch > 1
+        args = [
+            *cache_args(k_cache, k_scale, v_cache, v_scale, v_zero),
+            _ptr(block_table), int(block_table.stride(0)) if many else int(block_table.shape[1]),
+            int(block_table.shape[1]), int(pages_per_block), _ptr(seq_starts), _ptr(path),
+            int(path.stride(0)) if many else width, width, _ptr(accepted), batch, hkv, head_dim,
+        ]
+        return DeviceCall(self._lib, self._lib.k8v4_kv_keep_paged, args, dev, tensors)
+
+    # -- log probabilities ---------------------------------------------------------
+    def token_logprobs_workspace_bytes(self, rows: int, vocab: int, top: int) -> int:
+        """Scratch bytes :meth:`token_logprobs` needs (may be 0)."""
+        n = int(self._lib.k8v4_token_logprobs_workspace_bytes(int(rows), int(vocab), int(top)))
+        _require(n >= 0, "bad shape for the log probability workspace")
+        return n
+
+    def token_logprobs(self, logits, tokens, workspace, logprobs, ranks, entropy, top_ids, top_logprobs):
+        """Log probabilities, ranks, entropies and likeliest tokens of rows of logits.
+
+        ``logits`` ``[N, V]`` (fp16, bf16 or fp32, rows of any stride); ``tokens`` int32 or
+        int64 ``[N]`` with ``logprobs`` fp32 ``[N]`` and ``ranks`` int32 ``[N]`` (all three
+        None: not wanted); ``entropy`` fp32 ``[N]`` (None: not wanted), in nats; ``top_ids``
+        int64 and ``top_logprobs`` fp32 ``[N, K]`` (K up to 64; both None: not wanted), the K
+        likeliest tokens, of equal logits the lower index first.  Rank 1 is the likeliest
+        token.  Logits of minus infinity or NaN have no probability: rank 0, -inf; where a row
+        has fewer than K others, ids -1 and -inf.  ``workspace`` holds
+        :meth:`token_logprobs_workspace_bytes` bytes (None where that is 0)."""
+        bound = self.bind_token_logprobs(logits, tokens, workspace, logprobs, ranks, entropy, top_ids, top_logprobs)
+        if bound is not None:
+            bound()
+
+    def bind_token_logprobs(self, logits, tokens, workspace, logprobs, ranks, entropy, top_ids, top_logprobs):
+        """Validate one call; returns a :class:`DeviceCall` (None for no rows)."""
+        _require(logits.dim() == 2 and logits.dtype in _DTYPE_CODE, "logits float16, bfloat16 or float32 [N,V]")
+        rows, vocab = (int(x) for x in logits.shape)
+        _require(vocab >= 1 and (vocab == 1 or logits.stride(1) == 1), "logits rows must be contiguous")
+        tensors = (logits,)
+        _require((tokens is None) == (logprobs is None) and (tokens is None) == (ranks is None),
+                 "tokens, logprobs and ranks go together")
+        if tokens is not None:
+            _require(tokens.dtype in (torch.int32, torch.int64) and tokens.shape == (rows,) and tokens.is_contiguous(),
+                     "tokens must be a contiguous int32 or int64 [N]")
+            _require(ranks.dtype == torch.int32 and ranks.shape == (rows,) and ranks.is_contiguous(),
+                     "ranks must be a contiguous int32 [N]")
+            tensors += (tokens, logprobs, ranks)
+        for name, x in (("logprobs", logprobs), ("entropy", entropy)):
+            if x is not None:
+                _require(x.dtype == torch.float32 and x.shape == (rows,) and x.is_contiguous(),
+                         "%s must be a contiguous float32 [N]" % name)
+        if entropy is not None:
+            tensors += (entropy,)
+        _require((top_ids is None) == (top_logprobs is None), "top_ids and top_logprobs go together")
+        top = 0
+        if top_ids is not None:
+            _require(top_ids.dtype == torch.int64 and top_ids.dim() == 2 and top_ids.shape[0] == rows, "top_ids int64 [N,K]")
+            top = int(top_ids.shape[1])
+            _require(top <= 64, "0 to 64 likeliest tokens")
+            _require(top_logprobs.dtype == torch.float32 and top_logprobs.shape == top_ids.shape, "top_logprobs float32 [N,K]")
+            _require(top <= 1 or (top_ids.stride(1) == 1 and top_logprobs.stride(1) == 1),
+                     "top_ids/top_logprobs rows must be contiguous")
+            if top:
+                tensors += (top_ids, top_logprobs)
+        if workspace is not None:
+            _require(workspace.is_contiguous(), "log probability workspace must be a contiguous buffer")
+            tensors += (workspace,)
+        if rows == 0:
+            return None
+        dev = _on_gpu(*tensors)
+        many = rows > 1
+        args = [
+            _ptr(logits), _DTYPE_CODE[logits.dtype], int(logits.stride(0)) if many else vocab,
+            0 if tokens is None else _ptr(tokens), int(tokens is not None and tokens.dtype == torch.int64),
+            rows, vocab, top, 0 if tokens is None else _ptr(logprobs), 0 if tokens is None else _ptr(ranks),
+            0 if entropy is None else _ptr(entropy),
+            _ptr(top_ids) if top else 0, int(top_ids.stride(0)) if top and many else top,
+            _ptr(top_logprobs) if top else 0, int(top_logprobs.stride(0)) if top and many else top,
+            0 if workspace is None else _ptr(workspace),
+            0 if workspace is None else int(workspace.numel()) * workspace.element_size(),
+        ]
+        return DeviceCall(self._lib, self._lib.k8v4_token_logprobs, args, dev, tensors)
 
     # -- the Q-once tile and the ops that read it ----------------------------
     def q_quant_once(self, q_fp16, q8, q_scale):

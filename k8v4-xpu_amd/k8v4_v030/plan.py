@@ -73,6 +73,29 @@ def token_span(starts: Sequence[int], first_request: int, count: int, q_len: int
     return t0, t1 - t0
 
 
+def tree_depths(parents: Sequence[int]) -> list[int]:
+    """Depth of every node of a drafted tree (node 0 the root, ``parents[i] < i`` for the
+    others): what a node's position lies behind its sequence's context."""
+    depths: list[int] = []
+    for i, parent in enumerate(parents):
+        if i and not 0 <= int(parent) < i:
+            raise ValueError("node %d has parent %d; a parent comes before its children" % (i, int(parent)))
+        depths.append(depths[int(parent)] + 1 if i else 0)
+    return depths
+
+
+def tree_masks(parents: Sequence[int]) -> list[int]:
+    """The int64 words of a drafted tree's attention: bit j of word i is set where node
+    j is node i or on its branch to the root."""
+    if len(parents) > 64:
+        raise ValueError("a tree has at most 64 nodes, got %d" % len(parents))
+    tree_depths(parents)
+    words: list[int] = []
+    for i, parent in enumerate(parents):
+        words.append((words[int(parent)] if i else 0) | 1 << i)
+    return [w - (1 << 64) if w >> 63 else w for w in words]  # as signed words
+
+
 # The bytes of cache a batch has to save before a launch over a shared prefix is
 # used in a step whose attention is called eagerly either way.  The launch costs 2 to
 # 20 us more than the batch op where it saves nothing (a launch more, the sequences'
@@ -219,6 +242,8 @@ __all__ = [
     "scratch_capacity",
     "split_state_bytes",
     "token_span",
+    "tree_depths",
+    "tree_masks",
     "uniform_packed_q_len",
     "workspace_programs",
 ]
