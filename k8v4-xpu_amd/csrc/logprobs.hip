@@ -17,15 +17,24 @@ namespace k8v4 {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
 constexpr int kMaxTop = 64;
+constexpr int kMaxSlices = 64;  // one lane each when they are joined
+constexpr int kGroupLanes = 8;  // lanes whose vectors make a chunk
+constexpr int kBatch = 4;       // vectors of a thread in flight
+constexpr int kMaxListed = 256;
+constexpr int kSliceUnit = 2048;        // elements of a slice at least, and its length's unit
+constexpr int kMaxSliceLen = 1 << 18;   // its chunks' maxima fit the LDS
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kFarBelow = -1000.f;  // exp of it is 0
 
 struct LogprobArgs {
   const void *logits;
   int64_t row_stride;  // elements
   const void *tokens;  // nullable; int32 or int64
   int tokens64;
-  int64_t rows;
   int vocab, top;
+  int slices, slice_len;  // elements, a multiple of kThreads * 8
   float *logprobs;
   int32_t *ranks;
   float *entropy;  // nullable
@@ -33,24 +42,126 @@ struct LogprobArgs {
   int64_t ids_stride;
   float *top_logprobs;
   int64_t lps_stride;
+  char *ws;  // slices > 1: [row][slice] a Part and `top` Listed
 };
 
-template <typename T>
-__device__ __forceinline__ float logit(T x) {
-  const float f = static_cast<float>(x);
-  return f != f ? -INFINITY : f;
+// What a slice says of its row: the largest logit, the sums of the others against
+// it (see Sums), and how many of its tokens are ahead of the given one.
+struct Part {
+  float m, rest, mean;
+  int before;
+};
+struct Listed {
+  float x;
+  int i;
+};
+
+__host__ __device__ inline int64_t part_bytes(int top) {
+  return static_cast<int64_t>(sizeof(Part)) + top * static_cast<int64_t>(sizeof(Listed));
 }
+
+// A logit that is NaN counts as minus infinity.
+__device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x; }
 
 // Whether (x, i) comes ahead of (y, j).
 __device__ __forceinline__ bool ahead(float x, int i, float y, int j) { return x > y || (x == y && i < j); }
 
+// The largest of three without the compiler's quieting of each operand: a quiet
+// NaN gives way to the others, a signalling one makes the result NaN.
+__device__ __forceinline__ float max3_raw(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+// The next larger value of fp32 (x not NaN or plus infinity).
+__device__ __forceinline__ float next_above(float x) {
+  const int b = __float_as_int(x + 0.f);
+  return x == 0.f ? __int_as_float(1) : __int_as_float(b + (b < 0 ? -1 : 1));
+}
+
+// Sums over a set of logits with largest element m: r = sum exp(y) and q = sum y
+// exp(y), y = x - m, over all but one element of value m.
+struct Sums {
+  float m, r, q;  // m = -inf: the set is empty
+};
+// The sums against a larger maximum.  `own`: this holder counts the element left out.
+__device__ __forceinline__ void raise(Sums &s, float m, bool own) {
+  if (s.m == m) return;
+  if (s.m > -INFINITY) {
+    const float d = m == INFINITY ? kFarBelow : fmaxf(s.m - m, kFarBelow);
+    const float f = __builtin_amdgcn_exp2f(d * kLog2e);
+    s.r += own ? 1.f : 0.f;
+    s.q = f > 0.f ? (s.q + d * s.r) * f : 0.f;
+    s.r *= f;
+  }
+  s.m = m;
+}
+// Two disjoint sets as one.
+__device__ __forceinline__ Sums join(Sums a, Sums b) {
+  if (a.m < b.m) {
+    const Sums t = a;
+    a = b;
+    b = t;
+  }
+  const bool tie = a.m == b.m && a.m > -INFINITY;
+  raise(b, a.m, true);
+  a.r += b.r + (tie ? 1.f : 0.f);
+  a.q += b.q;
+  return a;
+}
+
+__device__ __forceinline__ float wave_max_f32(float x) {
+#pragma unroll
+  for (int m = 1; m < kWave; m <<= 1) x = fmaxf(x, __shfl_xor(x, m, kWave));
+  return x;
+}
+__device__ __forceinline__ float wave_sum_f32(float x) {
+#pragma unroll
+  for (int m = 1; m < kWave; m <<= 1) x += __shfl_xor(x, m, kWave);
+  return x;
+}
+
+// Max over eight consecutive lanes, without the LDS.
+template <int CTRL>
+__device__ __forceinline__ float max_dpp(float x) {
+  const int y = __builtin_amdgcn_update_dpp(__float_as_int(x), __float_as_int(x), CTRL, 0xF, 0xF, false);
+  return fmaxf(x, __int_as_float(y));
+}
+__device__ __forceinline__ float max_of_8(float x) {
+  x = max_dpp<0xB1>(x);   // quad_perm 1,0,3,2
+  x = max_dpp<0x4E>(x);   // quad_perm 2,3,0,1
+  return max_dpp<0x141>(x);  // row_half_mirror
+}
+
+template <typename T>
+struct Vec {
+  static constexpr int N = 16 / sizeof(T);
+  T x[N];
+};
+// Elements at .. at + N - 1 of a row; those from `end` on read as minus infinity.
+template <typename T>
+__device__ __forceinline__ void load_vec(const T *row, int at, int end, Vec<T> &v) {
+  if (at + Vec<T>::N <= end) {
+    __builtin_memcpy(v.x, row + at, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N; ++i) v.x[i] = at + i < end ? row[at + i] : static_cast<T>(-INFINITY);
+  }
+}
+
 struct Shared {
-  float x[kThreads / kWave];
-  int i[kThreads / kWave];
-  double d[kThreads / kWave];
+  Part part[kWaves];
+  float best[kThreads];
+  Listed list[kMaxListed];
+  Listed picked[kMaxTop], final[kMaxTop];
+  float red_x[kWaves];
+  int red_i[kWaves];
+  int count;
+  float floor;
 };
 
-// The foremost of the work-group's elements.
+// The foremost of the work-group's pairs, the same for every thread.
 __device__ void block_first(float &x, int &i, Shared &sh) {
 #pragma unroll
   for (int m = 1; m < kWave; m <<= 1) {
@@ -63,107 +174,369 @@ __device__ void block_first(float &x, int &i, Shared &sh) {
   }
   __syncthreads();
   if ((threadIdx.x & (kWave - 1)) == 0) {
-    sh.x[threadIdx.x / kWave] = x;
-    sh.i[threadIdx.x / kWave] = i;
+    sh.red_x[threadIdx.x / kWave] = x;
+    sh.red_i[threadIdx.x / kWave] = i;
   }
   __syncthreads();
-  x = sh.x[0];
-  i = sh.i[0];
+  x = sh.red_x[0];
+  i = sh.red_i[0];
 #pragma unroll
-  for (int w = 1; w < kThreads / kWave; ++w)
-    if (ahead(sh.x[w], sh.i[w], x, i)) {
-      x = sh.x[w];
-      i = sh.i[w];
+  for (int w = 1; w < kWaves; ++w)
+    if (ahead(sh.red_x[w], sh.red_i[w], x, i)) {
+      x = sh.red_x[w];
+      i = sh.red_i[w];
     }
 }
 
-__device__ double block_sum(double x, Shared &sh) {
-#pragma unroll
-  for (int m = 1; m < kWave; m <<= 1) x += __shfl_xor(x, m, kWave);
+// The foremost `want` of `n` pairs (x(e), id(e)) into `out`, in order, and their
+// number (fewer where the others are minus infinity).  Every thread calls it.  A
+// floor that at least `want` pairs reach, from one maximum a thread, leaves few to
+// rank; where too many reach it (ties), they are taken one at a time.
+template <typename X, typename I>
+__device__ int foremost(int n, int want, X x, I id, Listed *out, Shared &sh) {
+  const int t = threadIdx.x;
+  float best = -INFINITY;
+  for (int e = t; e < n; e += kThreads) best = fmaxf(best, x(e));
+  sh.best[t] = best;
+  if (t == 0) sh.count = 0;
   __syncthreads();
-  if ((threadIdx.x & (kWave - 1)) == 0) sh.d[threadIdx.x / kWave] = x;
-  __syncthreads();
-  double r = 0.0;
+  if (t < kWave) {
+    // The largest floor of 16 bits that `want` threads' maxima reach, bit by bit; as
+    // ordered integers, so that a bit set is a larger value.
+    uint32_t key[kWaves];
 #pragma unroll
-  for (int w = 0; w < kThreads / kWave; ++w) r += sh.d[w];
+    for (int w = 0; w < kWaves; ++w) {
+      const int bits = __float_as_int(sh.best[w * kWave + t] + 0.f);
+      key[w] = static_cast<uint32_t>(bits < 0 ? ~bits : bits | static_cast<int>(0x80000000u));
+    }
+    uint32_t floor = 0;
+#pragma unroll
+    for (int b = 31; b >= 16; --b) {
+      const uint32_t f = floor | 1u << b;
+      int reach = 0;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) reach += __popcll(__ballot(key[w] >= f));
+      if (reach >= want) floor = f;
+    }
+    const int back = floor & 0x80000000u ? static_cast<int>(floor & 0x7FFFFFFFu) : ~static_cast<int>(floor);
+    const float value = __int_as_float(back);
+    if (t == 0) sh.floor = value == value ? value : -INFINITY;  // (below minus infinity the bits are a NaN's)
+  }
+  __syncthreads();
+  const float floor = sh.floor;
+  for (int e = t; e < n; e += kThreads) {
+    const float v = x(e);
+    if (v >= floor && v > -INFINITY) {
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kMaxListed) sh.list[at] = {v, id(e)};
+    }
+  }
+  __syncthreads();
+  const int listed = sh.count;
+  if (listed <= kMaxListed) {
+    if (t < listed) {
+      const Listed mine = sh.list[t];
+      int rank = 0;
+      for (int j = 0; j < listed; ++j) rank += ahead(sh.list[j].x, sh.list[j].i, mine.x, mine.i);
+      if (rank < want) out[rank] = mine;
+    }
+    __syncthreads();
+    return min(listed, want);
+  }
+  float last = INFINITY;
+  int ilast = -1;
+  for (int k = 0; k < want; ++k) {
+    float v = -INFINITY;
+    int i = INT32_MAX;
+    for (int e = t; e < n; e += kThreads) {
+      const float y = x(e);
+      const int j = id(e);
+      if (ahead(last, ilast, y, j) && ahead(y, j, v, i)) {
+        v = y;
+        i = j;
+      }
+    }
+    block_first(v, i, sh);
+    if (!(v > -INFINITY)) {
+      __syncthreads();
+      return k;
+    }
+    if (t == 0) out[k] = {v, i};
+    last = v;
+    ilast = i;
+  }
+  __syncthreads();
+  return want;
+}
+
+struct Result {
+  float m, log_s, entropy;
+  bool some;
+};
+__device__ __forceinline__ Result result_of(const Sums &s) {
+  Result r;
+  r.m = s.m;
+  r.some = s.m > -INFINITY;
+  const double log_s = log1p(static_cast<double>(s.r));
+  r.log_s = static_cast<float>(log_s);
+  r.entropy = r.some ? static_cast<float>(log_s - static_cast<double>(s.q) / (1.0 + s.r)) : 0.f;
   return r;
+}
+__device__ __forceinline__ float logprob_of(const Result &r, float x) {
+  return r.some && x > -INFINITY ? (x == r.m ? 0.f : x - r.m) - r.log_s : -INFINITY;
+}
+
+__device__ __forceinline__ int64_t token_of(const LogprobArgs &a, int64_t row) {
+  if (!a.tokens) return -1;
+  return a.tokens64 ? static_cast<const int64_t *>(a.tokens)[row] : static_cast<const int32_t *>(a.tokens)[row];
+}
+template <typename T>
+__device__ __forceinline__ float token_logit(const LogprobArgs &a, int64_t row, int64_t token) {
+  if (token < 0 || token >= a.vocab) return -INFINITY;
+  return clean(static_cast<float>(static_cast<const T *>(a.logits)[row * a.row_stride + token]));
+}
+template <typename T>
+__device__ __forceinline__ void write_row(const LogprobArgs &a, int64_t row, const Result &r, int before, float xt) {
+  if (a.tokens) {
+    a.logprobs[row] = logprob_of(r, xt);
+    a.ranks[row] = xt > -INFINITY ? before + 1 : 0;
+  }
+  if (a.entropy) a.entropy[row] = r.entropy;
+}
+
+__device__ __forceinline__ void write_top(const LogprobArgs &a, int64_t row, const Result &r, int found, const Shared &sh) {
+  const int t = threadIdx.x;
+  if (t >= a.top) return;
+  a.top_ids[row * a.ids_stride + t] = t < found ? sh.final[t].i : -1;
+  a.top_logprobs[row * a.lps_stride + t] = t < found ? logprob_of(r, sh.final[t].x) : -INFINITY;
 }
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
+  constexpr int N = Vec<T>::N;
+  constexpr int CHUNK = kGroupLanes * N;  // elements, 128 bytes
+  constexpr int STEP = kThreads * N;      // elements of one vector of every thread
   __shared__ Shared sh;
-  const int64_t row = blockIdx.x;
+  extern __shared__ float values[];  // the largest of each chunk, later the picked chunks' tokens
+  const int t = threadIdx.x, lane = t & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(t / kWave);
+  const int64_t row = blockIdx.x / static_cast<unsigned>(a.slices);
+  const int slice = static_cast<int>(blockIdx.x - row * a.slices);
   const T *x = static_cast<const T *>(a.logits) + row * a.row_stride;
-  int64_t t = -1;
-  if (a.tokens)
-    t = a.tokens64 ? static_cast<const int64_t *>(a.tokens)[row] : static_cast<const int32_t *>(a.tokens)[row];
-  const bool inside = t >= 0 && t < a.vocab;
-  const float xt = inside ? logit(x[t]) : -INFINITY;
-  float m = -INFINITY;
-  int im = INT32_MAX;
-  int before = 0;
-  for (int i = threadIdx.x; i < a.vocab; i += kThreads) {
-    const float v = logit(x[i]);
-    if (ahead(v, i, m, im)) {
-      m = v;
-      im = i;
+  const int first = slice * a.slice_len;
+  const int end = static_cast<int>(min(static_cast<int64_t>(first) + a.slice_len, static_cast<int64_t>(a.vocab)));
+  const int64_t token = token_of(a, row);
+  const float xt = token_logit<T>(a, row, token);
+  // Ahead of the token: at lower indices what is not less, at higher ones what is larger.
+  const float above = xt < INFINITY ? next_above(xt) : NAN;  // nothing is larger than plus infinity
+  const bool ranked = xt > -INFINITY;
+
+  Sums s = {-INFINITY, 0.f, 0.f};  // m the same for the wave
+  int before = 0;                  // tokens ahead: of the wave, in scalars
+  int mixed = 0;                   // of the lane, in the run that holds the token
+
+  Vec<T> v[kBatch];
+#pragma unroll
+  for (int j = 0; j < kBatch; ++j) load_vec(x, first + j * STEP + t * N, end, v[j]);
+  for (int at = first; at < end; at += kBatch * STEP) {
+    float f[kBatch][N], vmax[kBatch];
+    bool usual = true;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[j][i] = static_cast<float>(v[j].x[i]);
+      float mx = max3_raw(f[j][0], f[j][1], f[j][2]);
+#pragma unroll
+      for (int i = 3; i + 1 < N; i += 2) mx = max3_raw(mx, f[j][i], f[j][i + 1]);
+      vmax[j] = max3_raw(mx, f[j][N - 1], f[j][N - 1]);
+      usual &= vmax[j] <= s.m;  // false for a NaN
     }
-    before += ahead(v, i, xt, static_cast<int>(t));
-  }
-  block_first(m, im, sh);
-  const bool some = m > -INFINITY;
-  double rest = 0.0, mean = 0.0;
-  for (int i = threadIdx.x; i < a.vocab && some; i += kThreads) {
-    const float v = logit(x[i]);
-    if (i == im) continue;
-    const float y = v == m ? 0.f : v - m, e = expf(y);
-    rest += e;
-    if (e > 0.f) mean += y * e;
-  }
-  rest = block_sum(rest, sh);
-  mean = block_sum(mean, sh);
-  before = static_cast<int>(block_sum(before, sh));
-  const float log_s = static_cast<float>(log1p(rest));
-  if (threadIdx.x == 0) {
-    const bool there = some && xt > -INFINITY;
-    if (a.tokens) {
-      a.logprobs[row] = there ? (xt == m ? 0.f : xt - m) - log_s : -INFINITY;
-      a.ranks[row] = there ? before + 1 : 0;
+    const int next = at + kBatch * STEP;
+    if (next < end) {
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) load_vec(x, next + j * STEP + t * N, end, v[j]);
     }
-    if (a.entropy) a.entropy[row] = some ? static_cast<float>(log1p(rest) - mean / (1.0 + rest)) : 0.f;
-  }
-  float last = INFINITY;
-  int ilast = -1;
-  for (int k = 0; k < a.top; ++k) {
-    float best = -INFINITY;
-    int ibest = INT32_MAX;
-    for (int i = threadIdx.x; i < a.vocab; i += kThreads) {
-      const float v = logit(x[i]);
-      if (ahead(last, ilast, v, i) && ahead(v, i, best, ibest)) {
-        best = v;
-        ibest = i;
+    const bool special = !__all(usual) || s.m == INFINITY;
+    int skip = -1;  // this lane's element left out of the sums
+    if (special) {
+      // A new maximum, a NaN, nothing so far, or plus infinities.
+      float mine = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        vmax[j] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          f[j][i] = clean(f[j][i]);
+          vmax[j] = fmaxf(vmax[j], f[j][i]);
+        }
+        mine = fmaxf(mine, vmax[j]);
+      }
+      const float m = wave_max_f32(mine);
+      if (m > s.m) {
+        raise(s, m, lane == 0);
+        const bool holder = lane == __builtin_ctzll(__ballot(mine == m));
+#pragma unroll
+        for (int j = kBatch - 1; j >= 0; --j)
+#pragma unroll
+          for (int i = N - 1; i >= 0; --i)
+            if (holder && f[j][i] == m) skip = j * N + i;
       }
     }
-    block_first(best, ibest, sh);
-    const bool there = best > -INFINITY;
-    if (threadIdx.x == 0) {
-      a.top_ids[row * a.ids_stride + k] = there ? ibest : -1;
-      a.top_logprobs[row * a.lps_stride + k] = there ? (best == m ? 0.f : best - m) - log_s : -INFINITY;
+    if (ranked) {
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int w0 = at + j * STEP + wave * kWave * N;  // the wave's first element
+        if (w0 + kWave * N <= token || w0 > token) {
+          const float bar = w0 > token ? above : xt;
+#pragma unroll
+          for (int i = 0; i < N; ++i) before += __popcll(__ballot(f[j][i] >= bar));
+        } else {
+#pragma unroll
+          for (int i = 0; i < N; ++i) mixed += f[j][i] >= (w0 + lane * N + i < token ? xt : above);
+        }
+      }
     }
-    last = best;
-    ilast = ibest;
+    if (a.top) {
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const float c = max_of_8(vmax[j]);
+        if ((lane & (kGroupLanes - 1)) == 0) values[(at - first + j * STEP + t * N) / CHUNK] = c;
+      }
+    }
+    if (special) {
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if (s.m == INFINITY && f[j][i] == INFINITY && skip != j * N + i) s.r += 1.f;
+          if (skip == j * N + i) f[j][i] = -INFINITY;
+        }
+    }
+    if (s.m > -INFINITY && s.m < INFINITY) {
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        float r = 0.f, q = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float y = fmaxf(f[j][i] - s.m, kFarBelow);  // a NaN or minus infinity: exp is 0
+          const float e = __builtin_amdgcn_exp2f(y * kLog2e);
+          r += e;
+          q = fmaf(y, e, q);
+        }
+        s.r += r;
+        s.q += q;
+      }
+    }
   }
+  s.r = wave_sum_f32(s.r);
+  s.q = wave_sum_f32(s.q);
+#pragma unroll
+  for (int m = 1; m < kWave; m <<= 1) mixed += __shfl_xor(mixed, m, kWave);
+  if (lane == 0) sh.part[wave] = {s.m, s.r, s.q, before + mixed};
+  __syncthreads();
+  s = {sh.part[0].m, sh.part[0].rest, sh.part[0].mean};
+  before = sh.part[0].before;
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) {
+    s = join(s, {sh.part[w].m, sh.part[w].rest, sh.part[w].mean});
+    before += sh.part[w].before;
+  }
+
+  int found = 0;
+  if (a.top) {
+    // The foremost `top` chunks hold the foremost `top` tokens: a token of another
+    // chunk has the largest of each of them ahead of it, chunks being runs of tokens.
+    const int chunks = (max(end - first, 0) + CHUNK - 1) / CHUNK;
+    const int picked = foremost(chunks, a.top, [&](int e) { return values[e]; }, [](int e) { return e; }, sh.picked, sh);
+    for (int e = t; e < picked * kGroupLanes; e += kThreads) {
+      Vec<T> w;
+      load_vec(x, first + sh.picked[e / kGroupLanes].i * CHUNK + e % kGroupLanes * N, end, w);
+#pragma unroll
+      for (int i = 0; i < N; ++i) values[e * N + i] = clean(static_cast<float>(w.x[i]));
+    }
+    __syncthreads();
+    found = foremost(
+        picked * CHUNK, a.top, [&](int e) { return values[e]; },
+        [&](int e) { return first + sh.picked[e / CHUNK].i * CHUNK + e % CHUNK; }, sh.final, sh);
+  }
+  if (a.slices == 1) {
+    const Result r = result_of(s);
+    if (t == 0) write_row<T>(a, row, r, before, xt);
+    write_top(a, row, r, found, sh);
+    return;
+  }
+  char *out = a.ws + blockIdx.x * part_bytes(a.top);
+  if (t == 0) *reinterpret_cast<Part *>(out) = {s.m, s.r, s.q, before};
+  if (t < a.top) reinterpret_cast<Listed *>(out + sizeof(Part))[t] = t < found ? sh.final[t] : Listed{-INFINITY, INT32_MAX};
+}
+
+// Joins the slices of one row.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void logprob_join_kernel(LogprobArgs a) {
+  __shared__ Shared sh;
+  extern __shared__ float values[];  // slices * top values, then their tokens
+  const int t = threadIdx.x, lane = t & (kWave - 1);
+  const int64_t row = blockIdx.x;
+  const float xt = token_logit<T>(a, row, token_of(a, row));
+  const char *parts = a.ws + row * a.slices * part_bytes(a.top);
+  const int n = a.slices * a.top;
+  int *ids = reinterpret_cast<int *>(values + n);
+  for (int e = t; e < n; e += kThreads) {
+    const int slice = e / a.top;
+    const Listed l = reinterpret_cast<const Listed *>(parts + slice * part_bytes(a.top) + sizeof(Part))[e - slice * a.top];
+    values[e] = l.x;
+    ids[e] = l.i;
+  }
+  Part p = {-INFINITY, 0.f, 0.f, 0};
+  if (lane < a.slices) p = *reinterpret_cast<const Part *>(parts + lane * part_bytes(a.top));
+  Sums s = {p.m, p.rest, p.mean};
+  int before = p.before;
+#pragma unroll
+  for (int m = 1; m < kWave; m <<= 1) {
+    const Sums o = {__shfl_xor(s.m, m, kWave), __shfl_xor(s.r, m, kWave), __shfl_xor(s.q, m, kWave)};
+    s = join(s, o);
+    before += __shfl_xor(before, m, kWave);
+  }
+  __syncthreads();
+  const int found = a.top ? foremost(n, a.top, [&](int e) { return values[e]; }, [&](int e) { return ids[e]; }, sh.final, sh) : 0;
+  const Result r = result_of(s);
+  if (t == 0) write_row<T>(a, row, r, before, xt);
+  write_top(a, row, r, found, sh);
+}
+
+// How many slices a row is cut into: enough work-groups for the chip (two a compute
+// unit), each of a few vectors a thread at least.
+int slices_of(int64_t rows, int64_t vocab) {
+  const int64_t wanted = (2 * static_cast<int64_t>(device_cus()) + rows - 1) / rows;
+  const int64_t most = (vocab + kSliceUnit - 1) / kSliceUnit;
+  const int64_t least = (vocab + kMaxSliceLen - 1) / kMaxSliceLen;
+  int64_t n = wanted < most ? wanted : most;
+  n = n < kMaxSlices ? n : kMaxSlices;
+  return static_cast<int>(n > least ? n : least);
+}
+
+template <typename T>
+int launch(LogprobArgs a, int64_t rows, hipStream_t s) {
+  constexpr int CHUNK = kGroupLanes * Vec<T>::N, ROUND = kBatch * kThreads * Vec<T>::N;
+  const int64_t chunks = static_cast<int64_t>((a.slice_len + ROUND - 1) / ROUND) * ROUND / CHUNK;
+  const int64_t floats = !a.top ? 0 : chunks > a.top * CHUNK ? chunks : a.top * CHUNK;
+  logprob_kernel<T><<<dim3(static_cast<unsigned>(rows * a.slices)), dim3(kThreads), floats * 4, s>>>(a);
+  int rc = launch_status("k8v4_token_logprobs");
+  if (rc || a.slices == 1) return rc;
+  logprob_join_kernel<T><<<dim3(static_cast<unsigned>(rows)), dim3(kThreads), a.slices * a.top * 8, s>>>(a);
+  return launch_status("k8v4_token_logprobs join");
 }
 
 constexpr int64_t kMaxVocab = int64_t(1) << 24;
+constexpr int64_t kMaxRows = int64_t(1) << 24;
 
 }  // namespace
 }  // namespace k8v4
 
 extern "C" int64_t k8v4_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top) {
   using namespace k8v4;
-  if (rows < 0 || rows > INT32_MAX || vocab < 1 || vocab > kMaxVocab || top < 0 || top > kMaxTop) return -1;
-  return 0;
+  if (rows < 0 || rows > kMaxRows || vocab < 1 || vocab > kMaxVocab || top < 0 || top > kMaxTop) return -1;
+  const int slices = rows ? slices_of(rows, vocab) : 1;
+  return slices == 1 ? 0 : rows * slices * part_bytes(top);
 }
 
 extern "C" int k8v4_token_logprobs(const void *logits, int dtype, int64_t row_stride, const void *tokens,
@@ -174,7 +547,7 @@ extern "C" int k8v4_token_logprobs(const void *logits, int dtype, int64_t row_st
   using namespace k8v4;
   clear_error();
   K8V4_REQUIRE(dtype == K8V4_F16 || dtype == K8V4_BF16 || dtype == K8V4_F32, "logits must be fp16, bf16 or fp32");
-  K8V4_REQUIRE(rows >= 0 && rows <= INT32_MAX, "rows must be 0 .. 2^31 - 1");
+  K8V4_REQUIRE(rows >= 0 && rows <= kMaxRows, "rows must be 0 .. %lld", static_cast<long long>(kMaxRows));
   K8V4_REQUIRE(vocab >= 1 && vocab <= kMaxVocab, "vocabulary must be 1 .. %lld", static_cast<long long>(kMaxVocab));
   K8V4_REQUIRE(top >= 0 && top <= kMaxTop, "0 to %d likeliest tokens, got %d", kMaxTop, top);
   if (rows == 0) return K8V4_OK;
@@ -198,7 +571,6 @@ extern "C" int k8v4_token_logprobs(const void *logits, int dtype, int64_t row_st
   a.row_stride = row_stride;
   a.tokens = tokens;
   a.tokens64 = tokens_are_int64 != 0;
-  a.rows = rows;
   a.vocab = static_cast<int>(vocab);
   a.top = top;
   a.logprobs = logprobs;
@@ -208,13 +580,10 @@ extern "C" int k8v4_token_logprobs(const void *logits, int dtype, int64_t row_st
   a.ids_stride = ids_stride;
   a.top_logprobs = top_logprobs;
   a.lps_stride = lps_stride;
-  const dim3 grid(static_cast<unsigned>(rows));
+  a.slices = slices_of(rows, vocab);
+  a.slice_len = static_cast<int>(((vocab + a.slices - 1) / a.slices + kSliceUnit - 1) / kSliceUnit * kSliceUnit);
+  a.ws = static_cast<char *>(workspace);
   auto s = static_cast<hipStream_t>(stream);
-  if (dtype == K8V4_F32)
-    logprob_kernel<float><<<grid, dim3(kThreads), 0, s>>>(a);
-  else if (dtype == K8V4_BF16)
-    logprob_kernel<__bf16><<<grid, dim3(kThreads), 0, s>>>(a);
-  else
-    logprob_kernel<_Float16><<<grid, dim3(kThreads), 0, s>>>(a);
-  return launch_status("k8v4_token_logprobs");
+  if (dtype == K8V4_F32) return launch<float>(a, rows, s);
+  return dtype == K8V4_BF16 ? launch<__bf16>(a, rows, s) : launch<_Float16>(a, rows, s);
 }
