@@ -566,9 +566,9 @@ __device__ __forceinline__ void attend_piece(const PieceArgs &a, char *lds_raw, 
 // over the four lanes of a row.
 constexpr int kWideWaves = 8;
 
-template <int D>
+template <int D, int TILES = D == 128 ? 3 : 2>
 struct Wide {
-  static constexpr int NT = D == 128 ? 3 : 2;    // row tiles a wave holds in registers
+  static constexpr int NT = TILES;               // row tiles a wave holds in registers
   static constexpr int ROWS = kWideWaves * 16 * NT;
   static constexpr int SLOTS = D == 128 ? 4 : 3;
   static constexpr int VROW = D / 2;
@@ -591,10 +591,13 @@ struct Wide {
 // chunk and written 64 at a time at one chunk, both conflict-free.
 __device__ __forceinline__ int vswz(int row) { return (row & 7) ^ ((row >> 3) & 1); }
 
-// Pages p0 .. p1 - 1 of the prefix for one row block of one KV head.
-template <int D, int HKV>
+// Pages p0 .. p1 - 1 of the prefix for one row block of one KV head, or (TREE) of a
+// sequence for a row block of its drafted tree, whose words lie in the LDS behind
+// everything else (kWideWordBytes).
+constexpr int kWideWordBytes = 64 * 8;
+template <int D, int HKV, int TILES = Wide<D>::NT, bool TREE = false>
 __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, int tid, int wg, int seg, int p0, int p1) {
-  using W = Wide<D>;
+  using W = Wide<D, TILES>;
   constexpr int NT = W::NT, KS = D / 64, DT = D / 16;
   lds_t *lds = (lds_t *)(lds_raw);
   const int lane = tid & (kWave - 1);
@@ -602,9 +605,19 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
   const int grp = wave >> 2;
   const int n = lane & 15, g = lane >> 4;
 
-  const int h = seg / a.wide_blocks, block = seg - h * a.wide_blocks;
+  const int b = TREE ? seg / a.per_seq : 0, sub = seg - b * a.per_seq * TREE;
+  const int h = sub / a.wide_blocks, block = sub - h * a.wide_blocks;
   const int row0 = block * W::ROWS + wave * 16 * NT;  // first row of this wave, of the head's tokens * 6
-  const int nrows = a.tokens * kGqa;
+  const int nrows = (TREE ? a.q_len : a.tokens) * kGqa;
+  const int len = TREE ? ((const const_i32_ptr)(a.seq_lens))[b] : 0;
+  const int own0 = TREE ? b * nrows : 0;  // the sequence's first row of the head's rows in the buffer
+  TreeRows tree{};
+  if constexpr (TREE) {
+    auto *words = reinterpret_cast<__attribute__((address_space(3))) uint64_t *>(lds + W::LDS_BYTES);
+    if (tid < a.q_len) words[tid] = static_cast<uint64_t>(a.tree_masks[b * a.mask_stride + tid]);
+    tree.words = words;
+    tree.context = len - a.q_len;
+  }
   const bool active = row0 < nrows;
   const int pages = p1 - p0;
 
@@ -618,18 +631,19 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int r = row0 + 16 * nt + n;
-    const int64_t at = h * a.head_rows + r;  // the buffer is padded to whole blocks
+    const int64_t at = h * a.head_rows + (TREE ? own0 + r : r);  // the buffer is padded to whole blocks
     const int rl = min(r, nrows - 1), tok = rl / kGqa, sb = tok / a.q_len;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[nt][ks] = *reinterpret_cast<const v4i *>(a.q8 + at * D + 64 * ks + 16 * g);
-    crow[nt] = a.q8_scale[h * a.head_rows + rl];
-    lim[nt] = a.seq_lens[sb] - a.q_len + (tok - sb * a.q_len) + 1;
+    crow[nt] = a.q8_scale[h * a.head_rows + (TREE ? own0 + rl : rl)];
+    lim[nt] = TREE ? len : a.seq_lens[sb] - a.q_len + (tok - sb * a.q_len) + 1;
   }
   // Physical pages, 64 at a time: lane l holds page p0 + 64 k + l.
   int ptab = -1;
   auto load_table = [&](int k) {
     const int p = min(p0 + 64 * k + lane, p1 - 1);
-    const int raw = a.prefix_table[a.ppb <= 1 ? p : p / a.ppb];
+    const int32_t *table = TREE ? a.block_table + static_cast<int64_t>(b) * a.bt_stride : a.prefix_table;
+    const int raw = table[a.ppb <= 1 ? p : p / a.ppb];
     const int64_t ph = a.ppb <= 1 ? raw : static_cast<int64_t>(raw) * a.ppb + p % a.ppb;
     ptab = ph >= 0 && ph < a.num_pages ? static_cast<int>(ph) : -1;
   };
@@ -637,12 +651,12 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const bool live = row0 + 16 * nt + n < nrows;
-    if (live && lim[nt] > 0) far = max(far, kFar - min(lim[nt], kFar));
-    if (!live) lim[nt] = a.prefix_pages * kPage;
+    if (!TREE && live && lim[nt] > 0) far = max(far, kFar - min(lim[nt], kFar));
+    if (!TREE && !live) lim[nt] = a.prefix_pages * kPage;
     const double f = live ? static_cast<double>(crow[nt]) : 0.0;
     crow[nt] = fmaxf(static_cast<float>(f * (static_cast<double>(kLog2e) / sqrt(static_cast<double>(D)))), 1e-30f);
   }
-  const int min_end = kFar - wave_max(far);
+  const int min_end = TREE ? max(tree.context, 0) : kFar - wave_max(far);
 
   // The lane for addresses that, kept over the loop, would be what is too many
   // for the registers at head dim 256: formed anew where they are used.
@@ -749,6 +763,11 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
   };
   auto scale_planes = [&](int i) __attribute__((always_inline)) {
     if (wave != 0) return;
+    if constexpr (TREE) {
+      // Tokens behind the last hold anything; their probabilities are zero, and so
+      // their V has to be.
+      if ((p0 + i) * kPage + lane >= len) plane_s = plane_z = 0.f;
+    }
     lds_t *planes = lds + (i % W::SLOTS) * W::SLOT_BYTES + W::S_OFF + 4 * lane;
     *reinterpret_cast<__attribute__((address_space(3))) float *>(planes) = plane_s * 0x1p20f;
     *reinterpret_cast<__attribute__((address_space(3))) float *>(planes + kPage * 4) = plane_z * (plane_s * -0.0625f);
@@ -898,12 +917,22 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
     }
     if (__builtin_expect(masked, 0)) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        [[maybe_unused]] uint64_t word = 0;
+        if constexpr (TREE) word = tree.words[min((row0 + 16 * nt + n) / kGqa, a.q_len - 1)];
 #pragma unroll
         for (int ml = 0; ml < 4; ++ml)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (tbase + 16 * ml + 4 * g + e >= min(lim[nt], seen_to)) t[nt][ml][e] = -INFINITY;
+          for (int e = 0; e < 4; ++e) {
+            const int tok = tbase + 16 * ml + 4 * g + e;
+            if constexpr (TREE) {
+              const int node = tok - tree.context;
+              if (tok >= min(len, seen_to) || (node >= 0 && !((word >> (node & 63)) & 1))) t[nt][ml][e] = -INFINITY;
+            } else {
+              if (tok >= min(lim[nt], seen_to)) t[nt][ml][e] = -INFINITY;
+            }
+          }
+      }
     }
     bool grow = false;
 #pragma unroll
@@ -1013,7 +1042,8 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
   // The state, as in the kernel above: a quarter of O / l (O is a sixteenth),
   // then m and l; lane (n, g) holds dims 32 q + 8 g .. + 7 of row n.
   if (active) {
-    char *state = a.ws + static_cast<int64_t>(wg + seg) * a.prefix_bytes;
+    char *state = TREE ? a.own_ws + static_cast<int64_t>(wg + seg) * a.own_bytes
+                       : a.ws + static_cast<int64_t>(wg + seg) * a.prefix_bytes;
     float2 *ml = reinterpret_cast<float2 *>(state + static_cast<int64_t>(W::ROWS) * D * 2);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -1044,7 +1074,8 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
 
 // Folds the states of one column slice of one output row (token, query head):
 // the prefix's for its group, then its sequence's own.
-template <int D, int TPU>
+// TREE: of a tree's row, whose wide form (a.wide_blocks) holds a KV head's rows alone.
+template <int D, int TPU, bool TREE = false>
 __global__ __launch_bounds__(TPU) void pieces_merge_kernel(PieceArgs a) {
   constexpr int NW = TPU / kWave;
   __shared__ float red[NW * 32 * 10];  // per wave and column: M, l, o[8]
@@ -1065,10 +1096,16 @@ __global__ __launch_bounds__(TPU) void pieces_merge_kernel(PieceArgs a) {
   const Axis ax = plan_axis(a, lane, b);
   // Pieces of the row's prefix segment and of its own one.
   int pf = 0, pn = 0, of = 0, on = 0;
-  const int sub = j / kGroup;
+  int sub = j / kGroup;
+  int orow = h * a.own_rows + (j - sub * kGroup) * kGqa + i6;
+  if (TREE && a.wide_blocks) {
+    const int r = j * kGqa + i6, block = r / a.own_rows;
+    sub = h * a.wide_blocks + block;
+    orow = r - block * a.own_rows;
+  }
   int ps = tok / kGroup;                                      // prefix segment
   int pr = h * a.prefix_rows + (tok - ps * kGroup) * kGqa + i6;  // the row in its states
-  if (a.wide_blocks) {
+  if (!TREE && a.wide_blocks) {
     const int r = tok * kGqa + i6, block = r / Wide<D>::ROWS;
     ps = h * a.wide_blocks + block;
     pr = r - block * Wide<D>::ROWS;
@@ -1087,12 +1124,11 @@ __global__ __launch_bounds__(TPU) void pieces_merge_kernel(PieceArgs a) {
     on = (first + pages - 1) / ax.unit - of + 1;
   }
   const int dcol = 8 * (slice * VPR + col);
-  const int orow = h * a.own_rows + (j - sub * kGroup) * kGqa + i6;
   const char *pbase = piece_state(a, pf, ps), *obase = piece_state(a, of, a.groups + os);
   const int64_t p_o = (static_cast<int64_t>(pr) * D + dcol) * 2;
   const int64_t p_ml = static_cast<int64_t>(a.wide_blocks ? 1 : a.hkv) * a.prefix_rows * D * 2 + pr * 8;
   const int64_t o_o = (static_cast<int64_t>(orow) * D + dcol) * 2;
-  const int64_t o_ml = static_cast<int64_t>(a.hkv) * a.own_rows * D * 2 + orow * 8;
+  const int64_t o_ml = static_cast<int64_t>(TREE && a.wide_blocks ? 1 : a.hkv) * a.own_rows * D * 2 + orow * 8;
 
   MergeAcc acc{-INFINITY, 0.f, (v8f){0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}};
   const int count = pn + on;

@@ -33,6 +33,30 @@ void tree_split_kernel(PieceArgs args) {
   });
 }
 
+// Many rows of one KV head: wide_piece in decode_pieces.h, TILES row tiles a wave.
+template <int D, int HKV, int TILES>
+__global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_per_eu(2, 2)))
+void tree_wide_kernel(PieceArgs args) {
+  using W = Wide<D, TILES>;
+  static_assert(W::LDS_BYTES + kWideWordBytes <= 163840, "no room for the mask words");
+  __shared__ __attribute__((aligned(16))) char lds[W::LDS_BYTES + kWideWordBytes];
+  const int wg = static_cast<int>(blockIdx.x);
+  walk_pieces<true>(args, wg, [&](const PieceArgs &a, int tid, int seg, int s0, int s1) {
+    wide_piece<D, HKV, TILES, true>(a, lds, tid, wg, seg, s0, s1);
+  });
+}
+
+template <int D, int HKV>
+void launch_wide(const PieceArgs &a, int tiles, hipStream_t s) {
+  const dim3 grid(a.grid), block(64 * kWideWaves);
+  if (tiles == 1)
+    tree_wide_kernel<D, HKV, 1><<<grid, block, 0, s>>>(a);
+  else if (D == 256 || tiles == 2)
+    tree_wide_kernel<D, HKV, 2><<<grid, block, 0, s>>>(a);
+  else
+    tree_wide_kernel<D, HKV, D == 256 ? 2 : 3><<<grid, block, 0, s>>>(a);
+}
+
 template <int HKV, int NWH, bool PH>
 void launch_split(const PieceArgs &a, int tiles, hipStream_t s) {
   const dim3 grid(a.grid), block(64 * HKV * NWH);
@@ -50,25 +74,45 @@ int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 // the states of the pieces.
 struct TreeShape {
   int64_t tokens, per_seq, head_rows, grid;
+  int64_t blocks;  // row blocks of a KV head in the wide form (0: eight nodes at a time)
+  int tiles;       // row tiles of a wave
   int own_rows;
   int64_t own_bytes;
   int64_t q_bytes, scale_bytes, state_bytes;
   int64_t bytes() const { return q_bytes + scale_bytes + state_bytes; }
 };
-TreeShape shape_of(int64_t batch, int nodes, int hkv, int head_dim) {
+TreeShape shape_of(bool wide, int64_t batch, int nodes, int hkv, int head_dim) {
   TreeShape s;
   s.tokens = batch * nodes;
-  s.per_seq = (nodes + kGroup - 1) / kGroup;
-  // One work-group per CU, two of the half-sized ones of two 128-dim heads.
-  s.grid = static_cast<int64_t>(device_cus()) * (hkv == 2 && head_dim == 128 ? 2 : 1);
-  s.own_rows = (nodes < kGroup ? nodes : kGroup) * kGqa;
-  s.own_bytes = static_cast<int64_t>(hkv) * s.own_rows * (2 * head_dim + 8);
-  s.head_rows = s.tokens * kGqa + 3 * 16;  // a last segment's tiles read rows behind the last token's
+  const int64_t rows = static_cast<int64_t>(nodes) * kGqa, state = 2 * head_dim + 8;
+  if (wide) {
+    const int most = head_dim == 128 ? Wide<128>::NT : Wide<256>::NT, tile_rows = kWideWaves * 16;
+    const int64_t tiles = (rows + tile_rows - 1) / tile_rows;
+    s.blocks = (tiles + most - 1) / most;
+    s.tiles = static_cast<int>((tiles + s.blocks - 1) / s.blocks);
+    s.own_rows = tile_rows * s.tiles;
+    s.per_seq = hkv * s.blocks;
+    s.own_bytes = s.own_rows * state;
+    s.grid = device_cus();
+    s.head_rows = s.tokens * kGqa + s.own_rows;  // a last block's tiles read rows behind the last token's
+  } else {
+    s.blocks = 0;
+    s.per_seq = (nodes + kGroup - 1) / kGroup;
+    s.own_rows = (nodes < kGroup ? nodes : kGroup) * kGqa;
+    s.tiles = (s.own_rows + 15) / 16;
+    s.own_bytes = hkv * s.own_rows * state;
+    // One work-group per CU, two of the half-sized ones of two 128-dim heads.
+    s.grid = static_cast<int64_t>(device_cus()) * (hkv == 2 && head_dim == 128 ? 2 : 1);
+    s.head_rows = s.tokens * kGqa + 3 * 16;
+  }
   s.q_bytes = round256(hkv * s.head_rows * head_dim);
   s.scale_bytes = round256(hkv * s.head_rows * 4);
   s.state_bytes = (s.grid + batch * s.per_seq) * s.own_bytes;
   return s;
 }
+
+// Which form serves trees of so many nodes.
+bool takes_wide(int nodes) { return nodes > kGroup; }
 
 constexpr int64_t kMaxBatch = int64_t(1) << 20;
 
@@ -94,7 +138,7 @@ int64_t tree_wait_timeouts() {
 extern "C" int64_t k8v4_attn_tree_workspace_bytes(int64_t batch, int nodes, int hkv, int head_dim) {
   using namespace k8v4;
   if (!valid_shape(batch, nodes, hkv, head_dim)) return -1;
-  return shape_of(batch, nodes, hkv, head_dim).bytes();
+  return shape_of(takes_wide(nodes), batch, nodes, hkv, head_dim).bytes();
 }
 
 extern "C" int k8v4_attn_tree(const void *q, int q_dtype, int64_t q_tok_stride, const int8_t *k_cache,
@@ -145,7 +189,7 @@ extern "C" int k8v4_attn_tree(const void *q, int q_dtype, int64_t q_tok_stride, 
               static_cast<long long>(need));
     return K8V4_ERR_WORKSPACE;
   }
-  const TreeShape sh = shape_of(batch, nodes, hkv, head_dim);
+  const TreeShape sh = shape_of(takes_wide(nodes), batch, nodes, hkv, head_dim);
   const int64_t table_pages = table_width * pages_per_block;
   K8V4_REQUIRE(batch * sh.per_seq * (table_pages + kPieceCost) < (int64_t(1) << 30), "batch too large for one call");
 
@@ -186,6 +230,7 @@ extern "C" int k8v4_attn_tree(const void *q, int q_dtype, int64_t q_tok_stride, 
   a.hkv = hkv;
   a.tokens = static_cast<int>(sh.tokens);
   a.per_seq = static_cast<int>(sh.per_seq);
+  a.wide_blocks = static_cast<int>(sh.blocks);
   a.grid = static_cast<int>(sh.grid);
   a.ws = a.own_ws = ws + sh.q_bytes + sh.scale_bytes;
   a.own_rows = sh.own_rows;
@@ -223,8 +268,20 @@ extern "C" int k8v4_attn_tree(const void *q, int q_dtype, int64_t q_tok_stride, 
   auto s = static_cast<hipStream_t>(stream);
   int rc = q_rows_launch(q, q_dtype == K8V4_BF16, q_tok_stride, sh.tokens, hkv, head_dim, sh.head_rows, q8, scales, s);
   if (rc) return rc;
-  const int tiles = (sh.own_rows + 15) / 16;
-  if (head_dim == 256) {
+  const int tiles = sh.tiles;
+  if (sh.blocks) {
+    if (head_dim == 256) {
+      if (hkv == 4)
+        launch_wide<256, 4>(a, tiles, s);
+      else
+        launch_wide<256, 2>(a, tiles, s);
+    } else {
+      if (hkv == 4)
+        launch_wide<128, 4>(a, tiles, s);
+      else
+        launch_wide<128, 2>(a, tiles, s);
+    }
+  } else if (head_dim == 256) {
     if (hkv == 4)
       launch_split<8, 1, true>(a, tiles, s);
     else
@@ -240,18 +297,18 @@ extern "C" int k8v4_attn_tree(const void *q, int q_dtype, int64_t q_tok_stride, 
   const dim3 mgrid(static_cast<unsigned>(merge_units));
   if (head_dim == 128) {
     if (tpu == 64)
-      pieces_merge_kernel<128, 64><<<mgrid, dim3(64), 0, s>>>(a);
+      pieces_merge_kernel<128, 64, true><<<mgrid, dim3(64), 0, s>>>(a);
     else if (tpu == 128)
-      pieces_merge_kernel<128, 128><<<mgrid, dim3(128), 0, s>>>(a);
+      pieces_merge_kernel<128, 128, true><<<mgrid, dim3(128), 0, s>>>(a);
     else
-      pieces_merge_kernel<128, 256><<<mgrid, dim3(256), 0, s>>>(a);
+      pieces_merge_kernel<128, 256, true><<<mgrid, dim3(256), 0, s>>>(a);
   } else {
     if (tpu == 64)
-      pieces_merge_kernel<256, 64><<<mgrid, dim3(64), 0, s>>>(a);
+      pieces_merge_kernel<256, 64, true><<<mgrid, dim3(64), 0, s>>>(a);
     else if (tpu == 128)
-      pieces_merge_kernel<256, 128><<<mgrid, dim3(128), 0, s>>>(a);
+      pieces_merge_kernel<256, 128, true><<<mgrid, dim3(128), 0, s>>>(a);
     else
-      pieces_merge_kernel<256, 256><<<mgrid, dim3(256), 0, s>>>(a);
+      pieces_merge_kernel<256, 256, true><<<mgrid, dim3(256), 0, s>>>(a);
   }
   return launch_status("k8v4_attn_tree merge");
 }
