@@ -54,8 +54,14 @@ struct PieceArgs {
   void *out;
   int out_dtype;
   int64_t out_tok_stride;  // elements
-  const int64_t *tree_masks;  // drafted trees: a word a query token (else unused)
+  // Drafted trees only:
+  const int64_t *tree_masks;  // a word a query token
   int64_t mask_stride;        // words between sequences
+  const uint16_t *q;          // wide form: the query rows as they are
+  int q_bf16;
+  int64_t q_tok_stride;   // elements
+  int shares;             // work-groups that take the same pages
+  int64_t share_bytes;    // bytes of one's state
 };
 
 // Length of sequence b's own segments on the axis: its pages behind the
@@ -97,8 +103,6 @@ struct Where {
   int seg;
   int base;
 };
-// MANY: any number of segments a sequence, else at most two.
-template <bool MANY>
 __device__ Where locate(const PieceArgs &a, int lane, int u) {
   Where w;
   const int pre = a.groups * prefix_cost(a);
@@ -117,7 +121,7 @@ __device__ Where locate(const PieceArgs &a, int lane, int u) {
       const int src = __builtin_ctzll(past);
       const int cost = __builtin_amdgcn_readlane(c, src);
       const int first = __builtin_amdgcn_readlane(incl, src) - cost * a.per_seq;
-      const int sub = MANY ? (u - first) / cost : u >= first + cost ? 1 : 0;
+      const int sub = u >= first + cost ? 1 : 0;  // at most two segments a sequence
       w.seg = __builtin_amdgcn_readfirstlane(a.groups + (b0 + src) * a.per_seq + sub);
       w.base = __builtin_amdgcn_readfirstlane(first + sub * cost);
       return w;
@@ -153,13 +157,13 @@ __device__ __forceinline__ args_ptr reread(args_ptr p) {
 
 // Calls piece(args, thread, segment, first page, last page + 1) for the pieces of
 // work-group wg, pages counted from the segment's first (uniform over it).
-template <bool MANY = false, typename Piece>
+template <typename Piece>
 __device__ __forceinline__ void walk_pieces(const PieceArgs &args, int wg, Piece piece) {
   int unit, seg, base;
   {
     const int lane = threadIdx.x & (kWave - 1);
     unit = plan_axis(args, lane, 0).unit;
-    const Where at = locate<MANY>(args, lane, wg * unit);
+    const Where at = locate(args, lane, wg * unit);
     seg = at.seg;
     base = at.base;
   }
@@ -181,6 +185,20 @@ __device__ __forceinline__ void walk_pieces(const PieceArgs &args, int wg, Piece
     const int s0 = max(u0 - first, 0), s1 = min(u1 - first, pages);
     if (s1 > s0) piece(a, tid, seg, s0, s1);
   }
+}
+
+// A work-group's place over drafted trees: its part of the axis, and which of the
+// `shares` work-groups that take the part's pages it is (one for every eight nodes;
+// in the wide form for every KV head and row block).  They are of one of the chip's
+// eight dies, eight ids apart, so that what one of them loads the others find in the
+// die's cache: over the dies' common memory the pages would be as slow as read again.
+struct TreePlace {
+  int part, share;
+};
+__device__ __forceinline__ TreePlace tree_place(const PieceArgs &a) {
+  const int id = static_cast<int>(blockIdx.x), slot = id >> 3;
+  const int part = slot / a.shares;
+  return {part * 8 + (id & 7), slot - part * a.shares};
 }
 
 // Pages s0 .. s1 - 1 of segment `seg` (counted from the segment's first page), by
@@ -221,7 +239,7 @@ __device__ __forceinline__ void attend_piece(const PieceArgs &a, char *lds_raw, 
   const bool shared = PREFIX && seg < a.groups;
   const int os = seg - a.groups;  // own segment
   const int b = shared ? 0 : os / a.per_seq;
-  const int sub = shared ? 0 : os - b * a.per_seq;
+  const int sub = TREE ? tree_place(a).share : shared ? 0 : os - b * a.per_seq;
   const int len = shared ? 0 : lens[b];
   const int p0 = (shared ? 0 : a.prefix_pages) + s0, p1 = (shared ? 0 : a.prefix_pages) + s1;
   const int L0 = shared ? a.prefix_pages * kPage : len;
@@ -444,7 +462,7 @@ __device__ __forceinline__ void attend_piece(const PieceArgs &a, char *lds_raw, 
   // then m and l.
   auto write_state = [&]() {
     const int srows = shared ? a.prefix_rows : a.own_rows;
-    char *state = piece_state(a, wg, seg);
+    char *state = piece_state(a, wg, seg) + (TREE ? sub * a.share_bytes : 0);
     _Float16 *obase = reinterpret_cast<_Float16 *>(state);
     float2 *mlbase = reinterpret_cast<float2 *>(state + static_cast<int64_t>(CFG::QHEADS) * srows * DQ * 2);
 #pragma unroll
@@ -566,11 +584,11 @@ __device__ __forceinline__ void attend_piece(const PieceArgs &a, char *lds_raw, 
 // over the four lanes of a row.
 constexpr int kWideWaves = 8;
 
-template <int D, int TILES = D == 128 ? 3 : 2>
+template <int D, int TILES = D == 128 ? 3 : 2, int RING = D == 128 ? 4 : 3>
 struct Wide {
   static constexpr int NT = TILES;               // row tiles a wave holds in registers
   static constexpr int ROWS = kWideWaves * 16 * NT;
-  static constexpr int SLOTS = D == 128 ? 4 : 3;
+  static constexpr int SLOTS = RING;             // pages in the LDS
   static constexpr int VROW = D / 2;
   static constexpr int K_BYTES = kPage * D;
   static constexpr int V_OFF = K_BYTES;
@@ -591,13 +609,65 @@ struct Wide {
 // chunk and written 64 at a time at one chunk, both conflict-free.
 __device__ __forceinline__ int vswz(int row) { return (row & 7) ^ ((row >> 3) & 1); }
 
+// Whether the wide form over drafted trees quantizes its query rows itself.  With one
+// 128-dim row tile a wave that costs a piece less than a launch ahead of it does
+// (13 nodes over 2,048 tokens 16.5 us against 17.0, 16 over four times 100,000 145
+// against 151); with more it is done again by every work-group for longer than the
+// launch takes (64 nodes over 2,048: 33.1 against 28.7; head dim 256, 13 nodes: 21.5
+// against 20.3).
+constexpr bool tree_quantizes(int head_dim, int tiles) { return head_dim == 128 && tiles == 1; }
+
+// A 16-row tile of query rows made int8 operands by the K rule (k_rule_code): lane (n,
+// g) holds dims 64 ks + 16 g .. + 15 of row n.  Codes are evaluated in fp32, whose
+// value before rounding is within 3e-5 of the rule's, and where that lies within
+// 2^-12 of a border (or the scale is too small for it) in float64, as the rule is written.
+template <int KS, typename V>
+__device__ __forceinline__ void quantize_tile(const V (&raw)[2 * KS], bool bf16, v4i (&codes)[KS], float &row_scale) {
+  float amax = 0.f;
+#pragma unroll
+  for (int c = 0; c < 2 * KS; ++c)
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      amax = fmaxf(amax, fabsf(half_bits_to_float(static_cast<uint16_t>(raw[c][e >> 1] >> (16 * (e & 1))), bf16)));
+  amax = xlane_max16_32(amax);
+  const double scale = amax == 0.f ? 0.0 : static_cast<double>(amax) / 127.0;
+  const double inv = amax == 0.f ? 0.0 : 1.0 / scale;
+  const float inv32 = static_cast<float>(inv);
+  const bool fast = inv32 <= 3.0e38f;
+  row_scale = static_cast<float>(scale);
+#pragma unroll
+  for (int c = 0; c < 2 * KS; ++c) {
+    uint32_t words[2] = {};
+    bool border = !fast;
+    auto value = [&](int e) { return half_bits_to_float(static_cast<uint16_t>(raw[c][e >> 1] >> (16 * (e & 1))), bf16); };
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = value(e), y = fabsf(x) * inv32 + 0.5f, m = floorf(y), fr = y - m;
+      const int32_t code = static_cast<int32_t>(m);
+      border |= fr < 0x1p-12f || fr > 1.f - 0x1p-12f;
+      words[e >> 2] |= (static_cast<uint32_t>(x < 0.f ? -code : code) & 0xFFu) << (8 * (e & 3));
+    }
+    if (__ballot(border)) {  // eight elements of all lanes
+      words[0] = words[1] = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        words[e >> 2] |= (static_cast<uint32_t>(k_rule_code(value(e), inv)) & 0xFFu) << (8 * (e & 3));
+    }
+    codes[c >> 1][2 * (c & 1)] = static_cast<int>(words[0]);
+    codes[c >> 1][2 * (c & 1) + 1] = static_cast<int>(words[1]);
+  }
+}
+
 // Pages p0 .. p1 - 1 of the prefix for one row block of one KV head, or (TREE) of a
 // sequence for a row block of its drafted tree, whose words lie in the LDS behind
 // everything else (kWideWordBytes).
 constexpr int kWideWordBytes = 64 * 8;
-template <int D, int HKV, int TILES = Wide<D>::NT, bool TREE = false>
+template <int D, int HKV, int TILES = Wide<D>::NT, bool TREE = false, int RING = Wide<D>::SLOTS>
 __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, int tid, int wg, int seg, int p0, int p1) {
-  using W = Wide<D, TILES>;
+  using W = Wide<D, TILES, RING>;
+  constexpr bool FUSED = TREE && tree_quantizes(D, TILES);
+  // Registers are short at head dim 256 and where two work-groups share a CU.
+  constexpr bool LEAN = D == 256 || RING < Wide<D>::SLOTS;
   constexpr int NT = W::NT, KS = D / 64, DT = D / 16;
   lds_t *lds = (lds_t *)(lds_raw);
   const int lane = tid & (kWave - 1);
@@ -605,12 +675,11 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
   const int grp = wave >> 2;
   const int n = lane & 15, g = lane >> 4;
 
-  const int b = TREE ? seg / a.per_seq : 0, sub = seg - b * a.per_seq * TREE;
+  const int sub = TREE ? tree_place(a).share : seg, b = TREE ? seg : 0;
   const int h = sub / a.wide_blocks, block = sub - h * a.wide_blocks;
   const int row0 = block * W::ROWS + wave * 16 * NT;  // first row of this wave, of the head's tokens * 6
   const int nrows = (TREE ? a.q_len : a.tokens) * kGqa;
   const int len = TREE ? ((const const_i32_ptr)(a.seq_lens))[b] : 0;
-  const int own0 = TREE ? b * nrows : 0;  // the sequence's first row of the head's rows in the buffer
   TreeRows tree{};
   if constexpr (TREE) {
     auto *words = reinterpret_cast<__attribute__((address_space(3))) uint64_t *>(lds + W::LDS_BYTES);
@@ -628,14 +697,24 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
   float crow[NT];
   int lim[NT];
   int far = 0;
+  typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+  [[maybe_unused]] v4u raw_q[FUSED ? NT : 1][2 * KS];
+  const int own0 = TREE ? b * nrows : 0;  // the sequence's first row of the head's rows in the buffer
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int r = row0 + 16 * nt + n;
     const int64_t at = h * a.head_rows + (TREE ? own0 + r : r);  // the buffer is padded to whole blocks
     const int rl = min(r, nrows - 1), tok = rl / kGqa, sb = tok / a.q_len;
+    if constexpr (FUSED) {
+      const uint16_t *src = a.q + (static_cast<int64_t>(b) * a.q_len + tok) * a.q_tok_stride + (h * kGqa + rl - tok * kGqa) * D;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[nt][ks] = *reinterpret_cast<const v4i *>(a.q8 + at * D + 64 * ks + 16 * g);
-    crow[nt] = a.q8_scale[h * a.head_rows + (TREE ? own0 + rl : rl)];
+      for (int c = 0; c < 2 * KS; ++c)
+        raw_q[nt][c] = *reinterpret_cast<const v4u *>(src + 64 * (c >> 1) + 16 * g + 8 * (c & 1));
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) qf[nt][ks] = *reinterpret_cast<const v4i *>(a.q8 + at * D + 64 * ks + 16 * g);
+      crow[nt] = a.q8_scale[h * a.head_rows + (TREE ? own0 + rl : rl)];
+    }
     lim[nt] = TREE ? len : a.seq_lens[sb] - a.q_len + (tok - sb * a.q_len) + 1;
   }
   // Physical pages, 64 at a time: lane l holds page p0 + 64 k + l.
@@ -648,6 +727,10 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
     ptab = ph >= 0 && ph < a.num_pages ? static_cast<int>(ph) : -1;
   };
   load_table(0);  // in the query rows' round trip
+  if constexpr (FUSED) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) quantize_tile<KS>(raw_q[nt], a.q_bf16, qf[nt], crow[nt]);
+  }
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const bool live = row0 + 16 * nt + n < nrows;
@@ -659,10 +742,10 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
   const int min_end = TREE ? max(tree.context, 0) : kFar - wave_max(far);
 
   // The lane for addresses that, kept over the loop, would be what is too many
-  // for the registers at head dim 256: formed anew where they are used.
+  // for the registers (LEAN): formed anew where they are used.
   auto fresh_lane = [&] {
     int l = lane;
-    if constexpr (D == 256) asm volatile("" : "+v"(l));
+    if constexpr (LEAN) asm volatile("" : "+v"(l));
     return l;
   };
   // Lane offsets of this wave's loads of a page: K rows (swizzled as in
@@ -711,14 +794,14 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
   };
   auto issue_k = [&](int i) __attribute__((always_inline)) {
     lds_t *dst = lds + (i % W::SLOTS) * W::SLOT_BYTES;
-    const Offsets off = D == 128 ? off0 : offsets(fresh_lane());
+    const Offsets off = !LEAN ? off0 : offsets(fresh_lane());
 #pragma unroll
     for (int k = 0; k < W::KPW; ++k)
       dma16s(kbase + static_cast<uint64_t>(ph) * k_ps, off.k[k], dst + (wave * W::KPW + k) * 1024);
   };
   auto issue_rest = [&](int i) __attribute__((always_inline)) {
     lds_t *dst = lds + (i % W::SLOTS) * W::SLOT_BYTES;
-    const Offsets off = D == 128 ? off0 : offsets(fresh_lane());
+    const Offsets off = !LEAN ? off0 : offsets(fresh_lane());
     if (D == 256 || wave >= 4) dma16s(vbase + static_cast<uint64_t>(ph) * v_ps, off.v, dst + W::V_OFF + vj * 1024);
     if (D == 256 || wave < 4) {
       // D = 128: waves 0 and 3 both fetch k_scale; D = 256: 0 and 3 .. 7.  A page
@@ -831,7 +914,7 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
   // of one operand (16 bytes a lane) and the NT products that use it.  Operands
   // are read AHEAD steps before their use (an LDS round trip takes about as
   // long as eight products), one step's code fenced off from the next.
-  constexpr int NV = 2 * DT, NK = 4 * KS, AHEAD = D == 128 ? 6 : 4;
+  constexpr int NV = 2 * DT, NK = 4 * KS, AHEAD = !LEAN ? 6 : 4;
   v4f kscale[4];  // of the page whose scores S holds: tokens 16 ml + 4 g ..
   auto read_kscale = [&](int i) {
 #pragma unroll
@@ -971,13 +1054,10 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
       }
     }
   };
-  // Ends a phase; with `wait`, `left` pages of this wave's loads may be under way.
-  auto end_phase = [&](bool wait, int left) {
+  // Ends a phase; with `wait`, all but SLOTS - 2 pages of this wave's loads are there.
+  auto end_phase = [&](bool wait) {
     if (wait) {
-      if (left == 2)
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * W::LOADS) : "memory");
-      else
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(W::LOADS) : "memory");
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((W::SLOTS - 2) * W::LOADS) : "memory");
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
@@ -996,13 +1076,13 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
   // the page is about to be read.
 #pragma unroll
   for (int i = 0; i < W::SLOTS - 1; ++i) issue(i);
-  end_phase(true, W::SLOTS - 2);
+  end_phase(true);
   read_planes(0);
   scale_planes(0);
-  end_phase(false, 0);
+  end_phase(false);
   if (grp) {  // group 1 sits out phase 0
     convert(0, std::false_type{});
-    end_phase(false, 0);
+    end_phase(false);
   }
   auto run = [&](auto compute) {
     constexpr bool C = decltype(compute)::value;
@@ -1013,7 +1093,7 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
         issue(i + W::SLOTS);
         convert(i + 1, std::true_type{});
       }
-      end_phase(true, W::SLOTS - 2);
+      end_phase(true);
     };
     phase(-1, std::false_type{});
     for (int i = 0; i < pages; ++i) {
@@ -1027,7 +1107,7 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
       }
       scale_planes(i + 1);
       convert(i + grp, std::false_type{});
-      end_phase(false, 0);
+      end_phase(false);
       // A(i + 1); behind the last page its scores are of no page and not used.
       phase(i, std::true_type{});
     }
@@ -1037,12 +1117,12 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
     run(std::true_type{});
   else
     run(std::false_type{});
-  if (!grp) end_phase(false, 0);
+  if (!grp) end_phase(false);
 
   // The state, as in the kernel above: a quarter of O / l (O is a sixteenth),
   // then m and l; lane (n, g) holds dims 32 q + 8 g .. + 7 of row n.
   if (active) {
-    char *state = TREE ? a.own_ws + static_cast<int64_t>(wg + seg) * a.own_bytes
+    char *state = TREE ? a.own_ws + static_cast<int64_t>(wg + seg) * a.own_bytes + tree_place(a).share * a.share_bytes
                        : a.ws + static_cast<int64_t>(wg + seg) * a.prefix_bytes;
     float2 *ml = reinterpret_cast<float2 *>(state + static_cast<int64_t>(W::ROWS) * D * 2);
 #pragma unroll
@@ -1098,10 +1178,15 @@ __global__ __launch_bounds__(TPU) void pieces_merge_kernel(PieceArgs a) {
   int pf = 0, pn = 0, of = 0, on = 0;
   int sub = j / kGroup;
   int orow = h * a.own_rows + (j - sub * kGroup) * kGqa + i6;
-  if (TREE && a.wide_blocks) {
-    const int r = j * kGqa + i6, block = r / a.own_rows;
-    sub = h * a.wide_blocks + block;
-    orow = r - block * a.own_rows;
+  int64_t share_at = 0;
+  if constexpr (TREE) {
+    if (a.wide_blocks) {
+      const int r = j * kGqa + i6, block = r / a.own_rows;
+      orow = r - block * a.own_rows;
+      sub = h * a.wide_blocks + block;
+    }
+    share_at = sub * a.share_bytes;
+    sub = 0;  // one segment a sequence
   }
   int ps = tok / kGroup;                                      // prefix segment
   int pr = h * a.prefix_rows + (tok - ps * kGroup) * kGqa + i6;  // the row in its states
@@ -1127,8 +1212,8 @@ __global__ __launch_bounds__(TPU) void pieces_merge_kernel(PieceArgs a) {
   const char *pbase = piece_state(a, pf, ps), *obase = piece_state(a, of, a.groups + os);
   const int64_t p_o = (static_cast<int64_t>(pr) * D + dcol) * 2;
   const int64_t p_ml = static_cast<int64_t>(a.wide_blocks ? 1 : a.hkv) * a.prefix_rows * D * 2 + pr * 8;
-  const int64_t o_o = (static_cast<int64_t>(orow) * D + dcol) * 2;
-  const int64_t o_ml = static_cast<int64_t>(TREE && a.wide_blocks ? 1 : a.hkv) * a.own_rows * D * 2 + orow * 8;
+  const int64_t o_o = share_at + (static_cast<int64_t>(orow) * D + dcol) * 2;
+  const int64_t o_ml = share_at + static_cast<int64_t>(TREE && a.wide_blocks ? 1 : a.hkv) * a.own_rows * D * 2 + orow * 8;
 
   MergeAcc acc{-INFINITY, 0.f, (v8f){0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}};
   const int count = pn + on;

@@ -8,10 +8,16 @@
 // k8v4_attn_batch (int8-quantized query rows, exact integer dot products, V as
 // (nibble - zero) * scale); a row that sees no key gives zeros.
 //
-// The work is cut as in decode_shared.hip, with no prefix: a sequence's segments
-// are its runs of eight nodes (48 rows of a KV head), each over all its pages.
-// Three launches: the query rows are quantized, the page runs attended to, their
-// states folded.
+// The work is cut as in decode_shared.hip, with no prefix: the sequences' pages make
+// the axis, and several work-groups share a part of it, either one for every eight
+// nodes (48 rows of all KV heads) or one for every KV head and block of its rows.
+// Three launches: the query rows are quantized (not where the second form does that
+// itself), the page runs attended to, their states folded.
+//
+// Roundings to fewer than 32 bits are the batch op's (probabilities, V scales or
+// dequantized V and a page run's output in fp16, the query int8): with them both
+// products run on the matrix cores at 16 and 8 bits.  Sums, maxima and the folding
+// are fp32.
 #include "decode_pieces.h"
 
 namespace k8v4 {
@@ -27,28 +33,39 @@ void tree_split_kernel(PieceArgs args) {
   using CFG = SplitConfig<128, NT, HKV, NWH, PH>;
   static_assert(CFG::LDS_BYTES + kTreeWordBytes <= CFG::LDS_MAX, "no room for the mask words");
   __shared__ __attribute__((aligned(16))) char lds[CFG::LDS_BYTES + kTreeWordBytes];
-  const int wg = static_cast<int>(blockIdx.x);
-  walk_pieces<true>(args, wg, [&](const PieceArgs &a, int tid, int seg, int s0, int s1) {
+  const int wg = tree_place(args).part;
+  walk_pieces(args, wg, [&](const PieceArgs &a, int tid, int seg, int s0, int s1) {
     attend_piece<NT, HKV, NWH, PH, false, HKV * NWH, true>(a, lds, tid, wg, seg, s0, s1);
   });
 }
 
+// Work-groups of the wide form on a CU.  With one 128-dim row tile a wave a phase is
+// short and mostly latency; two work-groups fill each other's gaps (8 nodes over four
+// times 100,000 tokens 98 us, with one work-group of four ring slots 126, of eight
+// slots 126).
+constexpr int wide_groups(int head_dim, int tiles) { return head_dim == 128 && tiles == 1 ? 2 : 1; }
+
 // Many rows of one KV head: wide_piece in decode_pieces.h, TILES row tiles a wave.
+// Bound by issue: 64 nodes over four times 100,000 tokens (4 KV heads, D 128) 264 us,
+// 1,073 TFLOP/s of products (two thirds of them fp16's share of the time); 16 nodes,
+// where unpacking a page for all waves weighs more, 129 us.
 template <int D, int HKV, int TILES>
-__global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_per_eu(2, 2)))
+__global__ __attribute__((amdgpu_flat_work_group_size(512, 512),
+                          amdgpu_waves_per_eu(2 * wide_groups(D, TILES), 2 * wide_groups(D, TILES))))
 void tree_wide_kernel(PieceArgs args) {
-  using W = Wide<D, TILES>;
-  static_assert(W::LDS_BYTES + kWideWordBytes <= 163840, "no room for the mask words");
+  constexpr int GROUPS = wide_groups(D, TILES), RING = GROUPS == 2 ? 3 : Wide<D>::SLOTS;
+  using W = Wide<D, TILES, RING>;
+  static_assert(W::LDS_BYTES + kWideWordBytes <= 163840 / GROUPS, "no room for the mask words");
   __shared__ __attribute__((aligned(16))) char lds[W::LDS_BYTES + kWideWordBytes];
-  const int wg = static_cast<int>(blockIdx.x);
-  walk_pieces<true>(args, wg, [&](const PieceArgs &a, int tid, int seg, int s0, int s1) {
-    wide_piece<D, HKV, TILES, true>(a, lds, tid, wg, seg, s0, s1);
+  const int wg = tree_place(args).part;
+  walk_pieces(args, wg, [&](const PieceArgs &a, int tid, int seg, int s0, int s1) {
+    wide_piece<D, HKV, TILES, true, RING>(a, lds, tid, wg, seg, s0, s1);
   });
 }
 
 template <int D, int HKV>
 void launch_wide(const PieceArgs &a, int tiles, hipStream_t s) {
-  const dim3 grid(a.grid), block(64 * kWideWaves);
+  const dim3 grid(a.grid * a.shares), block(64 * kWideWaves);
   if (tiles == 1)
     tree_wide_kernel<D, HKV, 1><<<grid, block, 0, s>>>(a);
   else if (D == 256 || tiles == 2)
@@ -59,7 +76,7 @@ void launch_wide(const PieceArgs &a, int tiles, hipStream_t s) {
 
 template <int HKV, int NWH, bool PH>
 void launch_split(const PieceArgs &a, int tiles, hipStream_t s) {
-  const dim3 grid(a.grid), block(64 * HKV * NWH);
+  const dim3 grid(a.grid * a.shares), block(64 * HKV * NWH);
   if (tiles == 1)
     tree_split_kernel<1, HKV, NWH, PH><<<grid, block, 0, s>>>(a);
   else if (tiles == 2)
@@ -73,11 +90,13 @@ int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 // What a call keeps in its workspace: the quantized query rows, their scales and
 // the states of the pieces.
 struct TreeShape {
-  int64_t tokens, per_seq, head_rows, grid;
+  int64_t tokens, head_rows;
+  int64_t grid;    // parts of the axis
+  int shares;      // work-groups of a part
   int64_t blocks;  // row blocks of a KV head in the wide form (0: eight nodes at a time)
   int tiles;       // row tiles of a wave
   int own_rows;
-  int64_t own_bytes;
+  int64_t share_bytes;
   int64_t q_bytes, scale_bytes, state_bytes;
   int64_t bytes() const { return q_bytes + scale_bytes + state_bytes; }
 };
@@ -85,34 +104,60 @@ TreeShape shape_of(bool wide, int64_t batch, int nodes, int hkv, int head_dim) {
   TreeShape s;
   s.tokens = batch * nodes;
   const int64_t rows = static_cast<int64_t>(nodes) * kGqa, state = 2 * head_dim + 8;
+  int64_t groups = device_cus();  // work-groups: one per CU
   if (wide) {
     const int most = head_dim == 128 ? Wide<128>::NT : Wide<256>::NT, tile_rows = kWideWaves * 16;
     const int64_t tiles = (rows + tile_rows - 1) / tile_rows;
     s.blocks = (tiles + most - 1) / most;
     s.tiles = static_cast<int>((tiles + s.blocks - 1) / s.blocks);
     s.own_rows = tile_rows * s.tiles;
-    s.per_seq = hkv * s.blocks;
-    s.own_bytes = s.own_rows * state;
-    s.grid = device_cus();
-    s.head_rows = s.tokens * kGqa + s.own_rows;  // a last block's tiles read rows behind the last token's
+    s.shares = static_cast<int>(hkv * s.blocks);
+    groups *= wide_groups(head_dim, s.tiles);
+    s.share_bytes = s.own_rows * state;
+    // A last block's tiles read rows behind the last token's.
+    s.head_rows = tree_quantizes(head_dim, s.tiles) ? 0 : s.tokens * kGqa + s.own_rows;
   } else {
+    if (hkv == 2 && head_dim == 128) groups *= 2;  // half-sized ones
     s.blocks = 0;
-    s.per_seq = (nodes + kGroup - 1) / kGroup;
     s.own_rows = (nodes < kGroup ? nodes : kGroup) * kGqa;
     s.tiles = (s.own_rows + 15) / 16;
-    s.own_bytes = hkv * s.own_rows * state;
-    // One work-group per CU, two of the half-sized ones of two 128-dim heads.
-    s.grid = static_cast<int64_t>(device_cus()) * (hkv == 2 && head_dim == 128 ? 2 : 1);
+    s.shares = (nodes + kGroup - 1) / kGroup;
+    s.share_bytes = hkv * s.own_rows * state;
     s.head_rows = s.tokens * kGqa + 3 * 16;
   }
+  const int64_t parts = groups / (8 * s.shares) * 8;
+  s.grid = parts > 8 ? parts : 8;
   s.q_bytes = round256(hkv * s.head_rows * head_dim);
   s.scale_bytes = round256(hkv * s.head_rows * 4);
-  s.state_bytes = (s.grid + batch * s.per_seq) * s.own_bytes;
+  s.state_bytes = (s.grid + batch) * s.shares * s.share_bytes;
   return s;
 }
 
-// Which form serves trees of so many nodes.
-bool takes_wide(int nodes) { return nodes > kGroup; }
+// Which form serves trees of so many nodes over tables of so many pages in all (of
+// the lengths the host knows no more): the wide form, or eight nodes at a time.  A
+// wide page costs about as much for 1 as for 20 nodes (unpacked once for all rows, in
+// phases that wait for each other), the other form's about the same for each run of
+// eight; over a few pages the latter has the longer chain, but for the wide form's
+// row blocks of two and three tiles a wave.  Measured, us, eight at a time / wide, at
+// so many pages (4,000 tokens of one sequence to 100,000 of four):
+//   D 128, 4 heads   4 nodes    63: 18.7 / 14.9   254: 19.8 / 20.2  1004: 27.8 / 29.1  6256: 68 / 93
+//                    8          63: 21.1 / 15.9   504: 25.8 / 24.6  1004: 30.9 / 30.1  6256: 71 / 98
+//                    16         63: 21.8 / 18.4  1004: 35.9 / 37.3  2004: 48.8 / 52.6  6256: 113 / 129
+//                    21         33: 21.4 / 18.4  1032: 46.1 / 40.9                     6256: 160 / 145
+//                    26        127: 25.6 / 24.8   504: 36.2 / 37.5  1004: 49.2 / 43.8
+//                    64         63: 26.2 / 35.2   254: 40.7 / 45.0   504: 54.0 / 44.7  6256: 395 / 264
+//   D 128, 2 heads   8          63: 19.0 / 15.4   504: 24.1 / 21.1  2004: 30.3 / 28.9  6256: 46 / 56
+//                    64        254: 30.8 / 37.1  1004: 51.1 / 50.4  2004: 74.7 / 65.1
+//   D 256, 2 heads   8          63: 21.5 / 18.2   504: 26.4 / 25.0  1004: 32.5 / 32.3  2004: 39.8 / 46.6
+//                    16         63: 21.7 / 21.3  1004: 38.9 / 37.8  2004: 55.0 / 53.9
+//                    42        127: 29.2 / 35.6   254: 36.8 / 36.7   504: 49.2 / 44.7  2004: 126 / 79
+//   D 256, 4 heads   8          63: 24.2 / 18.8   504: 33.2 / 32.1  1004: 42.5 / 46.8  2004: 56.8 / 75.1
+//                    42         63: 31.9 / 35.3   127: 39.9 / 36.6   504: 77.5 / 54.4  2004: 222 / 123
+bool takes_wide(int nodes, int64_t pages, int hkv, int head_dim) {
+  if (nodes <= 16) return pages <= 64 * nodes;
+  if (nodes <= 21 || (hkv == 4 && head_dim == 256)) return true;  // one row tile a wave, or half as much LDS a row
+  return pages > 384;
+}
 
 constexpr int64_t kMaxBatch = int64_t(1) << 20;
 
@@ -138,7 +183,10 @@ int64_t tree_wait_timeouts() {
 extern "C" int64_t k8v4_attn_tree_workspace_bytes(int64_t batch, int nodes, int hkv, int head_dim) {
   using namespace k8v4;
   if (!valid_shape(batch, nodes, hkv, head_dim)) return -1;
-  return shape_of(takes_wide(nodes), batch, nodes, hkv, head_dim).bytes();
+  // Either form, whatever the tables.
+  const int64_t narrow = shape_of(false, batch, nodes, hkv, head_dim).bytes();
+  const int64_t wide = shape_of(true, batch, nodes, hkv, head_dim).bytes();
+  return narrow > wide ? narrow : wide;
 }
 
 extern "C" int k8v4_attn_tree(const void *q, int q_dtype, int64_t q_tok_stride, const int8_t *k_cache,
@@ -189,9 +237,9 @@ extern "C" int k8v4_attn_tree(const void *q, int q_dtype, int64_t q_tok_stride, 
               static_cast<long long>(need));
     return K8V4_ERR_WORKSPACE;
   }
-  const TreeShape sh = shape_of(takes_wide(nodes), batch, nodes, hkv, head_dim);
   const int64_t table_pages = table_width * pages_per_block;
-  K8V4_REQUIRE(batch * sh.per_seq * (table_pages + kPieceCost) < (int64_t(1) << 30), "batch too large for one call");
+  const TreeShape sh = shape_of(takes_wide(nodes, batch * table_pages, hkv, head_dim), batch, nodes, hkv, head_dim);
+  K8V4_REQUIRE(batch * (table_pages + kPieceCost) < (int64_t(1) << 30), "batch too large for one call");
 
   PieceArgs a = {};
   char *ws = static_cast<char *>(workspace);
@@ -229,12 +277,17 @@ extern "C" int k8v4_attn_tree(const void *q, int q_dtype, int64_t q_tok_stride, 
   a.q_len = nodes;
   a.hkv = hkv;
   a.tokens = static_cast<int>(sh.tokens);
-  a.per_seq = static_cast<int>(sh.per_seq);
+  a.per_seq = 1;
   a.wide_blocks = static_cast<int>(sh.blocks);
   a.grid = static_cast<int>(sh.grid);
   a.ws = a.own_ws = ws + sh.q_bytes + sh.scale_bytes;
   a.own_rows = sh.own_rows;
-  a.own_bytes = sh.own_bytes;
+  a.own_bytes = sh.shares * sh.share_bytes;
+  a.q = static_cast<const uint16_t *>(q);
+  a.q_bf16 = q_dtype == K8V4_BF16;
+  a.q_tok_stride = q_tok_stride;
+  a.shares = sh.shares;
+  a.share_bytes = sh.share_bytes;
   a.out = out;
   a.out_dtype = out_dtype;
   a.out_tok_stride = out_tok_stride;
@@ -245,8 +298,7 @@ extern "C" int k8v4_attn_tree(const void *q, int q_dtype, int64_t q_tok_stride, 
   int tpu = 256;
   {
     const int vpr_max = head_dim / 8;
-    const int64_t segments = batch * sh.per_seq;
-    const int64_t avg = (sh.grid + segments - 1) / segments;
+    const int64_t avg = (sh.grid + batch - 1) / batch;
     int cs = vpr_max / 8;
     bool found = false;
     for (int threads : {64, 128, 256}) {
@@ -266,7 +318,7 @@ extern "C" int k8v4_attn_tree(const void *q, int q_dtype, int64_t q_tok_stride, 
   K8V4_REQUIRE(merge_units <= INT32_MAX / 2, "batch too large for one merge launch");
 
   auto s = static_cast<hipStream_t>(stream);
-  int rc = q_rows_launch(q, q_dtype == K8V4_BF16, q_tok_stride, sh.tokens, hkv, head_dim, sh.head_rows, q8, scales, s);
+  int rc = sh.head_rows == 0 ? K8V4_OK : q_rows_launch(q, q_dtype == K8V4_BF16, q_tok_stride, sh.tokens, hkv, head_dim, sh.head_rows, q8, scales, s);
   if (rc) return rc;
   const int tiles = sh.tiles;
   if (sh.blocks) {

@@ -10,7 +10,8 @@
 // taking the steps in order gives what reading everything first would.  A thread
 // owns a slice of a token's row in one region (16 bytes of K, 8 of V, a word of a
 // plane) and moves that slice of every node itself, eight nodes' loads in flight,
-// so no two threads touch the same bytes and nothing has to be waited for.
+// so no two threads touch the same bytes and nothing has to be waited for.  The
+// slots are found once for all of them, by one wave, a lane an entry.
 //
 // Bound by latency: a branch is a few rows of 1 to 2 KB, found by three dependent
 // loads (path, table, row).
@@ -37,52 +38,70 @@ struct KeepArgs {
 
 constexpr int kThreads = 192;  // slices of a token at most: 64 of K, 64 of V, 12 of the planes
 constexpr int kInFlight = 8;
+constexpr int kEntries = kWave;  // looked up together
 
 // Slot (page * 64 + row) of token t, -1 if it has none.
 __device__ __forceinline__ int64_t slot_of(const KeepArgs &a, const int32_t *row, int64_t t) {
-  if (t < 0 || t / kPage >= a.table_pages) return -1;
-  const int64_t p = t / kPage;
-  const int64_t page = static_cast<int64_t>(row[p / a.ppb]) * a.ppb + p % a.ppb;
+  if (t < 0 || t >= a.table_pages * kPage) return -1;
+  const uint32_t p = static_cast<uint32_t>(t / kPage), ppb = static_cast<uint32_t>(a.ppb);
+  const uint32_t entry = ppb == 1 ? p : p / ppb;
+  const int64_t page = static_cast<int64_t>(row[entry]) * a.ppb + (p - entry * ppb);
   return page >= 0 && page < a.num_pages ? page * kPage + t % kPage : -1;
 }
 
+struct Move {
+  int64_t from, to;  // slots
+};
+
 template <typename T>
-__device__ __forceinline__ void keep_slice(const KeepArgs &a, char *base, int64_t ps, int row_bytes, int off, int b) {
-  const int32_t *path = a.path + b * a.path_stride;
-  const int32_t *row = a.block_table + b * a.bt_stride;
-  const int64_t first = a.starts[b];
-  const int count = min(max(a.accepted[b], -1), a.width - 1) + 1;
+__device__ __forceinline__ void move_slice(char *base, int64_t ps, int row_bytes, int off, const Move *moves, int count) {
   for (int i0 = 0; i0 < count; i0 += kInFlight) {
-    int64_t src[kInFlight], dst[kInFlight];
-#pragma unroll
-    for (int u = 0; u < kInFlight; ++u) {
-      const int i = min(i0 + u, count - 1), node = path[i];
-      const bool moves = i0 + u < count && node > i;
-      const int64_t from = moves ? slot_of(a, row, first + node) : -1, to = moves ? slot_of(a, row, first + i) : -1;
-      src[u] = to < 0 ? -1 : from;
-      dst[u] = to;
-    }
     T x[kInFlight];
 #pragma unroll
-    for (int u = 0; u < kInFlight; ++u)
-      if (src[u] >= 0) x[u] = *reinterpret_cast<const T *>(base + src[u] / kPage * ps + src[u] % kPage * row_bytes + off);
+    for (int u = 0; u < kInFlight; ++u) {
+      const int64_t s = moves[min(i0 + u, count - 1)].from;
+      x[u] = *reinterpret_cast<const T *>(base + (s >> 6) * ps + (s & 63) * row_bytes + off);
+    }
 #pragma unroll
-    for (int u = 0; u < kInFlight; ++u)
-      if (src[u] >= 0) *reinterpret_cast<T *>(base + dst[u] / kPage * ps + dst[u] % kPage * row_bytes + off) = x[u];
+    for (int u = 0; u < kInFlight; ++u) {
+      if (i0 + u >= count) break;
+      const int64_t s = moves[i0 + u].to;
+      *reinterpret_cast<T *>(base + (s >> 6) * ps + (s & 63) * row_bytes + off) = x[u];
+    }
   }
 }
 
 __global__ __launch_bounds__(kThreads) void kv_keep_kernel(KeepArgs a) {
+  __shared__ Move moves[kEntries];
+  __shared__ int count;
   const int b = blockIdx.x, t = threadIdx.x;
   const int k_row = a.hkv * a.head_dim, v_row = k_row / 2, plane_row = a.hkv * 4;
   const int nk = k_row / 16, nv = v_row / 8;
-  if (t < nk) {
-    keep_slice<u32x4>(a, a.base[0], a.ps[0], k_row, 16 * t, b);
-  } else if (t < nk + nv) {
-    keep_slice<uint64_t>(a, a.base[2], a.ps[2], v_row, 8 * (t - nk), b);
-  } else if (t < nk + nv + 3 * a.hkv) {
-    const int p = (t - nk - nv) / a.hkv, r = p == 0 ? 1 : p + 2;
-    keep_slice<uint32_t>(a, a.base[r], a.ps[r], plane_row, 4 * ((t - nk - nv) % a.hkv), b);
+  const int kept = min(max(a.accepted[b], -1), a.width - 1) + 1;
+  for (int i0 = 0; i0 < kept; i0 += kEntries) {
+    if (t < kEntries) {
+      const int i = i0 + t;
+      const int node = i < kept ? a.path[b * a.path_stride + i] : -1;
+      const int32_t *row = a.block_table + b * a.bt_stride;
+      const int64_t first = a.starts[b];
+      Move m = {-1, -1};
+      if (node > i) m = {slot_of(a, row, first + node), slot_of(a, row, first + i)};
+      const bool moves_it = m.from >= 0 && m.to >= 0;
+      const uint64_t all = __ballot(moves_it);
+      if (moves_it) moves[__popcll(all & ((uint64_t(1) << t) - 1))] = m;
+      if (t == 0) count = __popcll(all);
+    }
+    __syncthreads();
+    const int n = count;
+    if (t < nk) {
+      move_slice<u32x4>(a.base[0], a.ps[0], k_row, 16 * t, moves, n);
+    } else if (t < nk + nv) {
+      move_slice<uint64_t>(a.base[2], a.ps[2], v_row, 8 * (t - nk), moves, n);
+    } else if (t < nk + nv + 3 * a.hkv) {
+      const int p = (t - nk - nv) / a.hkv, r = p == 0 ? 1 : p + 2;
+      move_slice<uint32_t>(a.base[r], a.ps[r], plane_row, 4 * ((t - nk - nv) % a.hkv), moves, n);
+    }
+    __syncthreads();
   }
 }
 

@@ -398,7 +398,7 @@ class _Ops:
                                  k_scale, v_cache, v_scale, v_zero, q_out):
         """Validate a rotated store once; returns a :class:`DeviceCall` (None when there are no tokens)."""
         _require(k_fp16.dim() == 3, "k_fp16 [T,HKV,D]")
-        ntok, hkv, head_dim = (int(x) for x in k_fp16.shape)
+        ntok, hkv, head_dim = k_fp16.shape
         _require(head_dim in (128, 256), "k_fp16 [T,HKV,D] with D in (128, 256)")
         _checked_hkv(hkv)
         _require(k_fp16.dtype == v_fp16.dtype, "k/v_fp16 dtypes differ")
@@ -411,33 +411,37 @@ class _Ops:
         _require(positions.dtype in (torch.int32, torch.int64) and positions.shape == (ntok,)
                  and positions.is_contiguous(), "positions must be a contiguous int32 or int64 [T]")
         _require(cos_sin.dtype in _DTYPE_CODE and cos_sin.dim() == 2, "cos_sin float16, bfloat16 or float32 [P,R]")
-        table_rows, rot = (int(x) for x in cos_sin.shape)
+        table_rows, rot = cos_sin.shape
         _require(rot % 16 == 0 and 16 <= rot <= head_dim and table_rows >= 1,
-                 "cos_sin [P,R] with R a multiple of 16 up to %d" % head_dim)
+                 "cos_sin [P,R] with R a multiple of 16 up to the head dim")
         _require(cos_sin.stride(1) == 1, "cos_sin rows must be contiguous")
         ks = _src_rows(k_fp16, "k_fp16", hkv, head_dim)
         vs = _src_rows(v_fp16, "v_fp16", hkv, head_dim)
         _require((q_fp16 is None) == (q_out is None), "q_fp16 and q_out go together")
         tensors = (k_fp16, v_fp16, positions, cos_sin, slot_mapping, k_cache, k_scale, v_cache, v_scale, v_zero)
-        qs = qos = GQA * hkv * head_dim
+        heads = GQA * hkv
+        q_ptr = out_ptr = 0
+        qs = qos = heads * head_dim
         if q_fp16 is not None:
-            _require(q_fp16.shape == (ntok, GQA * hkv, head_dim), "q_fp16 [T,%d,%d]" % (GQA * hkv, head_dim))
+            _require(q_fp16.shape == (ntok, heads, head_dim), "q_fp16 [T,HQ,D] with HQ = 6 * HKV")
             _require(q_fp16.dtype == k_fp16.dtype, "q/k_fp16 dtypes differ")
             _require(q_out.shape == q_fp16.shape and q_out.dtype == q_fp16.dtype, "q_out must match q_fp16")
-            qs = _src_rows(q_fp16, "q_fp16", GQA * hkv, head_dim)
-            qos = _src_rows(q_out, "q_out", GQA * hkv, head_dim)
+            qs = _src_rows(q_fp16, "q_fp16", heads, head_dim)
+            qos = _src_rows(q_out, "q_out", heads, head_dim)
+            q_ptr, out_ptr = q_fp16.data_ptr(), q_out.data_ptr()
+            _require(q_ptr != out_ptr or qs == qos, "q_out may be q_fp16 itself, not another view of its rows")
             tensors += (q_fp16, q_out)
         if ntok == 0:
             return None
         dev = _on_gpu(*tensors)
-        args = [
-            0 if q_fp16 is None else _ptr(q_fp16), _ptr(k_fp16), _ptr(v_fp16), _DTYPE_CODE[k_fp16.dtype], qs, ks, vs,
-            _ptr(positions), int(positions.dtype == torch.int64), _ptr(cos_sin), _DTYPE_CODE[cos_sin.dtype],
-            table_rows, int(cos_sin.stride(0)) if table_rows > 1 else rot, rot, int(bool(neox)),
-            _ptr(slot_mapping), ntok, hkv, head_dim,
+        args = (
+            q_ptr, k_fp16.data_ptr(), v_fp16.data_ptr(), _DTYPE_CODE[k_fp16.dtype], qs, ks, vs,
+            positions.data_ptr(), int(positions.dtype == torch.int64), cos_sin.data_ptr(), _DTYPE_CODE[cos_sin.dtype],
+            table_rows, cos_sin.stride(0) if table_rows > 1 else rot, rot, int(bool(neox)),
+            slot_mapping.data_ptr(), ntok, hkv, head_dim,
             *cache_args(k_cache, k_scale, v_cache, v_scale, v_zero),
-            0 if q_out is None else _ptr(q_out), qos,
-        ]
+            out_ptr, qos,
+        )
         return DeviceCall(self._lib, self._lib.k8v4_rope_kv_store_paged, args, dev, tensors)
 
     # -- decode / MTP verify ----------------------------------------------
@@ -1019,6 +1023,43 @@ class _Ops:
     def bind_accept_tree(self, draft_tokens, parents, target_tokens, seq_lens, path, out_tokens, accepted, next_lens,
                          num_nodes=None):
         """Validate one acceptance; returns a :class:`DeviceCall` (None for an empty batch)."""
+        shape, walk = draft_tokens.shape, path.shape
+        whole = seq_lens is not None and next_lens is not None and num_nodes is None
+        # The usual call in one condition; any other goes through the checks one by one.
+        if not (
+            whole and len(shape) == 2 and 1 <= shape[1] <= 64 and draft_tokens.dtype in (torch.int32, torch.int64)
+            and parents.dtype == path.dtype == accepted.dtype == seq_lens.dtype == next_lens.dtype == torch.int32
+            and target_tokens.dtype == out_tokens.dtype == torch.int64
+            and parents.shape == target_tokens.shape == shape and out_tokens.shape == walk and len(walk) == 2
+            and walk[0] == shape[0] and 1 <= walk[1] <= shape[1]
+            and accepted.shape == seq_lens.shape == next_lens.shape == shape[:1]
+            and draft_tokens.is_contiguous() and parents.is_contiguous() and target_tokens.is_contiguous()
+            and path.is_contiguous() and out_tokens.is_contiguous() and accepted.is_contiguous()
+            and seq_lens.is_contiguous() and next_lens.is_contiguous()
+        ):
+            self._check_accept(draft_tokens, parents, target_tokens, seq_lens, path, out_tokens, accepted, next_lens,
+                               num_nodes)
+        batch, nodes = shape
+        width = walk[1]
+        if batch == 0:
+            return None
+        tensors = (draft_tokens, parents, target_tokens, path, out_tokens, accepted)
+        tensors += tuple(x for x in (seq_lens, next_lens, num_nodes) if x is not None)
+        dev = _on_gpu(*tensors)
+        many = batch > 1
+        args = (
+            draft_tokens.data_ptr(), int(draft_tokens.dtype == torch.int64), draft_tokens.stride(0) if many else nodes,
+            parents.data_ptr(), parents.stride(0) if many else nodes, 0 if num_nodes is None else num_nodes.data_ptr(),
+            target_tokens.data_ptr(), target_tokens.stride(0) if many else nodes,
+            0 if seq_lens is None else seq_lens.data_ptr(), batch, nodes, width,
+            path.data_ptr(), path.stride(0) if many else width, out_tokens.data_ptr(),
+            out_tokens.stride(0) if many else width, accepted.data_ptr(),
+            0 if next_lens is None else next_lens.data_ptr(),
+        )
+        return DeviceCall(self._lib, self._lib.k8v4_accept_tree, args, dev, tensors)
+
+    @staticmethod
+    def _check_accept(draft_tokens, parents, target_tokens, seq_lens, path, out_tokens, accepted, next_lens, num_nodes):
         _require(draft_tokens.dim() == 2 and draft_tokens.dtype in (torch.int32, torch.int64),
                  "draft_tokens int32 or int64 [B,N]")
         batch, nodes = (int(x) for x in draft_tokens.shape)
@@ -1033,27 +1074,11 @@ class _Ops:
                         ("path", path), ("out_tokens", out_tokens)):
             _require(x.shape[1] == 1 or x.stride(1) == 1, "%s rows must be contiguous" % name)
         _require(next_lens is None or seq_lens is not None, "next_lens needs seq_lens")
-        tensors = (draft_tokens, parents, target_tokens, path, out_tokens, accepted)
         for name, x in (("accepted", accepted), ("seq_lens", seq_lens), ("next_lens", next_lens),
                         ("num_nodes", num_nodes)):
             if x is not None or name == "accepted":
                 _require(x is not None and x.dtype == torch.int32 and x.shape == (batch,) and x.is_contiguous(),
                          "%s must be a contiguous int32 [B]" % name)
-                if name != "accepted":
-                    tensors += (x,)
-        if batch == 0:
-            return None
-        dev = _on_gpu(*tensors)
-        many = batch > 1
-        args = [
-            _ptr(draft_tokens), int(draft_tokens.dtype == torch.int64), int(draft_tokens.stride(0)) if many else nodes,
-            _ptr(parents), int(parents.stride(0)) if many else nodes, 0 if num_nodes is None else _ptr(num_nodes),
-            _ptr(target_tokens), int(target_tokens.stride(0)) if many else nodes,
-            0 if seq_lens is None else _ptr(seq_lens), batch, nodes, width,
-            _ptr(path), int(path.stride(0)) if many else width, _ptr(out_tokens),
-            int(out_tokens.stride(0)) if many else width, _ptr(accepted), 0 if next_lens is None else _ptr(next_lens),
-        ]
-        return DeviceCall(self._lib, self._lib.k8v4_accept_tree, args, dev, tensors)
 
     def kv_keep_paged(self, k_cache, k_scale, v_cache, v_scale, v_zero, block_table, seq_starts, path, accepted,
                       pages_per_block):
@@ -1073,34 +1098,40 @@ class _Ops:
     def bind_kv_keep_paged(self, k_cache, k_scale, v_cache, v_scale, v_zero, block_table, seq_starts, path, accepted,
                            pages_per_block):
         """Validate one move; returns a :class:`DeviceCall` (None where there is nothing to move)."""
-        _require(k_cache.dim() == 4 and v_cache.dim() == 4, "k_cache [num_blocks,64,HKV,D] NHD")
-        hkv, head_dim = _checked_hkv(int(k_cache.shape[2])), int(k_cache.shape[3])
+        _require(k_cache.dim() == 4, "k_cache [num_blocks,64,HKV,D] NHD")
+        _pages, _tokens, hkv, head_dim = k_cache.shape
+        _checked_hkv(hkv)
         _require(head_dim in (128, 256), "k_cache head dim must be 128 or 256")
         check_paged_k(k_cache, k_scale, hkv, head_dim)
         check_paged_v(v_cache, v_scale, v_zero, hkv, head_dim)
         _require(k_cache.shape[0] == v_cache.shape[0], "k/v num_blocks")
-        _require(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1,
-                 "block_table must be int32 [B, W] with unit column stride")
-        batch = int(block_table.shape[0])
-        for name, x in (("seq_starts", seq_starts), ("accepted", accepted)):
-            _require(x.dtype == torch.int32 and x.shape == (batch,) and x.is_contiguous(),
-                     "%s must be a contiguous int32 [B]" % name)
-        _require(path.dtype == torch.int32 and path.dim() == 2 and path.shape[0] == batch, "path int32 [B,W]")
-        width = int(path.shape[1])
-        _require(width <= 1 or path.stride(1) == 1, "path rows must be contiguous")
+        table = block_table.shape
+        if not (
+            len(table) == 2 and path.dim() == 2 and path.shape[0] == table[0]
+            and block_table.dtype == seq_starts.dtype == path.dtype == accepted.dtype == torch.int32
+            and seq_starts.shape == accepted.shape == table[:1] and block_table.is_contiguous()
+            and path.is_contiguous() and seq_starts.is_contiguous() and accepted.is_contiguous()
+        ):
+            _require(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1,
+                     "block_table must be int32 [B, W] with unit column stride")
+            for name, x in (("seq_starts", seq_starts), ("accepted", accepted)):
+                _require(x.dtype == torch.int32 and x.shape == table[:1] and x.is_contiguous(),
+                         "%s must be a contiguous int32 [B]" % name)
+            _require(path.dtype == torch.int32 and path.dim() == 2 and path.shape[0] == table[0], "path int32 [B,W]")
+            _require(path.shape[1] <= 1 or path.stride(1) == 1, "path rows must be contiguous")
+        batch, width = path.shape
         _require(int(pages_per_block) >= 1, "pages_per_block")
         if batch == 0 or width == 0:
             return None
-        _require(int(block_table.shape[1]) > 0, "block_table width")
+        _require(table[1] > 0, "block_table width")
         tensors = (k_cache, k_scale, v_cache, v_scale, v_zero, block_table, seq_starts, path, accepted)
         dev = _on_gpu(*tensors)
-        many = batch > 1
-        args = [
+        args = (
             *cache_args(k_cache, k_scale, v_cache, v_scale, v_zero),
-            _ptr(block_table), int(block_table.stride(0)) if many else int(block_table.shape[1]),
-            int(block_table.shape[1]), int(pages_per_block), _ptr(seq_starts), _ptr(path),
-            int(path.stride(0)) if many else width, width, _ptr(accepted), batch, hkv, head_dim,
-        ]
+            block_table.data_ptr(), block_table.stride(0) if batch > 1 else table[1], table[1], int(pages_per_block),
+            seq_starts.data_ptr(), path.data_ptr(), path.stride(0) if batch > 1 else width, width,
+            accepted.data_ptr(), batch, hkv, head_dim,
+        )
         return DeviceCall(self._lib, self._lib.k8v4_kv_keep_paged, args, dev, tensors)
 
     # -- log probabilities ---------------------------------------------------------
@@ -1127,10 +1158,48 @@ class _Ops:
 
     def bind_token_logprobs(self, logits, tokens, workspace, logprobs, ranks, entropy, top_ids, top_logprobs):
         """Validate one call; returns a :class:`DeviceCall` (None for no rows)."""
+        shape = logits.shape
+        whole = tokens is not None and entropy is not None and top_ids is not None and workspace is not None
+        # The usual call in one condition; any other goes through the checks one by one.
+        if not (
+            whole and len(shape) == 2 and shape[1] >= 1 and logits.dtype in _DTYPE_CODE and logits.stride(1) == 1
+            and logprobs is not None and ranks is not None and top_logprobs is not None
+            and tokens.dtype in (torch.int32, torch.int64) and ranks.dtype == torch.int32
+            and logprobs.dtype == entropy.dtype == top_logprobs.dtype == torch.float32 and top_ids.dtype == torch.int64
+            and tokens.shape == logprobs.shape == ranks.shape == entropy.shape == shape[:1]
+            and top_ids.dim() == 2 and top_ids.shape[0] == shape[0] and top_ids.shape[1] <= 64
+            and top_logprobs.shape == top_ids.shape
+            and tokens.is_contiguous() and logprobs.is_contiguous() and ranks.is_contiguous()
+            and entropy.is_contiguous() and top_ids.is_contiguous() and top_logprobs.is_contiguous()
+            and workspace.is_contiguous()
+        ):
+            self._check_logprobs(logits, tokens, workspace, logprobs, ranks, entropy, top_ids, top_logprobs)
+        rows, vocab = shape
+        if rows == 0:
+            return None
+        top = 0 if top_ids is None else top_ids.shape[1]
+        tensors = (logits, tokens, logprobs, ranks, entropy, workspace) + ((top_ids, top_logprobs) if top else ())
+        if not whole:
+            tensors = tuple(x for x in tensors if x is not None)
+        dev = _on_gpu(*tensors)
+        many = rows > 1
+        args = (
+            logits.data_ptr(), _DTYPE_CODE[logits.dtype], logits.stride(0) if many else vocab,
+            0 if tokens is None else tokens.data_ptr(), int(tokens is not None and tokens.dtype == torch.int64),
+            rows, vocab, top, 0 if tokens is None else logprobs.data_ptr(), 0 if tokens is None else ranks.data_ptr(),
+            0 if entropy is None else entropy.data_ptr(),
+            top_ids.data_ptr() if top else 0, top_ids.stride(0) if top and many else top,
+            top_logprobs.data_ptr() if top else 0, top_logprobs.stride(0) if top and many else top,
+            0 if workspace is None else workspace.data_ptr(),
+            0 if workspace is None else workspace.numel() * workspace.element_size(),
+        )
+        return DeviceCall(self._lib, self._lib.k8v4_token_logprobs, args, dev, tensors)
+
+    @staticmethod
+    def _check_logprobs(logits, tokens, workspace, logprobs, ranks, entropy, top_ids, top_logprobs):
         _require(logits.dim() == 2 and logits.dtype in _DTYPE_CODE, "logits float16, bfloat16 or float32 [N,V]")
-        rows, vocab = (int(x) for x in logits.shape)
+        rows, vocab = logits.shape
         _require(vocab >= 1 and (vocab == 1 or logits.stride(1) == 1), "logits rows must be contiguous")
-        tensors = (logits,)
         _require((tokens is None) == (logprobs is None) and (tokens is None) == (ranks is None),
                  "tokens, logprobs and ranks go together")
         if tokens is not None:
@@ -1138,42 +1207,19 @@ class _Ops:
                      "tokens must be a contiguous int32 or int64 [N]")
             _require(ranks.dtype == torch.int32 and ranks.shape == (rows,) and ranks.is_contiguous(),
                      "ranks must be a contiguous int32 [N]")
-            tensors += (tokens, logprobs, ranks)
         for name, x in (("logprobs", logprobs), ("entropy", entropy)):
             if x is not None:
                 _require(x.dtype == torch.float32 and x.shape == (rows,) and x.is_contiguous(),
                          "%s must be a contiguous float32 [N]" % name)
-        if entropy is not None:
-            tensors += (entropy,)
         _require((top_ids is None) == (top_logprobs is None), "top_ids and top_logprobs go together")
-        top = 0
         if top_ids is not None:
             _require(top_ids.dtype == torch.int64 and top_ids.dim() == 2 and top_ids.shape[0] == rows, "top_ids int64 [N,K]")
-            top = int(top_ids.shape[1])
-            _require(top <= 64, "0 to 64 likeliest tokens")
+            _require(top_ids.shape[1] <= 64, "0 to 64 likeliest tokens")
             _require(top_logprobs.dtype == torch.float32 and top_logprobs.shape == top_ids.shape, "top_logprobs float32 [N,K]")
-            _require(top <= 1 or (top_ids.stride(1) == 1 and top_logprobs.stride(1) == 1),
+            _require(top_ids.shape[1] <= 1 or (top_ids.stride(1) == 1 and top_logprobs.stride(1) == 1),
                      "top_ids/top_logprobs rows must be contiguous")
-            if top:
-                tensors += (top_ids, top_logprobs)
         if workspace is not None:
             _require(workspace.is_contiguous(), "log probability workspace must be a contiguous buffer")
-            tensors += (workspace,)
-        if rows == 0:
-            return None
-        dev = _on_gpu(*tensors)
-        many = rows > 1
-        args = [
-            _ptr(logits), _DTYPE_CODE[logits.dtype], int(logits.stride(0)) if many else vocab,
-            0 if tokens is None else _ptr(tokens), int(tokens is not None and tokens.dtype == torch.int64),
-            rows, vocab, top, 0 if tokens is None else _ptr(logprobs), 0 if tokens is None else _ptr(ranks),
-            0 if entropy is None else _ptr(entropy),
-            _ptr(top_ids) if top else 0, int(top_ids.stride(0)) if top and many else top,
-            _ptr(top_logprobs) if top else 0, int(top_logprobs.stride(0)) if top and many else top,
-            0 if workspace is None else _ptr(workspace),
-            0 if workspace is None else int(workspace.numel()) * workspace.element_size(),
-        ]
-        return DeviceCall(self._lib, self._lib.k8v4_token_logprobs, args, dev, tensors)
 
     # -- the Q-once tile and the ops that read it ----------------------------
     def q_quant_once(self, q_fp16, q8, q_scale):
