@@ -26,7 +26,8 @@ constexpr int kMaxListed = 256;
 constexpr int kSliceUnit = 2048;        // elements of a slice at least, and its length's unit
 constexpr int kMaxSliceLen = 1 << 18;   // its chunks' maxima fit the LDS
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kFarBelow = -1000.f;  // exp of it is 0
+constexpr float kLn2 = 0.69314718055994531f;
+constexpr float kFarBelow = -1000.f;  // exp and 2 to the power of it are 0
 
 struct LogprobArgs {
   const void *logits;
@@ -111,27 +112,51 @@ __device__ __forceinline__ Sums join(Sums a, Sums b) {
   return a;
 }
 
-__device__ __forceinline__ float wave_max_f32(float x) {
-#pragma unroll
-  for (int m = 1; m < kWave; m <<= 1) x = fmaxf(x, __shfl_xor(x, m, kWave));
-  return x;
+// The sums as a wave forms them, its maximum m in every lane: in powers of two
+// against m2, the fp32 value of m log2(e), so that an element takes one fma, t = x
+// log2(e) - m2.  m itself then has t = off, some 2^-24 of m2, which `sums_of` takes out.
+// A maximum of 1e37 or more of either sign (its log2(e) may not exist) leaves
+// nothing but equal elements to the sums; t is not formed then.
+struct WaveSums {
+  float m, m2, off;
+  float r, q;  // sum 2^t, sum t 2^t, of the lane
+};
+__device__ __forceinline__ bool huge(float m) { return !(fabsf(m) < 1e37f); }
+// `own`: this lane counts the element left out so far.
+__device__ __forceinline__ void raise(WaveSums &s, float m, bool own) {
+  const float m2 = m * kLog2e;
+  if (s.m > -INFINITY) {
+    const float d = huge(m) || huge(s.m) ? kFarBelow : fmaxf(s.m2 - m2, kFarBelow);
+    const float f = __builtin_amdgcn_exp2f(d);
+    const float w = own ? fmaf(s.off, kLn2, 1.f) : 0.f;  // 2^off
+    s.r += w;
+    s.q = fmaf(d, s.r, fmaf(s.off, w, s.q)) * f;
+    s.r *= f;
+  }
+  s.m = m;
+  s.m2 = huge(m) ? 0.f : m2;
+  s.off = huge(m) ? 0.f : fmaf(m, kLog2e, -m2);
 }
+__device__ __forceinline__ Sums sums_of(const WaveSums &s, float r, float q) {
+  const float f = fmaf(-s.off, kLn2, 1.f);  // 2^-off
+  return {s.m, r * f, fmaf(-s.off, r, q) * f * kLn2};
+}
+
 __device__ __forceinline__ float wave_sum_f32(float x) {
 #pragma unroll
   for (int m = 1; m < kWave; m <<= 1) x += __shfl_xor(x, m, kWave);
   return x;
 }
 
-// Max over eight consecutive lanes, without the LDS.
-template <int CTRL>
-__device__ __forceinline__ float max_dpp(float x) {
-  const int y = __builtin_amdgcn_update_dpp(__float_as_int(x), __float_as_int(x), CTRL, 0xF, 0xF, false);
-  return fmaxf(x, __int_as_float(y));
-}
+// Max over eight consecutive lanes, without the LDS (x not NaN).  A lane's value is
+// read two states after it was written at the earliest, which the compiler, not
+// looking into the statement, does not see to.
 __device__ __forceinline__ float max_of_8(float x) {
-  x = max_dpp<0xB1>(x);   // quad_perm 1,0,3,2
-  x = max_dpp<0x4E>(x);   // quad_perm 2,3,0,1
-  return max_dpp<0x141>(x);  // row_half_mirror
+  asm("s_nop 4\n\tv_max_f32_dpp %0, %0, %0 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n\t"
+      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n\t"
+      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_half_mirror row_mask:0xf bank_mask:0xf"
+      : "+v"(x));
+  return x;
 }
 
 template <typename T>
@@ -188,21 +213,15 @@ __device__ void block_first(float &x, int &i, Shared &sh) {
     }
 }
 
-// The foremost `want` of `n` pairs (x(e), id(e)) into `out`, in order, and their
-// number (fewer where the others are minus infinity).  Every thread calls it.  A
-// floor that at least `want` pairs reach, from one maximum a thread, leaves few to
-// rank; where too many reach it (ties), they are taken one at a time.
-template <typename X, typename I>
-__device__ int foremost(int n, int want, X x, I id, Listed *out, Shared &sh) {
+// A value that at least `want` of the work-group's threads' maxima reach: the largest
+// of 16 bits (minus infinity if there is none).  Clears sh.count.
+__device__ float floor_of(float best, int want, Shared &sh) {
   const int t = threadIdx.x;
-  float best = -INFINITY;
-  for (int e = t; e < n; e += kThreads) best = fmaxf(best, x(e));
   sh.best[t] = best;
   if (t == 0) sh.count = 0;
   __syncthreads();
   if (t < kWave) {
-    // The largest floor of 16 bits that `want` threads' maxima reach, bit by bit; as
-    // ordered integers, so that a bit set is a larger value.
+    // Bit by bit, as ordered integers, so that a bit set is a larger value.
     uint32_t key[kWaves];
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
@@ -223,14 +242,24 @@ __device__ int foremost(int n, int want, X x, I id, Listed *out, Shared &sh) {
     if (t == 0) sh.floor = value == value ? value : -INFINITY;  // (below minus infinity the bits are a NaN's)
   }
   __syncthreads();
-  const float floor = sh.floor;
-  for (int e = t; e < n; e += kThreads) {
-    const float v = x(e);
+  return sh.floor;
+}
+
+// The foremost `want` of the pairs that each(take) names to every thread in turn, as
+// take(value, id), into `out`, in order, and their number (fewer where the others are
+// minus infinity); `best` is the largest value named to the thread.  Every thread
+// calls it.  The floor leaves few pairs to rank; where too many reach it (ties), they
+// are taken one at a time.
+template <typename Each>
+__device__ int foremost(float best, int want, Each each, Listed *out, Shared &sh) {
+  const int t = threadIdx.x;
+  const float floor = floor_of(best, want, sh);
+  each([&](float v, int id) {
     if (v >= floor && v > -INFINITY) {
       const int at = atomicAdd(&sh.count, 1);
-      if (at < kMaxListed) sh.list[at] = {v, id(e)};
+      if (at < kMaxListed) sh.list[at] = {v, id};
     }
-  }
+  });
   __syncthreads();
   const int listed = sh.count;
   if (listed <= kMaxListed) {
@@ -248,14 +277,12 @@ __device__ int foremost(int n, int want, X x, I id, Listed *out, Shared &sh) {
   for (int k = 0; k < want; ++k) {
     float v = -INFINITY;
     int i = INT32_MAX;
-    for (int e = t; e < n; e += kThreads) {
-      const float y = x(e);
-      const int j = id(e);
+    each([&](float y, int j) {
       if (ahead(last, ilast, y, j) && ahead(y, j, v, i)) {
         v = y;
         i = j;
       }
-    }
+    });
     block_first(v, i, sh);
     if (!(v > -INFINITY)) {
       __syncthreads();
@@ -267,6 +294,18 @@ __device__ int foremost(int n, int want, X x, I id, Listed *out, Shared &sh) {
   }
   __syncthreads();
   return want;
+}
+// The same of n pairs (x(e), id(e)).
+template <typename X, typename I>
+__device__ int foremost_of(int n, int want, X x, I id, Listed *out, Shared &sh) {
+  float best = -INFINITY;
+  for (int e = threadIdx.x; e < n; e += kThreads) best = fmaxf(best, x(e));
+  return foremost(
+      best, want,
+      [&](auto take) {
+        for (int e = threadIdx.x; e < n; e += kThreads) take(x(e), id(e));
+      },
+      out, sh);
 }
 
 struct Result {
@@ -311,34 +350,45 @@ __device__ __forceinline__ void write_top(const LogprobArgs &a, int64_t row, con
   a.top_logprobs[row * a.lps_stride + t] = t < found ? logprob_of(r, sh.final[t].x) : -INFINITY;
 }
 
-template <typename T>
+// A slice of a row.  Every thread takes kBatch 16-byte vectors of kBatch runs at a
+// time, the next ones under way; ONE: the slice is one such batch, whose elements
+// then stay in registers until the likeliest tokens are found.
+template <typename T, bool ONE>
 __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
   constexpr int N = Vec<T>::N;
   constexpr int CHUNK = kGroupLanes * N;  // elements, 128 bytes
   constexpr int STEP = kThreads * N;      // elements of one vector of every thread
   __shared__ Shared sh;
-  extern __shared__ float values[];  // the largest of each chunk, later the picked chunks' tokens
+  extern __shared__ float values[];  // the largest of each chunk, later the picked chunks' tokens (ONE: not used)
   const int t = threadIdx.x, lane = t & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(t / kWave);
   const int64_t row = blockIdx.x / static_cast<unsigned>(a.slices);
   const int slice = static_cast<int>(blockIdx.x - row * a.slices);
   const T *x = static_cast<const T *>(a.logits) + row * a.row_stride;
   const int first = slice * a.slice_len;
   const int end = static_cast<int>(min(static_cast<int64_t>(first) + a.slice_len, static_cast<int64_t>(a.vocab)));
+
+  Vec<T> v[kBatch];
+  auto load = [&](int at) __attribute__((always_inline)) {
+    if (at + kBatch * STEP <= end) {  // the same for all threads
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) __builtin_memcpy(v[j].x, x + at + j * STEP + t * N, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) load_vec(x, at + j * STEP + t * N, end, v[j]);
+    }
+  };
+  load(first);
   const int64_t token = token_of(a, row);
   const float xt = token_logit<T>(a, row, token);
   // Ahead of the token: at lower indices what is not less, at higher ones what is larger.
   const float above = xt < INFINITY ? next_above(xt) : NAN;  // nothing is larger than plus infinity
   const bool ranked = xt > -INFINITY;
 
-  Sums s = {-INFINITY, 0.f, 0.f};  // m the same for the wave
-  int before = 0;                  // tokens ahead: of the wave, in scalars
-  int mixed = 0;                   // of the lane, in the run that holds the token
-
-  Vec<T> v[kBatch];
-#pragma unroll
-  for (int j = 0; j < kBatch; ++j) load_vec(x, first + j * STEP + t * N, end, v[j]);
+  WaveSums s = {-INFINITY, 0.f, 0.f, 0.f, 0.f};
+  int before = 0;  // tokens ahead: of the wave, in scalars
+  int mixed = 0;   // of the lane, in the run that holds the token
+  float f[kBatch][N], vmax[kBatch];
   for (int at = first; at < end; at += kBatch * STEP) {
-    float f[kBatch][N], vmax[kBatch];
     bool usual = true;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
@@ -350,35 +400,34 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
       vmax[j] = max3_raw(mx, f[j][N - 1], f[j][N - 1]);
       usual &= vmax[j] <= s.m;  // false for a NaN
     }
-    const int next = at + kBatch * STEP;
-    if (next < end) {
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) load_vec(x, next + j * STEP + t * N, end, v[j]);
-    }
-    const bool special = !__all(usual) || s.m == INFINITY;
-    int skip = -1;  // this lane's element left out of the sums
+    if (!ONE && at + kBatch * STEP < end) load(at + kBatch * STEP);
+    const bool special = !__all(usual) || huge(s.m);
+    bool holder = false;  // of a new maximum, whose first element is left out of the sums
     if (special) {
-      // A new maximum, a NaN, nothing so far, or plus infinities.
-      float mine = -INFINITY;
+      // A new maximum, a vector of NaN (or with a signalling one), or nothing so far.
+      bool nan = ONE;  // (the elements are needed without NaN)
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        vmax[j] = -INFINITY;
+      for (int j = 0; j < kBatch; ++j) nan |= vmax[j] != vmax[j];
+      if (__any(nan)) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          f[j][i] = clean(f[j][i]);
-          vmax[j] = fmaxf(vmax[j], f[j][i]);
+        for (int j = 0; j < kBatch; ++j) {
+          vmax[j] = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            f[j][i] = clean(f[j][i]);
+            vmax[j] = fmaxf(vmax[j], f[j][i]);
+          }
         }
-        mine = fmaxf(mine, vmax[j]);
       }
-      const float m = wave_max_f32(mine);
+      float mine = vmax[0];
+#pragma unroll
+      for (int j = 1; j < kBatch; ++j) mine = fmaxf(mine, vmax[j]);
+      float m = mine;
+#pragma unroll
+      for (int d = 1; d < kWave; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, kWave));
       if (m > s.m) {
         raise(s, m, lane == 0);
-        const bool holder = lane == __builtin_ctzll(__ballot(mine == m));
-#pragma unroll
-        for (int j = kBatch - 1; j >= 0; --j)
-#pragma unroll
-          for (int i = N - 1; i >= 0; --i)
-            if (holder && f[j][i] == m) skip = j * N + i;
+        holder = lane == __builtin_ctzll(__ballot(mine == m));
       }
     }
     if (ranked) {
@@ -395,77 +444,108 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
         }
       }
     }
-    if (a.top) {
+    if (!ONE && a.top) {
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
         const float c = max_of_8(vmax[j]);
         if ((lane & (kGroupLanes - 1)) == 0) values[(at - first + j * STEP + t * N) / CHUNK] = c;
       }
     }
-    if (special) {
+    auto add = [&](int j, int i, float &r, float &q) __attribute__((always_inline)) {
+      const float y = fmaxf(fmaf(f[j][i], kLog2e, -s.m2), kFarBelow);  // a NaN or minus infinity: 2^y is 0
+      const float e = __builtin_amdgcn_exp2f(y);
+      r += e;
+      q = fmaf(y, e, q);
+    };
+    if (!special) {
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j)
+      for (int j = 0; j < kBatch; ++j) {
+        float r = 0.f, q = 0.f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          if (s.m == INFINITY && f[j][i] == INFINITY && skip != j * N + i) s.r += 1.f;
-          if (skip == j * N + i) f[j][i] = -INFINITY;
-        }
-    }
-    if (s.m > -INFINITY && s.m < INFINITY) {
+        for (int i = 0; i < N; ++i) add(j, i, r, q);
+        s.r += r;
+        s.q += q;
+      }
+    } else if (s.m > -INFINITY) {
+      const bool only_equal = huge(s.m);
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
         float r = 0.f, q = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const float y = fmaxf(f[j][i] - s.m, kFarBelow);  // a NaN or minus infinity: exp is 0
-          const float e = __builtin_amdgcn_exp2f(y * kLog2e);
-          r += e;
-          q = fmaf(y, e, q);
+          const bool equal = f[j][i] == s.m;
+          if (holder && equal)
+            holder = false;
+          else if (!only_equal)
+            add(j, i, r, q);
+          else if (equal)
+            r += 1.f;
         }
         s.r += r;
         s.q += q;
       }
     }
   }
-  s.r = wave_sum_f32(s.r);
-  s.q = wave_sum_f32(s.q);
+  const float r = wave_sum_f32(s.r), q = wave_sum_f32(s.q);
 #pragma unroll
   for (int m = 1; m < kWave; m <<= 1) mixed += __shfl_xor(mixed, m, kWave);
-  if (lane == 0) sh.part[wave] = {s.m, s.r, s.q, before + mixed};
+  if (lane == 0) {
+    const Sums w = sums_of(s, r, q);
+    sh.part[wave] = {w.m, w.r, w.q, before + mixed};
+  }
   __syncthreads();
-  s = {sh.part[0].m, sh.part[0].rest, sh.part[0].mean};
+  Sums sum = {sh.part[0].m, sh.part[0].rest, sh.part[0].mean};
   before = sh.part[0].before;
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) {
-    s = join(s, {sh.part[w].m, sh.part[w].rest, sh.part[w].mean});
+    sum = join(sum, {sh.part[w].m, sh.part[w].rest, sh.part[w].mean});
     before += sh.part[w].before;
   }
 
   int found = 0;
   if (a.top) {
-    // The foremost `top` chunks hold the foremost `top` tokens: a token of another
-    // chunk has the largest of each of them ahead of it, chunks being runs of tokens.
-    const int chunks = (max(end - first, 0) + CHUNK - 1) / CHUNK;
-    const int picked = foremost(chunks, a.top, [&](int e) { return values[e]; }, [](int e) { return e; }, sh.picked, sh);
-    for (int e = t; e < picked * kGroupLanes; e += kThreads) {
-      Vec<T> w;
-      load_vec(x, first + sh.picked[e / kGroupLanes].i * CHUNK + e % kGroupLanes * N, end, w);
+    if constexpr (ONE) {
+      float best = -INFINITY;
+      if (first < end) {
+        best = vmax[0];
 #pragma unroll
-      for (int i = 0; i < N; ++i) values[e * N + i] = clean(static_cast<float>(w.x[i]));
+        for (int j = 1; j < kBatch; ++j) best = fmaxf(best, vmax[j]);
+      }
+      found = foremost(
+          best, a.top,
+          [&](auto take) {
+            if (first >= end) return;
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+              for (int i = 0; i < N; ++i) take(f[j][i], first + j * STEP + t * N + i);
+          },
+          sh.final, sh);
+    } else {
+      // The foremost `top` chunks hold the foremost `top` tokens: a token of another
+      // chunk has the largest of each of them ahead of it, chunks being runs of tokens.
+      const int chunks = (max(end - first, 0) + CHUNK - 1) / CHUNK;
+      const int picked = foremost_of(chunks, a.top, [&](int e) { return values[e]; }, [](int e) { return e; }, sh.picked, sh);
+      for (int e = t; e < picked * kGroupLanes; e += kThreads) {
+        Vec<T> w;
+        load_vec(x, first + sh.picked[e / kGroupLanes].i * CHUNK + e % kGroupLanes * N, end, w);
+#pragma unroll
+        for (int i = 0; i < N; ++i) values[e * N + i] = clean(static_cast<float>(w.x[i]));
+      }
+      __syncthreads();
+      found = foremost_of(
+          picked * CHUNK, a.top, [&](int e) { return values[e]; },
+          [&](int e) { return first + sh.picked[e / CHUNK].i * CHUNK + e % CHUNK; }, sh.final, sh);
     }
-    __syncthreads();
-    found = foremost(
-        picked * CHUNK, a.top, [&](int e) { return values[e]; },
-        [&](int e) { return first + sh.picked[e / CHUNK].i * CHUNK + e % CHUNK; }, sh.final, sh);
   }
   if (a.slices == 1) {
-    const Result r = result_of(s);
-    if (t == 0) write_row<T>(a, row, r, before, xt);
-    write_top(a, row, r, found, sh);
+    const Result res = result_of(sum);
+    if (t == 0) write_row<T>(a, row, res, before, xt);
+    write_top(a, row, res, found, sh);
     return;
   }
   char *out = a.ws + blockIdx.x * part_bytes(a.top);
-  if (t == 0) *reinterpret_cast<Part *>(out) = {s.m, s.r, s.q, before};
+  if (t == 0) *reinterpret_cast<Part *>(out) = {sum.m, sum.r, sum.q, before};
   if (t < a.top) reinterpret_cast<Listed *>(out + sizeof(Part))[t] = t < found ? sh.final[t] : Listed{-INFINITY, INT32_MAX};
 }
 
@@ -497,7 +577,7 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(LogprobArgs a) {
     before += __shfl_xor(before, m, kWave);
   }
   __syncthreads();
-  const int found = a.top ? foremost(n, a.top, [&](int e) { return values[e]; }, [&](int e) { return ids[e]; }, sh.final, sh) : 0;
+  const int found = a.top ? foremost_of(n, a.top, [&](int e) { return values[e]; }, [&](int e) { return ids[e]; }, sh.final, sh) : 0;
   const Result r = result_of(s);
   if (t == 0) write_row<T>(a, row, r, before, xt);
   write_top(a, row, r, found, sh);
@@ -517,9 +597,14 @@ int slices_of(int64_t rows, int64_t vocab) {
 template <typename T>
 int launch(LogprobArgs a, int64_t rows, hipStream_t s) {
   constexpr int CHUNK = kGroupLanes * Vec<T>::N, ROUND = kBatch * kThreads * Vec<T>::N;
-  const int64_t chunks = static_cast<int64_t>((a.slice_len + ROUND - 1) / ROUND) * ROUND / CHUNK;
-  const int64_t floats = !a.top ? 0 : chunks > a.top * CHUNK ? chunks : a.top * CHUNK;
-  logprob_kernel<T><<<dim3(static_cast<unsigned>(rows * a.slices)), dim3(kThreads), floats * 4, s>>>(a);
+  const dim3 grid(static_cast<unsigned>(rows * a.slices));
+  if (a.slice_len <= ROUND) {
+    logprob_kernel<T, true><<<grid, dim3(kThreads), 0, s>>>(a);
+  } else {
+    const int64_t chunks = static_cast<int64_t>((a.slice_len + ROUND - 1) / ROUND) * ROUND / CHUNK;
+    const int64_t floats = !a.top ? 0 : chunks > a.top * CHUNK ? chunks : a.top * CHUNK;
+    logprob_kernel<T, false><<<grid, dim3(kThreads), floats * 4, s>>>(a);
+  }
   int rc = launch_status("k8v4_token_logprobs");
   if (rc || a.slices == 1) return rc;
   logprob_join_kernel<T><<<dim3(static_cast<unsigned>(rows)), dim3(kThreads), a.slices * a.top * 8, s>>>(a);
