@@ -11,6 +11,18 @@
 // S is kept as 1 + r with r the sum without one largest element, and log S as
 // log1p(r), so that a token of probability near 1 keeps its log to fp32's relative
 // accuracy.
+//
+// One pass.  A wave keeps one running maximum; a batch of elements below it, which
+// most are, takes one fma, one clamp (for NaN and minus infinity), one exponential and
+// two additions an element, a comparison with the given token (counted in scalars) and
+// half an instruction of a maximum; a batch with a new maximum rescales the sums.  The
+// maxima of 128-byte chunks go to the LDS; the K foremost chunks hold the K likeliest
+// tokens, which are read again and ranked.  Few rows are cut into slices and joined by
+// a second launch.
+//
+// Bound by memory, closely followed by issue (12 slots an element): 2048 x 152000 bf16
+// with 20 tokens a row 150 us, 4.1 TB/s (a sum over 2 GiB reads 4.0); calls of a few
+// rows by latency, two launches of about 8 and 5 us.
 #include "k8v4_common.h"
 
 namespace k8v4 {
@@ -583,10 +595,15 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(LogprobArgs a) {
   write_top(a, row, r, found, sh);
 }
 
-// How many slices a row is cut into: enough work-groups for the chip (two a compute
-// unit), each of a few vectors a thread at least.
+// How many slices a row is cut into: enough for two work-groups a compute unit, or
+// for four where that leaves a slice kLongSlice tokens.  Measured, two a unit / four, us:
+// 48 x 65537 fp16 17.7 / 24.5, 64 x 152000 bf16 30.6 / 31.2, 128 x 152000 fp32 35.2 /
+// 31.3, 256 x 152000 bf16 52.3 / 46.6 (one: 58.0; eight: 59.6), 512 x 32000 27.9 / 32.2.
+constexpr int64_t kLongSlice = 16384;
 int slices_of(int64_t rows, int64_t vocab) {
-  const int64_t wanted = (2 * static_cast<int64_t>(device_cus()) + rows - 1) / rows;
+  const int64_t units = device_cus();
+  const int64_t four = (4 * units + rows - 1) / rows;
+  const int64_t wanted = vocab >= four * kLongSlice ? four : (2 * units + rows - 1) / rows;
   const int64_t most = (vocab + kSliceUnit - 1) / kSliceUnit;
   const int64_t least = (vocab + kMaxSliceLen - 1) / kMaxSliceLen;
   int64_t n = wanted < most ? wanted : most;
