@@ -299,6 +299,42 @@ class Xe2K8V4Impl(AttentionImpl[Xe2K8V4Metadata]):
         v = _rows(value[:ntok], self.layout.hkv, self.layout.head_dim, "value")
         ops().kv_store_paged(k, v, slot_mapping, *regions)
 
+    def fused_rope_kvcache_supported(self) -> bool:
+        """Whether :meth:`do_rope_and_kv_cache_update` may stand for the model's rotation
+        and :meth:`do_kv_cache_update`."""
+        return True
+
+    def do_rope_and_kv_cache_update(
+        self,
+        layer: torch.nn.Module,
+        query: torch.Tensor,
+        key: torch.Tensor,
+        value: torch.Tensor,
+        positions: torch.Tensor,
+        cos_sin_cache: torch.Tensor,
+        is_neox: bool,
+        kv_cache: torch.Tensor,
+        layer_slot_mapping: torch.Tensor,
+    ) -> None:
+        """Rotate the step's query rows in place and store its keys, rotated, with its
+        values, in one launch.  ``key`` stays as it is (nothing here reads it again), and so
+        do query rows behind the slot map's; keys are quantized from the unrounded rotation."""
+        del layer
+        cache = _cache_tensor(kv_cache)
+        if layer_slot_mapping.ndim != 1:
+            raise RuntimeError("slot_mapping rank %d" % layer_slot_mapping.ndim)
+        ntok = int(layer_slot_mapping.shape[0])
+        if cache.numel() == 0 or ntok == 0:
+            return
+        if min(int(x.shape[0]) for x in (query, key, value, positions)) < ntok:
+            raise RuntimeError("query/key/value/positions shorter than slot_mapping")
+        lay = self.layout
+        regions = _regions(cache, lay)
+        q = _rows(query[:ntok], lay.hq, lay.head_dim, "query")
+        k = _rows(key[:ntok], lay.hkv, lay.head_dim, "key")
+        v = _rows(value[:ntok], lay.hkv, lay.head_dim, "value")
+        ops().rope_kv_store_paged(q, k, v, positions[:ntok], cos_sin_cache, is_neox, layer_slot_mapping, *regions, q)
+
     # -- attention -----------------------------------------------------------
     def forward(
         self,

@@ -651,7 +651,7 @@ class _Ops:
         _require(pages_per_block >= 1, "pages_per_block")
         _require(1 <= nodes <= 64, "1 to 64 nodes a tree")
         _require(q_fp16.dim() == 3, "q_fp16 [T,HQ,D]")
-        tokens, heads, head_dim = (int(x) for x in q_fp16.shape)
+        tokens, heads, head_dim = q_fp16.shape
         _require(head_dim in (128, 256), "q_fp16 [T,HQ,D] with D in (128, 256)")
         _require(heads % GQA == 0, "q_fp16 heads must be a multiple of GQA=6")
         hkv = _checked_hkv(heads // GQA)
@@ -677,16 +677,15 @@ class _Ops:
         _require(workspace.is_contiguous(), "workspace must be a contiguous buffer")
         tensors = (q_fp16, k_cache, k_scale, v_cache, v_scale, v_zero, block_table, seq_lens, tree_masks, out, workspace)
         dev = _on_gpu(*tensors)
-        row = heads * head_dim
-        args = [
-            _ptr(q_fp16), _DTYPE_CODE[q_fp16.dtype], int(q_fp16.stride(0)) if tokens > 1 else row,
+        row, width = heads * head_dim, block_table.shape[1]
+        args = (
+            q_fp16.data_ptr(), _DTYPE_CODE[q_fp16.dtype], q_fp16.stride(0) if tokens > 1 else row,
             *cache_args(k_cache, k_scale, v_cache, v_scale, v_zero),
-            _ptr(block_table), int(block_table.stride(0)) if batch > 1 else int(block_table.shape[1]),
-            int(block_table.shape[1]), pages_per_block, _ptr(seq_lens),
-            _ptr(tree_masks), int(tree_masks.stride(0)) if batch > 1 else nodes, batch, nodes, hkv, head_dim,
-            _ptr(out), _DTYPE_CODE[out.dtype], int(out.stride(0)) if tokens > 1 else row,
-            _ptr(workspace), int(workspace.numel()) * workspace.element_size(),
-        ]
+            block_table.data_ptr(), block_table.stride(0) if batch > 1 else width, width, pages_per_block,
+            seq_lens.data_ptr(), tree_masks.data_ptr(), tree_masks.stride(0) if batch > 1 else nodes, batch, nodes,
+            hkv, head_dim, out.data_ptr(), _DTYPE_CODE[out.dtype], out.stride(0) if tokens > 1 else row,
+            workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+        )
         return DeviceCall(self._lib, self._lib.k8v4_attn_tree, args, dev, tensors)
 
     # -- chunked prefill ----------------------------------------------------
@@ -877,45 +876,48 @@ class _Ops:
     def bind_kv_load_paged(self, k_cache, k_scale, v_cache, v_scale, v_zero, block_table, seq_starts, row_starts,
                            pages_per_block, k_out, v_out):
         """Validate a read once; returns a :class:`DeviceCall` (None when there are no rows)."""
-        outs = [x for x in (k_out, v_out) if x is not None]
-        _require(len(outs) > 0, "k_out or v_out")
+        out = v_out if k_out is None else k_out
+        _require(out is not None, "k_out or v_out")
         _require(k_cache.dim() == 4 and v_cache.dim() == 4, "k_cache [num_blocks,64,HKV,D] NHD")
-        hkv, head_dim = _checked_hkv(int(k_cache.shape[2])), int(k_cache.shape[3])
+        _pages, _tokens, hkv, head_dim = k_cache.shape
+        _checked_hkv(hkv)
         _require(head_dim in (128, 256), "k_cache head dim must be 128 or 256")
         check_paged_k(k_cache, k_scale, hkv, head_dim)
         check_paged_v(v_cache, v_scale, v_zero, hkv, head_dim)
         _require(k_cache.shape[0] == v_cache.shape[0], "k/v num_blocks")
         _require(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1,
                  "block_table must be int32 [B, W] with unit column stride")
-        batch = int(block_table.shape[0])
-        _require(row_starts.dtype == torch.int32 and row_starts.dim() == 1 and row_starts.shape[0] == batch + 1
-                 and row_starts.is_contiguous(), "row_starts must be a contiguous int32 [B + 1]")
+        batch, width = block_table.shape
+        _require(row_starts.dtype == torch.int32 and row_starts.shape == (batch + 1,) and row_starts.is_contiguous(),
+                 "row_starts must be a contiguous int32 [B + 1]")
         if seq_starts is not None:
-            _require(seq_starts.dtype == torch.int32 and seq_starts.dim() == 1 and seq_starts.shape[0] == batch
-                     and seq_starts.is_contiguous(), "seq_starts must be a contiguous int32 [B]")
+            _require(seq_starts.dtype == torch.int32 and seq_starts.shape == (batch,) and seq_starts.is_contiguous(),
+                     "seq_starts must be a contiguous int32 [B]")
         _require(int(pages_per_block) >= 1, "pages_per_block")
-        rows, dtype = int(outs[0].shape[0]) if outs[0].dim() else -1, outs[0].dtype
-        _require(dtype in (torch.float16, torch.bfloat16, torch.float32), "k/v_out float16, bfloat16 or float32")
-        for x in outs:
-            _require(x.dtype == dtype, "k/v_out dtypes differ")
-            _require(x.shape == (rows, hkv, head_dim), "k/v_out [N,%d,%d]" % (hkv, head_dim))
-            _require(x.stride(2) == 1 and x.stride(1) == head_dim, "k/v_out head/dim strides")
+        rows, dtype = out.shape[0] if out.dim() else -1, out.dtype
+        _require(dtype in _DTYPE_CODE, "k/v_out float16, bfloat16 or float32")
+        for x in (k_out, v_out):
+            if x is not None and not (
+                x.dtype == dtype and x.shape == (rows, hkv, head_dim) and x.stride()[1:] == (head_dim, 1)
+            ):
+                _require(x.dtype == dtype, "k/v_out dtypes differ")
+                _require(x.shape == (rows, hkv, head_dim), "k/v_out [N,%d,%d]" % (hkv, head_dim))
+                _require(False, "k/v_out head/dim strides")
         if rows == 0 or batch == 0:
             return None
-        _require(int(block_table.shape[1]) > 0, "block_table width")
-        tensors = (k_cache, k_scale, v_cache, v_scale, v_zero, block_table, row_starts, *outs)
-        if seq_starts is not None:
-            tensors += (seq_starts,)
+        _require(width > 0, "block_table width")
+        tensors = (k_cache, k_scale, v_cache, v_scale, v_zero, block_table, row_starts)
+        tensors += tuple(x for x in (k_out, v_out, seq_starts) if x is not None)
         dev = _on_gpu(*tensors)
         row = hkv * head_dim
-        args = [
+        args = (
             *cache_args(k_cache, k_scale, v_cache, v_scale, v_zero),
-            _ptr(block_table), int(block_table.stride(0)), int(block_table.shape[1]), int(pages_per_block),
-            0 if seq_starts is None else _ptr(seq_starts), _ptr(row_starts), batch, hkv, head_dim,
-            0 if k_out is None else _ptr(k_out), 0 if v_out is None else _ptr(v_out), _DTYPE_CODE[dtype],
-            row if k_out is None or rows == 1 else int(k_out.stride(0)),
-            row if v_out is None or rows == 1 else int(v_out.stride(0)), rows,
-        ]
+            block_table.data_ptr(), block_table.stride(0), width, int(pages_per_block),
+            0 if seq_starts is None else seq_starts.data_ptr(), row_starts.data_ptr(), batch, hkv, head_dim,
+            0 if k_out is None else k_out.data_ptr(), 0 if v_out is None else v_out.data_ptr(), _DTYPE_CODE[dtype],
+            row if k_out is None or rows == 1 else k_out.stride(0),
+            row if v_out is None or rows == 1 else v_out.stride(0), rows,
+        )
         return DeviceCall(self._lib, self._lib.k8v4_kv_load_paged, args, dev, tensors)
 
     # -- verification of drafted tokens ----------------------------------------
