@@ -285,7 +285,7 @@ int64_t k8v4_attn_noalloc_max_bytes(void);
 
 /*
  * Diagnostics, no counterpart in the reference: how many in-kernel waits of
- * the decode kernels (k8v4_attn_shared's too) on the current device gave up
+ * the decode kernels (k8v4_attn_shared's and k8v4_attn_tree's too) on the current device gave up
  * since the library was loaded (the paired-halves handshake of head dim 256 caps
  * each wait; a give-up means a wrong output).  Synchronizes with the device
  * (a copy from device memory); -1 on a HIP error.  Zero in a correct run.
@@ -450,7 +450,9 @@ int k8v4_rope_kv_store_paged(const void *q, const void *k, const void *v, int sr
  * tree and to every node i whose bit i is set in tree_masks[b][j] (int64
  * [batch], rows mask_stride apart, 0: one tree for all), itself only if its own
  * bit is; bits from `nodes` on, and nodes of a sequence shorter than its tree
- * that lie before its first token, are ignored.  A row that sees no key outputs zeros.
+ * that lie before its first token, are ignored.  A node that no row's mask of the
+ * sequence has (the padding of a smaller tree) need not have been stored, all
+ * others do.  A row that sees no key outputs zeros.
  * The chain's mask, 2^(j+1) - 1, gives what k8v4_attn_batch does.  Query
  * rows, cache, table, seq_lens (the tree's tokens counted), out and numerics as
  * in k8v4_attn_batch; page strides below 2^31 bytes.

@@ -402,9 +402,11 @@ __device__ __forceinline__ void pair_flag_wait(const lds_int *f, int target, int
 
 // What rows of a drafted tree see: the tokens ahead of `context`, and of the tree's
 // tokens behind them those whose bit is set in the row's word (row r's is words[r / 6]).
+// A token of the tree that none of the `count` words has may never have been stored:
+// its planes may hold anything and are not used.
 struct TreeRows {
   const __attribute__((address_space(3))) uint64_t *words;
-  int context;
+  int context, count;
 };
 
 // Softmax and P.V of one chunk whose scores chunk_qk produced; reads the V
@@ -433,9 +435,18 @@ __device__ __forceinline__ void chunk_softmax_pv(WaveState<D, NT> &st, const v4i
   float vsv[8] = {vsa[0], vsa[1], vsa[2], vsa[3], vsb[0], vsb[1], vsb[2], vsb[3]};
   float vzv[8] = {vza[0], vza[1], vza[2], vza[3], vzb[0], vzb[1], vzb[2], vzb[3]};
   if (__builtin_expect(masked, 0)) {
+    [[maybe_unused]] uint64_t any = 0;  // nodes that some row sees
+    if constexpr (TREE) {
+      for (int i = 0; i < tree.count; ++i) any |= tree.words[i];
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (tbase + chunk_token(g, i) >= L0) {  // unwritten tail: never use its planes
+      bool unused = tbase + chunk_token(g, i) >= L0;  // unwritten tail: never use its planes
+      if constexpr (TREE) {
+        const int node = tbase + chunk_token(g, i) - tree.context;
+        unused |= node >= 0 && !((any >> (node & 63)) & 1);
+      }
+      if (unused) {
         ksv[i] = 0.f;
         vsv[i] = 0.f;
         vzv[i] = 0.f;

@@ -146,6 +146,17 @@ __device__ __forceinline__ float lane_value(float x, int src) {
   return __int_as_float(__builtin_amdgcn_ds_bpermute(4 * src, __float_as_int(x)));
 }
 
+// OR over the wave, the same value in every lane (all 64 active).
+__device__ __forceinline__ uint32_t wave_or(uint32_t x) {
+  x |= __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr:1, 2, 4, 8
+  x |= __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+  x |= __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+  x |= __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+  x |= __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast:15, 31
+  x |= __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
+  return __builtin_amdgcn_readlane(x, kWave - 1);
+}
+
 // The arguments again, through a pointer the compiler knows nothing of: read
 // where they are used, instead of being held in scalar registers (more than
 // there are) across the pieces of a work-group.
@@ -275,6 +286,7 @@ __device__ __forceinline__ void attend_piece(const PieceArgs &a, char *lds_raw, 
     if (tid < kGroup) words[tid] = tid < ntok ? static_cast<uint64_t>(a.tree_masks[b * a.mask_stride + sub * kGroup + tid]) : 0;
     tree.words = words;
     tree.context = L0 - a.q_len;
+    tree.count = kGroup;
   }
 
   const int my0 = x0 + w;
@@ -661,7 +673,7 @@ __device__ __forceinline__ void quantize_tile(const V (&raw)[2 * KS], bool bf16,
 // Pages p0 .. p1 - 1 of the prefix for one row block of one KV head, or (TREE) of a
 // sequence for a row block of its drafted tree, whose words lie in the LDS behind
 // everything else (kWideWordBytes).
-constexpr int kWideWordBytes = 64 * 8;
+constexpr int kWideWordBytes = (64 + 1) * 8;
 template <int D, int HKV, int TILES = Wide<D>::NT, bool TREE = false, int RING = Wide<D>::SLOTS>
 __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, int tid, int wg, int seg, int p0, int p1) {
   using W = Wide<D, TILES, RING>;
@@ -683,9 +695,14 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
   TreeRows tree{};
   if constexpr (TREE) {
     auto *words = reinterpret_cast<__attribute__((address_space(3))) uint64_t *>(lds + W::LDS_BYTES);
-    if (tid < a.q_len) words[tid] = static_cast<uint64_t>(a.tree_masks[b * a.mask_stride + tid]);
+    uint64_t word = 0;
+    if (tid < a.q_len) words[tid] = word = static_cast<uint64_t>(a.tree_masks[b * a.mask_stride + tid]);
     tree.words = words;
     tree.context = len - a.q_len;
+    if (wave == 0) {
+      const uint32_t hi = wave_or(static_cast<uint32_t>(word >> 32)), lo = wave_or(static_cast<uint32_t>(word));
+      if (lane == 0) words[kWave] = static_cast<uint64_t>(hi) << 32 | lo;  // nodes that some row sees
+    }
   }
   const bool active = row0 < nrows;
   const int pages = p1 - p0;
@@ -847,9 +864,13 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
   auto scale_planes = [&](int i) __attribute__((always_inline)) {
     if (wave != 0) return;
     if constexpr (TREE) {
-      // Tokens behind the last hold anything; their probabilities are zero, and so
-      // their V has to be.
-      if ((p0 + i) * kPage + lane >= len) plane_s = plane_z = 0.f;
+      // Tokens behind the last, and nodes that no row sees, may hold anything; their
+      // probabilities are zero, and so their V has to be.
+      const int tok = (p0 + i) * kPage + lane, node = tok - tree.context;
+      if ((p0 + i + 1) * kPage > tree.context) {
+        const uint64_t any = tree.words[kWave];
+        if (tok >= len || (node >= 0 && !((any >> (node & 63)) & 1))) plane_s = plane_z = 0.f;
+      }
     }
     lds_t *planes = lds + (i % W::SLOTS) * W::SLOT_BYTES + W::S_OFF + 4 * lane;
     *reinterpret_cast<__attribute__((address_space(3))) float *>(planes) = plane_s * 0x1p20f;

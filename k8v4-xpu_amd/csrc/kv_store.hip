@@ -583,6 +583,7 @@ extern "C" int k8v4_rope_kv_store_paged(const void *q, const void *k, const void
   K8V4_REQUIRE(k && v && positions && cos_sin && slot_mapping && k_cache && k_scale && v_cache && v_scale && v_zero,
                "null pointer");
   K8V4_REQUIRE(!q == !q_out, "q and q_out go together");
+  K8V4_REQUIRE(!q || q != q_out || q_tok_stride == q_out_stride, "q_out may be q itself, not another view of its rows");
   const int64_t row = static_cast<int64_t>(hkv) * head_dim;
   K8V4_REQUIRE(k_tok_stride >= row && v_tok_stride >= row, "k/v token stride shorter than hkv*head_dim");
   K8V4_REQUIRE(!q || (q_tok_stride >= kGqa * row && q_out_stride >= kGqa * row), "q token stride shorter than HQ*D");

@@ -155,6 +155,18 @@ def test_masked_rows(gpu_ops, vocab, dtype):
         Rows(x, tokens, 20).run(gpu_ops).check()
 
 
+@pytest.mark.parametrize("dtype,bits", [(torch.bfloat16, 0x7F81), (torch.float16, 0x7C01), (torch.float32, 0x7F800001)])
+@pytest.mark.parametrize("vocab", [90, 20000])
+def test_signalling_nan(gpu_ops, dtype, bits, vocab):
+    """Beside the row's largest values, in the first batch of elements and in later ones."""
+    x = logits_of(4, vocab, dtype, 8)
+    whole = x.view(torch.int32 if dtype == torch.float32 else torch.int16)
+    for row, at in ((0, [0, 1, 2]), (1, [vocab - 1, vocab - 2, 5]), (2, list(range(1, 80, 2)))):
+        whole[row, torch.tensor(at, device=DEV)] = bits
+    x[0, 3], x[1, vocab - 3], x[2, 0] = 25.0, 25.0, 25.0
+    Rows(x, [3, vocab - 1, 0, 5], 9).run(gpu_ops).check()
+
+
 @pytest.mark.parametrize("vocab", [300, 9000, 152000])
 def test_sorted_and_equal_rows(gpu_ops, vocab):
     """Rows in ascending and descending order (the likeliest last or first), few distinct values."""

@@ -115,8 +115,8 @@ class Trees:
                 a[rows, heads] = torch.mm(p, v[:, h].abs().contiguous()).view(n, GQA, self.d)
         return o, a, r
 
-    def check(self, out):
-        o, a, r = self.want()
+    def check(self, out, want=None):
+        o, a, r = want or self.want()
         got = out.double()
         assert bool(torch.isfinite(got).all())
         eps = torch.finfo(out.dtype).eps / 2
@@ -212,6 +212,25 @@ def test_a_padding_sequence_may_hold_anything(gpu_ops):
     assert not out[20:40].any()
     st.q[20:40] = 0
     st.check(out)
+
+
+@pytest.mark.parametrize("hkv,d", SHAPES)
+@pytest.mark.parametrize("nodes", [6, 20, 50, 64])
+def test_nodes_that_nobody_sees_need_not_be_stored(gpu_ops, hkv, d, nodes):
+    """Trees of fewer nodes than the call's: the cache may hold NaN at the others."""
+    rng = random.Random(nodes)
+    real = [nodes // 2, 1, nodes - 1, nodes]
+    masks = [tree_masks(random_parents(rng, n)) + [0] * (nodes - n) for n in real]
+    for words in masks:
+        words[-1] = words[0] if words[-1] == 0 else words[-1]  # an absent node's row may see stored ones
+    st = Trees(gpu_ops, hkv, d, nodes, [500, 64 - real[1], 0, 3000], seed=nodes + 5, masks=masks)
+    want = st.want()
+    for b, n in enumerate(real):
+        t = torch.arange(st.lens[b] - nodes + n, st.lens[b])
+        page, row = st.table[b][t // PAGE].long().to(DEV), (t % PAGE).to(DEV)
+        for name in ("k_scale", "v_scale", "v_zero"):
+            st.cache.views[name][page, row] = math.nan
+    st.check(st.run(), want)
 
 
 def test_large_values(gpu_ops):
