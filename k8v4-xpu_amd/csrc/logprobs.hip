@@ -33,7 +33,7 @@ constexpr int kWaves = kThreads / kWave;
 constexpr int kMaxTop = 64;
 constexpr int kMaxSlices = 64;  // one lane each when they are joined
 constexpr int kGroupLanes = 8;  // lanes whose vectors make a chunk
-constexpr int kBatch = 4;       // vectors of a thread in flight
+constexpr int kStream = 4;      // vectors of a thread in flight
 constexpr int kMaxListed = 256;
 constexpr int kSliceUnit = 2048;        // elements of a slice at least, and its length's unit
 constexpr int kMaxSliceLen = 1 << 18;   // its chunks' maxima fit the LDS
@@ -362,12 +362,15 @@ __device__ __forceinline__ void write_top(const LogprobArgs &a, int64_t row, con
   a.top_logprobs[row * a.lps_stride + t] = t < found ? logprob_of(r, sh.final[t].x) : -INFINITY;
 }
 
-// A slice of a row.  Every thread takes kBatch 16-byte vectors of kBatch runs at a
-// time, the next ones under way; ONE: the slice is one such batch, whose elements
-// then stay in registers until the likeliest tokens are found.
-template <typename T, bool ONE>
+// A slice of a row.  Every thread takes kStream 16-byte vectors of as many runs at a
+// time, the next ones under way; HELD: the slice is one batch of HELD elements a
+// thread, which stay in registers until the likeliest tokens are found.  (Such a call
+// runs its code once, and most of its time is the code's way from memory: as few
+// elements a thread as the slice needs.)
+template <typename T, int HELD>
 __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
-  constexpr int N = Vec<T>::N;
+  constexpr int N = Vec<T>::N, kBatch = HELD ? HELD / N : kStream;
+  constexpr bool ONE = HELD != 0;
   constexpr int CHUNK = kGroupLanes * N;  // elements, 128 bytes
   constexpr int STEP = kThreads * N;      // elements of one vector of every thread
   __shared__ Shared sh;
@@ -595,15 +598,19 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(LogprobArgs a) {
   write_top(a, row, r, found, sh);
 }
 
-// How many slices a row is cut into: enough for two work-groups a compute unit, or
-// for four where that leaves a slice kLongSlice tokens.  Measured, two a unit / four, us:
-// 48 x 65537 fp16 17.7 / 24.5, 64 x 152000 bf16 30.6 / 31.2, 128 x 152000 fp32 35.2 /
-// 31.3, 256 x 152000 bf16 52.3 / 46.6 (one: 58.0; eight: 59.6), 512 x 32000 27.9 / 32.2.
-constexpr int64_t kLongSlice = 16384;
+// How many slices a row is cut into.  One that a work-group holds, or nearly, is not
+// cut (256 x 8000 bf16 10.0 us in one launch, 14.1 in slices and a second one).  Others
+// are for two work-groups a compute unit, or for four where that leaves slices that
+// are held in few registers, or long ones.  Measured, two a unit / four, us: 48 x 65537
+// fp16 17.7 / 16.1, 128 x 32000 fp32 23.1 / 19.0, 256 x 32000 bf16 26.7 / 29.6, 512 x
+// 32000 bf16 27.9 / 32.1, 128 x 152000 fp32 35.2 / 31.3, 256 x 152000 bf16 52.3 / 46.6
+// (one: 58.0; eight: 59.6).
+constexpr int64_t kHeldWhole = 8192, kShortSlice = 4096, kLongSlice = 16384;
 int slices_of(int64_t rows, int64_t vocab) {
+  if (vocab <= kHeldWhole) return 1;
   const int64_t units = device_cus();
-  const int64_t four = (4 * units + rows - 1) / rows;
-  const int64_t wanted = vocab >= four * kLongSlice ? four : (2 * units + rows - 1) / rows;
+  const int64_t four = (4 * units + rows - 1) / rows, two = (2 * units + rows - 1) / rows;
+  const int64_t wanted = vocab <= four * kShortSlice || vocab >= four * kLongSlice ? four : two;
   const int64_t most = (vocab + kSliceUnit - 1) / kSliceUnit;
   const int64_t least = (vocab + kMaxSliceLen - 1) / kMaxSliceLen;
   int64_t n = wanted < most ? wanted : most;
@@ -613,14 +620,18 @@ int slices_of(int64_t rows, int64_t vocab) {
 
 template <typename T>
 int launch(LogprobArgs a, int64_t rows, hipStream_t s) {
-  constexpr int CHUNK = kGroupLanes * Vec<T>::N, ROUND = kBatch * kThreads * Vec<T>::N;
-  const dim3 grid(static_cast<unsigned>(rows * a.slices));
-  if (a.slice_len <= ROUND) {
-    logprob_kernel<T, true><<<grid, dim3(kThreads), 0, s>>>(a);
+  constexpr int CHUNK = kGroupLanes * Vec<T>::N, ROUND = kStream * kThreads * Vec<T>::N;
+  const dim3 grid(static_cast<unsigned>(rows * a.slices)), block(kThreads);
+  if (a.slice_len <= 8 * kThreads) {
+    logprob_kernel<T, 8><<<grid, block, 0, s>>>(a);
+  } else if (a.slice_len <= 16 * kThreads) {
+    logprob_kernel<T, 16><<<grid, block, 0, s>>>(a);
+  } else if (a.slice_len <= 32 * kThreads && sizeof(T) == 2) {
+    logprob_kernel<T, sizeof(T) == 2 ? 32 : 16><<<grid, block, 0, s>>>(a);
   } else {
     const int64_t chunks = static_cast<int64_t>((a.slice_len + ROUND - 1) / ROUND) * ROUND / CHUNK;
     const int64_t floats = !a.top ? 0 : chunks > a.top * CHUNK ? chunks : a.top * CHUNK;
-    logprob_kernel<T, false><<<grid, dim3(kThreads), floats * 4, s>>>(a);
+    logprob_kernel<T, 0><<<grid, block, floats * 4, s>>>(a);
   }
   int rc = launch_status("k8v4_token_logprobs");
   if (rc || a.slices == 1) return rc;
