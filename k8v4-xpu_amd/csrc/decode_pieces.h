@@ -1217,7 +1217,7 @@ __global__ __launch_bounds__(TPU) void pieces_merge_kernel(PieceArgs a) {
     pr = r - block * Wide<D>::ROWS;
   }
   const int os = b * a.per_seq + sub;
-  if (a.groups) {
+  if (!TREE && a.groups) {
     const int first = ps * prefix_cost(a) + kPieceCost;
     pf = first / ax.unit;
     pn = (first + a.prefix_pages - 1) / ax.unit - pf + 1;
@@ -1247,7 +1247,7 @@ __global__ __launch_bounds__(TPU) void pieces_merge_kernel(PieceArgs a) {
 #pragma unroll
     for (int u = 0; u < kMergeMU; ++u) {
       const int s = min(s0 + u * SPI, count - 1);
-      const bool pre = s < pn;
+      const bool pre = !TREE && s < pn;
       const char *state = pre ? pbase + s * a.prefix_bytes : obase + (s - pn) * a.own_bytes;
       ml[u] = *reinterpret_cast<const float2 *>(state + (pre ? p_ml : o_ml));
       raw[u] = *reinterpret_cast<const v8h *>(state + (pre ? p_o : o_o));
