@@ -583,10 +583,10 @@ extern "C" int k8v4_rope_kv_store_paged(const void *q, const void *k, const void
   K8V4_REQUIRE(k && v && positions && cos_sin && slot_mapping && k_cache && k_scale && v_cache && v_scale && v_zero,
                "null pointer");
   K8V4_REQUIRE(!q == !q_out, "q and q_out go together");
-  K8V4_REQUIRE(!q || q != q_out || q_tok_stride == q_out_stride, "q_out may be q itself, not another view of its rows");
   const int64_t row = static_cast<int64_t>(hkv) * head_dim;
   K8V4_REQUIRE(k_tok_stride >= row && v_tok_stride >= row, "k/v token stride shorter than hkv*head_dim");
   K8V4_REQUIRE(!q || (q_tok_stride >= kGqa * row && q_out_stride >= kGqa * row), "q token stride shorter than HQ*D");
+  K8V4_REQUIRE(!q || q != q_out || q_tok_stride == q_out_stride, "q_out may be q itself, not another view of its rows");
   K8V4_REQUIRE(aligned(q, 2) && aligned(q_out, 2) && aligned(k, 2) && aligned(v, 2), "q/k/v pointers misaligned");
   K8V4_REQUIRE(aligned(cos_sin, table_dtype == K8V4_F32 ? 4 : 2) && aligned(positions, positions_are_int64 ? 8 : 4),
                "cos_sin or positions misaligned");

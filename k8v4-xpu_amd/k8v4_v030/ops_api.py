@@ -169,9 +169,10 @@ def _check(rc: int, lib) -> None:
         raise RuntimeError(lib.k8v4_last_error().decode("utf-8", "replace"))
 
 
-def _require(cond: bool, message: str) -> None:
+def _require(cond: bool, message: str, *parts) -> None:
+    """Raise with ``message`` (``parts`` put into it only then) unless ``cond``."""
     if not cond:
-        raise RuntimeError(message)
+        raise RuntimeError(message % parts if parts else message)
 
 
 def _checked_hkv(hkv: int) -> int:
@@ -279,6 +280,36 @@ def cache_args(k_cache, k_scale, v_cache, v_scale, v_zero) -> list[int]:
         v_scale.stride(0) * 4,
         v_zero.stride(0) * 4,
     ]
+
+
+def _checked_cache(k_cache, k_scale, v_cache, v_scale, v_zero):
+    """``(hkv, head_dim, cache_args)`` of five region views, each tensor's shape and
+    strides fetched once (the checks and messages of :func:`check_paged_k` and
+    :func:`check_paged_v`, to which anything unusual goes)."""
+    shape, ks = k_cache.shape, k_cache.stride()
+    if len(shape) == 4:
+        pages, rows, hkv, dim = shape
+        plane, cols = (pages, rows, hkv), dim // 2
+        s1, vs, s2, s3 = k_scale.stride(), v_cache.stride(), v_scale.stride(), v_zero.stride()
+        if (
+            rows == PAGE and hkv in (2, 4) and dim in (128, 256)
+            and k_cache.dtype == torch.int8 and v_cache.dtype == torch.uint8
+            and k_scale.dtype == v_scale.dtype == v_zero.dtype == torch.float32
+            and k_scale.shape == v_scale.shape == v_zero.shape == plane and v_cache.shape == (pages, rows, hkv, cols)
+            and ks[1:] == (hkv * dim, dim, 1) and vs[1:] == (hkv * cols, cols, 1)
+            and s1[1:] == s2[1:] == s3[1:] == (hkv, 1)
+        ):
+            return hkv, dim, (
+                k_cache.data_ptr(), k_scale.data_ptr(), v_cache.data_ptr(), v_scale.data_ptr(), v_zero.data_ptr(),
+                pages, ks[0], s1[0] * 4, vs[0], s2[0] * 4, s3[0] * 4,
+            )
+    _require(k_cache.dim() == 4 and v_cache.dim() == 4, "k_cache [num_blocks,64,HKV,D] NHD")
+    hkv, dim = _checked_hkv(int(k_cache.shape[2])), int(k_cache.shape[3])
+    _require(dim in (128, 256), "k_cache head dim must be 128 or 256")
+    check_paged_k(k_cache, k_scale, hkv, dim)
+    check_paged_v(v_cache, v_scale, v_zero, hkv, dim)
+    _require(k_cache.shape[0] == v_cache.shape[0], "k/v num_blocks")
+    return hkv, dim, tuple(cache_args(k_cache, k_scale, v_cache, v_scale, v_zero))
 
 
 def _src_rows(t: torch.Tensor, name: str, hkv: int, head_dim: int) -> int:
@@ -404,9 +435,8 @@ class _Ops:
         _require(k_fp16.dtype == v_fp16.dtype, "k/v_fp16 dtypes differ")
         _require(v_fp16.shape == k_fp16.shape, "v_fp16 must match k_fp16")
         _require(slot_mapping.dtype == torch.int64 and slot_mapping.is_contiguous(), "slot_mapping int64")
-        check_paged_k(k_cache, k_scale, hkv, head_dim)
-        check_paged_v(v_cache, v_scale, v_zero, hkv, head_dim)
-        _require(k_cache.shape[0] == v_cache.shape[0], "k/v num_blocks")
+        chkv, cdim, cache = _checked_cache(k_cache, k_scale, v_cache, v_scale, v_zero)
+        _require(chkv == hkv and cdim == head_dim, "k_cache [num_blocks,64,%d,%d] NHD", hkv, head_dim)
         _require(slot_mapping.shape == (ntok,), "slot_mapping [T]")
         _require(positions.dtype in (torch.int32, torch.int64) and positions.shape == (ntok,)
                  and positions.is_contiguous(), "positions must be a contiguous int32 or int64 [T]")
@@ -438,9 +468,7 @@ class _Ops:
             q_ptr, k_fp16.data_ptr(), v_fp16.data_ptr(), _DTYPE_CODE[k_fp16.dtype], qs, ks, vs,
             positions.data_ptr(), int(positions.dtype == torch.int64), cos_sin.data_ptr(), _DTYPE_CODE[cos_sin.dtype],
             table_rows, cos_sin.stride(0) if table_rows > 1 else rot, rot, int(bool(neox)),
-            slot_mapping.data_ptr(), ntok, hkv, head_dim,
-            *cache_args(k_cache, k_scale, v_cache, v_scale, v_zero),
-            out_ptr, qos,
+            slot_mapping.data_ptr(), ntok, hkv, head_dim, *cache, out_ptr, qos,
         )
         return DeviceCall(self._lib, self._lib.k8v4_rope_kv_store_paged, args, dev, tensors)
 
@@ -663,9 +691,8 @@ class _Ops:
         _require(tokens % nodes == 0, "T must be B*nodes")
         batch = tokens // nodes
         _require(batch >= 1, "empty batch")
-        check_paged_k(k_cache, k_scale, hkv, head_dim)
-        check_paged_v(v_cache, v_scale, v_zero, hkv, head_dim)
-        _require(k_cache.shape[0] == v_cache.shape[0], "k/v num_blocks")
+        chkv, cdim, cache = _checked_cache(k_cache, k_scale, v_cache, v_scale, v_zero)
+        _require(chkv == hkv and cdim == head_dim, "k_cache [num_blocks,64,%d,%d] NHD", hkv, head_dim)
         _require(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == batch,
                  "block_table int32 [B, splits]")
         _require(int(block_table.shape[1]) > 0, "block_table n_splits")
@@ -680,8 +707,7 @@ class _Ops:
         row, width = heads * head_dim, block_table.shape[1]
         args = (
             q_fp16.data_ptr(), _DTYPE_CODE[q_fp16.dtype], q_fp16.stride(0) if tokens > 1 else row,
-            *cache_args(k_cache, k_scale, v_cache, v_scale, v_zero),
-            block_table.data_ptr(), block_table.stride(0) if batch > 1 else width, width, pages_per_block,
+            *cache, block_table.data_ptr(), block_table.stride(0) if batch > 1 else width, width, pages_per_block,
             seq_lens.data_ptr(), tree_masks.data_ptr(), tree_masks.stride(0) if batch > 1 else nodes, batch, nodes,
             hkv, head_dim, out.data_ptr(), _DTYPE_CODE[out.dtype], out.stride(0) if tokens > 1 else row,
             workspace.data_ptr(), workspace.numel() * workspace.element_size(),
@@ -878,13 +904,7 @@ class _Ops:
         """Validate a read once; returns a :class:`DeviceCall` (None when there are no rows)."""
         out = v_out if k_out is None else k_out
         _require(out is not None, "k_out or v_out")
-        _require(k_cache.dim() == 4 and v_cache.dim() == 4, "k_cache [num_blocks,64,HKV,D] NHD")
-        _pages, _tokens, hkv, head_dim = k_cache.shape
-        _checked_hkv(hkv)
-        _require(head_dim in (128, 256), "k_cache head dim must be 128 or 256")
-        check_paged_k(k_cache, k_scale, hkv, head_dim)
-        check_paged_v(v_cache, v_scale, v_zero, hkv, head_dim)
-        _require(k_cache.shape[0] == v_cache.shape[0], "k/v num_blocks")
+        hkv, head_dim, cache = _checked_cache(k_cache, k_scale, v_cache, v_scale, v_zero)
         _require(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1,
                  "block_table must be int32 [B, W] with unit column stride")
         batch, width = block_table.shape
@@ -911,8 +931,7 @@ class _Ops:
         dev = _on_gpu(*tensors)
         row = hkv * head_dim
         args = (
-            *cache_args(k_cache, k_scale, v_cache, v_scale, v_zero),
-            block_table.data_ptr(), block_table.stride(0), width, int(pages_per_block),
+            *cache, block_table.data_ptr(), block_table.stride(0), width, int(pages_per_block),
             0 if seq_starts is None else seq_starts.data_ptr(), row_starts.data_ptr(), batch, hkv, head_dim,
             0 if k_out is None else k_out.data_ptr(), 0 if v_out is None else v_out.data_ptr(), _DTYPE_CODE[dtype],
             row if k_out is None or rows == 1 else k_out.stride(0),
@@ -1100,13 +1119,7 @@ class _Ops:
     def bind_kv_keep_paged(self, k_cache, k_scale, v_cache, v_scale, v_zero, block_table, seq_starts, path, accepted,
                            pages_per_block):
         """Validate one move; returns a :class:`DeviceCall` (None where there is nothing to move)."""
-        _require(k_cache.dim() == 4, "k_cache [num_blocks,64,HKV,D] NHD")
-        _pages, _tokens, hkv, head_dim = k_cache.shape
-        _checked_hkv(hkv)
-        _require(head_dim in (128, 256), "k_cache head dim must be 128 or 256")
-        check_paged_k(k_cache, k_scale, hkv, head_dim)
-        check_paged_v(v_cache, v_scale, v_zero, hkv, head_dim)
-        _require(k_cache.shape[0] == v_cache.shape[0], "k/v num_blocks")
+        hkv, head_dim, cache = _checked_cache(k_cache, k_scale, v_cache, v_scale, v_zero)
         table = block_table.shape
         if not (
             len(table) == 2 and path.dim() == 2 and path.shape[0] == table[0]
@@ -1129,8 +1142,7 @@ class _Ops:
         tensors = (k_cache, k_scale, v_cache, v_scale, v_zero, block_table, seq_starts, path, accepted)
         dev = _on_gpu(*tensors)
         args = (
-            *cache_args(k_cache, k_scale, v_cache, v_scale, v_zero),
-            block_table.data_ptr(), block_table.stride(0) if batch > 1 else table[1], table[1], int(pages_per_block),
+            *cache, block_table.data_ptr(), block_table.stride(0) if batch > 1 else table[1], table[1], int(pages_per_block),
             seq_starts.data_ptr(), path.data_ptr(), path.stride(0) if batch > 1 else width, width,
             accepted.data_ptr(), batch, hkv, head_dim,
         )

@@ -42,7 +42,7 @@ def rope(lib, **over):
     (dict(pos=None), "null"), (dict(table=None), "null"), (dict(slots=None), "null"), (dict(vz=None), "null"),
     (dict(q=None), "go together"), (dict(q_out=None), "go together"), (dict(k_stride=511), "k/v token stride"),
     (dict(v_stride=0), "k/v token stride"), (dict(q_stride=3000), "q token stride"), (dict(q_out_stride=1), "q token stride"),
-    (dict(q=P + 1), "misaligned"), (dict(v_rows=P + 1), "misaligned"), (dict(table=P + 2), "misaligned"),
+    (dict(q_out_stride=5000), "not another view"), (dict(q=P + 1), "misaligned"), (dict(v_rows=P + 1), "misaligned"), (dict(table=P + 2), "misaligned"),
     (dict(pos=P + 4), "misaligned"), (dict(pos=P + 2, pos64=0), "misaligned"), (dict(slots=P + 4), "misaligned"),
     (dict(k=P + 8), "misaligned"), (dict(v=P + 4), "misaligned"), (dict(k_ps=52232), "page strides"),
     (dict(v_ps=52228), "page strides"), (dict(ntok=2**40), "too many tokens"),
