@@ -689,7 +689,13 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
 
   const int sub = TREE ? tree_place(a).share : seg, b = TREE ? seg : 0;
   const int h = sub / a.wide_blocks, block = sub - h * a.wide_blocks;
-  const int row0 = block * W::ROWS + wave * 16 * NT;  // first row of this wave, of the head's tokens * 6
+  // First row of this wave, of the head's tokens * 6, and how far its tiles are apart.
+  // TREE: dealt in turn, so that the waves of a partly filled block differ by one tile
+  // and each SIMD's two share it (a wave's consecutive, D 256, 26 nodes over twelve
+  // times 8,000 tokens 60.9 -> 57.6 us, 30 nodes 65.9 -> 61.1; D 128, 50 nodes over four
+  // times 40,000 109 -> 103; full blocks the same).
+  constexpr int TILE_STEP = TREE ? 16 * kWideWaves : 16;
+  const int row0 = block * W::ROWS + wave * (TREE ? 16 : 16 * NT);
   const int nrows = (TREE ? a.q_len : a.tokens) * kGqa;
   const int len = TREE ? ((const const_i32_ptr)(a.seq_lens))[b] : 0;
   TreeRows tree{};
@@ -719,7 +725,7 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
   const int own0 = TREE ? b * nrows : 0;  // the sequence's first row of the head's rows in the buffer
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int r = row0 + 16 * nt + n;
+    const int r = row0 + TILE_STEP * nt + n;
     const int64_t at = h * a.head_rows + (TREE ? own0 + r : r);  // the buffer is padded to whole blocks
     const int rl = min(r, nrows - 1), tok = rl / kGqa, sb = tok / a.q_len;
     if constexpr (FUSED) {
@@ -750,7 +756,7 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
   }
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const bool live = row0 + 16 * nt + n < nrows;
+    const bool live = row0 + TILE_STEP * nt + n < nrows;
     if (!TREE && live && lim[nt] > 0) far = max(far, kFar - min(lim[nt], kFar));
     if (!TREE && !live) lim[nt] = a.prefix_pages * kPage;
     const double f = live ? static_cast<double>(crow[nt]) : 0.0;
@@ -943,7 +949,8 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
       kscale[ml] = *reinterpret_cast<__attribute__((address_space(3))) const v4f *>(
           lds + W::KS_OFF + ((i & 3) * kPage + 16 * ml + 4 * g) * 4);
   };
-  auto phase_a = [&](int i, auto with_v) __attribute__((always_inline)) {
+  auto phase_a = [&](int i, auto with_v, auto tiles) __attribute__((always_inline)) {
+    constexpr int NU = decltype(tiles)::value;
     __builtin_amdgcn_s_setprio(1);  // the products first, phase B in their gaps
     constexpr int FIRST = decltype(with_v)::value ? 0 : NV, LAST = NV + NK;
     const lds_t *vsrc = lds + W::V16_OFF + (i & 1) * W::V16_BYTES;
@@ -975,11 +982,11 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
         const v4i f = ring[x % AHEAD];
         ring[x % AHEAD] = operand(x + AHEAD);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NU; ++nt)
           O[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, f), P[nt][s], O[nt][j], 0, 0, 0);
         if (j == DT - 1) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) lsum[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, P[nt][s], lsum[nt], 0, 0, 0);
+          for (int nt = 0; nt < NU; ++nt) lsum[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, P[nt][s], lsum[nt], 0, 0, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -996,16 +1003,17 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
       const v4i f = ring[k % AHEAD];
       if (x + AHEAD < LAST) ring[k % AHEAD] = operand(x + AHEAD);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NU; ++nt)
         S[nt][ml] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, qf[nt][ks], ks ? S[nt][ml] : bias, 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_s_setprio(0);
   };
   // P = exp2(score - m - 2) of page i, see chunk_softmax_pv in decode_chunk.h.
-  auto softmax = [&](int i, bool there) __attribute__((always_inline)) {
+  auto softmax = [&](int i, bool there, auto tiles) __attribute__((always_inline)) {
+    constexpr int NU = decltype(tiles)::value;
     if constexpr (D == 256) read_kscale(i);
-    float t[NT][4][4], mx[NT];
+    float t[NU][4][4], mx[NU];
     const int tbase = (p0 + i) * kPage;
     const bool masked = !there || tbase + kPage > min_end;
     const int seen_to = there ? INT32_MAX : 0;
@@ -1016,14 +1024,14 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
       for (int e = 0; e < 4; ++e) {
         const float kb = -12582912.0f * ks[e];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) t[nt][ml][e] = fmaf(__int_as_float(S[nt][ml][e]), ks[e], kb);
+        for (int nt = 0; nt < NU; ++nt) t[nt][ml][e] = fmaf(__int_as_float(S[nt][ml][e]), ks[e], kb);
       }
     }
     if (__builtin_expect(masked, 0)) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int nt = 0; nt < NU; ++nt) {
         [[maybe_unused]] uint64_t word = 0;
-        if constexpr (TREE) word = tree.words[min((row0 + 16 * nt + n) / kGqa, a.q_len - 1)];
+        if constexpr (TREE) word = tree.words[min((row0 + TILE_STEP * nt + n) / kGqa, a.q_len - 1)];
 #pragma unroll
         for (int ml = 0; ml < 4; ++ml)
 #pragma unroll
@@ -1040,7 +1048,7 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
     }
     bool grow = false;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int nt = 0; nt < NU; ++nt) {
       float x = -INFINITY;
 #pragma unroll
       for (int ml = 0; ml < 4; ++ml)
@@ -1051,7 +1059,7 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
     }
     if (__ballot(grow)) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int nt = 0; nt < NU; ++nt) {
         const float mnew = fmaxf(m_run[nt], xlane_max16_32(mx[nt]) * crow[nt]);
         const float alpha = m_run[nt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[nt] - mnew);
         m_run[nt] = mnew;
@@ -1062,7 +1070,7 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
       }
     }
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int nt = 0; nt < NU; ++nt) {
       const float nm = -fmaxf(m_run[nt], -FLT_MAX) - kPLog2Offset;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
@@ -1105,11 +1113,11 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
     convert(0, std::false_type{});
     end_phase(false);
   }
-  auto run = [&](auto compute) {
-    constexpr bool C = decltype(compute)::value;
+  auto run = [&](auto tiles) {
+    constexpr bool C = decltype(tiles)::value != 0;
     auto phase = [&](int i, auto with_v) {
       if constexpr (C) {
-        phase_a(i, with_v);
+        phase_a(i, with_v, tiles);
       } else {
         issue(i + W::SLOTS);
         convert(i + 1, std::true_type{});
@@ -1120,10 +1128,10 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
     for (int i = 0; i < pages; ++i) {
       read_planes(i + 1);  // group 0's wave 0 scales them; the others read nothing of use
       if constexpr (C) {
-        softmax(i, (valid >> (i % W::SLOTS)) & 1u);
+        softmax(i, (valid >> (i % W::SLOTS)) & 1u, tiles);
         // Used here: its last steps would otherwise be moved over the barrier.
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) asm volatile("" : "+v"(P[nt][0]), "+v"(P[nt][1]));
+        for (int nt = 0; nt < decltype(tiles)::value; ++nt) asm volatile("" : "+v"(P[nt][0]), "+v"(P[nt][1]));
         __builtin_amdgcn_sched_barrier(0);
       }
       scale_planes(i + 1);
@@ -1134,10 +1142,13 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
     }
   };
   // Waves whose rows lie behind the batch's only move and dequantize pages.
-  if (active)
-    run(std::true_type{});
+  constexpr bool FEWER = TREE && NT > 1;
+  if (active && (!FEWER || row0 + TILE_STEP * (NT - 1) < nrows))
+    run(std::integral_constant<int, NT>{});
+  else if (FEWER && active)
+    run(std::integral_constant<int, FEWER ? NT - 1 : 0>{});  // without its last tile
   else
-    run(std::false_type{});
+    run(std::integral_constant<int, 0>{});
   if (!grp) end_phase(false);
 
   // The state, as in the kernel above: a quarter of O / l (O is a sixteenth),
@@ -1148,8 +1159,8 @@ __device__ __forceinline__ void wide_piece(const PieceArgs &a, char *lds_raw, in
     float2 *ml = reinterpret_cast<float2 *>(state + static_cast<int64_t>(W::ROWS) * D * 2);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int lr = wave * 16 * NT + 16 * nt + n;
-      if (row0 + 16 * nt + n < nrows) {
+      const int lr = row0 - block * W::ROWS + TILE_STEP * nt + n;
+      if (row0 + TILE_STEP * nt + n < nrows) {
         const bool seen = lim[nt] > 0 && m_run[nt] != -INFINITY;
         const float l = seen ? lsum[nt][0] : 0.f;
         const float f = l > 0.f ? 4.f / l : 0.f;
