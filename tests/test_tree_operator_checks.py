@@ -234,3 +234,14 @@ def test_another_view_of_the_query_as_output(lib, cpu):
     args[0], args[12] = buf[:3], buf[::2][:3]
     with pytest.raises(RuntimeError, match="not another view"):
         ops_api.ops().rope_kv_store_paged(*args)
+
+
+def test_more_than_a_launch_takes_is_refused(lib):
+    # 2^32 threads of a launch at most.
+    refused(lib, rope, "too many tokens", ntok=1 << 27)
+    refused(lib, rope, "too many tokens", ntok=1 << 26)  # its queries
+    refused(lib, accept, "batch", batch=1 << 24)
+    refused(lib, keep, "batch", batch=1 << 24)
+    refused(lib, logprobs, "too many rows", rows=1 << 24)
+    refused(lib, logprobs, "too many rows", rows=(1 << 24) // 2, vocab=1 << 19, stride=1 << 19)  # two slices a row
+    assert lib.k8v4_token_logprobs_workspace_bytes((1 << 24) - 1, 1000, 5) == 0
