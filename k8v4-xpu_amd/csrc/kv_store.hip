@@ -236,12 +236,14 @@ __global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs a) {
 // Lane `sub` of the D / 16 lanes of a head holds eight first and eight second
 // members of pairs 8 sub .. 8 sub + 7, whichever way they lie, so it needs the same
 // eight cosines and sines in both layouts and no other lane's dims.  A wave takes
-// all query heads of one token, whose cosines and sines it reads once; the keys and
-// values, four times the arithmetic, go to waves of their own, ahead of the queries'.
+// all query heads of one token, whose cosines and sines it reads once; the keys, four
+// times the arithmetic, and the values go to waves of their own, ahead of the
+// queries'.  (Values behind the keys in one wave: a single token 5.0 us instead of 3.8,
+// 16,223 tokens the same.)
 //
 // Bound by memory: 15.7 KB a token with four KV heads of 128 dims, most of it the
 // queries read and written; 16,223 tokens take 56 us, 4.6 TB/s, where a copy reaches
-// 4.9.  A single token takes 5 us, the launch and two round trips (slot and
+// 4.9.  A single token takes 3.8 us, the launch and two round trips (slot and
 // position, then its angles).
 struct RopeArgs {
   StoreArgs kv;
@@ -361,36 +363,52 @@ __device__ __forceinline__ void rope_queries(const RopeArgs &a, int64_t token, i
   }
 }
 
+// Even waves take keys, odd ones the same tokens' values.
 template <int D, int HKV>
 __device__ __forceinline__ void rope_store(const RopeArgs &ra, int64_t wave, int lane) {
 #pragma clang fp contract(off)
   constexpr int LPU = D / 16, UPW = kWave / LPU;
   const StoreArgs &a = ra.kv;
   const int sub = lane % LPU;
-  int64_t unit = wave * UPW + lane / LPU;
+  int64_t unit = (wave >> 1) * UPW + lane / LPU;
   const bool live = unit < a.units;
   if (!live) unit = a.units - 1;  // keep the group's shuffles on real data
   const int64_t token = unit / HKV;
   const int head = static_cast<int>(unit - token * HKV);
   const int64_t slot = a.slots[token];
   const int64_t pos = position_of(ra, token);
-  const RopeLane l = rope_lane(ra, sub);
-  const uint16_t *ksrc = a.k + token * a.k_tok_stride + head * D, *vsrc = a.v + token * a.v_tok_stride + head * D;
-  const u32x4 kw0 = load8(ksrc + l.d0), kw1 = load8(ksrc + l.d1);
-  const u32x4 vw0 = load8(vsrc + 16 * sub), vw1 = load8(vsrc + 16 * sub + 8);
   const bool there = pos >= 0 && pos < ra.table_rows;
+  const int64_t page = slot >= 0 ? slot / kPage : -1;
+  const bool stores = live && there && page >= 0 && page < a.num_pages;
+  const int64_t cell = (slot - page * kPage) * HKV + head;
+  if (wave & 1) {
+    const uint16_t *src = a.v + token * a.v_tok_stride + head * D + 16 * sub;
+    const u32x4 w0 = load8(src), w1 = load8(src + 8);
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = elem(i < 8 ? w0 : w1, i & 7, a.bf16);
+    float lo = x[0], hi = x[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) {
+      lo = fminf(lo, x[i]);
+      hi = fmaxf(hi, x[i]);
+    }
+    lo = group_min<LPU>(lo);
+    hi = group_max<LPU>(hi);
+    if (stores) store_v<D>(a, x, lo, hi, page, cell, sub);
+    return;
+  }
+  const RopeLane l = rope_lane(ra, sub);
+  const uint16_t *ksrc = a.k + token * a.k_tok_stride + head * D;
+  const u32x4 kw0 = load8(ksrc + l.d0), kw1 = load8(ksrc + l.d1);
   float c[8] = {}, s[8] = {};
   if (there && l.rotates) {
     load_angles(ra, pos * ra.table_stride + 8 * sub, c);
     load_angles(ra, pos * ra.table_stride + ra.rot / 2 + 8 * sub, s);
   }
-  float vx[16];
   double kx[16];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    kx[i] = elem(i < 8 ? kw0 : kw1, i & 7, a.bf16);
-    vx[i] = elem(i < 8 ? vw0 : vw1, i & 7, a.bf16);
-  }
+  for (int i = 0; i < 16; ++i) kx[i] = elem(i < 8 ? kw0 : kw1, i & 7, a.bf16);
   if (l.rotates) {
     if (ra.neox)
       rotate(true, c, s, kx);
@@ -398,20 +416,11 @@ __device__ __forceinline__ void rope_store(const RopeArgs &ra, int64_t wave, int
       rotate(false, c, s, kx);
   }
   double amax = 0.0;
-  float lo = vx[0], hi = vx[0];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    amax = fmax(amax, fabs(kx[i]));
-    lo = fminf(lo, vx[i]);
-    hi = fmaxf(hi, vx[i]);
-  }
+  for (int i = 0; i < 16; ++i) amax = fmax(amax, fabs(kx[i]));
 #pragma unroll
   for (int m = 1; m < LPU; m <<= 1) amax = fmax(amax, __shfl_xor(amax, m, kWave));
-  lo = group_min<LPU>(lo);
-  hi = group_max<LPU>(hi);
-  const int64_t page = slot >= 0 ? slot / kPage : -1;
-  if (!live || !there || page < 0 || page >= a.num_pages) return;
-  const int64_t cell = (slot - page * kPage) * HKV + head;
+  if (!stores) return;
 
   // The K rule, see kv_store_kernel; here the values are float64 themselves.
   const double k_scale = amax == 0.0 ? 0.0 : amax / 127.0;
@@ -443,13 +452,12 @@ __device__ __forceinline__ void rope_store(const RopeArgs &ra, int64_t wave, int
   if (sub == 0)
     *reinterpret_cast<float *>(reinterpret_cast<char *>(a.k_scale) + page * a.ks_ps + cell * 4) =
         static_cast<float>(k_scale);
-  store_v<D>(a, vx, lo, hi, page, cell, sub);
 }
 
 template <int D, int HKV>
 __global__ __launch_bounds__(256) void rope_store_kernel(RopeArgs a) {
   const int lane = threadIdx.x & (kWave - 1);
-  const int64_t w = threadIdx.x / kWave;
+  const int64_t w = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
   if (static_cast<int64_t>(blockIdx.x) < a.kv_blocks) {
     rope_store<D, HKV>(a, static_cast<int64_t>(blockIdx.x) * 4 + w, lane);
     return;
@@ -637,7 +645,7 @@ extern "C" int k8v4_rope_kv_store_paged(const void *q, const void *k, const void
   a.neox = neox != 0;
   a.ntok = ntok;
   const int upw = kWave / (head_dim / 16);
-  a.kv_blocks = ((a.kv.units + upw - 1) / upw + 3) / 4;
+  a.kv_blocks = ((a.kv.units + upw - 1) / upw + 1) / 2;
   const int64_t blocks = a.kv_blocks + (q ? (ntok + 3) / 4 : 0);
   K8V4_REQUIRE(blocks < (int64_t(1) << 24), "too many tokens for one launch");  // 2^32 threads
   const dim3 grid(static_cast<unsigned>(blocks));
