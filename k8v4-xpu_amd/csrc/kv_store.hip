@@ -241,8 +241,8 @@ __global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs a) {
 // queries'.  (Values behind the keys in one wave: a single token 5.0 us instead of 3.8,
 // 16,223 tokens the same.)
 //
-// Bound by memory: 15.7 KB a token with four KV heads of 128 dims, most of it the
-// queries read and written; 16,223 tokens take 56 us, 4.6 TB/s, where a copy reaches
+// Bound by memory: 15.4 KB a token with four KV heads of 128 dims, most of it the
+// queries read and written; 16,223 tokens take 56 us, 4.5 TB/s, where a copy reaches
 // 4.9.  A single token takes 3.8 us, the launch and two round trips (slot and
 // position, then its angles).
 struct RopeArgs {
