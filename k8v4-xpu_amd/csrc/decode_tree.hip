@@ -144,18 +144,24 @@ TreeShape shape_of(bool wide, int64_t batch, int nodes, int hkv, int head_dim) {
 //                    8          63: 21.1 / 15.9   504: 25.8 / 24.6  1004: 30.9 / 30.1  6256: 71 / 98
 //                    16         63: 21.8 / 18.4  1004: 35.9 / 37.3  2004: 48.8 / 52.6  6256: 113 / 129
 //                    21         33: 21.4 / 18.4  1032: 46.1 / 40.9                     6256: 160 / 145
-//                    26        127: 25.6 / 24.8   504: 36.2 / 37.5  1004: 49.2 / 43.8
+//                    26         63: 22.1 / 20.2   252: 30.7 / 29.1   504: 41.1 / 34.9  1004: 50.9 / 43.1
+//                    32         63: 22.9 / 21.2   252: 32.0 / 29.8   504: 42.5 / 36.9
+//                    42         63: 24.3 / 27.0   126: 29.2 / 27.0   252: 37.1 / 34.9
 //                    64         63: 26.2 / 35.2   254: 40.7 / 45.0   504: 54.0 / 44.7  6256: 395 / 264
 //   D 128, 2 heads   8          63: 19.0 / 15.4   504: 24.1 / 21.1  2004: 30.3 / 28.9  6256: 46 / 56
+//                    32         63: 20.8 / 21.0   126: 22.5 / 21.6   252: 26.2 / 25.9
+//                    42         63: 22.7 / 23.3   126: 24.8 / 27.1   252: 27.2 / 27.3
 //                    64        254: 30.8 / 37.1  1004: 51.1 / 50.4  2004: 74.7 / 65.1
 //   D 256, 2 heads   8          63: 21.5 / 18.2   504: 26.4 / 25.0  1004: 32.5 / 32.3  2004: 39.8 / 46.6
 //                    16         63: 21.7 / 21.3  1004: 38.9 / 37.8  2004: 55.0 / 53.9
+//                    26        126: 26.7 / 27.1   252: 31.4 / 33.1   504: 40.9 / 38.3
 //                    42        127: 29.2 / 35.6   254: 36.8 / 36.7   504: 49.2 / 44.7  2004: 126 / 79
 //   D 256, 4 heads   8          63: 24.2 / 18.8   504: 33.2 / 32.1  1004: 42.5 / 46.8  2004: 56.8 / 75.1
 //                    42         63: 31.9 / 35.3   127: 39.9 / 36.6   504: 77.5 / 54.4  2004: 222 / 123
 bool takes_wide(int nodes, int64_t pages, int hkv, int head_dim) {
   if (nodes <= 16) return pages <= 64 * nodes;
   if (nodes <= 21 || (hkv == 4 && head_dim == 256)) return true;  // one row tile a wave, or half as much LDS a row
+  if (head_dim == 128 && (nodes <= 32 || (nodes <= 42 && hkv == 4 && pages > 96))) return true;  // two
   return pages > 384;
 }
 

@@ -2,8 +2,8 @@
 
 Which kernel int8k_int4v_attn_tree takes depends on the nodes and on the pages that
 the tables have room for: eight nodes at a time up to 16 nodes over more than 64 pages
-a node, and from 22 on over up to 384 pages (but for four heads of 256 dims), all rows
-of a KV head otherwise.  Here tables are widened by entries that no length reaches, so
+a node, and from 22 (256 dims) or 33 on over up to 384 pages (but for four heads of 256
+dims, and some of 42 nodes and fewer), all rows of a KV head otherwise.  Here tables are widened by entries that no length reaches, so
 that short sequences take either.  Tolerances are test_gpu_tree's and, for bytes, none.
 """
 from __future__ import annotations
