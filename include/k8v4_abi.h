@@ -424,7 +424,9 @@ int64_t k8v4_verify_drafts_workspace_bytes(int64_t batch, int64_t vocab);
  * rotated.  neox: pair i is dims (i, i + rotary_dim / 2), else (2 i, 2 i + 1);
  * a pair (x, y) becomes (x c - y s, y c + x s).
  * Keys: the rotated row in float64, unrounded, goes through the K rule; a
- * token without a slot stores nothing.  Values as in k8v4_kv_store_paged.
+ * token without a slot stores nothing; no two tokens of a call have the same slot
+ * (which of them a head's key and value would be of is not defined).  Values as in
+ * k8v4_kv_store_paged.
  * q: [ntok, 6*hkv, head_dim] of src_dtype (NULL with q_out NULL: none), head
  * stride head_dim; q_out: the rotated rows, computed in fp32 and rounded once;
  * may be q itself (same strides), must not overlap it otherwise.  All tokens'

@@ -417,9 +417,10 @@ class _Ops:
         both None: no queries); ``positions`` int32 or int64 ``[T]``; ``cos_sin``
         ``[P, R]`` (fp16, bf16 or fp32), row p the R / 2 cosines, then the sines of
         position p, R a multiple of 16 up to D; ``neox``: pairs are dims (i, i + R / 2),
-        else (2 i, 2 i + 1).  Keys are quantized from the unrounded rotation.  A token
-        without a slot stores nothing; one whose position lies outside the table neither,
-        and its query rows become zeros."""
+        else (2 i, 2 i + 1).  Keys are quantized from the unrounded rotation.  Slots
+        are distinct; a token without one (negative, or past the last page) stores nothing;
+        one whose position lies outside the table neither, and its query rows become
+        zeros."""
         bound = self.bind_rope_kv_store_paged(q_fp16, k_fp16, v_fp16, positions, cos_sin, neox, slot_mapping, k_cache,
                                               k_scale, v_cache, v_scale, v_zero, q_out)
         if bound is not None:
