@@ -126,19 +126,21 @@ __device__ __forceinline__ Sums join(Sums a, Sums b) {
 
 // The sums as a wave forms them, its maximum m in every lane: in powers of two
 // against m2, the fp32 value of m log2(e), so that an element takes one fma, t = x
-// log2(e) - m2.  m itself then has t = off, some 2^-24 of m2, which `sums_of` takes out.
-// A maximum of 1e37 or more of either sign (its log2(e) may not exist) leaves
-// nothing but equal elements to the sums; t is not formed then.
+// log2(e) - m2.  m itself then has t = off, some 2^-24 of m2, which `sums_of` takes out
+// by 2^off = 1 + off ln 2: below 4096 |off| is 2^-12 at most and the square left out
+// (off ln 2)^2 / 2 < 2^-26.  From there on (`far`, infinities too) t is (x - m) log2(e),
+// a subtraction more an element, with m2 and off 0.
 struct WaveSums {
   float m, m2, off;
   float r, q;  // sum 2^t, sum t 2^t, of the lane
 };
-__device__ __forceinline__ bool huge(float m) { return !(fabsf(m) < 1e37f); }
+__device__ __forceinline__ bool far(float m) { return !(fabsf(m) < 4096.f); }
 // `own`: this lane counts the element left out so far.
 __device__ __forceinline__ void raise(WaveSums &s, float m, bool own) {
-  const float m2 = m * kLog2e;
+  const float m2 = far(m) ? 0.f : m * kLog2e;
+  const float off = far(m) ? 0.f : fmaf(m, kLog2e, -m2);
   if (s.m > -INFINITY) {
-    const float d = huge(m) || huge(s.m) ? kFarBelow : fmaxf(s.m2 - m2, kFarBelow);
+    const float d = fmaxf(fmaf(s.m - m, kLog2e, off - s.off), kFarBelow);
     const float f = __builtin_amdgcn_exp2f(d);
     const float w = own ? fmaf(s.off, kLn2, 1.f) : 0.f;  // 2^off
     s.r += w;
@@ -146,8 +148,8 @@ __device__ __forceinline__ void raise(WaveSums &s, float m, bool own) {
     s.r *= f;
   }
   s.m = m;
-  s.m2 = huge(m) ? 0.f : m2;
-  s.off = huge(m) ? 0.f : fmaf(m, kLog2e, -m2);
+  s.m2 = m2;
+  s.off = off;
 }
 __device__ __forceinline__ Sums sums_of(const WaveSums &s, float r, float q) {
   const float f = fmaf(-s.off, kLn2, 1.f);  // 2^-off
@@ -416,7 +418,7 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
       usual &= vmax[j] <= s.m;  // false for a NaN
     }
     if (!ONE && at + kBatch * STEP < end) load(at + kBatch * STEP);
-    const bool special = !__all(usual) || huge(s.m);
+    const bool special = !__all(usual) || far(s.m);
     bool holder = false;  // of a new maximum, whose first element is left out of the sums
     if (special) {
       // A new maximum, a vector of NaN (or with a signalling one), or nothing so far.
@@ -466,8 +468,8 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
         if ((lane & (kGroupLanes - 1)) == 0) values[(at - first + j * STEP + t * N) / CHUNK] = c;
       }
     }
-    auto add = [&](int j, int i, float &r, float &q) __attribute__((always_inline)) {
-      const float y = fmaxf(fmaf(f[j][i], kLog2e, -s.m2), kFarBelow);  // a NaN or minus infinity: 2^y is 0
+    auto add = [&](float t, float &r, float &q) __attribute__((always_inline)) {
+      const float y = fmaxf(t, kFarBelow);  // a NaN or minus infinity: 2^y is 0
       const float e = __builtin_amdgcn_exp2f(y);
       r += e;
       q = fmaf(y, e, q);
@@ -477,12 +479,12 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
       for (int j = 0; j < kBatch; ++j) {
         float r = 0.f, q = 0.f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) add(j, i, r, q);
+        for (int i = 0; i < N; ++i) add(fmaf(f[j][i], kLog2e, -s.m2), r, q);
         s.r += r;
         s.q += q;
       }
     } else if (s.m > -INFINITY) {
-      const bool only_equal = huge(s.m);
+      const float base = far(s.m) ? s.m : 0.f;
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
         float r = 0.f, q = 0.f;
@@ -491,10 +493,8 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
           const bool equal = f[j][i] == s.m;
           if (holder && equal)
             holder = false;
-          else if (!only_equal)
-            add(j, i, r, q);
-          else if (equal)
-            r += 1.f;
+          else
+            add(equal ? s.off : fmaf(f[j][i] - base, kLog2e, -s.m2), r, q);  // (equal: of infinities no difference)
         }
         s.r += r;
         s.q += q;
