@@ -79,8 +79,15 @@ __device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x;
 // Whether (x, i) comes ahead of (y, j).
 __device__ __forceinline__ bool ahead(float x, int i, float y, int j) { return x > y || (x == y && i < j); }
 
-// The largest of three without the compiler's quieting of each operand: a quiet
-// NaN gives way to the others, a signalling one makes the result NaN.
+// A NaN of either kind gives way to the other operand of a maximum.  (In the mode that
+// kernels begin in, a signalling one makes the result NaN, and as an instruction of three
+// is two maxima, the second then drops what the first should have kept.)  The wave's
+// MODE bit for it, cleared ahead of all loads, so ahead of the maxima over them.
+__device__ __forceinline__ void nan_gives_way() {
+  asm volatile("s_setreg_imm32_b32 hwreg(HW_REG_MODE, 9, 1), 0" ::: "memory");
+}
+// The largest of three, without the compiler's quieting of each operand: NaN only if all
+// are, once nan_gives_way() was called.
 __device__ __forceinline__ float max3_raw(float a, float b, float c) {
   float r;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
@@ -377,6 +384,7 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
   constexpr int STEP = kThreads * N;      // elements of one vector of every thread
   __shared__ Shared sh;
   extern __shared__ float values[];  // the largest of each chunk, later the picked chunks' tokens (ONE: not used)
+  nan_gives_way();
   const int t = threadIdx.x, lane = t & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(t / kWave);
   const int64_t row = blockIdx.x / static_cast<unsigned>(a.slices);
   const int slice = static_cast<int>(blockIdx.x - row * a.slices);
@@ -415,13 +423,13 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
 #pragma unroll
       for (int i = 3; i + 1 < N; i += 2) mx = max3_raw(mx, f[j][i], f[j][i + 1]);
       vmax[j] = max3_raw(mx, f[j][N - 1], f[j][N - 1]);
-      usual &= vmax[j] <= s.m;  // false for a NaN
+      usual &= vmax[j] <= s.m;  // false for NaN
     }
     if (!ONE && at + kBatch * STEP < end) load(at + kBatch * STEP);
     const bool special = !__all(usual) || far(s.m);
     bool holder = false;  // of a new maximum, whose first element is left out of the sums
     if (special) {
-      // A new maximum, a vector of NaN (or with a signalling one), or nothing so far.
+      // A new maximum, a vector of NaN, or nothing so far.
       bool nan = ONE;  // (the elements are needed without NaN)
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) nan |= vmax[j] != vmax[j];
