@@ -270,6 +270,7 @@ class Xe2K8V4Impl(AttentionImpl[Xe2K8V4Metadata]):
         self.scale = float(scale)
         self.kv_cache_dtype = kv_cache_dtype
         self.kv_sharing_target_layer_name = kv_sharing_target_layer_name
+        self.rotary_dims = _rotary_dims(_engine_config(), int(head_size))
 
     # -- store ---------------------------------------------------------------
     def do_kv_cache_update(
@@ -301,8 +302,9 @@ class Xe2K8V4Impl(AttentionImpl[Xe2K8V4Metadata]):
 
     def fused_rope_kvcache_supported(self) -> bool:
         """Whether :meth:`do_rope_and_kv_cache_update` may stand for the model's rotation
-        and :meth:`do_kv_cache_update`."""
-        return True
+        and :meth:`do_kv_cache_update`: every rotary dim that the engine's model names is
+        one the fused store takes (a model that names none rotates whole heads)."""
+        return all(0 < r <= self.layout.head_dim and r % 16 == 0 for r in self.rotary_dims)
 
     def do_rope_and_kv_cache_update(
         self,
@@ -442,6 +444,35 @@ class Xe2K8V4Impl(AttentionImpl[Xe2K8V4Metadata]):
 def _runs_alone(width: int, seq_len: int, layout) -> bool:
     _check_covers(seq_len, width)
     return ops().prefill_uses_tiles(seq_len, width, layout.hkv, layout.head_dim)
+
+
+def _engine_config():
+    """The config of the engine that is making its layers, None outside one."""
+    try:
+        from vllm.config import get_current_vllm_config
+
+        return get_current_vllm_config()
+    except (ImportError, AssertionError):
+        return None
+
+
+def _rotary_dims(cfg, head_dim: int) -> tuple[int, ...]:
+    """The rotary dims that the model's config names, in any of its usual places: in dims
+    (``rotary_dim``) or as a part of the head's (``partial_rotary_factor``, ``rotary_pct``),
+    by itself or among the rope parameters, which may be one set for every kind of layer."""
+    model = getattr(cfg, "model_config", None)
+    hf = getattr(model, "hf_text_config", None) or getattr(model, "hf_config", None)
+    places = [{n: getattr(hf, n, None) for n in ("rotary_dim", "partial_rotary_factor", "rotary_pct")}]
+    for name in ("rope_parameters", "rope_scaling"):
+        rope = getattr(hf, name, None)
+        if isinstance(rope, dict):
+            places += [rope, *(x for x in rope.values() if isinstance(x, dict))]
+    dims = []
+    for place in places:
+        if place.get("rotary_dim") is not None:
+            dims.append(int(place["rotary_dim"]))
+        dims += [int(head_dim * float(place[n])) for n in ("partial_rotary_factor", "rotary_pct") if place.get(n) is not None]
+    return tuple(dims)
 
 
 def _engine_shares_prefixes(cfg) -> bool:
