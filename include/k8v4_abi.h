@@ -457,7 +457,9 @@ int k8v4_rope_kv_store_paged(const void *q, const void *k, const void *v, int sr
  * others do.  A row that sees no key outputs zeros.
  * The chain's mask, 2^(j+1) - 1, gives what k8v4_attn_batch does.  Query
  * rows, cache, table, seq_lens (the tree's tokens counted), out and numerics as
- * in k8v4_attn_batch; page strides below 2^31 bytes.
+ * in k8v4_attn_batch; page strides below 2^31 bytes.  Which of two kernels runs
+ * depends on the nodes and on the pages that the tables have room for, not on the
+ * lengths: a table_width no larger than the longest sequence needs is served best.
  * workspace: >= k8v4_attn_tree_workspace_bytes(batch, nodes, hkv, head_dim)
  * bytes, 16-byte aligned.  Calls that may overlap (other streams, captured
  * graphs) need one each.

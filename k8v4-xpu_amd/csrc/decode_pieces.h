@@ -204,8 +204,8 @@ __device__ __forceinline__ void walk_pieces(const PieceArgs &args, int wg, Piece
 // in the wide form for every KV head and row block).  They are of one of the chip's
 // eight dies, eight ids apart, so that what one of them loads the others find in the
 // die's cache: over the dies' common memory the pages would be as slow as read again
-// (eight nodes at a time over four times 100,000 tokens, 64 nodes 452 us with ids in
-// the order of the shares, 395 so; 16 nodes 123 and 116).
+// (eight nodes at a time over four times 100,000 tokens, 64 nodes 467 us with ids in
+// the order of the shares, 406 so; 16 nodes 120 and 112).
 struct TreePlace {
   int part, share;
 };
@@ -625,11 +625,11 @@ struct Wide {
 __device__ __forceinline__ int vswz(int row) { return (row & 7) ^ ((row >> 3) & 1); }
 
 // Whether the wide form over drafted trees quantizes its query rows itself.  With one
-// 128-dim row tile a wave that costs a piece less than a launch ahead of it does
-// (13 nodes over 2,048 tokens 16.5 us against 17.0, 16 over four times 100,000 145
-// against 151); with more it is done again by every work-group for longer than the
-// launch takes (64 nodes over 2,048: 33.1 against 28.7; head dim 256, 13 nodes: 21.5
-// against 20.3).
+// 128-dim row tile a wave that costs a short call less than a launch ahead of it does
+// (13 nodes over 2,048 tokens 17.1 us against 17.6) and a long one nothing (16 over four
+// times 100,000 133 and 132); with more it is done again by every work-group for longer
+// than the launch takes (64 nodes over 2,048: 33.1 against 28.7; head dim 256, 13 nodes:
+// 21.5 against 20.3).
 constexpr bool tree_quantizes(int head_dim, int tiles) { return head_dim == 128 && tiles == 1; }
 
 // A 16-row tile of query rows made int8 operands by the K rule (k_rule_code): lane (n,

@@ -46,9 +46,9 @@ void tree_split_kernel(PieceArgs args) {
 constexpr int wide_groups(int head_dim, int tiles) { return head_dim == 128 && tiles == 1 ? 2 : 1; }
 
 // Many rows of one KV head: wide_piece in decode_pieces.h, TILES row tiles a wave.
-// Bound by issue: 64 nodes over four times 100,000 tokens (4 KV heads, D 128) 264 us,
-// 1,073 TFLOP/s of products (two thirds of them fp16's share of the time); 16 nodes,
-// where unpacking a page for all waves weighs more, 129 us.
+// Bound by issue: 64 nodes over four times 100,000 tokens (4 KV heads, D 128) 271 us,
+// 1,045 TFLOP/s of products (two thirds of them fp16's share of the time); 16 nodes,
+// where unpacking a page for all waves weighs more, 133 us.
 template <int D, int HKV, int TILES>
 __global__ __attribute__((amdgpu_flat_work_group_size(512, 512),
                           amdgpu_waves_per_eu(2 * wide_groups(D, TILES), 2 * wide_groups(D, TILES))))
@@ -134,7 +134,8 @@ TreeShape shape_of(bool wide, int64_t batch, int nodes, int hkv, int head_dim) {
 }
 
 // Which form serves trees of so many nodes over tables of so many pages in all (of
-// the lengths the host knows no more): the wide form, or eight nodes at a time.  A
+// the lengths the host knows no more: a table wider than its sequences need has the
+// form of longer ones, with their costs): the wide form, or eight nodes at a time.  A
 // wide page costs about as much for 1 as for 20 nodes (unpacked once for all rows, in
 // phases that wait for each other), the other form's about the same for each run of
 // eight; over a few pages the latter has the longer chain, but for the wide form's
@@ -142,22 +143,33 @@ TreeShape shape_of(bool wide, int64_t batch, int nodes, int hkv, int head_dim) {
 // so many pages (4,000 tokens of one sequence to 100,000 of four):
 //   D 128, 4 heads   4 nodes    63: 18.7 / 14.9   254: 19.8 / 20.2  1004: 27.8 / 29.1  6256: 68 / 93
 //                    8          63: 21.1 / 15.9   504: 25.8 / 24.6  1004: 30.9 / 30.1  6256: 71 / 98
-//                    16         63: 21.8 / 18.4  1004: 35.9 / 37.3  2004: 48.8 / 52.6  6256: 113 / 129
+//                    16         63: 21.8 / 18.4  1004: 35.9 / 37.3  2004: 48.8 / 52.6  6256: 112 / 133
+//                    17         63: 22.2 / 19.1  1008: 53.0 / 45.0                     6256: 159 / 138
 //                    21         33: 21.4 / 18.4  1032: 46.1 / 40.9                     6256: 160 / 145
 //                    26         63: 22.1 / 20.2   252: 30.7 / 29.1   504: 41.1 / 34.9  1004: 50.9 / 43.1
 //                    32         63: 22.9 / 21.2   252: 32.0 / 29.8   504: 42.5 / 36.9
 //                    42         63: 24.3 / 27.0   126: 29.2 / 27.0   252: 37.1 / 34.9
-//                    64         63: 26.2 / 35.2   254: 40.7 / 45.0   504: 54.0 / 44.7  6256: 395 / 264
+//                    64         63: 26.2 / 35.2   254: 40.7 / 45.0   504: 54.0 / 44.7  6256: 406 / 271
 //   D 128, 2 heads   8          63: 19.0 / 15.4   504: 24.1 / 21.1  2004: 30.3 / 28.9  6256: 46 / 56
+//                    21         63: 20.5 / 19.0  1008: 36.8 / 33.4                     6256: 88 / 77
 //                    32         63: 20.8 / 21.0   126: 22.5 / 21.6   252: 26.2 / 25.9
 //                    42         63: 22.7 / 23.3   126: 24.8 / 27.1   252: 27.2 / 27.3
-//                    64        254: 30.8 / 37.1  1004: 51.1 / 50.4  2004: 74.7 / 65.1
+//                    64        254: 30.8 / 37.1   504: 43.1 / 45.0   756: 55.8 / 53.9
+//                             1004: 51.1 / 50.4  2004: 74.7 / 65.1
 //   D 256, 2 heads   8          63: 21.5 / 18.2   504: 26.4 / 25.0  1004: 32.5 / 32.3  2004: 39.8 / 46.6
 //                    16         63: 21.7 / 21.3  1004: 38.9 / 37.8  2004: 55.0 / 53.9
+//                    21         63: 23.5 / 22.7  1008: 55.9 / 45.8                     6256: 190 / 140
 //                    26        126: 26.7 / 27.1   252: 31.4 / 33.1   504: 40.9 / 38.3
 //                    42        127: 29.2 / 35.6   254: 36.8 / 36.7   504: 49.2 / 44.7  2004: 126 / 79
 //   D 256, 4 heads   8          63: 24.2 / 18.8   504: 33.2 / 32.1  1004: 42.5 / 46.8  2004: 56.8 / 75.1
+//                    21         63: 28.3 / 23.7  1008: 88.4 / 70.9                     6256: 363 / 269
+//                    26         63: 28.0 / 26.7
 //                    42         63: 31.9 / 35.3   127: 39.9 / 36.6   504: 77.5 / 54.4  2004: 222 / 123
+//                    50         63: 34.7 / 35.0   126: 44.6 / 43.6   252: 59.8 / 51.1
+//                    64         63: 36.6 / 35.4   252: 61.1 / 52.9   504: 110 / 90.4
+// The lines are simple, and next to them the slower form may be taken: by up to 4 % (4
+// nodes at 254 pages, 16 at 1,004, 64 of two 128-dim heads from 384 to about 700), and
+// by a tenth for about 42 nodes of four 256-dim heads over one sequence of 4,000 tokens.
 bool takes_wide(int nodes, int64_t pages, int hkv, int head_dim) {
   if (nodes <= 16) return pages <= 64 * nodes;
   if (nodes <= 21 || (hkv == 4 && head_dim == 256)) return true;  // one row tile a wave, or half as much LDS a row

@@ -21,7 +21,7 @@
 // a second launch.
 //
 // Bound by memory, closely followed by issue (12 slots an element): 2048 x 152000 bf16
-// with 20 tokens a row 150 us, 4.1 TB/s (a sum over 2 GiB reads 4.0); calls of a few
+// with 20 tokens a row 145 us, 4.3 TB/s (a sum over 2 GiB reads 4.0); calls of a few
 // rows by latency, two launches of about 7 and 5 us.
 #include "k8v4_common.h"
 
@@ -607,12 +607,12 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(LogprobArgs a) {
 }
 
 // How many slices a row is cut into.  One that a work-group holds, or nearly, is not
-// cut (256 x 8000 bf16 10.0 us in one launch, 14.1 in slices and a second one).  Others
+// cut (256 x 8000 bf16 11.4 us in one launch, 16.8 in slices and a second one).  Others
 // are for two work-groups a compute unit, or for four where that leaves slices that
 // are held in few registers, or long ones.  Measured, two a unit / four, us: 48 x 65537
-// fp16 17.7 / 16.1, 128 x 32000 fp32 23.1 / 19.0, 256 x 32000 bf16 26.7 / 29.6, 512 x
-// 32000 bf16 27.9 / 32.1, 128 x 152000 fp32 35.2 / 31.3, 256 x 152000 bf16 52.3 / 46.6
-// (one: 58.0; eight: 59.6).
+// fp16 17.0 / 15.7, 128 x 32000 fp32 22.4 / 18.8, 256 x 32000 bf16 25.5 / 28.5, 512 x
+// 32000 bf16 26.0 / 30.8, 128 x 152000 fp32 38.1 / 35.0, 256 x 152000 bf16 48.7 / 44.1
+// (one: 53.0; eight: 56.7).
 constexpr int64_t kHeldWhole = 8192, kShortSlice = 4096, kLongSlice = 16384;
 int slices_of(int64_t rows, int64_t vocab) {
   if (vocab <= kHeldWhole) return 1;

@@ -667,7 +667,8 @@ class _Ops:
         ``tree_masks[b, j]`` (int64 ``[B, nodes]``; a row expanded over the batch is one
         tree for all; :func:`k8v4_v030.plan.tree_masks` makes them from parents).  The
         other arguments and the numerics are the batch op's; ``workspace`` holds
-        :meth:`attn_tree_workspace_bytes` bytes."""
+        :meth:`attn_tree_workspace_bytes` bytes.  The kernel is chosen by the table's
+        width: short contexts are served best with no wider a table than they need."""
         self.bind_int8k_int4v_attn_tree(q_fp16, k_cache, k_scale, v_cache, v_scale, v_zero, block_table, seq_lens,
                                         tree_masks, workspace, out, nodes, pages_per_block)()
 
